@@ -444,7 +444,7 @@ def _compact(s):
 
 def _write(s):
     if own:
-        s.cache.write(s.layer, s.k.data_ptr(), s.v.data_ptr(), s.offsets.data_ptr(), s.rows,
+        s.cache.write(s.layer, s.k.data_ptr(), s.v.data_ptr(), s.offsets.data_ptr(), s.rows, source_rows=s.k.shape[0],
                       index=0 if s.index is None else s.index.data_ptr(), k_stride=s.k.stride(0), v_stride=s.v.stride(0),
                       stream=torch.cuda.current_stream().cuda_stream)
         return {"keys": s.keys, "values": s.values}
