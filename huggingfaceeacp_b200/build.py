@@ -4,7 +4,7 @@ with the source tree).
     python -m huggingfaceeacp_b200.build          # product libraries
     python -m huggingfaceeacp_b200.build --all    # plus the test oracle
 
-libhf_cuda.so : csrc/hf_cuda.cu for sm_100a (nvcc -gencode arch=compute_100a,code=sm_100a)
+libhf_cuda.so : csrc/hf_cuda.cu + csrc/operators.cu for sm_100a (nvcc -gencode arch=compute_100a,code=sm_100a)
 libhf_host.so : host/int8_blocks.cpp + host/synthetic.cpp (F16C, pthreads)
 libhf.so      : host/hf_decoder.cpp, the C++ HF:: surface over the two above
 """
@@ -47,11 +47,23 @@ def build_host(force=False):
 def build_cuda(force=False):
     os.makedirs(LIB, exist_ok=True)
     csrc = os.path.join(PKG, "csrc")
-    sources = [os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".cu", ".cuh"))]
+    headers = [os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith(".cuh")]
+    headers += [os.path.join(INCLUDE, "hf_cuda.h"), os.path.join(PKG, "host", "safetensors.h")]
     target = os.path.join(LIB, "libhf_cuda.so")
-    if force or _stale(target, sources + [os.path.join(INCLUDE, "hf_cuda.h"), os.path.join(PKG, "host", "safetensors.h")]):
-        _run([NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", f"-I{INCLUDE}",
-              os.path.join(csrc, "hf_cuda.cu"), "-o", target])
+    objects, compiling = [], []
+    for source in ("hf_cuda.cu", "operators.cu"):
+        path, obj = os.path.join(csrc, source), os.path.join(LIB, source[:-3] + ".o")
+        objects.append(obj)
+        if force or _stale(obj, [path, *headers]):
+            cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-c", f"-I{INCLUDE}", path,
+                   "-o", obj]
+            print("+", " ".join(cmd), flush=True)
+            compiling.append((cmd, subprocess.Popen(cmd)))
+    for cmd, process in compiling:
+        if process.wait():
+            raise subprocess.CalledProcessError(process.returncode, cmd)
+    if compiling or _stale(target, objects):
+        _run([NVCC, *ARCH, "-shared", *objects, "-o", target])
     return target
 
 

@@ -23,6 +23,7 @@
 #include "attention.cuh"
 #include "attention_tc.cuh"
 #include "gemv.cuh"
+#include "launch.cuh"
 #include "misc.cuh"
 #include "persistent.cuh"
 #include "rows_mma.cuh"
@@ -126,29 +127,6 @@ struct Layer
     float* in_norm = nullptr;
     float* post_norm = nullptr;
 };
-
-template <typename Kernel, typename... Args>
-cudaError_t launch(bool pdl, Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args)
-{
-    cudaLaunchConfig_t config = {};
-    config.gridDim = grid;
-    config.blockDim = block;
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute[0].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attribute;
-    config.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
-int sm_count(int device)
-{
-    int sms = 0;
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    return sms > 0 ? sms : 1;
-}
 
 // Opt-in shared memory for every kernel that needs more than 48 KiB, once per
 // device.

@@ -1,0 +1,395 @@
+// libhf_cuda.so: the serving operators on device pointers of include/hf_cuda.h
+// (paged cache steps, packed prompt attention, tree attention). They hold no
+// state: every check is made on the host before the first launch.
+#include <hf_cuda.h>
+
+#include "attention_rows.cuh"
+#include "launch.cuh"
+#include "pages.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace hfk;
+
+static_assert(kPagePositions == HF_PAGE_ROWS && kTreeNodes == HF_TREE_NODES, "the header's sizes");
+
+namespace
+{
+// Makes the device that holds `p` current, and the caller's again at the end.
+class DeviceOf
+{
+public:
+    explicit DeviceOf(const void* p)
+    {
+        int device = 0;
+        if (!on_device(p, &device))
+            return;
+        if (cudaGetDevice(&before) != cudaSuccess || (device != before && cudaSetDevice(device) != cudaSuccess))
+        {
+            status = HF_E_CUDA;
+            return;
+        }
+        changed = device != before;
+        current = device;
+        status = HF_OK;
+    }
+    ~DeviceOf()
+    {
+        if (changed)
+            cudaSetDevice(before);
+    }
+    DeviceOf(const DeviceOf&) = delete;
+
+    // The other buffers of the call: on the same device too.
+    template <typename... P>
+    bool holds(const P*... p) const
+    {
+        return (here(p) && ...);
+    }
+
+    int status = HF_E_INVALID;
+    int current = 0;
+
+private:
+    static bool on_device(const void* p, int* device)
+    {
+        cudaPointerAttributes a;
+        if (cudaPointerGetAttributes(&a, p) != cudaSuccess)
+        {
+            cudaGetLastError();
+            return false;
+        }
+        *device = a.device;
+        return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged;
+    }
+    bool here(const void* p) const
+    {
+        int device = 0;
+        return !p || (on_device(p, &device) && device == current);
+    }
+    int before = 0;
+    bool changed = false;
+};
+
+int size_of(int dtype)
+{
+    return dtype == HF_DTYPE_F32 ? 4 : dtype == HF_DTYPE_BF16 || dtype == HF_DTYPE_F16 ? 2 : 0;
+}
+
+bool aligned(const void* p)
+{
+    return p && (uintptr_t) p % 16 == 0;
+}
+
+// A row stride in elements: the width when 0; false when rows would overlap or
+// are not 16-byte aligned.
+bool row_stride(int64_t* stride, int64_t width, int size)
+{
+    if (*stride == 0)
+        *stride = width;
+    return *stride >= width && *stride <= (int64_t) 1 << 40 && *stride * size % 16 == 0;
+}
+
+int status_of(cudaError_t e)
+{
+    return e == cudaSuccess ? HF_OK : HF_E_CUDA;
+}
+
+// ---- the cache ---------------------------------------------------------------
+
+// Sizes only; the layer stride is filled in.
+int check_cache_sizes(const hf_page_cache* cache, hf_page_cache* c)
+{
+    if (!cache)
+        return HF_E_INVALID;
+    *c = *cache;
+    const int size = size_of(c->dtype);
+    if (!size || c->layers < 1 || c->pages < 1 || c->sequences < 1 || c->table_stride < 1
+        || c->table_stride > (1 << 20) || c->pages > (1 << 26))
+        return HF_E_INVALID;
+    if (c->kv_width < 8 || c->kv_width % 8 || c->kv_width > (1 << 20))
+        return HF_E_SHAPE;
+    const int64_t layer = (int64_t) c->pages * kPagePositions * c->kv_width;
+    if (c->layer_stride == 0)
+        c->layer_stride = layer;
+    return c->layer_stride >= layer && c->layer_stride * size % 16 == 0 ? HF_OK : HF_E_INVALID;
+}
+
+int check_cache(const hf_page_cache* cache, hf_page_cache* c)
+{
+    if (const int rc = check_cache_sizes(cache, c))
+        return rc;
+    return aligned(c->keys) && aligned(c->values) && c->table && c->lengths && c->refs ? HF_OK : HF_E_INVALID;
+}
+
+uint64_t book_bytes(const hf_page_cache& c)
+{
+    const uint64_t copies = std::max(c.sequences, c.pages);
+    return 4 * (4 + 3 * copies + 2 * (uint64_t) c.sequences + 2 * (uint64_t) c.pages);
+}
+
+PageBook book_of(const hf_page_cache& c, void* workspace)
+{
+    PageBook b = {};
+    const int size = size_of(c.dtype);
+    b.keys = (char*) c.keys;
+    b.values = (char*) c.values;
+    b.layer_bytes = c.layer_stride * size;
+    b.row_bytes = c.kv_width * size;
+    b.layers = c.layers;
+    b.pages = c.pages;
+    b.sequences = c.sequences;
+    b.table_stride = c.table_stride;
+    b.table = c.table;
+    b.lengths = c.lengths;
+    b.refs = c.refs;
+    b.copy_count = (int*) workspace;
+    b.copies = (PageCopy*) (b.copy_count + 4);
+    b.per_sequence = (int*) (b.copies + std::max(c.sequences, c.pages));
+    b.free_ids = b.per_sequence + 2 * (size_t) c.sequences;
+    b.renamed = b.free_ids + c.pages;
+    return b;
+}
+
+int copy_rows(const PageBook& b, int most, int device, cudaStream_t stream)
+{
+    const long long units = (long long) most * b.layers * 2;
+    const int grid = (int) std::min<long long>(std::max<long long>(units, 1), (long long) sm_count(device) * 8);
+    return status_of(launch(true, pages_copy_rows, dim3(grid), dim3(256), 0, stream, b));
+}
+
+// ---- the attentions -----------------------------------------------------------
+
+// Checks of what both attentions share; fills the kernels' call.
+int check_attention(int dtype, int heads, int kv_heads, int width, int rows, float scale)
+{
+    if (!size_of(dtype) || heads < 1 || kv_heads < 1 || rows < 1 || !std::isfinite(scale))
+        return HF_E_INVALID;
+    if (heads % kv_heads || heads / kv_heads > 128 || width < 8 || width % 8 || width > 256
+        || (int64_t) heads * width > (1 << 24))
+        return HF_E_SHAPE;
+    return HF_OK;
+}
+
+template <typename Call>
+int check_rows(const Call& call, int size, int heads, int kv_heads, int width, AttnCall* a)
+{
+    int64_t q = call.q_stride, k = call.k_stride, v = call.v_stride, o = call.out_stride;
+    if (!aligned(call.q) || !aligned(call.k) || !aligned(call.v) || !aligned(call.out) || !call.offsets
+        || !row_stride(&q, (int64_t) heads * width, size) || !row_stride(&k, (int64_t) kv_heads * width, size)
+        || !row_stride(&v, (int64_t) kv_heads * width, size) || !row_stride(&o, (int64_t) heads * width, size))
+        return HF_E_INVALID;
+    a->q = call.q;
+    a->k = call.k;
+    a->v = call.v;
+    a->out = call.out;
+    a->q_stride = q;
+    a->k_stride = k;
+    a->v_stride = v;
+    a->out_stride = o;
+    a->offsets = call.offsets;
+    a->rows = call.rows;
+    a->heads = heads;
+    a->kv_heads = kv_heads;
+    a->group = heads / kv_heads;
+    a->width = width;
+    a->scale_log2 = (float) (call.scale * 1.4426950408889634);
+    return HF_OK;
+}
+
+template <bool Tree>
+int run_rows(int dtype, const AttnCall& a, cudaStream_t stream)
+{
+    const long long units = (long long) a.rows * a.heads;
+    const dim3 grid((unsigned) ((units + 7) / 8));
+    cudaError_t e = dtype == HF_DTYPE_F32    ? launch(false, attention_rows<float, Tree>, grid, dim3(256), 0, stream, a)
+                    : dtype == HF_DTYPE_BF16 ? launch(false, attention_rows<__nv_bfloat16, Tree>, grid, dim3(256), 0, stream, a)
+                                             : launch(false, attention_rows<__half, Tree>, grid, dim3(256), 0, stream, a);
+    return status_of(e);
+}
+
+int check_packed_sizes(const hf_attention_packed* call)
+{
+    if (!call || call->sequences < 1)
+        return HF_E_INVALID;
+    return check_attention(call->dtype, call->heads, call->kv_heads, call->head_width, call->rows, call->scale);
+}
+
+int check_tree_sizes(const hf_page_cache* cache, hf_page_cache* c, const hf_attention_tree* call)
+{
+    if (const int rc = check_cache_sizes(cache, c))
+        return rc;
+    if (!call || call->layer < 0 || call->layer >= c->layers || call->max_nodes < 1 || call->max_length < 0)
+        return HF_E_INVALID;
+    if (const int rc = check_attention(c->dtype, call->heads, call->kv_heads, call->head_width, call->rows, call->scale))
+        return rc;
+    if (call->max_nodes > HF_TREE_NODES || c->kv_width != call->kv_heads * call->head_width)
+        return HF_E_SHAPE;
+    return HF_OK;
+}
+} // namespace
+
+extern "C" {
+int hf_cuda_pages_workspace(const hf_page_cache* cache, uint64_t* bytes)
+{
+    hf_page_cache c;
+    if (!bytes)
+        return HF_E_INVALID;
+    *bytes = 0;
+    if (const int rc = check_cache_sizes(cache, &c))
+        return rc;
+    *bytes = book_bytes(c);
+    return HF_OK;
+}
+
+int hf_cuda_pages_update(const hf_page_cache* cache, const int32_t* release, int32_t releases, const int32_t* forks,
+                         int32_t fork_count, const int32_t* grow, int32_t* result, void* workspace,
+                         uint64_t workspace_bytes, void* stream)
+{
+    hf_page_cache c;
+    if (const int rc = check_cache(cache, &c))
+        return rc;
+    if (releases < 0 || releases > c.sequences || fork_count < 0 || fork_count > c.sequences || !result
+        || (releases && !release) || (fork_count && !forks) || !aligned(workspace))
+        return HF_E_INVALID;
+    if (workspace_bytes < book_bytes(c))
+        return HF_E_CAPACITY;
+    const DeviceOf on(c.keys);
+    if (on.status)
+        return on.status;
+    if (!on.holds(c.values, c.table, c.lengths, c.refs, releases ? release : nullptr, fork_count ? forks : nullptr, grow,
+                  result, workspace))
+        return HF_E_INVALID;
+    const PageBook b = book_of(c, workspace);
+    cudaStream_t s = (cudaStream_t) stream;
+    const cudaError_t e = launch(false, pages_update_book, dim3(1), dim3(kBookThreads), 0, s, b, release, (int) releases,
+                                 forks, (int) fork_count, grow, result);
+    if (e != cudaSuccess || !grow)
+        return status_of(e);
+    return copy_rows(b, c.sequences, on.current, s);
+}
+
+int hf_cuda_pages_compact(const hf_page_cache* cache, int32_t* live, void* workspace, uint64_t workspace_bytes,
+                          void* stream)
+{
+    hf_page_cache c;
+    if (const int rc = check_cache(cache, &c))
+        return rc;
+    if (!live || !aligned(workspace))
+        return HF_E_INVALID;
+    if (workspace_bytes < book_bytes(c))
+        return HF_E_CAPACITY;
+    const DeviceOf on(c.keys);
+    if (on.status)
+        return on.status;
+    if (!on.holds(c.values, c.table, c.lengths, c.refs, live, workspace))
+        return HF_E_INVALID;
+    const PageBook b = book_of(c, workspace);
+    cudaStream_t s = (cudaStream_t) stream;
+    const cudaError_t e = launch(false, pages_compact_book, dim3(1), dim3(kBookThreads), 0, s, b, live);
+    if (e != cudaSuccess)
+        return HF_E_CUDA;
+    return copy_rows(b, c.pages / 2 + 1, on.current, s);
+}
+
+int hf_cuda_pages_write(const hf_page_cache* cache, int32_t layer, const void* k, const void* v, int64_t k_stride,
+                        int64_t v_stride, int32_t source_rows, const int32_t* offsets, const int32_t* index,
+                        int32_t rows, void* stream)
+{
+    hf_page_cache c;
+    if (const int rc = check_cache(cache, &c))
+        return rc;
+    const int size = size_of(c.dtype);
+    if (layer < 0 || layer >= c.layers || rows < 0 || source_rows < 0 || !offsets || !aligned(k) || !aligned(v)
+        || !row_stride(&k_stride, c.kv_width, size) || !row_stride(&v_stride, c.kv_width, size))
+        return HF_E_INVALID;
+    if (rows == 0 || source_rows == 0)
+        return HF_OK;
+    const DeviceOf on(c.keys);
+    if (on.status)
+        return on.status;
+    if (!on.holds(c.values, c.table, c.lengths, k, v, offsets, index))
+        return HF_E_INVALID;
+    PageWrite w = {};
+    w.keys = (char*) c.keys + layer * c.layer_stride * size;
+    w.values = (char*) c.values + layer * c.layer_stride * size;
+    w.k = (const char*) k;
+    w.v = (const char*) v;
+    w.k_stride = k_stride * size;
+    w.v_stride = v_stride * size;
+    w.row_bytes = c.kv_width * size;
+    w.pages = c.pages;
+    w.sequences = c.sequences;
+    w.table_stride = c.table_stride;
+    w.table = c.table;
+    w.lengths = c.lengths;
+    w.offsets = offsets;
+    w.index = index;
+    w.rows = rows;
+    w.source_rows = source_rows;
+    return status_of(launch(false, pages_write_rows, dim3((unsigned) (rows + 7) / 8), dim3(256), 0, (cudaStream_t) stream, w));
+}
+
+int hf_cuda_attention_packed_workspace(const hf_attention_packed* call, uint64_t* bytes)
+{
+    if (!bytes)
+        return HF_E_INVALID;
+    *bytes = 0;
+    return check_packed_sizes(call);
+}
+
+int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
+{
+    if (const int rc = check_packed_sizes(call))
+        return rc;
+    AttnCall a = {};
+    if (const int rc = check_rows(*call, size_of(call->dtype), call->heads, call->kv_heads, call->head_width, &a))
+        return rc;
+    a.sequences = call->sequences;
+    const DeviceOf on(a.q);
+    if (on.status)
+        return on.status;
+    if (!on.holds(a.k, a.v, a.out, a.offsets))
+        return HF_E_INVALID;
+    return run_rows<false>(call->dtype, a, (cudaStream_t) stream);
+}
+
+int hf_cuda_attention_tree_workspace(const hf_page_cache* cache, const hf_attention_tree* call, uint64_t* bytes)
+{
+    hf_page_cache c;
+    if (!bytes)
+        return HF_E_INVALID;
+    *bytes = 0;
+    return check_tree_sizes(cache, &c, call);
+}
+
+int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* call, void* stream)
+{
+    hf_page_cache c;
+    if (const int rc = check_tree_sizes(cache, &c, call))
+        return rc;
+    AttnCall a = {};
+    const int size = size_of(c.dtype);
+    if (const int rc = check_rows(*call, size, call->heads, call->kv_heads, call->head_width, &a))
+        return rc;
+    if (!aligned(c.keys) || !aligned(c.values) || !c.table || !c.lengths || !call->parents)
+        return HF_E_INVALID;
+    a.sequences = c.sequences;
+    a.parents = call->parents;
+    a.key_pages = (const char*) c.keys + call->layer * c.layer_stride * size;
+    a.value_pages = (const char*) c.values + call->layer * c.layer_stride * size;
+    a.table = c.table;
+    a.lengths = c.lengths;
+    a.pages = c.pages;
+    a.table_stride = c.table_stride;
+    a.max_nodes = call->max_nodes;
+    a.max_length = std::min(call->max_length, c.table_stride * kPagePositions);
+    const DeviceOf on(a.q);
+    if (on.status)
+        return on.status;
+    if (!on.holds(a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
+        return HF_E_INVALID;
+    return run_rows<true>(c.dtype, a, (cudaStream_t) stream);
+}
+}

@@ -1,0 +1,414 @@
+// The steps of a paged K/V cache whose book (table, lengths, reference counts)
+// lives on the device: update (release, fork, grow), compact, write. No
+// counterpart in the reference, whose cache is one contiguous window
+// (Decoder.cpp:199-203).
+//
+// update and compact are two kernels each: one CTA does the bookkeeping on a
+// few thousand integers, leaving a list of page copies in the workspace, and a
+// grid copies the rows of all layers. Which page goes where is a prefix sum
+// over ids, so the result does not depend on the order in which threads run;
+// the only atomics add and subtract integers.
+#pragma once
+
+#include "common.cuh"
+
+namespace hfk
+{
+constexpr int kPageLog = 6; // positions of a page: 64
+constexpr int kPagePositions = 1 << kPageLog;
+constexpr int kBookThreads = 1024;
+
+struct PageCopy
+{
+    int source, target, rows;
+};
+
+// The cache as the kernels see it; layer_bytes and row_bytes are of one pool.
+struct PageBook
+{
+    char* keys;
+    char* values;
+    long long layer_bytes;
+    int row_bytes;
+    int layers, pages, sequences, table_stride;
+    int* table;
+    int* lengths;
+    int* refs;
+    // workspace
+    int* copy_count;
+    PageCopy* copies; // [max(sequences, pages)]
+    int* per_sequence; // [2][sequences]
+    int* free_ids;     // [pages]
+    int* renamed;      // [pages]
+};
+
+__device__ __forceinline__ bool page_there(int id, int pages)
+{
+    return (unsigned) id < (unsigned) pages;
+}
+
+// The table entries that a sequence of `length` positions uses.
+__device__ __forceinline__ int pages_of(long long length, int stride)
+{
+    const long long n = (length + kPagePositions - 1) >> kPageLog;
+    return n < 0 ? 0 : (n > stride ? stride : (int) n);
+}
+
+// Exclusive prefix sum over the CTA, and the CTA's total. All threads call it.
+__device__ __forceinline__ int block_scan(int v, int* total)
+{
+    __shared__ int warps[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+        if (lane >= o)
+            sum += up;
+    }
+    __syncthreads(); // the last call's reads of `warps` are done
+    if (lane == 31)
+        warps[warp] = sum;
+    __syncthreads();
+    const int w = lane < (int) (blockDim.x >> 5) ? warps[lane] : 0;
+    int before = lane < warp ? w : 0, all = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+    {
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+    }
+    *total = all;
+    return before + sum - v;
+}
+
+// One CTA. refs, table and lengths are read through L2 (__ldcg) where another
+// thread of the CTA may have changed them in an earlier phase.
+__global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook b, const int* release, int releases,
+                                                                  const int* forks, int fork_count, const int* grow,
+                                                                  int* result)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kWarps = kBookThreads / 32;
+    pdl_wait();
+    pdl_trigger();
+
+    for (int i = warp; i < releases; i += kWarps)
+    {
+        const int s = release[i];
+        if ((unsigned) s >= (unsigned) b.sequences)
+            continue;
+        int length = 0;
+        if (lane == 0)
+            length = atomicExch(&b.lengths[s], 0); // a second listing finds 0
+        length = __shfl_sync(0xFFFFFFFFu, length, 0);
+        const int held = pages_of(length, b.table_stride);
+        int* row = b.table + (size_t) s * b.table_stride;
+        for (int j = lane; j < held; j += 32)
+        {
+            const int id = row[j];
+            if (page_there(id, b.pages))
+                atomicSub(&b.refs[id], 1);
+            row[j] = -1;
+        }
+    }
+    __syncthreads();
+
+    // Forks: every pair's length is taken before any target is filled.
+    int* fork_length = b.per_sequence;
+    for (int i = warp; i < fork_count; i += kWarps)
+    {
+        const int source = forks[2 * i], target = forks[2 * i + 1];
+        bool ok = (unsigned) source < (unsigned) b.sequences && (unsigned) target < (unsigned) b.sequences
+                  && __ldcg(&b.lengths[target]) <= 0;
+        for (int e = lane; e < i && ok; e += 32)
+            ok = forks[2 * e + 1] != target;
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (lane == 0)
+            fork_length[i] = ok ? __ldcg(&b.lengths[source]) : 0;
+    }
+    __syncthreads();
+    for (int i = warp; i < fork_count; i += kWarps)
+    {
+        const int length = __ldcg(&fork_length[i]);
+        if (length <= 0)
+            continue;
+        const int held = pages_of(length, b.table_stride);
+        const int* from = b.table + (size_t) forks[2 * i] * b.table_stride;
+        int* to = b.table + (size_t) forks[2 * i + 1] * b.table_stride;
+        for (int j = lane; j < held; j += 32)
+        {
+            const int id = __ldcg(&from[j]);
+            to[j] = id;
+            if (page_there(id, b.pages))
+                atomicAdd(&b.refs[id], 1);
+        }
+        if (lane == 0)
+            b.lengths[forks[2 * i + 1]] = length;
+    }
+    __syncthreads();
+
+    // Growth: last[s] is the partly filled page that sequence s would write
+    // into, -1 when there is none; it is copied while more than one sequence
+    // holds it, those before s that have moved off it no longer counted.
+    int* last = b.per_sequence;
+    int* first = b.per_sequence + b.sequences;
+    int wanted = 0, past = 0;
+    if (grow)
+    {
+        for (int s = tid; s < b.sequences; s += kBookThreads)
+        {
+            const int length = max(__ldcg(&b.lengths[s]), 0);
+            int id = -1;
+            if (grow[s] > 0 && (length & (kPagePositions - 1)) && length >> kPageLog < b.table_stride)
+                id = __ldcg(&b.table[(size_t) s * b.table_stride + (length >> kPageLog)]);
+            last[s] = page_there(id, b.pages) && __ldcg(&b.refs[id]) > 1 ? id : -1;
+        }
+        __syncthreads();
+        for (int base = 0; base < b.sequences; base += kBookThreads)
+        {
+            const int s = base + tid;
+            int need = 0, over = 0;
+            if (s < b.sequences && grow[s] > 0)
+            {
+                const int length = max(__ldcg(&b.lengths[s]), 0);
+                const long long grown = (long long) length + grow[s];
+                over = grown > (long long) b.table_stride * kPagePositions;
+                need = over ? 0 : pages_of(grown, b.table_stride) - pages_of(length, b.table_stride);
+                const int id = __ldcg(&last[s]);
+                if (id >= 0)
+                {
+                    int holders = __ldcg(&b.refs[id]);
+                    for (int e = 0; e < s; ++e)
+                        holders -= __ldcg(&last[e]) == id;
+                    need += holders > 1 ? 1 : 0;
+                    if (holders > 1)
+                        need |= 1 << 30; // the copy, kept beside the count
+                }
+            }
+            int total, overs;
+            const int before = block_scan(need & 0x3FFFFFFF, &total);
+            block_scan(over, &overs);
+            if (s < b.sequences)
+                first[s] = (wanted + before) | (need & (1 << 30));
+            wanted = min(wanted + total, 1 << 29); // need <= 2^20: no sum overflows; this many are never there
+            past += overs;
+        }
+    }
+    // The free ids, ascending, as far as they are wanted, and how many there are.
+    int room = 0;
+    for (int base = 0; base < b.pages; base += 4 * kBookThreads)
+    {
+        int free_here[4], n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const int id = base + 4 * tid + k;
+            free_here[k] = id < b.pages && __ldcg(&b.refs[id]) <= 0;
+            n += free_here[k];
+        }
+        int total;
+        int at = room + block_scan(n, &total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (free_here[k])
+            {
+                if (at < wanted)
+                    b.free_ids[at] = base + 4 * tid + k;
+                ++at;
+            }
+        room += total;
+    }
+    __syncthreads();
+    const bool fits = wanted <= room && past == 0;
+    int copied = 0;
+    if (grow && fits)
+        for (int base = 0; base < b.sequences; base += kBookThreads)
+        {
+            const int s = base + tid;
+            const bool grows = s < b.sequences && grow[s] > 0;
+            const int entry = grows ? __ldcg(&first[s]) : 0;
+            const bool copies = entry & (1 << 30);
+            int total;
+            const int slot = copied + block_scan(copies, &total);
+            copied += total;
+            if (!grows)
+                continue;
+            int* row = b.table + (size_t) s * b.table_stride;
+            const int length = max(__ldcg(&b.lengths[s]), 0);
+            const int held = pages_of(length, b.table_stride);
+            const int need = pages_of((long long) length + grow[s], b.table_stride) - held;
+            int at = entry & 0x3FFFFFFF;
+            if (copies)
+            {
+                const int id = __ldcg(&last[s]), fresh = __ldcg(&b.free_ids[at++]);
+                b.copies[slot] = {id, fresh, length & (kPagePositions - 1)};
+                row[held - 1] = fresh;
+                b.refs[fresh] = 1;
+                atomicSub(&b.refs[id], 1);
+            }
+            for (int j = 0; j < need; ++j)
+            {
+                const int fresh = __ldcg(&b.free_ids[at + j]);
+                row[held + j] = fresh;
+                b.refs[fresh] = 1;
+            }
+            b.lengths[s] = length + grow[s];
+        }
+    if (tid == 0)
+    {
+        *b.copy_count = copied;
+        result[0] = fits ? room - wanted : room;
+        result[1] = max(wanted - room, 0);
+        result[2] = past;
+    }
+}
+
+// One CTA: counts the held pages, pairs those above the count with the free
+// ids below it, renames the table's entries and moves the counts.
+__global__ void __launch_bounds__(kBookThreads) pages_compact_book(const PageBook b, int* live_out)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    pdl_trigger();
+    int live = 0;
+    {
+        int mine = 0;
+        for (int id = tid; id < b.pages; id += kBookThreads)
+            mine += b.refs[id] > 0;
+        block_scan(mine, &live);
+    }
+    int leaves = 0, holes = 0;
+    for (int base = 0; base < b.pages; base += kBookThreads)
+    {
+        const int id = base + tid;
+        const bool held = id < b.pages && b.refs[id] > 0;
+        const bool leaves_here = held && id >= live, hole = id < live && !held;
+        int total;
+        const int at = leaves + block_scan(leaves_here, &total);
+        leaves += total;
+        const int hole_at = holes + block_scan(hole, &total);
+        holes += total;
+        if (leaves_here)
+            b.renamed[at] = id; // for now the list of those that leave
+        if (hole)
+            b.free_ids[hole_at] = id;
+    }
+    __syncthreads();
+    for (int i = tid; i < leaves; i += kBookThreads)
+    {
+        const int source = __ldcg(&b.renamed[i]), target = __ldcg(&b.free_ids[i]);
+        b.copies[i] = {source, target, kPagePositions};
+        b.refs[target] = b.refs[source];
+        b.refs[source] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < leaves; i += kBookThreads)
+        b.renamed[b.copies[i].source] = b.copies[i].target;
+    __syncthreads();
+    for (int s = warp; s < b.sequences; s += kBookThreads / 32)
+    {
+        int* row = b.table + (size_t) s * b.table_stride;
+        const int held = pages_of(b.lengths[s], b.table_stride);
+        for (int j = lane; j < held; j += 32)
+        {
+            const int id = row[j];
+            if (page_there(id, b.pages) && id >= live)
+                row[j] = __ldcg(&b.renamed[id]);
+        }
+    }
+    if (tid == 0)
+    {
+        *b.copy_count = leaves;
+        *live_out = live;
+    }
+}
+
+// The rows in use of every listed page, in all layers, keys and values: one
+// unit is a listed page of one layer's pool, taken by the grid's CTAs in turn.
+__global__ void __launch_bounds__(256) pages_copy_rows(const PageBook b)
+{
+    pdl_wait();
+    const int count = *(volatile const int*) b.copy_count;
+    const int units = count * b.layers * 2;
+    const size_t page_bytes = (size_t) kPagePositions * b.row_bytes;
+    for (int u = blockIdx.x; u < units; u += gridDim.x)
+    {
+        const PageCopy c = b.copies[u / (2 * b.layers)];
+        const int layer = u / 2 % b.layers;
+        char* pool = (u & 1 ? b.values : b.keys) + (long long) layer * b.layer_bytes;
+        const uint4* from = reinterpret_cast<const uint4*>(pool + c.source * page_bytes);
+        uint4* to = reinterpret_cast<uint4*>(pool + c.target * page_bytes);
+        const int n = c.rows * (b.row_bytes / 16);
+        for (int i = threadIdx.x; i < n; i += blockDim.x)
+            to[i] = from[i];
+    }
+}
+
+struct PageWrite
+{
+    char* keys; // the layer's
+    char* values;
+    const char* k;
+    const char* v;
+    long long k_stride, v_stride; // bytes
+    int row_bytes, pages, sequences, table_stride;
+    const int* table;
+    const int* lengths;
+    const int* offsets;
+    const int* index;
+    int rows, source_rows;
+};
+
+// offsets[s] as the calls take it: within [0, rows].
+__device__ __forceinline__ int bounded_offset(const int* offsets, int s, int rows)
+{
+    return min(max(offsets[s], 0), rows);
+}
+
+// The sequence whose rows hold r: the last s with offsets[s] <= r, -1 for none.
+__device__ __forceinline__ int sequence_of(const int* offsets, int sequences, int rows, int r)
+{
+    int low = -1, high = sequences; // offsets[low] <= r < offsets[high]
+    while (high - low > 1)
+    {
+        const int mid = (low + high) / 2;
+        if (bounded_offset(offsets, mid, rows) <= r)
+            low = mid;
+        else
+            high = mid;
+    }
+    return low >= 0 && low < sequences && r < bounded_offset(offsets, low + 1, rows) ? low : -1;
+}
+
+// One warp a row.
+__global__ void __launch_bounds__(256) pages_write_rows(const PageWrite w)
+{
+    pdl_wait();
+    pdl_trigger();
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= w.rows)
+        return;
+    const int s = sequence_of(w.offsets, w.sequences, w.rows, r);
+    if (s < 0)
+        return;
+    const long long position = (long long) w.lengths[s] - bounded_offset(w.offsets, s + 1, w.rows) + r;
+    if (position < 0 || position >= (long long) w.table_stride << kPageLog)
+        return;
+    const int id = w.table[(size_t) s * w.table_stride + (position >> kPageLog)];
+    const int source = w.index ? w.index[r] : r;
+    if (!page_there(id, w.pages) || (unsigned) source >= (unsigned) w.source_rows)
+        return;
+    const size_t at = ((size_t) id * kPagePositions + (position & (kPagePositions - 1))) * w.row_bytes;
+    const uint4* k = reinterpret_cast<const uint4*>(w.k + source * w.k_stride);
+    const uint4* v = reinterpret_cast<const uint4*>(w.v + source * w.v_stride);
+    uint4* keys = reinterpret_cast<uint4*>(w.keys + at);
+    uint4* values = reinterpret_cast<uint4*>(w.values + at);
+    for (int i = lane; i < w.row_bytes / 16; i += 32)
+    {
+        keys[i] = k[i];
+        values[i] = v[i];
+    }
+}
+} // namespace hfk

@@ -47,6 +47,11 @@ TRACE_LOGITS_EVENTS = ("logits.staged", "logits.limbs", "logits.done", "logits.l
 KERNEL_QKV, KERNEL_ATTENTION, KERNEL_OUTPUT, KERNEL_GATE_UP, KERNEL_DOWN, KERNEL_LOGITS = range(6)
 KERNEL_NAMES = ("qkv_rope", "attention", "o_proj_residual", "gate_up_geglu", "down_residual", "logits_argmax")
 
+# Element types of the serving operators (hf_cuda.h HF_DTYPE_*), a cache page's positions, the most drafted nodes.
+F32, BF16, F16 = range(3)
+PAGE_ROWS = 64
+TREE_NODES = 64
+
 # Tensor ids (DecoderWeights.h:53-116).
 EMBEDDING, FINAL_NORM, INPUT_NORM, QUERY, KEY, VALUE, OUTPUT, GATE_UP, DOWN, POST_NORM = range(10)
 Q8_TENSORS = (QUERY, KEY, VALUE, OUTPUT, GATE_UP, DOWN)
@@ -192,6 +197,40 @@ class SamplingStruct(ctypes.Structure):
                 ("seed", ctypes.c_uint64)]
 
 
+class PageCacheStruct(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("kv_width", ctypes.c_int32),
+        ("sequences", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+        ("layer_stride", ctypes.c_int64),
+        ("keys", _vp),
+        ("values", _vp),
+        ("table", _vp),
+        ("lengths", _vp),
+        ("refs", _vp),
+    ]
+
+
+_ROW_FIELDS = [(n, _vp) for n in ("q", "k", "v", "out")] + [
+    (n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class PackedStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "heads", "kv_heads", "head_width", "sequences", "rows")] + [
+        ("scale", ctypes.c_float), *_ROW_FIELDS, ("offsets", _vp), ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_uint64)]
+
+
+class TreeStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "head_width", "rows", "max_nodes", "max_length",
+                                              "layer")] + [
+        ("scale", ctypes.c_float), *_ROW_FIELDS, ("offsets", _vp), ("parents", _vp), ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_uint64)]
+
+
 def cuda() -> ctypes.CDLL:
     global _cuda
     if _cuda is None:
@@ -255,6 +294,17 @@ def cuda() -> ctypes.CDLL:
         lib.hf_cuda_argmax_noalloc.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp]
         lib.hf_cuda_time_kernel.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_float),
                                             ctypes.POINTER(ctypes.c_double)]
+        lib.hf_cuda_pages_workspace.argtypes = [ctypes.POINTER(PageCacheStruct), ctypes.POINTER(ctypes.c_uint64)]
+        lib.hf_cuda_pages_update.argtypes = [ctypes.POINTER(PageCacheStruct), _vp, ctypes.c_int32, _vp, ctypes.c_int32,
+                                             _vp, _vp, _vp, ctypes.c_uint64, _vp]
+        lib.hf_cuda_pages_compact.argtypes = [ctypes.POINTER(PageCacheStruct), _vp, _vp, ctypes.c_uint64, _vp]
+        lib.hf_cuda_pages_write.argtypes = [ctypes.POINTER(PageCacheStruct), ctypes.c_int32, _vp, _vp, ctypes.c_int64,
+                                            ctypes.c_int64, ctypes.c_int32, _vp, _vp, ctypes.c_int32, _vp]
+        lib.hf_cuda_attention_packed_workspace.argtypes = [ctypes.POINTER(PackedStruct), ctypes.POINTER(ctypes.c_uint64)]
+        lib.hf_cuda_attention_packed.argtypes = [ctypes.POINTER(PackedStruct), _vp]
+        lib.hf_cuda_attention_tree_workspace.argtypes = [ctypes.POINTER(PageCacheStruct), ctypes.POINTER(TreeStruct),
+                                                         ctypes.POINTER(ctypes.c_uint64)]
+        lib.hf_cuda_attention_tree.argtypes = [ctypes.POINTER(PageCacheStruct), ctypes.POINTER(TreeStruct), _vp]
         _cuda = lib
     return _cuda
 
@@ -645,6 +695,106 @@ class Linear:
 
     def __exit__(self, *exc):
         self.close()
+
+
+# ---- serving operators on device addresses (hf_cuda_pages_*, hf_cuda_attention_*) ----
+def _refused(rc: int, what: str):
+    if rc:
+        raise HFError(rc, f"the engine refused the {what}")
+
+
+class PageCache:
+    """A paged K/V cache in the caller's device memory (hf_page_cache): `keys`, `values`, `table`, `lengths` and `refs` are
+    device addresses. Nothing is kept beyond them; a workspace of `workspace_bytes` serves update and compact."""
+
+    def __init__(self, dtype: int, layers: int, pages: int, kv_width: int, sequences: int, table_stride: int, keys: int,
+                 values: int, table: int, lengths: int, refs: int, layer_stride: int = 0):
+        self.lib = cuda()
+        self.struct = PageCacheStruct(dtype, layers, pages, kv_width, sequences, table_stride, layer_stride, keys, values,
+                                      table, lengths, refs)
+        self.ref = ctypes.byref(self.struct)
+
+    @property
+    def workspace_bytes(self) -> int:
+        size = ctypes.c_uint64(0)
+        _refused(self.lib.hf_cuda_pages_workspace(self.ref, ctypes.byref(size)), "page cache")
+        return size.value
+
+    def update(self, result: int, workspace: int, workspace_bytes: int, release: int = 0, releases: int = 0,
+               forks: int = 0, fork_count: int = 0, grow: int = 0, stream: int | None = None):
+        """Releases, forks, then grows sequences (hf_cuda_pages_update)."""
+        rc = self.lib.hf_cuda_pages_update(self.ref, release, releases, forks, fork_count, grow, result, workspace,
+                                           workspace_bytes, stream)
+        _refused(rc, "page update")
+
+    def compact(self, live: int, workspace: int, workspace_bytes: int, stream: int | None = None):
+        """Moves the held pages to the lowest ids (hf_cuda_pages_compact)."""
+        _refused(self.lib.hf_cuda_pages_compact(self.ref, live, workspace, workspace_bytes, stream), "page compaction")
+
+    def write(self, layer: int, k: int, v: int, offsets: int, rows: int, source_rows: int | None = None, index: int = 0,
+              k_stride: int = 0, v_stride: int = 0, stream: int | None = None):
+        """Writes K/V rows to the sequences' last positions (hf_cuda_pages_write)."""
+        rc = self.lib.hf_cuda_pages_write(self.ref, layer, k, v, k_stride, v_stride,
+                                          rows if source_rows is None else source_rows, offsets, index, rows, stream)
+        _refused(rc, "page write")
+
+
+class PackedAttention:
+    """Causal attention of packed prompts (hf_cuda_attention_packed) for one choice of heads; run() takes device addresses.
+    `scale` defaults to head_width ** -0.5."""
+
+    def __init__(self, dtype: int, heads: int, kv_heads: int, head_width: int, scale: float | None = None):
+        self.lib = cuda()
+        self.call = PackedStruct(dtype, heads, kv_heads, head_width)
+        self.call.scale = head_width ** -0.5 if scale is None else scale
+        self.ref = ctypes.byref(self.call)
+
+    def workspace_bytes(self, sequences: int, rows: int) -> int:
+        size = ctypes.c_uint64(0)
+        self.call.sequences, self.call.rows = sequences, rows
+        _refused(self.lib.hf_cuda_attention_packed_workspace(self.ref, ctypes.byref(size)), "packed attention")
+        return size.value
+
+    def run(self, q: int, k: int, v: int, out: int, offsets: int, sequences: int, rows: int, q_stride: int = 0,
+            k_stride: int = 0, v_stride: int = 0, out_stride: int = 0, workspace: int = 0, workspace_bytes: int = 0,
+            stream: int | None = None):
+        c = self.call
+        c.q, c.k, c.v, c.out, c.offsets, c.sequences, c.rows = q, k, v, out, offsets, sequences, rows
+        c.q_stride, c.k_stride, c.v_stride, c.out_stride = q_stride, k_stride, v_stride, out_stride
+        c.workspace, c.workspace_bytes = workspace, workspace_bytes
+        _refused(self.lib.hf_cuda_attention_packed(self.ref, stream), "packed attention")
+
+
+class TreeAttention:
+    """Attention of drafted trees, or of single tokens, over a layer of a PageCache (hf_cuda_attention_tree) for one choice
+    of heads; run() takes device addresses. `scale` defaults to head_width ** -0.5."""
+
+    def __init__(self, dtype: int, heads: int, kv_heads: int, head_width: int, scale: float | None = None):
+        self.lib = cuda()
+        self.call = TreeStruct(heads, kv_heads, head_width)
+        self.dtype = dtype
+        self.call.scale = head_width ** -0.5 if scale is None else scale
+        self.ref = ctypes.byref(self.call)
+
+    def workspace_bytes(self, sequences: int, rows: int, max_nodes: int, max_length: int) -> int:
+        size, c = ctypes.c_uint64(0), self.call
+        cache = PageCacheStruct(self.dtype, 1, 1, c.kv_heads * c.head_width, sequences, 1)
+        c.rows, c.max_nodes, c.max_length, c.layer = rows, max_nodes, max_length, 0
+        _refused(self.lib.hf_cuda_attention_tree_workspace(ctypes.byref(cache), self.ref, ctypes.byref(size)),
+                 "tree attention")
+        return size.value
+
+    def run(self, cache: PageCache, layer: int, q: int, k: int, v: int, out: int, offsets: int, parents: int, rows: int,
+            max_nodes: int, max_length: int, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, out_stride: int = 0,
+            workspace: int = 0, workspace_bytes: int = 0, stream: int | None = None):
+        c = self.call
+        c.q, c.k, c.v, c.out, c.offsets, c.parents, c.rows = q, k, v, out, offsets, parents, rows
+        c.q_stride, c.k_stride, c.v_stride, c.out_stride = q_stride, k_stride, v_stride, out_stride
+        c.max_nodes, c.max_length, c.layer, c.workspace, c.workspace_bytes = (max_nodes, max_length, layer, workspace,
+                                                                              workspace_bytes)
+        if cache.struct.dtype != self.dtype:
+            raise HFError(HF_E_INVALID, "the cache holds another element type")
+        _refused(self.lib.hf_cuda_attention_tree(cache.ref, self.ref, stream), "tree attention")
 
 
 NCCL_ID_BYTES = 128  # hf_cuda.h HF_NCCL_ID_BYTES

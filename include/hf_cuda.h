@@ -380,6 +380,159 @@ void hf_cuda_linear_destroy(hf_linear* lin);
 int hf_cuda_quantize_q8(const float* values, int64_t first, int64_t count, int64_t element_count,
                         uint8_t* destination, void* stream);
 
+/* ---- serving operators on device pointers: a paged K/V cache and the
+ * attentions around it. No counterpart in the reference, whose one sequence
+ * has one contiguous cache and attends for one prompt at a time
+ * (Decoder.cpp:199-203, 400, Kernels/MultiQueryAttention.h:138-341). They use
+ * no context: every pointer is the caller's DEVICE memory on one device (the
+ * calls switch to it and back), nothing is allocated, and each is asynchronous
+ * on `stream` (a cudaStream_t of that device, null = the legacy default
+ * stream) and can be captured into a CUDA graph. A `workspace` holds nothing
+ * between calls; calls that may overlap on the GPU (other streams, graphs
+ * replayed side by side) need one each. Element type of queries, keys, values,
+ * outputs and pages: HF_DTYPE_*; scores, softmax statistics and sums are fp32
+ * in all of them. Refused before anything is launched: a null pointer, a count
+ * out of range, memory that is not 16-byte aligned or not device memory, a
+ * stride that is no multiple of 16 bytes (HF_E_INVALID); a shape they do not
+ * serve (HF_E_SHAPE); a workspace that is too small (HF_E_CAPACITY). What the
+ * host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
+ * bounded by the kernels: offsets are taken as ascending within [0, rows],
+ * lengths within the bounds given, and a page id outside the pool is a page
+ * that is not there (its positions are not attended, read or written). */
+enum { HF_DTYPE_F32 = 0, HF_DTYPE_BF16 = 1, HF_DTYPE_F16 = 2 };
+
+/* Causal attention of packed prompts: row i of sequence s (rows
+ * [offsets[s], offsets[s + 1]) of q, k, v and out) attends to that sequence's
+ * rows up to i; query head h reads kv head h / (heads / kv_heads). Rows of q and
+ * out are [heads][head_width], of k and v [kv_heads][head_width], `*_stride`
+ * elements apart (0 = packed; views of one fused q|k|v row are fine). Rows
+ * outside every sequence are neither read nor written. head_width is a multiple
+ * of 8 up to 256, heads / kv_heads at most 128. `scale` multiplies the scores.
+ * A value or key row that holds infinities or NaN reaches only the rows that
+ * attend to it. */
+typedef struct hf_attention_packed
+{
+    int32_t dtype;
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t head_width;
+    int32_t sequences;
+    int32_t rows; /* rows that q, k, v and out hold */
+    float scale;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t out_stride;
+    const int32_t* offsets; /* [sequences + 1] */
+    void* workspace;        /* may be null when hf_cuda_attention_packed_workspace gives 0 */
+    uint64_t workspace_bytes;
+} hf_attention_packed;
+/* The workspace bytes of a call with these sizes (pointers are not looked at). */
+int hf_cuda_attention_packed_workspace(const hf_attention_packed* call, uint64_t* bytes);
+int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream);
+
+/* A paged K/V cache: `pages` pages of HF_PAGE_ROWS positions, each position
+ * kv_width (= kv_heads * head_width, a multiple of 8) elements, in every one of
+ * `layers` layers: layer l's page p begins at keys + l * layer_stride + p *
+ * HF_PAGE_ROWS * kv_width (layer_stride in elements, 0 = pages * HF_PAGE_ROWS *
+ * kv_width). Sequence s holds lengths[s] positions, position j in page
+ * table[s * table_stride + j / HF_PAGE_ROWS]; entries past its last page are
+ * -1. refs[p] counts the table entries that name page p: 0 = free. A fresh cache
+ * is a table of -1 and zeros elsewhere. */
+typedef struct hf_page_cache
+{
+    int32_t dtype;
+    int32_t layers;
+    int32_t pages;
+    int32_t kv_width;
+    int32_t sequences;
+    int32_t table_stride;
+    int64_t layer_stride;
+    void* keys;
+    void* values;
+    int32_t* table;   /* [sequences][table_stride] */
+    int32_t* lengths; /* [sequences] */
+    int32_t* refs;    /* [pages] */
+} hf_page_cache;
+/* The workspace bytes of hf_cuda_pages_update and hf_cuda_pages_compact. */
+int hf_cuda_pages_workspace(const hf_page_cache* cache, uint64_t* bytes);
+
+/* A serving step's bookkeeping, in this order:
+ *  release  the `releases` sequences listed (at most `sequences`; one listed
+ *           twice is released once, ids out of range are ignored) give their
+ *           pages back and have length 0;
+ *  fork     of `fork_count` pairs (source, target), each target that is empty and
+ *           that no earlier pair names becomes a copy of its source as the
+ *           releases left it, sharing all of its pages; other pairs are ignored;
+ *  grow     every sequence s grows by grow[s] positions (grow null = none, counts
+ *           below 1 ignored), as if one after another: if its last page is
+ *           partly filled and another sequence still holds it, the sequence
+ *           gets a page of its own with the rows in use copied (every layer, keys
+ *           and values); then the pages that its new positions need. Pages are
+ *           taken in ascending order of the free ids. When the free pages do not
+ *           suffice, or a sequence would pass its table row, nothing grows.
+ * result [3] receives the free pages left, the pages that were missing (0 = it
+ * fitted) and the sequences that would have passed their table row. The new
+ * positions' rows hold what the page held before until they are written. */
+int hf_cuda_pages_update(const hf_page_cache* cache, const int32_t* release, int32_t releases, const int32_t* forks,
+                         int32_t fork_count, const int32_t* grow, int32_t* result, void* workspace,
+                         uint64_t workspace_bytes, void* stream);
+/* Moves the held pages to the lowest ids: with L pages held, those with ids of
+ * L and above go to the free ids below L, both ascending, in every layer, and
+ * table and refs follow. live [1] receives L; pages from L on are free. */
+int hf_cuda_pages_compact(const hf_page_cache* cache, int32_t* live, void* workspace, uint64_t workspace_bytes,
+                          void* stream);
+/* Writes K/V rows of one layer into the pages: rows [offsets[s], offsets[s + 1])
+ * go to the last positions of sequence s (the positions it has just grown by).
+ * Row r comes from row index[r] of k and v ([source_rows][kv_width], `*_stride`
+ * elements apart, 0 = packed), or from row r when index is null; an index out of
+ * range leaves its position as it was. The pages written must not be shared. */
+int hf_cuda_pages_write(const hf_page_cache* cache, int32_t layer, const void* k, const void* v, int64_t k_stride,
+                        int64_t v_stride, int32_t source_rows, const int32_t* offsets, const int32_t* index,
+                        int32_t rows, void* stream);
+
+/* Attention of drafted token trees over a layer of the cache: sequence s drafts
+ * rows [offsets[s], offsets[s + 1]) of q, k, v and out (at most max_nodes <=
+ * HF_TREE_NODES; rows past that are left as they were). parents[r] is the index,
+ * within its sequence, of the node before row r, -1 for one that follows the
+ * cache; it comes before its child (anything else counts as -1). A node attends to
+ * its sequence's cached positions [0, lengths[s]) (at most max_length) and to
+ * the nodes on its path: itself, its parent, and so on. One node with parent -1
+ * is an ordinary decode step, whose own key and value are in k and v. Drafted
+ * rows stay out of the cache: hf_cuda_pages_write puts the accepted ones there.
+ * heads, strides, `scale` and rows as in hf_attention_packed. */
+#define HF_TREE_NODES 64
+typedef struct hf_attention_tree
+{
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t head_width;
+    int32_t rows; /* rows that q, k, v and out hold */
+    int32_t max_nodes;
+    int32_t max_length;
+    int32_t layer;
+    float scale;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t out_stride;
+    const int32_t* offsets; /* [cache->sequences + 1] */
+    const int32_t* parents; /* [rows] */
+    void* workspace;
+    uint64_t workspace_bytes;
+} hf_attention_tree;
+/* The workspace bytes of a call with these sizes over `cache` (pointers are not looked at). */
+int hf_cuda_attention_tree_workspace(const hf_page_cache* cache, const hf_attention_tree* call, uint64_t* bytes);
+int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,565 @@
+"""The serving operators on device pointers (hf_cuda_attention_packed, hf_cuda_attention_tree, hf_cuda_pages_*) against plain
+64-bit implementations (serving_reference.py): types, head layouts, lengths around the page and tile borders, strided
+views, empty sequences, garbage outside the rows in use, captured graphs, and a serving run of all of them together."""
+import math
+
+import pytest
+
+import serving_reference as ref
+from huggingfaceeacp_b200 import native
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+PAGE = native.PAGE_ROWS
+TYPES = ["f32", "bf16", "f16"]
+HEADS = [(8, 1, 256), (8, 2, 128), (4, 4, 64), (6, 2, 96), (7, 1, 80), (3, 3, 8), (10, 2, 40), (2, 2, 200)]
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _offsets(lengths, begin=0):
+    at = [begin]
+    for n in lengths:
+        at.append(at[-1] + n)
+    return at
+
+
+def _normal(g, *shape, dtype):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def _fused(g, rows, heads, kv_heads, width, dtype):
+    """q, k, v as views of one [rows, q | k | v] buffer, and its row stride."""
+    qkv = _normal(g, rows, (heads + 2 * kv_heads) * width, dtype=dtype)
+    parts = qkv.split([heads * width, kv_heads * width, kv_heads * width], 1)
+    return [x.unflatten(1, (-1, width)) for x in parts], qkv.stride(0)
+
+
+def _room(size):
+    return torch.full((max(size, 16),), 255, dtype=torch.uint8, device="cuda")
+
+
+def _run_packed(code, q, k, v, out, lengths, stride, scale=None, begin=0, stream=None):
+    heads, width = q.shape[1:]
+    plan = native.PackedAttention(code, heads, k.shape[1], width, scale=scale)
+    offsets = _ints(_offsets(lengths, begin))
+    room = _room(plan.workspace_bytes(len(lengths), len(q)))
+    plan.run(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), len(lengths), len(q),
+             q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(), workspace_bytes=room.numel(),
+             stream=_stream() if stream is None else stream)
+    return offsets, room
+
+
+# ---- packed prompts ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+def test_packed_prompts_of_every_layout(kind, heads):
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    lengths = [1, 0, 130, 17, 64, 3]
+    g = torch.Generator("cuda").manual_seed(1)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, max(lengths))
+
+
+@pytest.mark.parametrize("lengths", [[1], [2], [15], [16], [63], [65], [127], [128], [129], [191, 193], [257], [500, 1, 300]],
+                         ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(8, 1, 256), (8, 2, 128), (2, 2, 64)], ids=str)
+def test_packed_prompts_around_the_tile_borders(kind, lengths, heads):
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    g = torch.Generator("cuda").manual_seed(2)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride, scale=0.11)
+    expected, size = ref.packed(q, k, v, lengths, 0.11)
+    ref.close(out, expected, size, q, k, 0.11, max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_packed_prompts_of_many_sequences(kind):
+    code, dtype = ref.TYPES[kind]
+    lengths = [(i * 37) % 23 for i in range(150)]
+    g = torch.Generator("cuda").manual_seed(3)
+    (q, k, v), stride = _fused(g, sum(lengths), 4, 2, 64, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, 64 ** -0.5)
+    ref.close(out, expected, size, q, k, 64 ** -0.5, max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(8, 1, 256), (4, 2, 128), (5, 5, 72)], ids=str)
+def test_packed_rows_outside_every_sequence_are_left_alone(kind, heads):
+    """Rows before the first and behind the last sequence hold NaN and infinities: neither read nor written."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    lengths, before, behind = [70, 9], 5, 77
+    g = torch.Generator("cuda").manual_seed(4)
+    (q, k, v), stride = _fused(g, before + sum(lengths) + behind, h, kv, d, dtype)
+    for x in (q, k, v):
+        x[:before] = math.inf
+        x[before + sum(lengths):] = math.nan
+    out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride, begin=before)
+    used = slice(before, before + sum(lengths))
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5, begin=before)
+    ref.close(out[used], expected[used], size[used], q[used], k[used], d ** -0.5, max(lengths))
+    assert bool((out[:before] == 7.0).all()) and bool((out[before + sum(lengths):] == 7.0).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_packed_garbage_reaches_only_the_rows_that_attend_to_it(kind, value):
+    code, dtype = ref.TYPES[kind]
+    lengths, h, kv, d, bad = [90, 40], 8, 2, 128, 60
+    g = torch.Generator("cuda").manual_seed(5)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    clean = [x.clone() for x in (q, k, v)]
+    v[bad, :, 3] = value
+    k[bad, 0, 1] = math.nan  # kv head 0: the whole row of its query heads
+    out = torch.empty(q.shape, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(*clean, lengths, d ** -0.5)
+    fine = torch.ones(sum(lengths), h, d, dtype=torch.bool, device="cuda")
+    fine[bad:lengths[0], :, 3] = False
+    fine[bad:lengths[0], : h // kv] = False
+    where = fine.nonzero(as_tuple=True)
+    tol = ref.tolerance(expected, size, *clean[:2], d ** -0.5, max(lengths), dtype)
+    assert bool(((out.double() - expected).abs() <= tol)[where].all())
+    assert bool(torch.isnan(out[bad:lengths[0], : h // kv]).all())
+    got = out[bad:lengths[0], h // kv:, 3].float()
+    assert bool((torch.isnan(got) if math.isnan(value) else got == value).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_packed_scores_far_apart(kind):
+    """Large scores: the running maximum rises from tile to tile, and weights underflow to zero."""
+    code, dtype = ref.TYPES[kind]
+    lengths, d = [400], 64
+    g = torch.Generator("cuda").manual_seed(6)
+    (q, k, v), stride = _fused(g, 400, 4, 2, d, dtype)
+    k *= (torch.arange(400, device="cuda") / 40.0).to(dtype)[:, None, None]
+    q *= 2
+    out = torch.empty(q.shape, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, 400)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 3e4, 1e-6])
+def test_packed_fp32_keeps_its_digits_at_any_magnitude(scale):
+    """Rows of very different size, in one tile too: the relative error stays that of fp32."""
+    lengths, d = [300], 256
+    g = torch.Generator("cuda").manual_seed(7)
+    (q, k, v), stride = _fused(g, 300, 8, 1, d, torch.float32)
+    v *= scale
+    k *= 10.0 ** (torch.arange(300, device="cuda") % 5 - 3)[:, None, None]
+    out = torch.empty(q.shape, device="cuda")
+    _run_packed(native.F32, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, 300)
+
+
+# ---- trees ---------------------------------------------------------------------------------------------------------
+
+
+class Cache:
+    def __init__(self, kind, layers, pages, kv_heads, width, lengths, stride, seed, table=None):
+        code, dtype = ref.TYPES[kind]
+        g = torch.Generator("cuda").manual_seed(seed)
+        self.keys = _normal(g, layers, pages, PAGE, kv_heads * width, dtype=dtype)
+        self.values = _normal(g, layers, pages, PAGE, kv_heads * width, dtype=dtype)
+        order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        if table is None:
+            table, at = [], 0
+            for n in lengths:
+                held = -(-n // PAGE)
+                table.append(order[at : at + held] + [-1] * (stride - held))
+                at += held
+        refs = [sum(row[: -(-max(n, 0) // PAGE)].count(p) for row, n in zip(table, lengths)) for p in range(pages)]
+        self.shape = (pages, PAGE, kv_heads, width)
+        self.table, self.lengths, self.refs = _ints(table), _ints(lengths), _ints(refs)
+        self.native = native.PageCache(code, layers, pages, kv_heads * width, len(lengths), stride, self.keys.data_ptr(),
+                                       self.values.data_ptr(), self.table.data_ptr(), self.lengths.data_ptr(),
+                                       self.refs.data_ptr())
+        self.room = _room(self.native.workspace_bytes)
+        self.result = _ints([-9, -9, -9])
+        self.kind, self.code, self.dtype = kind, code, dtype
+
+    def kw(self):
+        return {"workspace": self.room.data_ptr(), "workspace_bytes": self.room.numel(), "stream": _stream()}
+
+    def book(self):
+        return ref.Book(self.keys, self.values, self.table.tolist(), self.lengths.tolist(), self.refs.tolist())
+
+    def same(self, book):
+        assert self.table.tolist() == book.table
+        assert self.lengths.tolist() == book.lengths
+        assert self.refs.tolist() == book.refs
+        for got, want in ((self.keys, book.keys), (self.values, book.values)):
+            assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
+def _tree(cache, layer, heads, kv_heads, width, nodes, parents, seed, max_length, max_nodes=None, poison=False):
+    g = torch.Generator("cuda").manual_seed(seed)
+    (q, k, v), stride = _fused(g, sum(nodes) + 2, heads, kv_heads, width, cache.dtype)
+    if poison:
+        for x in (q, k, v):
+            x[sum(nodes):] = math.nan
+    out = torch.full(q.shape, 7.0, dtype=cache.dtype, device="cuda")
+    plan = native.TreeAttention(cache.code, heads, kv_heads, width)
+    offsets, up = _ints(_offsets(nodes)), _ints([p for row in parents for p in row] + [-1, -1])
+    most = max_nodes or max(1, max(nodes))
+    room = _room(plan.workspace_bytes(len(nodes), len(q), most, max_length))
+    plan.run(cache.native, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(),
+             len(q), most, max_length, q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(),
+             workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q, k, v, nodes, parents, cache.keys[layer].view(cache.shape), cache.values[layer].view(cache.shape),
+                              cache.table.tolist(), cache.lengths.tolist(), width ** -0.5)
+    n = sum(nodes)
+    if n:
+        keys = max(cache.lengths.tolist()) + 64
+        everything = torch.cat([k[:n], cache.keys[layer].view(-1, kv_heads, width)])
+        ref.close(out[:n], expected[:n], size[:n], q[:n], everything, width ** -0.5, keys)
+    assert bool((out[n:] == 7.0).all())
+
+
+def _branching(n, seed):
+    """Parents of a random tree of n nodes, several of them following the cache."""
+    g = torch.Generator().manual_seed(seed)
+    return [-1 if i == 0 else int(torch.randint(-1, i, (1,), generator=g)) for i in range(n)]
+
+
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+def test_trees_of_every_layout(kind, heads):
+    h, kv, d = heads
+    lengths, nodes = [0, 1, 63, 64, 65, 200, 5], [3, 1, 0, 12, 7, 1, 20]
+    cache = Cache(kind, 2, 20, kv, d, lengths, 5, 11)
+    parents = [_branching(n, i) for i, n in enumerate(nodes)]
+    _tree(cache, 1, h, kv, d, nodes, parents, 12, 200)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(8, 1, 256), (8, 2, 128), (16, 8, 64)], ids=str)
+@pytest.mark.parametrize("lengths", [[0, 0], [1, 64], [700, 130], [4097, 3]], ids=str)
+@pytest.mark.parametrize("nodes", [[1, 1], [64, 33], [0, 16]], ids=str)
+def test_trees_of_one_to_64_nodes(kind, heads, lengths, nodes):
+    h, kv, d = heads
+    cache = Cache(kind, 1, 80, kv, d, lengths, 66, 13)
+    _tree(cache, 0, h, kv, d, nodes, [_branching(n, 20 + i) for i, n in enumerate(nodes)], 14, max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_decode_steps_of_many_sequences(kind):
+    lengths = [(i * 97) % 300 for i in range(40)]
+    cache = Cache(kind, 1, 260, 2, 128, lengths, 6, 15)
+    _tree(cache, 0, 8, 2, 128, [1] * 40, [[-1]] * 40, 16, 300)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_tree_garbage_in_the_cache_is_not_read(kind):
+    """Page rows past a length, free pages, and drafted rows behind the last sequence hold NaN."""
+    lengths = [70, 1, 129]
+    cache = Cache(kind, 1, 12, 2, 64, lengths, 4, 17)
+    for pool in (cache.keys, cache.values):
+        held = torch.zeros(12, PAGE, dtype=torch.bool)
+        for row, n in zip(cache.table.tolist(), lengths):
+            for j in range(n):
+                held[row[j // PAGE], j % PAGE] = True
+        pool[0][~held.cuda()] = math.nan
+    _tree(cache, 0, 8, 2, 64, [5, 1, 9], [_branching(n, n) for n in (5, 1, 9)], 18, 129, poison=True)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_tree_siblings_do_not_reach_each_other(kind):
+    """A sibling's value of NaN or infinity stays with its own descendants."""
+    code, dtype = ref.TYPES[kind]
+    lengths, parents, h, kv, d = [100], [-1, 0, 0, 1, 2, 2], 4, 1, 128
+    cache = Cache(kind, 1, 3, kv, d, lengths, 2, 19)
+    g = torch.Generator("cuda").manual_seed(20)
+    q, k, v = (_normal(g, 6, n, d, dtype=dtype) for n in (h, kv, kv))
+    v[1], v[2] = math.inf, math.nan
+    out = torch.empty_like(q)
+    plan = native.TreeAttention(code, h, kv, d)
+    offsets, up = _ints([0, 6]), _ints(parents)
+    room = _room(plan.workspace_bytes(1, 6, 6, 100))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(), 6, 6,
+             100, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q, k, v, [6], [parents], cache.keys[0].view(cache.shape), cache.values[0].view(cache.shape),
+                              cache.table.tolist(), lengths, d ** -0.5)
+    ref.close(out[:1], expected[:1], size[:1], q, k, d ** -0.5, 200)
+    assert bool((out[[1, 3]] == math.inf).all()) and bool(torch.isnan(out[[2, 4, 5]]).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_tree_pages_that_are_not_there_and_bounds(kind):
+    """Page ids outside the pool are not attended; lengths and node counts are bounded by the call's."""
+    lengths = [200, 130]
+    cache = Cache(kind, 1, 6, 1, 64, lengths, 4, 21, table=[[2, -1, 5, 77777], [-5, 0, 6, -1]])
+    _tree(cache, 0, 4, 1, 64, [3, 4], [[-1, 0, 1], [-1, -1, 1, 5]], 22, 200)
+    # Both sequences have more positions than max_length, the second more nodes than max_nodes.
+    g = torch.Generator("cuda").manual_seed(23)
+    (q, k, v), stride = _fused(g, 7, 4, 1, 64, cache.dtype)
+    out = torch.full(q.shape, 7.0, dtype=cache.dtype, device="cuda")
+    plan, offsets, up = native.TreeAttention(cache.code, 4, 1, 64), _ints([0, 2, 7]), _ints([-1, 0, -1, 0, 1, 2, 3])
+    room = _room(plan.workspace_bytes(2, 7, 3, 100))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(), 7, 3,
+             100, q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(), workspace_bytes=room.numel(),
+             stream=_stream())
+    expected, size = ref.tree(q[:5], k[:5], v[:5], [2, 3], [[-1, 0], [-1, 0, 1]], cache.keys[0].view(cache.shape),
+                              cache.values[0].view(cache.shape), cache.table.tolist(), [100, 100], 64 ** -0.5)
+    ref.close(out[:5], expected, size, q[:5], cache.keys[0].view(-1, 1, 64), 64 ** -0.5, 200)
+    assert bool((out[5:] == 7.0).all())
+
+
+# ---- the cache's steps ---------------------------------------------------------------------------------------------
+
+
+def _update(cache, release=(), forks=(), grow=None):
+    book = cache.book()
+    expected = book.update(release, forks, grow)
+    lists = [_ints(list(release)), _ints([x for pair in forks for x in pair]), None if grow is None else _ints(grow)]
+    cache.native.update(cache.result.data_ptr(), release=lists[0].data_ptr() if release else 0, releases=len(release),
+                        forks=lists[1].data_ptr() if forks else 0, fork_count=len(forks),
+                        grow=0 if grow is None else lists[2].data_ptr(), **cache.kw())
+    assert cache.result.tolist() == expected
+    cache.same(book)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_update_releases_forks_and_grows(kind):
+    cache = Cache(kind, 3, 30, 2, 40, [100, 64, 0, 5, 130, 0, 0, 63], 4, 31)
+    _update(cache, grow=[1, 1, 1, 1, 1, 0, 0, 1])
+    _update(cache, release=[4, 4, -1, 99, 3], forks=[(0, 5), (7, 6), (0, 5), (1, 4), (0, 1), (2, 2), (0, -1), (88, 3)])
+    _update(cache, grow=[1, 3, 0, 70, 0, 2, 65, 1])
+    _update(cache, release=[0], forks=[(5, 0), (5, 3), (6, 2)], grow=[1, 0, 2, 3, -4, 1, 1, 0])
+    _update(cache)
+
+
+def test_update_copies_a_shared_page_for_all_but_the_last_that_grows():
+    cache = Cache("f32", 2, 12, 1, 32, [70, 0, 0, 0], 3, 32)
+    _update(cache, forks=[(0, 1), (0, 2), (0, 3)], grow=[1, 1, 1, 1])
+    assert sorted(cache.refs.tolist(), reverse=True)[:6] == [4, 1, 1, 1, 1, 0]
+
+
+def test_update_that_does_not_fit_grows_nothing():
+    cache = Cache("bf16", 1, 6, 1, 64, [64, 128, 10], 3, 33)
+    _update(cache, grow=[1, 60, 200])   # four pages wanted, two free
+    _update(cache, grow=[1, 65, 1])     # the second would pass its row of three pages
+    _update(cache, release=[1], grow=[1, 64, 100])
+
+
+def test_update_of_many_sequences_and_pages():
+    n = 1500
+    lengths = [(i * 53) % 200 if i % 3 else 0 for i in range(n)]
+    cache = Cache("f16", 1, 9000, 1, 8, lengths, 5, 34)
+    _update(cache, release=list(range(0, n, 7)), forks=[(i + 1, i) for i in range(0, n - 1, 3)],
+            grow=[i % 3 for i in range(n)])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_compact_moves_held_pages_down(kind):
+    cache = Cache(kind, 3, 40, 2, 40, [300, 64, 0, 5, 130, 129, 0], 6, 35)
+    _update(cache, release=[0], forks=[(4, 6), (5, 2)])
+    for _ in range(2):
+        book = cache.book()
+        live = book.compact()
+        cache.native.compact(cache.result.data_ptr(), **cache.kw())
+        assert cache.result.tolist()[0] == live
+        cache.same(book)
+
+
+@pytest.mark.parametrize("pages,lengths", [(5, [0, 0]), (4, [256, 0]), (3000, [64 * 40 + i for i in range(20)])])
+def test_compact_of_empty_full_and_large_pools(pages, lengths):
+    cache = Cache("bf16", 2, pages, 1, 8, lengths, 45, 36)
+    book = cache.book()
+    live = book.compact()
+    cache.native.compact(cache.result.data_ptr(), **cache.kw())
+    assert cache.result.tolist()[0] == live
+    cache.same(book)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("picked", [False, True])
+def test_write_puts_rows_at_the_last_positions(kind, picked):
+    lengths, counts = [100, 64, 3, 0, 130], [70, 64, 5, 0, 1]
+    cache = Cache(kind, 3, 12, 2, 24, lengths, 4, 37)
+    offsets = _offsets(counts)
+    rows = offsets[-1]
+    g = torch.Generator("cuda").manual_seed(38)
+    kv = _normal(g, rows + 9, 2 * 48, dtype=cache.dtype)
+    k, v = kv.split(48, 1)
+    index = [(i * 7) % (rows + 9) for i in range(rows)]
+    index[3], index[4] = -1, rows + 9
+    book = cache.book()
+    book.write(1, k, v, offsets, index if picked else None)
+    at, which = _ints(offsets), _ints(index)
+    cache.native.write(1, k.data_ptr(), v.data_ptr(), at.data_ptr(), rows, source_rows=len(kv),
+                       index=which.data_ptr() if picked else 0, k_stride=kv.stride(0), v_stride=kv.stride(0), stream=_stream())
+    cache.same(book)
+
+
+def test_layers_further_apart_than_their_pages():
+    """layer_stride: the layers' pools are slices of a larger buffer."""
+    cache = Cache("f32", 2, 8, 1, 16, [70, 0], 3, 39)
+    wide = torch.randn(2, 2, 8, PAGE, 16, device="cuda")  # [layer][keys, values]
+    cache.keys, cache.values = wide[:, 0], wide[:, 1]
+    cache.native.struct.keys, cache.native.struct.values = cache.keys.data_ptr(), cache.values.data_ptr()
+    cache.native.struct.layer_stride = wide.stride(0)
+    book = cache.book()
+    assert book.update(forks=[(0, 1)], grow=[3, 3]) == [5, 0, 0]
+    forks, grow = _ints([0, 1]), _ints([3, 3])
+    cache.native.update(cache.result.data_ptr(), forks=forks.data_ptr(), fork_count=1, grow=grow.data_ptr(), **cache.kw())
+    assert cache.result.tolist() == [5, 0, 0]
+    assert torch.equal(cache.keys, book.keys) and torch.equal(cache.values, book.values)
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_a_serving_run_of_all_of_them(kind):
+    """Prompts enter packed, a beam forks, drafted trees are read and their accepted rows written, sequences leave, the pool is
+    compacted: at each step the tree attention equals attention over the tokens kept on the side."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, layers = 8, 2, 64, 2
+    lengths = [90, 30, 64]
+    cache = Cache(kind, layers, 24, kv, d, [0] * 5, 5, 41)
+    g = torch.Generator("cuda").manual_seed(42)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.empty(q.shape, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, 90)
+    _update(cache, grow=lengths + [0, 0])
+    offsets = _ints(_offsets(lengths + [0, 0]))
+    cache.native.write(1, k.data_ptr(), v.data_ptr(), offsets.data_ptr(), len(q), k_stride=stride, v_stride=stride,
+                       stream=_stream())
+    at = _offsets(lengths)
+    kept = [(k[a:b].clone(), v[a:b].clone()) for a, b in zip(at, at[1:])] + [None, None]
+    _update(cache, forks=[(0, 3), (1, 4)])
+    kept[3], kept[4] = kept[0], kept[1]
+    for step in range(4):
+        live = [s for s in range(5) if kept[s] is not None]
+        nodes = [5 + s if s in live else 0 for s in range(5)]
+        parents = [_branching(n, 50 + step * 5 + s) for s, n in enumerate(nodes)]
+        (q, k, v), stride = _fused(g, sum(nodes), h, kv, d, dtype)
+        out = torch.empty(q.shape, dtype=dtype, device="cuda")
+        plan = native.TreeAttention(code, h, kv, d)
+        room = _room(plan.workspace_bytes(5, len(q), 9, 200))
+        starts, up = _offsets(nodes), _ints([p for row in parents for p in row])
+        offsets = _ints(starts)
+        plan.run(cache.native, 1, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(),
+                 len(q), 9, 200, q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(),
+                 workspace_bytes=room.numel(), stream=_stream())
+        chosen = []
+        for s in live:
+            rows = slice(starts[s], starts[s + 1])
+            n, length = nodes[s], len(kept[s][0])
+            keys, values = (torch.cat([kept[s][i], x[rows]]) for i, x in enumerate((k, v)))
+            seen = torch.zeros(n, length + n, dtype=torch.bool, device="cuda")
+            seen[:, :length] = True
+            for i in range(n):
+                seen[i, [length + j for j in ref.path(parents[s], i)]] = True
+            expected, size = ref.attend(q[rows], keys, values, seen, d ** -0.5)
+            ref.close(out[rows], expected, size, q[rows], keys, d ** -0.5, length + n)
+            accepted = sorted(ref.path(parents[s], n - 1))
+            chosen.append((s, [starts[s] + i for i in accepted]))
+        grow = [0] * 5
+        for s, rows in chosen:
+            grow[s] = len(rows)
+            kept[s] = tuple(torch.cat([x, y[rows]]) for x, y in zip(kept[s], (k, v)))
+        _update(cache, grow=grow)
+        offsets, index = _ints(_offsets(grow)), _ints([r for _, rows in chosen for r in rows])
+        cache.native.write(1, k.data_ptr(), v.data_ptr(), offsets.data_ptr(), index.numel(), source_rows=len(q),
+                           index=index.data_ptr(), k_stride=stride, v_stride=stride, stream=_stream())
+        if step == 1:
+            _update(cache, release=[0, 2])
+            kept[0] = kept[2] = None
+            book = cache.book()
+            live_pages = book.compact()
+            cache.native.compact(cache.result.data_ptr(), **cache.kw())
+            assert cache.result.tolist()[0] == live_pages
+            cache.same(book)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_captured_calls_replay_on_new_inputs(kind):
+    """Each call captured into a graph on a side stream; the replay reads what the buffers hold then."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, lengths = 8, 2, 64, [100, 29]
+    cache = Cache(kind, 1, 12, kv, d, [0, 0], 5, 43)
+    g = torch.Generator("cuda").manual_seed(44)
+    (q, k, v), stride = _fused(g, 129, h, kv, d, dtype)
+    out, tree_out = torch.empty(q.shape, dtype=dtype, device="cuda"), torch.empty(2, h, d, dtype=dtype, device="cuda")
+    plan, step = native.PackedAttention(code, h, kv, d), native.TreeAttention(code, h, kv, d)
+    room = _room(plan.workspace_bytes(2, 129) + step.workspace_bytes(2, 2, 1, 200))
+    offsets, two, up, grow = _ints([0, 100, 129]), _ints([0, 1, 2]), _ints([-1, -1]), _ints(lengths)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        s = _stream()
+        at = {"workspace": room.data_ptr(), "workspace_bytes": room.numel(), "stream": s}
+        plan.run(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), 2, 129, q_stride=stride,
+                 k_stride=stride, v_stride=stride, **at)
+        cache.native.update(cache.result.data_ptr(), grow=grow.data_ptr(), **cache.kw())
+        cache.native.write(0, k.data_ptr(), v.data_ptr(), offsets.data_ptr(), 129, k_stride=stride, v_stride=stride, stream=s)
+        step.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), tree_out.data_ptr(), two.data_ptr(), up.data_ptr(),
+                 2, 1, 200, q_stride=stride, k_stride=stride, v_stride=stride, **at)
+        cache.native.compact(cache.result.data_ptr(), **cache.kw())
+    for seed in (1, 2):
+        fresh = _normal(torch.Generator("cuda").manual_seed(seed), 129, stride, dtype=dtype)
+        q._base.copy_(fresh) if q._base is not None else None
+        cache.table.fill_(-1), cache.lengths.zero_(), cache.refs.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+        ref.close(out, expected, size, q, k, d ** -0.5, 100)
+        expected, size = ref.tree(q[:2], k[:2], v[:2], [1, 1], [[-1], [-1]], cache.keys[0].view(cache.shape),
+                                  cache.values[0].view(cache.shape), cache.table.tolist(), lengths, d ** -0.5)
+        ref.close(tree_out, expected, size, q[:2], k, d ** -0.5, 200)
+        assert cache.lengths.tolist() == lengths
+
+
+def test_two_calls_side_by_side():
+    """The same operators on two streams at once, each with its own workspace."""
+    h, kv, d, lengths = 8, 1, 256, [200, 333]
+    runs = []
+    for i in range(2):
+        g = torch.Generator("cuda").manual_seed(60 + i)
+        (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, torch.float32)
+        runs.append((q, k, v, stride, torch.empty(q.shape, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    kept = [_run_packed(native.F32, q, k, v, out, lengths, stride, stream=s.cuda_stream)
+            for q, k, v, stride, out, s in runs for _ in range(3)]
+    torch.cuda.synchronize()
+    assert len(kept) == 6
+    for q, k, v, _, out, _ in runs:
+        expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+        ref.close(out, expected, size, q, k, d ** -0.5, 333)
+
+
+def test_host_memory_is_refused():
+    q = torch.zeros(64, 8, 64)
+    on = torch.zeros(64, 8, 64, device="cuda")
+    plan, offsets = native.PackedAttention(native.F32, 8, 8, 64), _ints([0, 64])
+    for args in ((q, on, on, on), (on, q, on, on), (on, on, on, q)):
+        with pytest.raises(native.HFError) as e:
+            plan.run(*(x.data_ptr() for x in args), offsets.data_ptr(), 1, 64, stream=_stream())
+        assert e.value.code == native.HF_E_INVALID
