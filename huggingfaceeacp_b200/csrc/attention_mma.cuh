@@ -1,0 +1,649 @@
+// Attention of packed prompts and drafted trees in bf16 and fp16 on the
+// 5th-generation tensor cores: scores S = Q K^T and rows O = P V as
+// tcgen05.mma with fp32 accumulators in TMEM, one pass over the keys with the
+// running maximum and sum of a softmax.
+//
+// Work. A query tile is 128 rows: `tile_tokens` consecutive tokens x the heads
+// that share one kv head (row = token * group + head), so short prompts and
+// single tokens fill it as far as they can and a causal tile's ragged edge is
+// a few tokens wide. A CTA takes NQ query tiles of one kv head, over the same
+// keys, in tiles of 64 (a page).
+//
+// Roles (one warp each, and one warpgroup a query tile):
+//  warp 0   copies: query tiles once, then key and value tiles through a ring,
+//           in the order the MMAs use them (tensor maps; a page is one box);
+//  warp 1   MMAs: S of the next tile is issued before O of this one, so the
+//           tensor core has work while the softmax runs. S has two buffers a
+//           query tile;
+//  warpgroups 1 ..  softmax, a thread a row (its TMEM lane): the tile's scores
+//           to registers, maximum, weights, the weights in T back over the
+//           scores (P, the A operand of O += P V), at the end the row itself.
+// The maximum that the weights are taken against follows the true one lazily:
+// only when it would rise by more than 8 (weights up to 2^8) is O scaled in
+// TMEM, which after the first tiles is rare. Weights are rounded to T for the
+// tensor core (half a step relative to each), their sum is kept in fp32
+// unrounded.
+//
+// Value rows past a sequence's last key are set to zero in shared memory before
+// the MMA (their weights are 0, but 0 x NaN is not). Inside a sequence a
+// masked value that is not finite makes the tile's sums NaN for rows that do not
+// attend to it: every row that comes out not finite is taken again by
+// attention_row, which reads only what the row attends to.
+//
+// A tree's keys may be cut into chunks over several CTAs (`chunk_tiles` tiles
+// each): each leaves its rows' maximum, sum and unnormalised O in the
+// workspace, and attention_join puts them together.
+#pragma once
+
+#include "attention_rows.cuh"
+#include "tcgen05.cuh"
+
+namespace hfk
+{
+constexpr int kKeyTile = 64;
+static_assert(kKeyTile == kPagePositions, "a key tile is a page");
+
+// Set when a bounded wait ran out (hf_cuda_operators_sync reports it).
+__device__ unsigned g_operator_error;
+
+struct MmaCall
+{
+    AttnCall a;
+    int tile_tokens;  // tokens of a query tile: 128 / group
+    int row_tiles;    // a tree's CTAs along its nodes
+    int chunk_tiles;  // key tiles of a chunk (a tree's)
+    int chunks;       // most chunks of a sequence; 1: the rows are finished here
+    float* part_o;    // [chunks][rows][heads][width]
+    float2* part_ml;  // [chunks][rows][heads]
+};
+
+template <int D, int NQ>
+struct MmaShape
+{
+    static constexpr int kBlocks = D / 64;                 // 64-channel blocks of a row
+    static constexpr int kQueryBytes = NQ * 128 * D * 2;
+    static constexpr int kStageBytes = kKeyTile * D * 2;   // one K or V tile
+    static constexpr int kBox = kKeyTile * 128;            // one block of it
+    static constexpr int kBuffers = D == 256 ? 4 : 2;      // of scores, a query tile
+    static constexpr int kScoreColumns = NQ * kBuffers * kKeyTile;
+    static constexpr int kTmem = kScoreColumns + NQ * D <= 256 ? 256 : 512;
+    static constexpr int kCtas = kTmem == 256 ? 2 : 1;     // a SM
+    static constexpr int kHead = 1024;                     // barriers and the tile's place
+    static constexpr int kBudget = kCtas == 2 ? 113 * 1024 : 227 * 1024;
+    static constexpr int kStagesFit = (kBudget - kHead - kQueryBytes) / kStageBytes;
+    static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
+    static constexpr int kSmem = kHead + kQueryBytes + kStages * kStageBytes;
+    static constexpr int kThreads = 128 + 128 * NQ;
+    static_assert(kScoreColumns + NQ * D <= kTmem && kStages >= 4, "what an SM holds");
+};
+
+// The CTA's place, found once by warp 0.
+struct MmaPlace
+{
+    int sequence; // -1: nothing to do
+    int begin, length; // its first row, its rows (a tree's nodes)
+    int token0, kv_head, chunk;
+    int cached, tiles_cached; // a tree's
+    int first_tile, tiles;    // the CTA's key tiles
+    bool whole;               // the only chunk: finish the rows
+};
+
+struct MmaHead
+{
+    uint64_t full[12], empty[12], query, scores[2][4], weights[2][4], done[2][4];
+    uint32_t tmem;
+    MmaPlace place;
+    int parents[kTreeNodes];
+};
+
+// Bounded waits, of a warp together and of one thread.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity)
+{
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)))
+        return true;
+    flag_error(&g_operator_error, kErrWaitTimeout);
+    return false;
+}
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, unsigned parity)
+{
+    if (mbar_wait(bar, parity))
+        return true;
+    flag_error(&g_operator_error, kErrWaitTimeout);
+    return false;
+}
+
+// The sequences' tiles of `step` tokens in descending order of their place (the
+// longest rows of keys first), equal places in the sequences' order: unit r of
+// them, by a whole warp.
+__device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequence, int& tile)
+{
+    const int lane = threadIdx.x & 31;
+    auto tiles_of = [&](int s) {
+        if (s >= a.sequences)
+            return 0;
+        const int n = bounded_offset(a.offsets, s + 1, a.rows) - bounded_offset(a.offsets, s, a.rows);
+        return n > 0 ? (n + step - 1) / step : 0;
+    };
+    auto from = [&](int t) { // tiles whose place is t or above
+        int sum = 0;
+        for (int s = lane; s < a.sequences; s += 32)
+            sum += max(tiles_of(s) - t, 0);
+        return __reduce_add_sync(0xFFFFFFFFu, sum);
+    };
+    int low = 0, high = (a.rows + step - 1) / step; // from(low) > r >= from(high)
+    sequence = -1;
+    if (from(0) <= r)
+        return;
+    while (high - low > 1)
+    {
+        const int mid = (low + high) / 2;
+        if (from(mid) > r)
+            low = mid;
+        else
+            high = mid;
+    }
+    tile = low;
+    int skip = r - from(low + 1);
+    for (int base = 0; base < a.sequences; base += 32)
+    {
+        unsigned has = __ballot_sync(0xFFFFFFFFu, tiles_of(base + lane) > low);
+        const int n = __popc(has);
+        if (skip < n)
+        {
+            while (skip--)
+                has &= has - 1;
+            sequence = base + __ffs(has) - 1;
+            return;
+        }
+        skip -= n;
+    }
+}
+
+template <typename T, int D, int NQ, bool Tree>
+__global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kCtas)
+    attention_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kpages,
+                  const __grid_constant__ CUtensorMap vpages, const MmaCall c)
+{
+    using Shape = MmaShape<D, NQ>;
+    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks, B = Shape::kBuffers;
+    constexpr int kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    MmaHead& h = *reinterpret_cast<MmaHead*>(smem);
+    static_assert(sizeof(MmaHead) <= Shape::kHead, "the head's room");
+    uint8_t* queries = smem + Shape::kHead;
+    uint8_t* ring = queries + Shape::kQueryBytes;
+    const AttnCall& a = c.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == 0)
+    {
+        MmaPlace p = {};
+        p.sequence = -1;
+        const int step = c.tile_tokens * NQ;
+        if (Tree)
+        {
+            int u = blockIdx.x;
+            p.chunk = u % c.chunks, u /= c.chunks;
+            p.kv_head = u % a.kv_heads, u /= a.kv_heads;
+            p.token0 = u % c.row_tiles * step;
+            const int s = u / c.row_tiles;
+            p.begin = bounded_offset(a.offsets, s, a.rows);
+            p.length = min(bounded_offset(a.offsets, s + 1, a.rows) - p.begin, a.max_nodes);
+            p.cached = min(max(a.lengths[s], 0), a.max_length);
+            p.tiles_cached = (p.cached + kKeyTile - 1) / kKeyTile;
+            p.first_tile = p.chunk * c.chunk_tiles;
+            p.tiles = min(c.chunk_tiles, p.tiles_cached + 1 - p.first_tile); // + 1: the drafted tile
+            p.whole = p.tiles_cached < c.chunk_tiles;
+            if (p.token0 < p.length && p.tiles > 0)
+                p.sequence = s;
+        }
+        else
+        {
+            int s, tile = 0;
+            p.kv_head = blockIdx.x % a.kv_heads;
+            find_tile(a, step, blockIdx.x / a.kv_heads, s, tile);
+            if (s >= 0)
+            {
+                p.sequence = s;
+                p.begin = bounded_offset(a.offsets, s, a.rows);
+                p.length = bounded_offset(a.offsets, s + 1, a.rows) - p.begin;
+                p.token0 = tile * step;
+                p.tiles = (min(p.token0 + step, p.length) - 1) / kKeyTile + 1;
+                p.whole = true;
+            }
+        }
+        if (lane == 0)
+            h.place = p;
+    }
+    else if (warp == 1)
+    {
+        tc_alloc(&h.tmem, Shape::kTmem);
+    }
+    else if (warp == 2 && lane == 0)
+    {
+        for (int s = 0; s < S; ++s)
+        {
+            mbar_init(&h.full[s], 1);
+            mbar_init(&h.empty[s], 1);
+        }
+        mbar_init(&h.query, 1);
+        for (int q = 0; q < NQ; ++q)
+            for (int b = 0; b < B; ++b)
+            {
+                mbar_init(&h.scores[q][b], 1);
+                mbar_init(&h.weights[q][b], 4); // an arrival a warp
+                mbar_init(&h.done[q][b], 1);
+            }
+        mbar_fence_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (Tree)
+        pdl_trigger(); // attention_join may take its place; it waits for this grid's end
+    const MmaPlace p = h.place;
+    const uint32_t tmem = h.tmem;
+    if (p.sequence < 0)
+    {
+        if (warp == 1)
+            tc_dealloc(tmem, Shape::kTmem);
+        return;
+    }
+    // Key tiles of query tile q: a prompt's tile ends with its last token's.
+    auto tiles_of = [&](int q) {
+        const int t0 = p.token0 + q * c.tile_tokens;
+        if (t0 >= p.length)
+            return 0;
+        return Tree ? p.tiles : (min(t0 + c.tile_tokens, p.length) - 1) / kKeyTile + 1;
+    };
+    const int tiles = p.tiles;
+    const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+
+    if (warp == 0)
+    {
+        int put = 0, ids = -1;
+        bool ok = true;
+        if (lane == 0)
+        {
+            mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
+            for (int q = 0; q < NQ; ++q)
+                for (int b = 0; b < kBlocks; ++b)
+                    tensor_load(queries + (q * kBlocks + b) * 128 * 128, &qmap, 64 * b, p.kv_head * a.group,
+                                p.begin + p.token0 + q * c.tile_tokens, &h.query);
+        }
+        auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id) {
+            const int stage = put % S;
+            if (put >= S && !thread_wait(&h.empty[stage], (put / S - 1) & 1))
+                return false;
+            const int t = p.first_tile + j;
+            const bool cached = Tree && t < p.tiles_cached;
+            // A page that is not there is read past the pool's end: zeros.
+            const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                   : p.begin + (Tree ? 0 : j * kKeyTile);
+            mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
+            for (int b = 0; b < kBlocks; ++b)
+                tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
+                            p.kv_head, row, &h.full[stage]);
+            ++put;
+            return true;
+        };
+        int id_before = -1; // tile j - 1's page
+        for (int j = 0; j <= tiles; ++j)
+        {
+            int id = -1;
+            if (Tree)
+            {
+                if ((j & 31) == 0)
+                {
+                    const int t = p.first_tile + j + lane;
+                    ids = t < p.tiles_cached ? table[t] : -1;
+                }
+                id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
+            }
+            if (lane == 0 && ok)
+                ok = (j == tiles || load(j, &kmap, &kpages, id)) && (j == 0 || load(j - 1, &vmap, &vpages, id_before));
+            id_before = id;
+            __syncwarp();
+        }
+        // Every copy has landed before the CTA may end (only a failed run gets here early).
+        if (lane == 0 && !ok)
+        {
+            mbar_wait(&h.query, 0);
+            for (int i = max(0, put - S); i < put; ++i)
+                mbar_wait(&h.full[i % S], (i / S) & 1);
+        }
+        __syncwarp();
+    }
+    else if (warp == 1)
+    {
+        constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false), kRows = tc_idesc16(kType, D, true);
+        const uint32_t qbase = smem_addr(queries), rbase = smem_addr(ring);
+        int n[NQ];
+        for (int q = 0; q < NQ; ++q)
+            n[q] = tiles_of(q);
+        int taken = 0;
+        bool ok = warp_wait(&h.query, 0);
+        // S of tile j, from the stage that is next in the ring.
+        auto scores = [&](int j) {
+            const int stage = taken % S;
+            if (!warp_wait(&h.full[stage], (taken / S) & 1))
+                return false;
+            for (int q = 0; q < NQ; ++q)
+            {
+                if (j >= n[q])
+                    continue;
+                // The buffer's last weights (tile j - B) have been read.
+                if (j >= B && !warp_wait(&h.done[q][j % B], (j / B - 1) & 1))
+                    return false;
+                tc_fence_after();
+                if (lane == 0)
+                {
+                    const uint32_t d = tmem + (q * B + j % B) * kKeyTile;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                    {
+                        const uint64_t qa = tc_desc(qbase + (q * kBlocks + i / 4) * 128 * 128 + (i & 3) * 32);
+                        const uint64_t kb = tc_desc(rbase + stage * Shape::kStageBytes + i / 4 * Shape::kBox + (i & 3) * 32);
+                        tc_mma(d, qa, kb, kScores, i > 0);
+                    }
+                    tc_commit(&h.scores[q][j % B]);
+                }
+                __syncwarp();
+            }
+            if (lane == 0)
+                tc_commit(&h.empty[stage]);
+            ++taken;
+            __syncwarp();
+            return true;
+        };
+        auto rows = [&](int j) {
+            const int stage = taken % S;
+            if (!warp_wait(&h.full[stage], (taken / S) & 1))
+                return false;
+            const int t = p.first_tile + j;
+            const int valid = !Tree                 ? p.length - j * kKeyTile
+                              : t < p.tiles_cached ? p.cached - t * kKeyTile
+                                                    : p.length;
+            if (valid < kKeyTile)
+            {
+                const int bytes = (kKeyTile - valid) * 128;
+                for (int b = 0; b < kBlocks; ++b)
+                    for (int i = lane * 16; i < bytes; i += 512)
+                        *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128 + i) =
+                            make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+                __syncwarp();
+            }
+            for (int q = 0; q < NQ; ++q)
+            {
+                if (j >= n[q])
+                    continue;
+                if (!warp_wait(&h.weights[q][j % B], (j / B) & 1))
+                    return false;
+                tc_fence_after();
+                if (lane == 0)
+                {
+                    const uint32_t d = tmem + Shape::kScoreColumns + q * D, pa = tmem + (q * B + j % B) * kKeyTile;
+#pragma unroll
+                    for (int i = 0; i < kKeyTile / 16; ++i)
+                        tc_mma_ts(d, pa + i * 8, tc_desc_mn(rbase + stage * Shape::kStageBytes + i * 2048, Shape::kBox),
+                                  kRows, j > 0 || i > 0);
+                    tc_commit(&h.done[q][j % B]);
+                }
+                __syncwarp();
+            }
+            if (lane == 0)
+                tc_commit(&h.empty[stage]);
+            ++taken;
+            __syncwarp();
+            return true;
+        };
+        ok = ok && scores(0);
+        for (int j = 0; j < tiles && ok; ++j)
+            ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
+        // A failed run: the MMAs issued so far end before TMEM is given back.
+        if (!ok && lane == 0)
+        {
+            tc_commit(&h.query);
+            mbar_wait(&h.query, 1);
+        }
+        __syncwarp();
+    }
+    else if (warp >= 4)
+    {
+        const int q = (warp - 4) >> 2, quarter = warp & 3;
+        const int row = quarter * 32 + lane; // the TMEM lane
+        const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
+        const uint32_t obase = tmem + lanes + Shape::kScoreColumns + q * D;
+        const int n = tiles_of(q);
+        const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
+        const bool real = row < c.tile_tokens * a.group && token < p.length;
+        unsigned long long path = 0;
+        if (Tree)
+        {
+            // The warpgroup's copy of the sequence's parents; a row's path from it.
+            for (int i = tid & 127; i < p.length; i += 128)
+                h.parents[i] = a.parents[p.begin + i];
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");
+            if (real)
+                path = tree_path(h.parents, token);
+        }
+        const float scale = a.scale_log2;
+        float m = -INFINITY, l = 0.f;
+        int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
+        bool ok = true;
+        for (int j = 0; j < n; ++j)
+        {
+            const int t = p.first_tile + j;
+            const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
+            const uint32_t sbase = tmem + lanes + (q * B + j % B) * kKeyTile;
+            if (!warp_wait(&h.scores[q][j % B], (j / B) & 1))
+            {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t r[64];
+            tc_ld32(sbase, r);
+            tc_ld32(sbase + 32, r + 32);
+            tc_wait_ld32(r);
+            tc_wait_ld32(r + 32);
+            float* s = reinterpret_cast<float*>(r);
+            // What the row does not attend to.
+            if (Tree && t >= p.tiles_cached)
+            {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    s[i] = path >> i & 1 ? s[i] : -INFINITY;
+            }
+            else
+            {
+                const int limit = !Tree                        ? token - j * kKeyTile + 1
+                                  : page_there(id, a.pages) ? p.cached - t * kKeyTile
+                                                             : 0;
+                if (limit < kKeyTile)
+                {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        s[i] = i < limit ? s[i] : -INFINITY;
+                }
+            }
+            id = id_next;
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < 64; ++i)
+                top[i & 3] = fmaxf(top[i & 3], s[i]);
+            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+            if (j == 0)
+                m = m_tile;
+            else
+            {
+                const bool rises = m_tile > m + 8.f;
+                if (__any_sync(0xFFFFFFFFu, rises))
+                {
+                    // O of tile j - 1 is complete before it is scaled.
+                    if (!warp_wait(&h.done[q][(j - 1) % B], ((j - 1) / B) & 1))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const float alpha = rises ? exp2_approx(m - m_tile) : 1.f;
+                    l *= alpha;
+                    m = rises ? m_tile : m;
+#pragma unroll 1
+                    for (int b = 0; b < D; b += 16)
+                    {
+                        uint32_t o[16];
+                        tc_ld16(obase + b, o);
+                        tc_wait_ld(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tc_st16(obase + b, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : -m;
+            float sum[4] = {};
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+            {
+                const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale),
+                                            make_float2(base, base));
+                const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
+                sum[2 * (i & 1)] += e0;
+                sum[2 * (i & 1) + 1] += e1;
+                w[i] = pack_pair<T>(e0, e1);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_st32(sbase, w);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&h.weights[q][j % B]);
+        }
+        if (ok && n > 0)
+            ok = warp_wait(&h.done[q][(n - 1) % B], ((n - 1) / B) & 1);
+        if (n > 0)
+        {
+            tc_fence_after();
+            const int at = p.begin + token; // the row of q and out
+            const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
+            const bool whole = !Tree || p.whole;
+            const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
+            bool finite = true;
+#pragma unroll 1
+            for (int b = 0; b < D; b += 16)
+            {
+                uint32_t o[16];
+                tc_ld16(obase + b, o);
+                tc_wait_ld(o);
+                if (b >= a.width || !real)
+                    continue;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        const float v = __uint_as_float(o[8 * g + i]);
+                        finite = finite && fabsf(v) < INFINITY;
+                        x[i] = scaled == 0.f ? 0.f : v * scaled;
+                    }
+                    if (b + 8 * g < a.width)
+                    {
+                        if (whole)
+                            store8((T*) a.out + at * a.out_stride + (size_t) head * a.width + b + 8 * g, x);
+                        else
+                            store8(c.part_o + part * a.width + b + 8 * g, x);
+                    }
+                }
+            }
+            if (Tree && !whole && real)
+                c.part_ml[part] = make_float2(m, l);
+            // Rows that came out not finite: again, from what they attend to only.
+            unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !(finite && fabsf(l) < INFINITY));
+            while (again)
+            {
+                const int who = __ffs(again) - 1;
+                again &= again - 1;
+                const int at1 = __shfl_sync(0xFFFFFFFFu, at, who), head1 = __shfl_sync(0xFFFFFFFFu, head, who);
+                if (whole)
+                    attention_row<T, Tree>(a, p.sequence, p.begin, at1, head1);
+                else
+                {
+                    const RowKeys keys = row_keys<Tree>(a, p.sequence, p.begin, at1);
+                    const int from = p.first_tile * kKeyTile;
+                    const bool last = p.first_tile + tiles > p.tiles_cached;
+                    const int to = last ? keys.cached + keys.drafted : (p.first_tile + tiles) * kKeyTile;
+                    float x[8] = {}, acc[8], m1, l1;
+                    if (lane * 8 < a.width)
+                        load8((const T*) a.q + at1 * a.q_stride + (size_t) head1 * a.width + lane * 8, x);
+                    attend_row<T, Tree>(a, keys, p.kv_head, x, from, to, m1, l1, acc);
+                    const size_t part1 = ((size_t) p.chunk * a.rows + at1) * a.heads + head1;
+                    if (lane * 8 < a.width)
+                        store8(c.part_o + part1 * a.width + lane * 8, acc);
+                    if (lane == 0)
+                        c.part_ml[part1] = make_float2(m1, l1);
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1)
+        tc_dealloc(tmem, Shape::kTmem);
+}
+
+// Joins a tree's chunks: a warp a (row, head), lane c the channels [8 c, 8 c + 8).
+// Rows of one chunk are finished already.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join(const MmaCall c)
+{
+    pdl_wait();
+    const AttnCall& a = c.a;
+    const long long unit = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int row = (int) (unit / a.heads), head = (int) (unit % a.heads), at = (threadIdx.x & 31) * 8;
+    if (row >= a.rows)
+        return;
+    const int s = sequence_of(a.offsets, a.sequences, a.rows, row);
+    if (s < 0 || row - bounded_offset(a.offsets, s, a.rows) >= a.max_nodes)
+        return;
+    const int tiles = (min(max(a.lengths[s], 0), a.max_length) + kKeyTile - 1) / kKeyTile + 1;
+    const int chunks = (tiles + c.chunk_tiles - 1) / c.chunk_tiles;
+    if (chunks == 1)
+        return;
+    float m = -INFINITY;
+    for (int i = 0; i < chunks; ++i)
+        m = fmaxf(m, c.part_ml[((size_t) i * a.rows + row) * a.heads + head].x);
+    float l = 0.f, acc[8] = {};
+    for (int i = 0; i < chunks; ++i)
+    {
+        const size_t part = ((size_t) i * a.rows + row) * a.heads + head;
+        const float2 ml = c.part_ml[part];
+        if (ml.y == 0.f) // nothing attended in this chunk
+            continue;
+        const float w = ml.x == m ? 1.f : exp2f(ml.x - m);
+        l += w * ml.y;
+        if (at < a.width)
+        {
+            float x[8];
+            load8(c.part_o + part * a.width + at, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                acc[e] = fmaf(w, x[e], acc[e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        acc[e] = l == 0.f ? 0.f : acc[e] * inv;
+    if (at < a.width)
+        store8((T*) a.out + row * a.out_stride + (size_t) head * a.width + at, acc);
+}
+} // namespace hfk

@@ -3,11 +3,13 @@
 // state: every check is made on the host before the first launch.
 #include <hf_cuda.h>
 
+#include "attention_mma.cuh"
 #include "attention_rows.cuh"
 #include "launch.cuh"
 #include "pages.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 using namespace hfk;
@@ -106,7 +108,7 @@ int check_cache_sizes(const hf_page_cache* cache, hf_page_cache* c)
     *c = *cache;
     const int size = size_of(c->dtype);
     if (!size || c->layers < 1 || c->pages < 1 || c->sequences < 1 || c->table_stride < 1
-        || c->table_stride > (1 << 20) || c->pages > (1 << 26))
+        || c->table_stride > (1 << 20) || c->pages >= (1 << 25))
         return HF_E_INVALID;
     if (c->kv_width < 8 || c->kv_width % 8 || c->kv_width > (1 << 20))
         return HF_E_SHAPE;
@@ -164,7 +166,7 @@ int copy_rows(const PageBook& b, int most, int device, cudaStream_t stream)
 // Checks of what both attentions share; fills the kernels' call.
 int check_attention(int dtype, int heads, int kv_heads, int width, int rows, float scale)
 {
-    if (!size_of(dtype) || heads < 1 || kv_heads < 1 || rows < 1 || !std::isfinite(scale))
+    if (!size_of(dtype) || heads < 1 || kv_heads < 1 || rows < 1 || !(scale > 0.f) || !std::isfinite(scale))
         return HF_E_INVALID;
     if (heads % kv_heads || heads / kv_heads > 128 || width < 8 || width % 8 || width > 256
         || (int64_t) heads * width > (1 << 24))
@@ -198,6 +200,147 @@ int check_rows(const Call& call, int size, int heads, int kv_heads, int width, A
     return HF_OK;
 }
 
+// ---- tensor maps ---------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder()
+{
+    static std::atomic<EncodeTiled> known {nullptr};
+    if (EncodeTiled e = known.load(std::memory_order_relaxed))
+        return e;
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess
+        || found != cudaDriverEntryPointSuccess)
+        return nullptr;
+    known.store((EncodeTiled) f, std::memory_order_relaxed);
+    return (EncodeTiled) f;
+}
+
+// [rows][heads][width] 16-bit elements, rows `stride` elements apart, in boxes of
+// 64 channels x box_heads x box_rows with the 128-byte swizzle; zeros outside.
+bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int heads, int64_t rows, int64_t stride,
+                 int box_heads, int box_rows)
+{
+    const EncodeTiled encode = encoder();
+    const cuuint64_t dims[3] = {(cuuint64_t) width, (cuuint64_t) heads, (cuuint64_t) rows};
+    const cuuint64_t strides[2] = {(cuuint64_t) width * 2, (cuuint64_t) stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t) box_heads, (cuuint32_t) box_rows}, ones[3] = {1, 1, 1};
+    return encode
+           && encode(map, dtype == HF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                     const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+                  == CUDA_SUCCESS;
+}
+
+// ---- attention_mma ---------------------------------------------------------------
+constexpr int kSms = 148; // a B200's; the work is cut for it wherever the call is checked
+
+// How a tree's keys are cut: `chunks` chunks of `chunk_tiles` key tiles at most.
+// A CTA a (sequence, kv head, row tile, chunk): chunks enough for about three
+// CTAs a place on the GPU at the longest length, so that shorter sequences and
+// the last CTAs leave little of it idle, but at least four tiles each.
+struct TreePlan
+{
+    int row_tiles, chunk_tiles, chunks;
+};
+
+TreePlan tree_plan(int sequences, int heads, int kv_heads, int width, int max_nodes, int max_length)
+{
+    const int tokens = 128 / (heads / kv_heads);
+    const int row_tiles = (max_nodes + tokens - 1) / tokens;
+    const int tiles = (max_length + kKeyTile - 1) / kKeyTile + 1;
+    const int64_t units = (int64_t) sequences * kv_heads * row_tiles, places = kSms * (width <= 128 ? 2 : 1);
+    const int64_t wanted = std::min<int64_t>((3 * places + units - 1) / units, (tiles + 3) / 4);
+    const int chunk_tiles = (int) ((tiles + wanted - 1) / std::max<int64_t>(wanted, 1));
+    return {row_tiles, chunk_tiles, (tiles + chunk_tiles - 1) / chunk_tiles};
+}
+
+uint64_t part_bytes(const TreePlan& plan, int rows, int heads, int width)
+{
+    return plan.chunks == 1 ? 0 : (uint64_t) plan.chunks * rows * heads * (4 * (uint64_t) width + 8);
+}
+
+template <typename T, int D, int NQ, bool Tree>
+int launch_mma(const CUtensorMap (&maps)[5], const MmaCall& c, int64_t ctas, int device, cudaStream_t stream)
+{
+    using Shape = MmaShape<D, NQ>;
+    const auto kernel = attention_mma<T, D, NQ, Tree>;
+    static std::atomic<uint64_t> ready {0}; // devices whose kernel has its shared memory
+    const uint64_t bit = 1ull << (device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit))
+    {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess)
+            return HF_E_CUDA;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return status_of(launch(false, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
+                            maps[1], maps[2], maps[3], maps[4], c));
+}
+
+template <typename T>
+int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
+{
+    MmaCall c = {};
+    c.a = a;
+    c.tile_tokens = 128 / a.group;
+    c.chunks = 1;
+    // Two query tiles a CTA read the keys half as often; with fewer of them
+    // than SMs the rows are spread over twice the CTAs instead.
+    const int64_t pairs = (int64_t) a.rows * a.heads / 256;
+    const int nq = a.width <= 128 && pairs >= kSms ? 2 : 1;
+    const int64_t ctas = ((int64_t) a.rows / (c.tile_tokens * nq) + a.sequences) * a.kv_heads;
+    CUtensorMap maps[5] = {};
+    if (!encode_rows(&maps[0], dtype, a.q, a.width, a.heads, a.rows, a.q_stride, a.group, c.tile_tokens)
+        || !encode_rows(&maps[1], dtype, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kKeyTile)
+        || !encode_rows(&maps[2], dtype, a.v, a.width, a.kv_heads, a.rows, a.v_stride, 1, kKeyTile))
+        return HF_E_CUDA;
+    if (ctas > INT32_MAX)
+        return HF_E_SHAPE;
+    if (a.width > 128)
+        return launch_mma<T, 256, 1, false>(maps, c, ctas, device, stream);
+    if (a.width > 64)
+        return nq == 2 ? launch_mma<T, 128, 2, false>(maps, c, ctas, device, stream)
+                       : launch_mma<T, 128, 1, false>(maps, c, ctas, device, stream);
+    return nq == 2 ? launch_mma<T, 64, 2, false>(maps, c, ctas, device, stream)
+                   : launch_mma<T, 64, 1, false>(maps, c, ctas, device, stream);
+}
+
+template <typename T>
+int tree_mma(int dtype, const AttnCall& a, const TreePlan& plan, void* workspace, int device, cudaStream_t stream)
+{
+    MmaCall c = {};
+    c.a = a;
+    c.tile_tokens = 128 / a.group;
+    c.row_tiles = plan.row_tiles;
+    c.chunk_tiles = plan.chunk_tiles;
+    c.chunks = plan.chunks;
+    const uint64_t parts = (uint64_t) plan.chunks * a.rows * a.heads;
+    c.part_o = (float*) workspace;
+    c.part_ml = (float2*) (c.part_o + parts * a.width);
+    const int64_t ctas = (int64_t) a.sequences * a.kv_heads * plan.row_tiles * plan.chunks;
+    CUtensorMap maps[5] = {};
+    const int64_t positions = (int64_t) a.pages * kPagePositions;
+    if (ctas > INT32_MAX)
+        return HF_E_SHAPE;
+    if (!encode_rows(&maps[0], dtype, a.q, a.width, a.heads, a.rows, a.q_stride, a.group, c.tile_tokens)
+        || !encode_rows(&maps[1], dtype, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kKeyTile)
+        || !encode_rows(&maps[2], dtype, a.v, a.width, a.kv_heads, a.rows, a.v_stride, 1, kKeyTile)
+        || !encode_rows(&maps[3], dtype, a.key_pages, a.width, a.kv_heads, positions, a.kv_heads * a.width, 1, kKeyTile)
+        || !encode_rows(&maps[4], dtype, a.value_pages, a.width, a.kv_heads, positions, a.kv_heads * a.width, 1, kKeyTile))
+        return HF_E_CUDA;
+    const int rc = a.width > 128  ? launch_mma<T, 256, 1, true>(maps, c, ctas, device, stream)
+                   : a.width > 64 ? launch_mma<T, 128, 1, true>(maps, c, ctas, device, stream)
+                                  : launch_mma<T, 64, 1, true>(maps, c, ctas, device, stream);
+    if (rc || plan.chunks == 1)
+        return rc;
+    const dim3 grid((unsigned) (((int64_t) a.rows * a.heads + 7) / 8));
+    return status_of(launch(true, attention_join<T>, grid, dim3(256), 0, stream, c));
+}
+
 template <bool Tree>
 int run_rows(int dtype, const AttnCall& a, cudaStream_t stream)
 {
@@ -228,9 +371,35 @@ int check_tree_sizes(const hf_page_cache* cache, hf_page_cache* c, const hf_atte
         return HF_E_SHAPE;
     return HF_OK;
 }
+
+uint64_t tree_workspace(const hf_page_cache& c, const hf_attention_tree& call)
+{
+    if (c.dtype == HF_DTYPE_F32)
+        return 0;
+    const TreePlan plan = tree_plan(c.sequences, call.heads, call.kv_heads, call.head_width, call.max_nodes, call.max_length);
+    return part_bytes(plan, call.rows, call.heads, call.head_width);
+}
 } // namespace
 
 extern "C" {
+int hf_cuda_operators_sync(int device, void* stream)
+{
+    int before = 0;
+    if (cudaGetDevice(&before) != cudaSuccess || cudaSetDevice(device) != cudaSuccess)
+        return HF_E_CUDA;
+    unsigned error = 0;
+    cudaError_t e = cudaStreamSynchronize((cudaStream_t) stream);
+    if (e == cudaSuccess)
+        e = cudaMemcpyFromSymbol(&error, g_operator_error, sizeof(error));
+    if (e == cudaSuccess && error)
+    {
+        const unsigned none = 0;
+        e = cudaMemcpyToSymbol(g_operator_error, &none, sizeof(none));
+    }
+    cudaSetDevice(before);
+    return e != cudaSuccess ? HF_E_CUDA : error ? HF_E_DEVICE : HF_OK;
+}
+
 int hf_cuda_pages_workspace(const hf_page_cache* cache, uint64_t* bytes)
 {
     hf_page_cache c;
@@ -352,7 +521,11 @@ int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
         return on.status;
     if (!on.holds(a.k, a.v, a.out, a.offsets))
         return HF_E_INVALID;
-    return run_rows<false>(call->dtype, a, (cudaStream_t) stream);
+    cudaStream_t st = (cudaStream_t) stream;
+    if (call->dtype == HF_DTYPE_F32)
+        return run_rows<false>(call->dtype, a, st);
+    return call->dtype == HF_DTYPE_BF16 ? packed_mma<__nv_bfloat16>(call->dtype, a, on.current, st)
+                                        : packed_mma<__half>(call->dtype, a, on.current, st);
 }
 
 int hf_cuda_attention_tree_workspace(const hf_page_cache* cache, const hf_attention_tree* call, uint64_t* bytes)
@@ -361,7 +534,10 @@ int hf_cuda_attention_tree_workspace(const hf_page_cache* cache, const hf_attent
     if (!bytes)
         return HF_E_INVALID;
     *bytes = 0;
-    return check_tree_sizes(cache, &c, call);
+    if (const int rc = check_tree_sizes(cache, &c, call))
+        return rc;
+    *bytes = tree_workspace(c, *call);
+    return HF_OK;
 }
 
 int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* call, void* stream)
@@ -385,11 +561,21 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
     a.table_stride = c.table_stride;
     a.max_nodes = call->max_nodes;
     a.max_length = std::min(call->max_length, c.table_stride * kPagePositions);
+    const TreePlan plan = tree_plan(c.sequences, a.heads, a.kv_heads, a.width, a.max_nodes, call->max_length);
+    const uint64_t bytes = tree_workspace(c, *call);
+    if (bytes && !aligned(call->workspace))
+        return HF_E_INVALID;
+    if (call->workspace_bytes < bytes)
+        return HF_E_CAPACITY;
     const DeviceOf on(a.q);
     if (on.status)
         return on.status;
-    if (!on.holds(a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
+    if (!on.holds(bytes ? call->workspace : nullptr, a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
         return HF_E_INVALID;
-    return run_rows<true>(c.dtype, a, (cudaStream_t) stream);
+    cudaStream_t st = (cudaStream_t) stream;
+    if (c.dtype == HF_DTYPE_F32)
+        return run_rows<true>(c.dtype, a, st);
+    return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, plan, call->workspace, on.current, st)
+                                    : tree_mma<__half>(c.dtype, a, plan, call->workspace, on.current, st);
 }
 }

@@ -58,10 +58,10 @@
 
 #include "common.cuh"
 #include "gemv.cuh"
+#include "tcgen05.cuh"
 
 namespace hfk
 {
-constexpr int kTcRows = 128;                             // weight rows per tile (the MMA's M)
 constexpr int kTcChunk = 64;                             // columns per stage (one 128-byte swizzle atom of fp16)
 constexpr int kTcQuantBytes = kTcRows * kTcChunk;        // 8 KiB
 constexpr int kTcBlockBytes = kTcQuantBytes + kTcRows * 2 * 2; // + two fp16 scales per row
@@ -114,108 +114,6 @@ __host__ __device__ constexpr size_t tc_weight_bytes(size_t N, size_t K)
 __host__ __device__ constexpr size_t tc_x_bytes(size_t m_pad, size_t K)
 {
     return m_pad * K * 2 * sizeof(__half);
-}
-
-// ---- tcgen05 / TMEM primitives (inline PTX, sm_100a) ----------------------
-__device__ __forceinline__ void tc_fence_before()
-{
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tc_fence_after()
-{
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-// Makes this thread's generic-proxy shared-memory stores visible to the
-// tensor core's (async proxy) reads.
-__device__ __forceinline__ void fence_proxy_async()
-{
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major operand with 128-byte swizzle:
-// start address >> 4, leading offset 1 (unused for this layout), stride 1024
-// bytes between 8-row groups, descriptor version 1, layout 2 (SWIZZLE_128B).
-__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr)
-{
-    return (uint64_t) ((saddr >> 4) & 0x3FFFu) | ((uint64_t) 1 << 16) | ((uint64_t) (1024 >> 4) << 32)
-           | ((uint64_t) 1 << 46) | ((uint64_t) 2 << 61);
-}
-
-// Instruction descriptor of kind::f16: D f32, A and B f16, both K-major,
-// N = nx, M = 128.
-__host__ __device__ constexpr uint32_t tc_idesc(int nx)
-{
-    return (1u << 4) | ((uint32_t) (nx >> 3) << 17) | ((uint32_t) (kTcRows >> 4) << 24);
-}
-
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
-{
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// The same with the A operand in TMEM (K-major: lane = row, two fp16 per
-// 32-bit column, the lower k in the low half).
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
-                                          uint32_t accumulate)
-{
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// 32 lanes x 16 consecutive 32-bit columns from registers (thread t: lane
-// taddr's lane + t), then the wait for this thread's TMEM stores.
-__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                 "%13, %14, %15, %16};" ::"r"(taddr),
-                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-
-__device__ __forceinline__ void tc_wait_st()
-{
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// Arrives on `bar` once every MMA this thread issued so far has completed.
-__device__ __forceinline__ void tc_commit(uint64_t* bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-
-// 32 lanes x 16 consecutive 32-bit columns: thread t gets lane (taddr's lane
-// + t), columns col .. col + 15. The values are usable after tc_wait_ld(r).
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                 "%13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15])
-                 : "r"(taddr));
-}
-
-// Waits for this thread's TMEM loads; naming r as read and written keeps the
-// compiler from using r before the wait.
-__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[16])
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15])
-                 :
-                 : "memory");
 }
 
 // ---- weight blocks (once per upload) --------------------------------------

@@ -294,6 +294,7 @@ def cuda() -> ctypes.CDLL:
         lib.hf_cuda_argmax_noalloc.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp]
         lib.hf_cuda_time_kernel.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_float),
                                             ctypes.POINTER(ctypes.c_double)]
+        lib.hf_cuda_operators_sync.argtypes = [ctypes.c_int, _vp]
         lib.hf_cuda_pages_workspace.argtypes = [ctypes.POINTER(PageCacheStruct), ctypes.POINTER(ctypes.c_uint64)]
         lib.hf_cuda_pages_update.argtypes = [ctypes.POINTER(PageCacheStruct), _vp, ctypes.c_int32, _vp, ctypes.c_int32,
                                              _vp, _vp, _vp, ctypes.c_uint64, _vp]
@@ -701,6 +702,13 @@ class Linear:
 def _refused(rc: int, what: str):
     if rc:
         raise HFError(rc, f"the engine refused the {what}")
+
+
+def operators_sync(device: int = 0, stream: int | None = None):
+    """Waits for `stream`; raises when an operator's kernel gave up a wait on `device` (hf_cuda_operators_sync)."""
+    rc = cuda().hf_cuda_operators_sync(device, stream)
+    if rc:
+        raise HFError(rc, "an operator's kernel gave up a wait" if rc == HF_E_DEVICE else "CUDA error")
 
 
 class PageCache:

@@ -398,8 +398,13 @@ int hf_cuda_quantize_q8(const float* values, int64_t first, int64_t count, int64
  * host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
  * bounded by the kernels: offsets are taken as ascending within [0, rows],
  * lengths within the bounds given, and a page id outside the pool is a page
- * that is not there (its positions are not attended, read or written). */
+ * that is not there (its positions are not attended, read or written). Waits
+ * inside the kernels are bounded: one that ran out leaves NaN rows and is
+ * reported by hf_cuda_operators_sync. */
 enum { HF_DTYPE_F32 = 0, HF_DTYPE_BF16 = 1, HF_DTYPE_F16 = 2 };
+/* Waits for `stream`; HF_E_DEVICE when a wait of an operator's kernel has run out on
+ * `device` since the last call (and clears it). */
+int hf_cuda_operators_sync(int device, void* stream);
 
 /* Causal attention of packed prompts: row i of sequence s (rows
  * [offsets[s], offsets[s + 1]) of q, k, v and out) attends to that sequence's
@@ -407,7 +412,7 @@ enum { HF_DTYPE_F32 = 0, HF_DTYPE_BF16 = 1, HF_DTYPE_F16 = 2 };
  * out are [heads][head_width], of k and v [kv_heads][head_width], `*_stride`
  * elements apart (0 = packed; views of one fused q|k|v row are fine). Rows
  * outside every sequence are neither read nor written. head_width is a multiple
- * of 8 up to 256, heads / kv_heads at most 128. `scale` multiplies the scores.
+ * of 8 up to 256, heads / kv_heads at most 128. `scale` (> 0) multiplies the scores.
  * A value or key row that holds infinities or NaN reaches only the rows that
  * attend to it. */
 typedef struct hf_attention_packed

@@ -84,7 +84,7 @@ def test_packed_arguments(bad, kind):
 
 
 def test_packed_scale_and_type():
-    for scale in (float("nan"), float("inf")):
+    for scale in (float("nan"), float("inf"), 0.0, -0.5):
         assert _code(native.PackedAttention(native.F32, 8, 2, 64, scale=scale).workspace_bytes, 1, 1) == native.HF_E_INVALID
     assert _code(native.PackedAttention(5, 8, 2, 64).workspace_bytes, 1, 1) == native.HF_E_INVALID
 
