@@ -1,0 +1,785 @@
+// Attention of packed prompts and drafted trees in fp32 on the 5th-generation
+// tensor cores, every operand as two fp16 halves.
+//
+// Arithmetic. x 2^e = hi + lo with hi = fp16(x 2^e) and lo = fp16(x 2^e - hi) keeps 22
+// bits and more of every x that is not tiny next to the largest one under the
+// same exponent e, and a product is hi.hi' + hi.lo' + lo.hi' in fp32 (the
+// dropped lo.lo' is below 2^-22 of it). The tensor core's fp32 additions
+// truncate, so no chain is long at full size: the scores keep hi.hi' (a step
+// per 16 channels) and the small rest in accumulators of their own, and the
+// values' products of one 64-key tile (the small ones first, then 4 steps of
+// hi.hi') are added to the row's fp32 sums in registers, rounded to nearest.
+// Exponents: of a query, its row's; of keys and values a tile's (prompts:
+// split_tiles takes the tile's largest value) or the CTA's (trees: from 16 of its keys);
+// the weights 2^(s - m) are taken times 2^14, which cancels in the end. Where an
+// exponent does not fit its tile (values 2^16 apart, or more than 16 times the
+// trees' sample) the tile's factor is NaN, and like every row that comes out
+// not finite, its rows are taken again by attention_row.
+//
+// Work. As in attention_mma: 128 rows (tokens x a kv head's heads) a CTA, 64-key
+// tiles, heaviest first. K and V pass through a ring of 16 KB stages, each 64
+// keys x 64 channels: the hi half and the lo half. A prompt's keys serve many
+// CTAs, so split_tiles writes their halves to the workspace once and the stages
+// are tensor-map copies; a tree's keys are read once, so its stages arrive in
+// fp32 (the same 16 KB) and a warpgroup of converters turns them into halves in
+// place.
+//
+// Roles: warp 0 copies; warp 1 MMAs: S = [hi.hi' | small] as one MMA of hi with
+// [hi' ; lo'] (N = 128) and one of lo with hi' (N = 64) a step, then O of a tile in
+// three passes of 4 steps over 128 channels; warpgroups 1 and 2 a row's softmax
+// (half of the keys each) and its sums (half of the channels each); in trees
+// warpgroup 3 converts. S is free for the next tile once it is in registers; the
+// weights' halves have two buffers.
+#pragma once
+
+#include "attention_mma.cuh"
+
+namespace hfk
+{
+// The two halves of x under a power-of-two factor, two values at a time.
+__device__ __forceinline__ void split_pair(float x, float y, float factor, uint32_t& hi, uint32_t& lo)
+{
+    const float2 v = __fmul2_rn(make_float2(x, y), make_float2(factor, factor));
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2 back = __half22float2(h);
+    const __half2 l = __floats2half2_rn(v.x - back.x, v.y - back.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// 2^e with `largest` 2^e in [2^top / 2, 2^top); 1 for nothing or for what lies
+// outside the normal range by far.
+__device__ __forceinline__ float split_factor(float largest, int top)
+{
+    if (!(largest > 0.f))
+        return 1.f;
+    const int exponent = (int) (__float_as_uint(largest) >> 23) - 126; // largest in [2^(exponent - 1), 2^exponent)
+    const int e = min(max(top - exponent, -120), 120);
+    return __uint_as_float((uint32_t) (127 + e) << 23);
+}
+
+__device__ __forceinline__ float finite_abs(float x)
+{
+    const float v = fabsf(x);
+    return v < INFINITY ? v : 0.f;
+}
+
+struct LimbCall
+{
+    MmaCall c;
+    __half* limbs;    // a prompt's K hi, K lo, V hi, V lo: [4][rows][kv_heads][width]
+    float* factors;   // what undoes a tile's exponents: [2][kv_heads][tiles]
+    int tiles;        // rows / 64 + sequences: tile j of sequence s is (begin_s / 64) + s + j
+};
+
+// One CTA a (tile, kv head, K or V) of packed prompts: 8 rows a warp, 8 channels
+// a lane, read once and kept.
+__global__ void __launch_bounds__(256) split_tiles(const __grid_constant__ LimbCall l)
+{
+    __shared__ float row_max[kKeyTile];
+    pdl_trigger();
+    const AttnCall& a = l.c.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, at = lane * 8;
+    const int tile = blockIdx.x, kv_head = blockIdx.y, values = blockIdx.z;
+    int low = -1, high = a.sequences; // first(low) <= tile < first(high)
+    while (high - low > 1)
+    {
+        const int mid = (low + high) / 2;
+        if (bounded_offset(a.offsets, mid, a.rows) / kKeyTile + mid <= tile)
+            low = mid;
+        else
+            high = mid;
+    }
+    if (low < 0)
+        return;
+    const int begin = bounded_offset(a.offsets, low, a.rows);
+    const int first = (tile - begin / kKeyTile - low) * kKeyTile;
+    const int count = min(bounded_offset(a.offsets, low + 1, a.rows) - begin - first, kKeyTile);
+    if (count <= 0)
+        return;
+    const float* source = (const float*) (values ? a.v : a.k);
+    const long long stride = values ? a.v_stride : a.k_stride;
+    float x[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        const int r = warp * 8 + i;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[i][e] = 0.f;
+        if (r < count && at < a.width)
+            load8(source + (begin + first + r) * stride + (size_t) kv_head * a.width + at, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            m = fmaxf(m, finite_abs(x[i][e]));
+        m = warp_max(m);
+        if (lane == 0)
+            row_max[warp * 8 + i] = m;
+    }
+    __syncthreads();
+    const float m0 = row_max[lane], m1 = row_max[lane + 32];
+    const float largest = warp_max(fmaxf(m0, m1));
+    // The smallest row that counts: of values any, of keys the first that is not
+    // zero (a row attends to a tile's keys from the first on).
+    const unsigned some0 = __ballot_sync(0xFFFFFFFFu, m0 > 0.f), some1 = __ballot_sync(0xFFFFFFFFu, m1 > 0.f);
+    float smallest = -warp_max(-fminf(m0 > 0.f ? m0 : INFINITY, m1 > 0.f ? m1 : INFINITY));
+    if (!values && (some0 | some1))
+        smallest = row_max[some0 ? __ffs(some0) - 1 : 31 + __ffs(some1)];
+    const float factor = split_factor(largest, 15);
+    if (tid == 0)
+    {
+        const bool fits = largest == 0.f || largest * 0x1p-16f <= smallest;
+        l.factors[((size_t) values * a.kv_heads + kv_head) * l.tiles + tile] = fits ? 1.f / factor : NAN;
+    }
+    const size_t limb = (size_t) a.rows * a.kv_heads * a.width;
+    if (at < a.width)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            const int r = warp * 8 + i;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                split_pair(x[i][2 * e], x[i][2 * e + 1], factor, hi[e], lo[e]);
+            if (r < count)
+            {
+                __half* to = l.limbs + 2 * values * limb + ((size_t) (begin + first + r) * a.kv_heads + kv_head) * a.width + at;
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + limb) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+    }
+}
+
+template <int D, bool Tree>
+struct LimbShape
+{
+    static constexpr int kBlocks = D / 64;
+    static constexpr int kBox = kKeyTile * 128;          // 64 keys x 64 channels of one half
+    static constexpr int kStageBytes = 2 * kBox;
+    static constexpr int kQueryHalf = kBlocks * 128 * 128;
+    static constexpr int kHead = 3072;
+    static constexpr int kStagesFit = (227 * 1024 - kHead - 2 * kQueryHalf) / kStageBytes;
+    static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit / 2 * 2; // pairs stay together
+    static constexpr int kSmem = kHead + 2 * kQueryHalf + kStages * kStageBytes;
+    static constexpr int kParts = D == 256 ? 2 : 1;      // O in parts of up to 128 channels
+    static constexpr int kPart = D / kParts;
+    static constexpr int kRowBuffers = D == 256 ? 1 : 2; // of O
+    static constexpr int kThreads = Tree ? 512 : 384;
+    // Registers a thread, by warpgroup; at launch 168 or 128 each: the shares
+    // add up to that (3 x 168, 4 x 128).
+    static constexpr int kLaunchRegisters = Tree ? 128 : 168;
+    static constexpr int kRegistersIssue = 40, kRegistersRows = Tree ? 200 : 232, kRegistersConvert = 72;
+    static_assert(kRegistersIssue + 2 * kRegistersRows + (Tree ? kRegistersConvert : 0)
+                      <= kLaunchRegisters * kThreads / 128,
+                  "what the CTA was launched with");
+    static constexpr int kScores = 0, kWeights = 128, kRows = 256; // TMEM columns
+    static_assert(kRows + kRowBuffers * D <= 512 && kStages >= 6 && kSmem <= 227 * 1024, "what an SM holds");
+};
+
+struct LimbHead
+{
+    uint64_t full[12], ready[12], empty[12], query, scores, scores_read, weights[2], done[2][2], free[2][2];
+    uint32_t tmem;
+    int misfit;              // a tree's value outside the sampled exponent's range
+    unsigned sample[2];      // its largest K and V, as bits
+    MmaPlace place;
+    int parents[kTreeNodes];
+};
+
+template <int N>
+__device__ __forceinline__ void set_registers_up()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_registers_down()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+template <int D, bool Tree>
+__global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
+    attention_limbs(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const __grid_constant__ CUtensorMap kmap2, const __grid_constant__ CUtensorMap vmap2,
+                    const __grid_constant__ LimbCall lc)
+{
+    // Prompts: the maps of K hi, V hi, K lo, V lo. Trees: drafted K, V, paged K, V in fp32.
+    using Shape = LimbShape<D, Tree>;
+    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks, kHalf = D / 2;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    LimbHead& h = *reinterpret_cast<LimbHead*>(smem);
+    float(*exchange)[2][128] = reinterpret_cast<float(*)[2][128]>(smem + Shape::kHead - 2048); // [tile parity][warpgroup][row]
+    static_assert(sizeof(LimbHead) <= Shape::kHead - 2048, "the head's room");
+    uint8_t* queries = smem + Shape::kHead;
+    uint8_t* ring = queries + 2 * Shape::kQueryHalf;
+    const MmaCall& c = lc.c;
+    const AttnCall& a = c.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == 0)
+    {
+        const MmaPlace p = find_place<Tree>(c, c.tile_tokens);
+        if (lane == 0)
+        {
+            h.place = p;
+            h.misfit = 0;
+            h.sample[0] = h.sample[1] = 0;
+        }
+    }
+    else if (warp == 1)
+    {
+        tc_alloc(&h.tmem, 512);
+    }
+    else if (warp == 2 && lane == 0)
+    {
+        for (int s = 0; s < S; ++s)
+        {
+            mbar_init(&h.full[s], 1);
+            mbar_init(&h.ready[s], 4); // an arrival a converter warp
+            mbar_init(&h.empty[s], 1);
+        }
+        mbar_init(&h.query, 8); // an arrival a row warp
+        mbar_init(&h.scores, 1);
+        mbar_init(&h.scores_read, 8);
+        for (int b = 0; b < 2; ++b)
+        {
+            mbar_init(&h.weights[b], 8);
+            for (int i = 0; i < 2; ++i)
+            {
+                mbar_init(&h.done[b][i], 1);
+                mbar_init(&h.free[b][i], Shape::kParts == 2 ? 4 : 8);
+            }
+        }
+        mbar_fence_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (Tree)
+        pdl_trigger(); // attention_join may take its place; it waits for this grid's end
+    else
+        pdl_wait(); // split_tiles' halves
+    const MmaPlace p = h.place;
+    const uint32_t tmem = h.tmem;
+    if (p.sequence < 0)
+    {
+        if (warp == 1)
+            tc_dealloc(tmem, 512);
+        return;
+    }
+    const int tiles = p.tiles;
+    const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+    // Keys of tile j that are there.
+    auto valid_of = [&](int j) {
+        const int t = p.first_tile + j;
+        return min(kKeyTile, !Tree                 ? p.length - j * kKeyTile
+                             : t < p.tiles_cached ? p.cached - t * kKeyTile
+                                                   : p.length);
+    };
+
+    if (warp < 4)
+    {
+        set_registers_down<Shape::kRegistersIssue>();
+        if (warp == 0)
+        {
+            int put = 0, ids = -1;
+            bool ok = true;
+            // A tile's K or V, block by block.
+            auto load = [&](int j, bool values, int id) {
+                const bool cached = Tree && p.first_tile + j < p.tiles_cached;
+                const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                       : p.begin + (Tree ? 0 : j * kKeyTile);
+                for (int b = 0; b < kBlocks; ++b)
+                {
+                    const int stage = put % S;
+                    if (put >= S && !thread_wait(&h.empty[stage], (put / S - 1) & 1))
+                        return false;
+                    uint8_t* to = ring + stage * Shape::kStageBytes;
+                    mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
+                    if (Tree)
+                    {
+                        const CUtensorMap* map = cached ? (values ? &vmap2 : &kmap2) : (values ? &vmap : &kmap);
+                        tensor_load(to, map, 64 * b, p.kv_head, row, &h.full[stage]);
+                        tensor_load(to + Shape::kBox, map, 64 * b + 32, p.kv_head, row, &h.full[stage]);
+                    }
+                    else
+                    {
+                        tensor_load(to, values ? &vmap : &kmap, 64 * b, p.kv_head, row, &h.full[stage]);
+                        tensor_load(to + Shape::kBox, values ? &vmap2 : &kmap2, 64 * b, p.kv_head, row, &h.full[stage]);
+                    }
+                    ++put;
+                }
+                return true;
+            };
+            int id_before = -1; // tile j - 1's page
+            for (int j = 0; j <= tiles; ++j)
+            {
+                int id = -1;
+                if (Tree)
+                {
+                    if ((j & 31) == 0)
+                    {
+                        const int t = p.first_tile + j + lane;
+                        ids = t < p.tiles_cached ? table[t] : -1;
+                    }
+                    id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
+                }
+                if (lane == 0 && ok)
+                    ok = (j == tiles || load(j, false, id)) && (j == 0 || load(j - 1, true, id_before));
+                id_before = id;
+                __syncwarp();
+            }
+            // Every copy has landed before the CTA may end (only a failed run gets here early).
+            if (lane == 0 && !ok)
+                for (int i = max(0, put - S); i < put; ++i)
+                    mbar_wait(&h.full[i % S], (i / S) & 1);
+            __syncwarp();
+        }
+        else if (warp == 1)
+        {
+            constexpr uint32_t kWide = tc_idesc16(0, 128, false), kNarrow = tc_idesc16(0, 64, false),
+                               kValues = tc_idesc16(0, Shape::kPart, true);
+            const uint32_t qhi = smem_addr(queries), qlo = qhi + Shape::kQueryHalf, rbase = smem_addr(ring);
+            uint64_t* landed = Tree ? h.ready : h.full;
+            int taken = 0;
+            auto scores = [&](int j) {
+                // S of tile j - 1 is in registers.
+                if (j > 0 && !warp_wait(&h.scores_read, (j - 1) & 1))
+                    return false;
+                for (int b = 0; b < kBlocks; ++b)
+                {
+                    const int stage = taken % S;
+                    if (!warp_wait(&landed[stage], (taken / S) & 1))
+                        return false;
+                    tc_fence_after();
+                    if (lane == 0)
+                    {
+                        const uint32_t k = rbase + stage * Shape::kStageBytes;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                        {
+                            const uint32_t at = b * 128 * 128 + i * 32;
+                            tc_mma(tmem + Shape::kScores, tc_desc(qhi + at), tc_desc(k + i * 32), kWide, b > 0 || i > 0);
+                            tc_mma(tmem + Shape::kScores + 64, tc_desc(qlo + at), tc_desc(k + i * 32), kNarrow, 1);
+                        }
+                        tc_commit(&h.empty[stage]);
+                        if (b == kBlocks - 1)
+                            tc_commit(&h.scores);
+                    }
+                    ++taken;
+                    __syncwarp();
+                }
+                return true;
+            };
+            auto rows = [&](int j) {
+                if (!warp_wait(&h.weights[j & 1], (j / 2) & 1))
+                    return false;
+                constexpr int RB = Shape::kRowBuffers, kEach = kBlocks / Shape::kParts; // stages a part
+                const int valid = valid_of(j), buffer = j % RB;
+                for (int part = 0; part < Shape::kParts; ++part)
+                {
+                    const int stage = taken % S;
+                    for (int e = 0; e < kEach; ++e)
+                        if (!warp_wait(&landed[stage + e], (taken / S) & 1))
+                            return false;
+                    if (!Tree && valid < kKeyTile)
+                    {
+                        // Rows past the sequence's end: weights of 0, but 0 x NaN is not.
+                        const int bytes = (kKeyTile - valid) * 128;
+                        for (int box = 0; box < 2 * kEach; ++box)
+                            for (int i = lane * 16; i < bytes; i += 512)
+                                *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + box * Shape::kBox + valid * 128
+                                                          + i) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    if (j >= RB && !warp_wait(&h.free[buffer][part], (j / RB - 1) & 1))
+                        return false;
+                    tc_fence_after();
+                    if (lane == 0)
+                    {
+                        const uint32_t d = tmem + Shape::kRows + buffer * D + part * Shape::kPart;
+                        const uint32_t hi = tmem + Shape::kWeights + (j & 1) * 64, lo = hi + 32;
+                        const uint32_t v = rbase + stage * Shape::kStageBytes;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc_mma_ts(d, hi + i * 8, tc_desc_mn(v + Shape::kBox + i * 2048, Shape::kStageBytes), kValues, i > 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc_mma_ts(d, lo + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc_mma_ts(d, hi + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
+                        for (int e = 0; e < kEach; ++e)
+                            tc_commit(&h.empty[stage + e]);
+                        tc_commit(&h.done[buffer][part]);
+                    }
+                    taken += kEach;
+                    __syncwarp();
+                }
+                return true;
+            };
+            bool ok = warp_wait(&h.query, 0);
+            tc_fence_after();
+            ok = ok && scores(0);
+            for (int j = 0; j < tiles && ok; ++j)
+                ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
+            // A failed run: the MMAs issued so far end before TMEM is given back.
+            if (!ok && lane == 0)
+            {
+                mbar_init(&h.query, 1);
+                mbar_fence_init();
+                tc_commit(&h.query);
+                mbar_wait(&h.query, 0);
+            }
+            __syncwarp();
+        }
+    }
+    else if (warp < 12)
+    {
+        set_registers_up<Shape::kRegistersRows>();
+        const int group = (warp - 4) >> 2, quarter = warp & 3;
+        const int row = quarter * 32 + lane; // the TMEM lane
+        const uint32_t lanes = tmem + ((uint32_t) (quarter * 32) << 16);
+        const int token = p.token0 + row / a.group, head = p.kv_head * a.group + row % a.group;
+        const bool real = row < c.tile_tokens * a.group && token < p.length;
+
+        // The queries' halves, a row a warp: lane c the channels [8 c, 8 c + 8).
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i)
+        {
+            const int r = (warp - 4) * 16 + i, t = p.token0 + r / a.group;
+            float x[8] = {};
+            if (r < c.tile_tokens * a.group && t < p.length && lane * 8 < a.width)
+                load8((const float*) a.q + (p.begin + t) * a.q_stride + (size_t) (p.kv_head * a.group + r % a.group) * a.width
+                          + lane * 8, x);
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                m = fmaxf(m, finite_abs(x[e]));
+            const float factor = split_factor(warp_max(m), 15);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                split_pair(x[2 * e], x[2 * e + 1], factor, hi[e], lo[e]);
+            if (lane < D / 8)
+            {
+                uint8_t* to = queries + (lane >> 3) * 128 * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            if (lane == 0)
+                exchange[0][0][r] = 1.f / factor;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(&h.query);
+        unsigned long long path = 0;
+        if (Tree)
+            for (int i = tid - 128; i < p.length; i += 256)
+                h.parents[i] = a.parents[p.begin + i];
+        named_barrier(1, 256);
+        float row_factor = exchange[0][0][row] * a.scale_log2;
+        if (Tree && real)
+            path = tree_path(h.parents, token);
+        const float* kfactors = nullptr;
+        const float* vfactors = nullptr;
+        float kfactor = 1.f, vfactor = 1.f;
+        if (Tree)
+        {
+            named_barrier(2, 384); // the converters' sample
+            kfactor = 1.f / split_factor(__uint_as_float(h.sample[0]), 11);
+            vfactor = 1.f / split_factor(__uint_as_float(h.sample[1]), 11);
+        }
+        else
+        {
+            kfactors = lc.factors + (size_t) p.kv_head * lc.tiles + p.begin / kKeyTile + p.sequence;
+            vfactors = kfactors + (size_t) a.kv_heads * lc.tiles;
+        }
+        named_barrier(1, 256); // the row factors are read: `exchange` is free
+
+        float acc[kHalf];
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+            acc[i] = 0.f;
+        float m = -INFINITY, l = 0.f, alpha_before = 1.f, vfactor_before = 1.f;
+        int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
+        bool ok = true;
+        // After a wait that ran out the loop goes on without waits, so that the
+        // warps' barriers still match.
+        // acc = acc * alpha + (O of tile j) * factor
+        auto drain = [&](int j, float alpha, float factor) {
+            constexpr int RB = Shape::kRowBuffers;
+            const int buffer = j % RB, part = Shape::kParts == 2 ? group : 0;
+            ok = ok && warp_wait(&h.done[buffer][part], (j / RB) & 1);
+            tc_fence_after();
+            const uint32_t at = lanes + Shape::kRows + buffer * D + group * kHalf;
+            const bool scales = __any_sync(0xFFFFFFFFu, alpha != 1.f);
+#pragma unroll
+            for (int b = 0; b < kHalf; b += 16)
+            {
+                uint32_t o[16];
+                tc_ld16(at + b, o);
+                tc_wait_ld(o);
+                if (scales)
+                {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[b + i] *= alpha;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    acc[b + i] = fmaf(__uint_as_float(o[i]), factor, acc[b + i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0)
+                mbar_arrive(&h.free[buffer][part]);
+        };
+        for (int j = 0; j < tiles; ++j)
+        {
+            const int t = p.first_tile + j;
+            const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
+            if (!Tree)
+            {
+                kfactor = kfactors[j];
+                vfactor = vfactors[j];
+            }
+            ok = ok && warp_wait(&h.scores, j & 1);
+            tc_fence_after();
+            float s[32];
+#pragma unroll
+            for (int b = 0; b < 32; b += 16)
+            {
+                uint32_t large[16], small[16];
+                tc_ld16(lanes + Shape::kScores + group * 32 + b, large);
+                tc_ld16(lanes + Shape::kScores + 64 + group * 32 + b, small);
+                tc_wait_ld(large);
+                tc_wait_ld(small);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[b + i] = __uint_as_float(large[i]) + __uint_as_float(small[i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0)
+                mbar_arrive(&h.scores_read);
+            // What the row does not attend to.
+            if (Tree && t >= p.tiles_cached)
+            {
+                const uint32_t bits = (uint32_t) (path >> (32 * group));
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    s[i] = bits >> i & 1 ? s[i] : -INFINITY;
+            }
+            else
+            {
+                const int limit = (!Tree                        ? token - j * kKeyTile + 1
+                                   : page_there(id, a.pages) ? p.cached - t * kKeyTile
+                                                              : 0)
+                                  - 32 * group;
+                if (limit < 32)
+                {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        s[i] = i < limit ? s[i] : -INFINITY;
+                }
+            }
+            id = id_next;
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < 32; ++i)
+                top[i & 3] = fmaxf(top[i & 3], s[i]);
+            const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            exchange[j & 1][group][row] = mine;
+            named_barrier(1, 256);
+            const float factor = row_factor * kfactor;
+            const float m_new = fmaxf(m, fmaxf(mine, exchange[j & 1][group ^ 1][row]) * factor);
+            const float alpha = m == m_new ? 1.f : exp2_approx(m - m_new);
+            const float base = 14.f - (m_new == -INFINITY ? 0.f : m_new);
+            m = m_new;
+            float sum[4] = {};
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(factor, factor),
+                                            make_float2(base, base));
+                const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
+                sum[2 * (i & 1)] += e0;
+                sum[2 * (i & 1) + 1] += e1;
+                const __half2 hh = __floats2half2_rn(e0, e1);
+                const float2 back = __half22float2(hh);
+                hi[i] = *reinterpret_cast<const uint32_t*>(&hh);
+                lo[i] = pack_pair<__half>(e0 - back.x, e1 - back.y);
+            }
+            l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            // The MMAs that read this buffer two tiles back ended before S of this tile.
+            const uint32_t wbase = lanes + Shape::kWeights + (j & 1) * 64 + group * 16;
+            tc_st16(wbase, hi);
+            tc_st16(wbase + 32, lo);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0)
+                mbar_arrive(&h.weights[j & 1]);
+            if (j > 0)
+                drain(j - 1, alpha_before, vfactor_before);
+            alpha_before = alpha;
+            vfactor_before = vfactor;
+        }
+        drain(tiles - 1, alpha_before, vfactor_before);
+        exchange[tiles & 1][group][row] = l;
+        named_barrier(1, 256);
+        l += exchange[tiles & 1][group ^ 1][row];
+        const bool whole = !Tree || p.whole;
+        const int at = p.begin + token;
+        const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
+        // The weights' 2^14: cancels in a finished row, is taken off a chunk's.
+        const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 0x1p-14f;
+        bool finite = l < INFINITY && (!Tree || !h.misfit);
+        float* to = whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width : c.part_o + part * a.width;
+#pragma unroll
+        for (int b = 0; b < kHalf; b += 4)
+        {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                finite = finite && fabsf(acc[b + i]) < INFINITY;
+                x[i] = scaled == 0.f ? 0.f : acc[b + i] * scaled;
+            }
+            if (real && group * kHalf + b < a.width)
+                *reinterpret_cast<float4*>(to + group * kHalf + b) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        if (Tree && !whole && real && group == 0)
+            c.part_ml[part] = make_float2(m, l * 0x1p-14f);
+        exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
+        named_barrier(1, 256);
+        // Rows that came out not finite: again, half of them by each warpgroup's warp.
+        unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && (!finite || exchange[(tiles & 1) ^ 1][group ^ 1][row] != 0.f));
+        again &= group ? 0xAAAAAAAAu : 0x55555555u;
+        while (again)
+        {
+            const int who = __ffs(again) - 1;
+            again &= again - 1;
+            take_again<float, Tree>(c, h.place, __shfl_sync(0xFFFFFFFFu, at, who), __shfl_sync(0xFFFFFFFFu, head, who));
+        }
+        tc_fence_before();
+    }
+    else if (Tree)
+    {
+        set_registers_down<Shape::kRegistersConvert>();
+        const int t = tid - 384;
+        // The exponents: the largest of 16 keys spread over the CTA's, an eighth
+        // of their channels a thread.
+        {
+            const int end = min((p.first_tile + tiles) * kKeyTile, p.cached), from = p.first_tile * kKeyTile;
+            const int key = t >> 3;
+            const float* k = nullptr;
+            const float* v = nullptr;
+            if (end > from)
+            {
+                const int j = from + (int) ((long long) (end - from) * key / 16);
+                const int page = table[j >> kPageLog];
+                if (page_there(page, a.pages))
+                {
+                    const size_t at = (((size_t) page << kPageLog) + (j & (kPagePositions - 1))) * a.kv_heads + p.kv_head;
+                    k = (const float*) a.key_pages + at * a.width;
+                    v = (const float*) a.value_pages + at * a.width;
+                }
+            }
+            else
+            {
+                const int r = p.begin + p.length * key / 16;
+                k = (const float*) a.k + r * a.k_stride + (size_t) p.kv_head * a.width;
+                v = (const float*) a.v + r * a.v_stride + (size_t) p.kv_head * a.width;
+            }
+            float mk = 0.f, mv = 0.f;
+            for (int i = (t & 7) * 4; k && i < a.width; i += 32)
+            {
+                const float4 x = *reinterpret_cast<const float4*>(k + i), y = *reinterpret_cast<const float4*>(v + i);
+                mk = fmaxf(fmaxf(mk, fmaxf(finite_abs(x.x), finite_abs(x.y))), fmaxf(finite_abs(x.z), finite_abs(x.w)));
+                mv = fmaxf(fmaxf(mv, fmaxf(finite_abs(y.x), finite_abs(y.y))), fmaxf(finite_abs(y.z), finite_abs(y.w)));
+            }
+            mk = warp_max(mk), mv = warp_max(mv);
+            if (lane == 0)
+            {
+                atomicMax(&h.sample[0], __float_as_uint(mk));
+                atomicMax(&h.sample[1], __float_as_uint(mv));
+            }
+        }
+        named_barrier(2, 384); // with the row warps, who wait for the exponents
+        const float factors[2] = {split_factor(__uint_as_float(h.sample[0]), 11),
+                                  split_factor(__uint_as_float(h.sample[1]), 11)};
+        // A stage: thread t holds 32 channels (one fp32 box's row) of key t / 2.
+        const int key = t >> 1, box = t & 1;
+        int taken = 0;
+        bool misfit = false, ok = true;
+        auto convert = [&](int j, int values) {
+            const bool there = key < valid_of(j);
+            const float factor = factors[values];
+            for (int b = 0; b < kBlocks; ++b)
+            {
+                const int stage = taken % S;
+                ok = ok && warp_wait(&h.full[stage], (taken / S) & 1);
+                uint8_t* at = ring + stage * Shape::kStageBytes + key * 128;
+                uint32_t hi[16], lo[16];
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                {
+                    float4 x = *reinterpret_cast<const float4*>(at + box * Shape::kBox + ((i ^ (key & 7)) << 4));
+                    if (!there)
+                        x = make_float4(0.f, 0.f, 0.f, 0.f); // behind the sequence: whatever the page holds
+                    largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+                    split_pair(x.x, x.y, factor, hi[2 * i], lo[2 * i]);
+                    split_pair(x.z, x.w, factor, hi[2 * i + 1], lo[2 * i + 1]);
+                }
+                // Too large for fp16, or values so small that their halves lose digits.
+                largest *= factor;
+                misfit = misfit || largest > 60000.f || (values && largest > 0.f && largest < 0x1p-6f);
+                named_barrier(3, 128); // all of the stage's fp32 is in registers
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const int chunk = ((box * 4 + i) ^ (key & 7)) << 4;
+                    *reinterpret_cast<uint4*>(at + chunk) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+                    *reinterpret_cast<uint4*>(at + Shape::kBox + chunk) =
+                        make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+                }
+                if (misfit)
+                    h.misfit = 1;
+                fence_proxy_async();
+                __syncwarp();
+                if (ok && lane == 0)
+                    mbar_arrive(&h.ready[stage]);
+                ++taken;
+            }
+        };
+        for (int j = 0; j <= tiles; ++j)
+        {
+            if (j < tiles)
+                convert(j, 0);
+            if (j > 0)
+                convert(j - 1, 1);
+        }
+    }
+    __syncthreads();
+    if (warp == 1)
+        tc_dealloc(tmem, 512);
+}
+} // namespace hfk

@@ -159,11 +159,79 @@ __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequen
     }
 }
 
+// Where CTA blockIdx.x works, its rows in steps of `step` tokens; by a whole warp.
+template <bool Tree>
+__device__ inline MmaPlace find_place(const MmaCall& c, int step)
+{
+    const AttnCall& a = c.a;
+    MmaPlace p = {};
+    p.sequence = -1;
+    if (Tree)
+    {
+        int u = blockIdx.x;
+        p.chunk = u % c.chunks, u /= c.chunks;
+        p.kv_head = u % a.kv_heads, u /= a.kv_heads;
+        p.token0 = u % c.row_tiles * step;
+        const int s = u / c.row_tiles;
+        p.begin = bounded_offset(a.offsets, s, a.rows);
+        p.length = min(bounded_offset(a.offsets, s + 1, a.rows) - p.begin, a.max_nodes);
+        p.cached = min(max(a.lengths[s], 0), a.max_length);
+        p.tiles_cached = (p.cached + kKeyTile - 1) / kKeyTile;
+        p.first_tile = p.chunk * c.chunk_tiles;
+        p.tiles = min(c.chunk_tiles, p.tiles_cached + 1 - p.first_tile); // + 1: the drafted tile
+        p.whole = p.tiles_cached < c.chunk_tiles;
+        if (p.token0 < p.length && p.tiles > 0)
+            p.sequence = s;
+    }
+    else
+    {
+        int s, tile = 0;
+        p.kv_head = blockIdx.x % a.kv_heads;
+        find_tile(a, step, blockIdx.x / a.kv_heads, s, tile);
+        if (s >= 0)
+        {
+            p.sequence = s;
+            p.begin = bounded_offset(a.offsets, s, a.rows);
+            p.length = bounded_offset(a.offsets, s + 1, a.rows) - p.begin;
+            p.token0 = tile * step;
+            p.tiles = (min(p.token0 + step, p.length) - 1) / kKeyTile + 1;
+            p.whole = true;
+        }
+    }
+    return p;
+}
+
+// A row that came out not finite, by a whole warp: the same keys again, read
+// only where the row attends to them.
+template <typename T, bool Tree>
+__device__ __noinline__ void take_again(const MmaCall& c, const MmaPlace& p, int row, int head)
+{
+    const AttnCall& a = c.a;
+    if (!Tree || p.whole)
+    {
+        attention_row<T, Tree>(a, p.sequence, p.begin, row, head);
+        return;
+    }
+    const int at = (threadIdx.x & 31) * 8;
+    const RowKeys keys = row_keys<Tree>(a, p.sequence, p.begin, row);
+    const int from = p.first_tile * kKeyTile, end = p.first_tile + p.tiles;
+    const int to = end > p.tiles_cached ? keys.cached + keys.drafted : end * kKeyTile;
+    float q[8] = {}, acc[8], m, l;
+    if (at < a.width)
+        load8((const T*) a.q + row * a.q_stride + (size_t) head * a.width + at, q);
+    attend_row<T, Tree>(a, keys, p.kv_head, q, from, to, m, l, acc);
+    const size_t part = ((size_t) p.chunk * a.rows + row) * a.heads + head;
+    if (at < a.width)
+        store8(c.part_o + part * a.width + at, acc);
+    if (at == 0)
+        c.part_ml[part] = make_float2(m, l);
+}
+
 template <typename T, int D, int NQ, bool Tree>
 __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kCtas)
     attention_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap kpages,
-                  const __grid_constant__ CUtensorMap vpages, const MmaCall c)
+                  const __grid_constant__ CUtensorMap vpages, const __grid_constant__ MmaCall c)
 {
     using Shape = MmaShape<D, NQ>;
     constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks, B = Shape::kBuffers;
@@ -178,41 +246,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 
     if (warp == 0)
     {
-        MmaPlace p = {};
-        p.sequence = -1;
-        const int step = c.tile_tokens * NQ;
-        if (Tree)
-        {
-            int u = blockIdx.x;
-            p.chunk = u % c.chunks, u /= c.chunks;
-            p.kv_head = u % a.kv_heads, u /= a.kv_heads;
-            p.token0 = u % c.row_tiles * step;
-            const int s = u / c.row_tiles;
-            p.begin = bounded_offset(a.offsets, s, a.rows);
-            p.length = min(bounded_offset(a.offsets, s + 1, a.rows) - p.begin, a.max_nodes);
-            p.cached = min(max(a.lengths[s], 0), a.max_length);
-            p.tiles_cached = (p.cached + kKeyTile - 1) / kKeyTile;
-            p.first_tile = p.chunk * c.chunk_tiles;
-            p.tiles = min(c.chunk_tiles, p.tiles_cached + 1 - p.first_tile); // + 1: the drafted tile
-            p.whole = p.tiles_cached < c.chunk_tiles;
-            if (p.token0 < p.length && p.tiles > 0)
-                p.sequence = s;
-        }
-        else
-        {
-            int s, tile = 0;
-            p.kv_head = blockIdx.x % a.kv_heads;
-            find_tile(a, step, blockIdx.x / a.kv_heads, s, tile);
-            if (s >= 0)
-            {
-                p.sequence = s;
-                p.begin = bounded_offset(a.offsets, s, a.rows);
-                p.length = bounded_offset(a.offsets, s + 1, a.rows) - p.begin;
-                p.token0 = tile * step;
-                p.tiles = (min(p.token0 + step, p.length) - 1) / kKeyTile + 1;
-                p.whole = true;
-            }
-        }
+        const MmaPlace p = find_place<Tree>(c, c.tile_tokens * NQ);
         if (lane == 0)
             h.place = p;
     }
@@ -573,24 +607,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 const int who = __ffs(again) - 1;
                 again &= again - 1;
                 const int at1 = __shfl_sync(0xFFFFFFFFu, at, who), head1 = __shfl_sync(0xFFFFFFFFu, head, who);
-                if (whole)
-                    attention_row<T, Tree>(a, p.sequence, p.begin, at1, head1);
-                else
-                {
-                    const RowKeys keys = row_keys<Tree>(a, p.sequence, p.begin, at1);
-                    const int from = p.first_tile * kKeyTile;
-                    const bool last = p.first_tile + tiles > p.tiles_cached;
-                    const int to = last ? keys.cached + keys.drafted : (p.first_tile + tiles) * kKeyTile;
-                    float x[8] = {}, acc[8], m1, l1;
-                    if (lane * 8 < a.width)
-                        load8((const T*) a.q + at1 * a.q_stride + (size_t) head1 * a.width + lane * 8, x);
-                    attend_row<T, Tree>(a, keys, p.kv_head, x, from, to, m1, l1, acc);
-                    const size_t part1 = ((size_t) p.chunk * a.rows + at1) * a.heads + head1;
-                    if (lane * 8 < a.width)
-                        store8(c.part_o + part1 * a.width + lane * 8, acc);
-                    if (lane == 0)
-                        c.part_ml[part1] = make_float2(m1, l1);
-                }
+                take_again<T, Tree>(c, h.place, at1, head1);
             }
         }
         tc_fence_before();
@@ -603,7 +620,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 // Joins a tree's chunks: a warp a (row, head), lane c the channels [8 c, 8 c + 8).
 // Rows of one chunk are finished already.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join(const MmaCall c)
+__global__ void __launch_bounds__(256) attention_join(const __grid_constant__ MmaCall c)
 {
     pdl_wait();
     const AttnCall& a = c.a;

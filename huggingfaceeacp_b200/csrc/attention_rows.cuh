@@ -251,23 +251,4 @@ __device__ void attention_row(const AttnCall& a, int s, int begin, int row, int 
     if (c < a.width)
         store8((T*) a.out + row * a.out_stride + (size_t) h * a.width + c, acc);
 }
-
-// One warp a (row, head).
-template <typename T, bool Tree>
-__global__ void __launch_bounds__(256) attention_rows(const AttnCall a)
-{
-    pdl_wait();
-    pdl_trigger();
-    const long long unit = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int row = (int) (unit / a.heads), h = (int) (unit % a.heads);
-    if (row >= a.rows)
-        return;
-    const int s = sequence_of(a.offsets, a.sequences, a.rows, row);
-    if (s < 0)
-        return;
-    const int begin = bounded_offset(a.offsets, s, a.rows);
-    if (Tree && row - begin >= a.max_nodes)
-        return;
-    attention_row<T, Tree>(a, s, begin, row, h);
-}
 } // namespace hfk

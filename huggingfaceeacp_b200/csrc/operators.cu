@@ -3,6 +3,7 @@
 // state: every check is made on the host before the first launch.
 #include <hf_cuda.h>
 
+#include "attention_limbs.cuh"
 #include "attention_mma.cuh"
 #include "attention_rows.cuh"
 #include "launch.cuh"
@@ -219,18 +220,23 @@ EncodeTiled encoder()
     return (EncodeTiled) f;
 }
 
-// [rows][heads][width] 16-bit elements, rows `stride` elements apart, in boxes of
-// 64 channels x box_heads x box_rows with the 128-byte swizzle; zeros outside.
+// [rows][heads][width] elements, rows `stride` elements apart, in boxes of 128
+// bytes of channels x box_heads x box_rows with the 128-byte swizzle; zeros
+// outside.
 bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int heads, int64_t rows, int64_t stride,
                  int box_heads, int box_rows)
 {
     const EncodeTiled encode = encoder();
+    const int size = size_of(dtype);
+    const CUtensorMapDataType type = dtype == HF_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dtype == HF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const cuuint64_t dims[3] = {(cuuint64_t) width, (cuuint64_t) heads, (cuuint64_t) rows};
-    const cuuint64_t strides[2] = {(cuuint64_t) width * 2, (cuuint64_t) stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t) box_heads, (cuuint32_t) box_rows}, ones[3] = {1, 1, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t) width * size, (cuuint64_t) stride * size};
+    const cuuint32_t box[3] = {(cuuint32_t) (128 / size), (cuuint32_t) box_heads, (cuuint32_t) box_rows};
+    const cuuint32_t ones[3] = {1, 1, 1};
     return encode
-           && encode(map, dtype == HF_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                     const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           && encode(map, type, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                   == CUDA_SUCCESS;
@@ -248,12 +254,12 @@ struct TreePlan
     int row_tiles, chunk_tiles, chunks;
 };
 
-TreePlan tree_plan(int sequences, int heads, int kv_heads, int width, int max_nodes, int max_length)
+TreePlan tree_plan(int dtype, int sequences, int heads, int kv_heads, int width, int max_nodes, int max_length)
 {
     const int tokens = 128 / (heads / kv_heads);
     const int row_tiles = (max_nodes + tokens - 1) / tokens;
     const int tiles = (max_length + kKeyTile - 1) / kKeyTile + 1;
-    const int64_t units = (int64_t) sequences * kv_heads * row_tiles, places = kSms * (width <= 128 ? 2 : 1);
+    const int64_t units = (int64_t) sequences * kv_heads * row_tiles, places = kSms * (dtype != HF_DTYPE_F32 && width <= 128 ? 2 : 1);
     const int64_t wanted = std::min<int64_t>((3 * places + units - 1) / units, (tiles + 3) / 4);
     const int chunk_tiles = (int) ((tiles + wanted - 1) / std::max<int64_t>(wanted, 1));
     return {row_tiles, chunk_tiles, (tiles + chunk_tiles - 1) / chunk_tiles};
@@ -309,19 +315,31 @@ int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
                    : launch_mma<T, 64, 1, false>(maps, c, ctas, device, stream);
 }
 
+// A tree's call and its CTAs.
+int64_t tree_call(MmaCall* c, const AttnCall& a, const TreePlan& plan, void* workspace)
+{
+    c->a = a;
+    c->tile_tokens = 128 / a.group;
+    c->row_tiles = plan.row_tiles;
+    c->chunk_tiles = plan.chunk_tiles;
+    c->chunks = plan.chunks;
+    c->part_o = (float*) workspace;
+    c->part_ml = (float2*) (c->part_o + (size_t) plan.chunks * a.rows * a.heads * a.width);
+    return (int64_t) a.sequences * a.kv_heads * plan.row_tiles * plan.chunks;
+}
+
+template <typename T>
+int join(const MmaCall& c, cudaStream_t stream)
+{
+    const dim3 grid((unsigned) (((int64_t) c.a.rows * c.a.heads + 7) / 8));
+    return status_of(launch(true, attention_join<T>, grid, dim3(256), 0, stream, c));
+}
+
 template <typename T>
 int tree_mma(int dtype, const AttnCall& a, const TreePlan& plan, void* workspace, int device, cudaStream_t stream)
 {
     MmaCall c = {};
-    c.a = a;
-    c.tile_tokens = 128 / a.group;
-    c.row_tiles = plan.row_tiles;
-    c.chunk_tiles = plan.chunk_tiles;
-    c.chunks = plan.chunks;
-    const uint64_t parts = (uint64_t) plan.chunks * a.rows * a.heads;
-    c.part_o = (float*) workspace;
-    c.part_ml = (float2*) (c.part_o + parts * a.width);
-    const int64_t ctas = (int64_t) a.sequences * a.kv_heads * plan.row_tiles * plan.chunks;
+    const int64_t ctas = tree_call(&c, a, plan, workspace);
     CUtensorMap maps[5] = {};
     const int64_t positions = (int64_t) a.pages * kPagePositions;
     if (ctas > INT32_MAX)
@@ -335,21 +353,85 @@ int tree_mma(int dtype, const AttnCall& a, const TreePlan& plan, void* workspace
     const int rc = a.width > 128  ? launch_mma<T, 256, 1, true>(maps, c, ctas, device, stream)
                    : a.width > 64 ? launch_mma<T, 128, 1, true>(maps, c, ctas, device, stream)
                                   : launch_mma<T, 64, 1, true>(maps, c, ctas, device, stream);
-    if (rc || plan.chunks == 1)
-        return rc;
-    const dim3 grid((unsigned) (((int64_t) a.rows * a.heads + 7) / 8));
-    return status_of(launch(true, attention_join<T>, grid, dim3(256), 0, stream, c));
+    return rc || plan.chunks == 1 ? rc : join<T>(c, stream);
 }
 
-template <bool Tree>
-int run_rows(int dtype, const AttnCall& a, cudaStream_t stream)
+// ---- attention_limbs (fp32) --------------------------------------------------------
+// A prompt's workspace: the halves of K and V, then the tiles' factors.
+int limb_tiles(int rows, int sequences)
 {
-    const long long units = (long long) a.rows * a.heads;
-    const dim3 grid((unsigned) ((units + 7) / 8));
-    cudaError_t e = dtype == HF_DTYPE_F32    ? launch(false, attention_rows<float, Tree>, grid, dim3(256), 0, stream, a)
-                    : dtype == HF_DTYPE_BF16 ? launch(false, attention_rows<__nv_bfloat16, Tree>, grid, dim3(256), 0, stream, a)
-                                             : launch(false, attention_rows<__half, Tree>, grid, dim3(256), 0, stream, a);
-    return status_of(e);
+    return rows / kKeyTile + sequences;
+}
+
+uint64_t limb_bytes(int rows, int sequences, int kv_heads, int width)
+{
+    return 8 * (uint64_t) rows * kv_heads * width + 8 * (uint64_t) kv_heads * limb_tiles(rows, sequences);
+}
+
+template <int D, bool Tree>
+int launch_limbs(const CUtensorMap (&maps)[4], const LimbCall& l, int64_t ctas, int device, cudaStream_t stream)
+{
+    using Shape = LimbShape<D, Tree>;
+    const auto kernel = attention_limbs<D, Tree>;
+    static std::atomic<uint64_t> ready {0}; // devices whose kernel has its shared memory
+    const uint64_t bit = 1ull << (device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit))
+    {
+        // The warpgroups' register shares assume this count at launch.
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, kernel) != cudaSuccess || f.numRegs != Shape::kLaunchRegisters
+            || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess)
+            return HF_E_CUDA;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return status_of(launch(!Tree, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
+                            maps[1], maps[2], maps[3], l));
+}
+
+int packed_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t stream)
+{
+    LimbCall l = {};
+    l.c.a = a;
+    l.c.tile_tokens = 128 / a.group;
+    l.c.chunks = 1;
+    l.limbs = (__half*) workspace;
+    l.tiles = limb_tiles(a.rows, a.sequences);
+    const size_t limb = (size_t) a.rows * a.kv_heads * a.width;
+    l.factors = (float*) (l.limbs + 4 * limb);
+    const int64_t ctas = ((int64_t) a.rows / l.c.tile_tokens + a.sequences) * a.kv_heads;
+    if (ctas > INT32_MAX || a.kv_heads > 65535)
+        return HF_E_SHAPE;
+    CUtensorMap maps[4] = {};
+    const int limb_of[4] = {0, 2, 1, 3}; // K hi, V hi, K lo, V lo
+    for (int i = 0; i < 4; ++i)
+        if (!encode_rows(&maps[i], HF_DTYPE_F16, l.limbs + limb_of[i] * limb, a.width, a.kv_heads, a.rows,
+                         (int64_t) a.kv_heads * a.width, 1, kKeyTile))
+            return HF_E_CUDA;
+    if (launch(false, split_tiles, dim3(l.tiles, a.kv_heads, 2), dim3(256), 0, stream, l) != cudaSuccess)
+        return HF_E_CUDA;
+    return a.width > 128  ? launch_limbs<256, false>(maps, l, ctas, device, stream)
+           : a.width > 64 ? launch_limbs<128, false>(maps, l, ctas, device, stream)
+                          : launch_limbs<64, false>(maps, l, ctas, device, stream);
+}
+
+int tree_limbs(const AttnCall& a, const TreePlan& plan, void* workspace, int device, cudaStream_t stream)
+{
+    LimbCall l = {};
+    MmaCall& c = l.c;
+    const int64_t ctas = tree_call(&c, a, plan, workspace);
+    if (ctas > INT32_MAX)
+        return HF_E_SHAPE;
+    CUtensorMap maps[4] = {};
+    const int64_t positions = (int64_t) a.pages * kPagePositions, kvw = (int64_t) a.kv_heads * a.width;
+    if (!encode_rows(&maps[0], HF_DTYPE_F32, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kKeyTile)
+        || !encode_rows(&maps[1], HF_DTYPE_F32, a.v, a.width, a.kv_heads, a.rows, a.v_stride, 1, kKeyTile)
+        || !encode_rows(&maps[2], HF_DTYPE_F32, a.key_pages, a.width, a.kv_heads, positions, kvw, 1, kKeyTile)
+        || !encode_rows(&maps[3], HF_DTYPE_F32, a.value_pages, a.width, a.kv_heads, positions, kvw, 1, kKeyTile))
+        return HF_E_CUDA;
+    const int rc = a.width > 128  ? launch_limbs<256, true>(maps, l, ctas, device, stream)
+                   : a.width > 64 ? launch_limbs<128, true>(maps, l, ctas, device, stream)
+                                  : launch_limbs<64, true>(maps, l, ctas, device, stream);
+    return rc || plan.chunks == 1 ? rc : join<float>(c, stream);
 }
 
 int check_packed_sizes(const hf_attention_packed* call)
@@ -372,11 +454,14 @@ int check_tree_sizes(const hf_page_cache* cache, hf_page_cache* c, const hf_atte
     return HF_OK;
 }
 
+uint64_t packed_workspace(const hf_attention_packed& call)
+{
+    return call.dtype == HF_DTYPE_F32 ? limb_bytes(call.rows, call.sequences, call.kv_heads, call.head_width) : 0;
+}
+
 uint64_t tree_workspace(const hf_page_cache& c, const hf_attention_tree& call)
 {
-    if (c.dtype == HF_DTYPE_F32)
-        return 0;
-    const TreePlan plan = tree_plan(c.sequences, call.heads, call.kv_heads, call.head_width, call.max_nodes, call.max_length);
+    const TreePlan plan = tree_plan(c.dtype, c.sequences, call.heads, call.kv_heads, call.head_width, call.max_nodes, call.max_length);
     return part_bytes(plan, call.rows, call.heads, call.head_width);
 }
 } // namespace
@@ -505,7 +590,10 @@ int hf_cuda_attention_packed_workspace(const hf_attention_packed* call, uint64_t
     if (!bytes)
         return HF_E_INVALID;
     *bytes = 0;
-    return check_packed_sizes(call);
+    if (const int rc = check_packed_sizes(call))
+        return rc;
+    *bytes = packed_workspace(*call);
+    return HF_OK;
 }
 
 int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
@@ -516,14 +604,19 @@ int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
     if (const int rc = check_rows(*call, size_of(call->dtype), call->heads, call->kv_heads, call->head_width, &a))
         return rc;
     a.sequences = call->sequences;
+    const uint64_t bytes = packed_workspace(*call);
+    if (bytes && !aligned(call->workspace))
+        return HF_E_INVALID;
+    if (call->workspace_bytes < bytes)
+        return HF_E_CAPACITY;
     const DeviceOf on(a.q);
     if (on.status)
         return on.status;
-    if (!on.holds(a.k, a.v, a.out, a.offsets))
+    if (!on.holds(bytes ? call->workspace : nullptr, a.k, a.v, a.out, a.offsets))
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
     if (call->dtype == HF_DTYPE_F32)
-        return run_rows<false>(call->dtype, a, st);
+        return packed_limbs(a, call->workspace, on.current, st);
     return call->dtype == HF_DTYPE_BF16 ? packed_mma<__nv_bfloat16>(call->dtype, a, on.current, st)
                                         : packed_mma<__half>(call->dtype, a, on.current, st);
 }
@@ -561,7 +654,7 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
     a.table_stride = c.table_stride;
     a.max_nodes = call->max_nodes;
     a.max_length = std::min(call->max_length, c.table_stride * kPagePositions);
-    const TreePlan plan = tree_plan(c.sequences, a.heads, a.kv_heads, a.width, a.max_nodes, call->max_length);
+    const TreePlan plan = tree_plan(c.dtype, c.sequences, a.heads, a.kv_heads, a.width, a.max_nodes, call->max_length);
     const uint64_t bytes = tree_workspace(c, *call);
     if (bytes && !aligned(call->workspace))
         return HF_E_INVALID;
@@ -574,7 +667,7 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
     if (c.dtype == HF_DTYPE_F32)
-        return run_rows<true>(c.dtype, a, st);
+        return tree_limbs(a, plan, call->workspace, on.current, st);
     return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, plan, call->workspace, on.current, st)
                                     : tree_mma<__half>(c.dtype, a, plan, call->workspace, on.current, st);
 }
