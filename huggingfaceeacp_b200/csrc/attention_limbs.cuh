@@ -185,7 +185,7 @@ struct LimbShape
 
 struct LimbHead
 {
-    uint64_t full[12], ready[12], empty[12], query, scores, scores_read, weights[2], done[2][2], free[2][2];
+    uint64_t full[12], ready[12], empty[12], query, scores, scores_read, weights[2], done[2][2], free[2][2], drained;
     uint32_t tmem;
     int misfit;              // a tree's value outside the sampled exponent's range
     unsigned sample[2];      // its largest K and V, as bits
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
     uint8_t* ring = queries + 2 * Shape::kQueryHalf;
     const MmaCall& c = lc.c;
     const AttnCall& a = c.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
     if (warp == 0)
     {
@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         }
         mbar_init(&h.query, 8); // an arrival a row warp
         mbar_init(&h.scores, 1);
+        mbar_init(&h.drained, 1);
         mbar_init(&h.scores_read, 8);
         for (int b = 0; b < 2; ++b)
         {
@@ -364,23 +365,18 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     if (!warp_wait(&landed[stage], (taken / S) & 1))
                         return false;
                     tc_fence_after();
-                    if (lane == 0)
-                    {
-                        const uint32_t k = rbase + stage * Shape::kStageBytes;
+                    const uint32_t k = rbase + stage * Shape::kStageBytes;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                        {
-                            const uint32_t at = b * 128 * 128 + i * 32;
-                            tc_mma(tmem + Shape::kScores, tc_desc(qhi + at), tc_desc(k + i * 32), kWide, b > 0 || i > 0);
-                            tc_mma(tmem + Shape::kScores + 64, tc_desc(qlo + at), tc_desc(k + i * 32), kNarrow, 1);
-                        }
-                        tc_commit(&h.empty[stage]);
-                        if (b == kBlocks - 1)
-                            tc_commit(&h.scores);
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        const uint32_t at = b * 128 * 128 + i * 32;
+                        tc_mma_warp(tmem + Shape::kScores, tc_desc(qhi + at), tc_desc(k + i * 32), kWide, b > 0 || i > 0);
+                        tc_mma_warp(tmem + Shape::kScores + 64, tc_desc(qlo + at), tc_desc(k + i * 32), kNarrow, 1);
                     }
+                    tc_commit_warp(&h.empty[stage]);
                     ++taken;
-                    __syncwarp();
                 }
+                tc_commit_warp(&h.scores);
                 return true;
             };
             auto rows = [&](int j) {
@@ -408,26 +404,22 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     if (j >= RB && !warp_wait(&h.free[buffer][part], (j / RB - 1) & 1))
                         return false;
                     tc_fence_after();
-                    if (lane == 0)
-                    {
-                        const uint32_t d = tmem + Shape::kRows + buffer * D + part * Shape::kPart;
-                        const uint32_t hi = tmem + Shape::kWeights + (j & 1) * 64, lo = hi + 32;
-                        const uint32_t v = rbase + stage * Shape::kStageBytes;
+                    const uint32_t d = tmem + Shape::kRows + buffer * D + part * Shape::kPart;
+                    const uint32_t hi = tmem + Shape::kWeights + (j & 1) * 64, lo = hi + 32;
+                    const uint32_t v = rbase + stage * Shape::kStageBytes;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc_mma_ts(d, hi + i * 8, tc_desc_mn(v + Shape::kBox + i * 2048, Shape::kStageBytes), kValues, i > 0);
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma_ts_warp(d, hi + i * 8, tc_desc_mn(v + Shape::kBox + i * 2048, Shape::kStageBytes), kValues, i > 0);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc_mma_ts(d, lo + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma_ts_warp(d, lo + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc_mma_ts(d, hi + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
-                        for (int e = 0; e < kEach; ++e)
-                            tc_commit(&h.empty[stage + e]);
-                        tc_commit(&h.done[buffer][part]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma_ts_warp(d, hi + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
+                    for (int e = 0; e < kEach; ++e)
+                        tc_commit_warp(&h.empty[stage + e]);
+                    tc_commit_warp(&h.done[buffer][part]);
                     taken += kEach;
-                    __syncwarp();
                 }
                 return true;
             };
@@ -437,14 +429,11 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             for (int j = 0; j < tiles && ok; ++j)
                 ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
             // A failed run: the MMAs issued so far end before TMEM is given back.
-            if (!ok && lane == 0)
+            if (!ok)
             {
-                mbar_init(&h.query, 1);
-                mbar_fence_init();
-                tc_commit(&h.query);
-                mbar_wait(&h.query, 0);
+                tc_commit_warp(&h.drained);
+                mbar_wait(&h.drained, 0);
             }
-            __syncwarp();
         }
     }
     else if (warp < 12)

@@ -90,7 +90,7 @@ struct MmaPlace
 
 struct MmaHead
 {
-    uint64_t full[12], empty[12], query, scores[2][4], weights[2][4], done[2][4];
+    uint64_t full[12], empty[12], query, scores[2][4], weights[2][4], done[2][4], drained[2];
     uint32_t tmem;
     MmaPlace place;
     int parents[kTreeNodes];
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
     uint8_t* queries = smem + Shape::kHead;
     uint8_t* ring = queries + Shape::kQueryBytes;
     const AttnCall& a = c.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
     if (warp == 0)
     {
@@ -259,9 +259,11 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         for (int s = 0; s < S; ++s)
         {
             mbar_init(&h.full[s], 1);
-            mbar_init(&h.empty[s], 1);
+            mbar_init(&h.empty[s], NQ); // an arrival an MMA warp
         }
         mbar_init(&h.query, 1);
+        for (int q = 0; q < NQ; ++q)
+            mbar_init(&h.drained[q], 1);
         for (int q = 0; q < NQ; ++q)
             for (int b = 0; b < B; ++b)
             {
@@ -349,100 +351,79 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         }
         __syncwarp();
     }
-    else if (warp == 1)
+    else if (warp <= NQ)
     {
+        const int q = warp - 1;
         constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false), kRows = tc_idesc16(kType, D, true);
-        const uint32_t qbase = smem_addr(queries), rbase = smem_addr(ring);
-        int n[NQ];
-        for (int q = 0; q < NQ; ++q)
-            n[q] = tiles_of(q);
+        const uint32_t qbase = smem_addr(queries) + q * Shape::kQueryBytes / NQ, rbase = smem_addr(ring);
+        const uint32_t sbase = tmem + q * B * kKeyTile, obase = tmem + Shape::kScoreColumns + q * D;
+        const int n = tiles_of(q);
         int taken = 0;
-        bool ok = warp_wait(&h.query, 0);
         // S of tile j, from the stage that is next in the ring.
         auto scores = [&](int j) {
             const int stage = taken % S;
             if (!warp_wait(&h.full[stage], (taken / S) & 1))
                 return false;
-            for (int q = 0; q < NQ; ++q)
+            if (j < n)
             {
-                if (j >= n[q])
-                    continue;
                 // The buffer's last weights (tile j - B) have been read.
                 if (j >= B && !warp_wait(&h.done[q][j % B], (j / B - 1) & 1))
                     return false;
                 tc_fence_after();
-                if (lane == 0)
-                {
-                    const uint32_t d = tmem + (q * B + j % B) * kKeyTile;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                    {
-                        const uint64_t qa = tc_desc(qbase + (q * kBlocks + i / 4) * 128 * 128 + (i & 3) * 32);
-                        const uint64_t kb = tc_desc(rbase + stage * Shape::kStageBytes + i / 4 * Shape::kBox + (i & 3) * 32);
-                        tc_mma(d, qa, kb, kScores, i > 0);
-                    }
-                    tc_commit(&h.scores[q][j % B]);
-                }
-                __syncwarp();
+                for (int i = 0; i < D / 16; ++i)
+                    tc_mma_warp(sbase + j % B * kKeyTile, tc_desc(qbase + i / 4 * 128 * 128 + (i & 3) * 32),
+                                tc_desc(rbase + stage * Shape::kStageBytes + i / 4 * Shape::kBox + (i & 3) * 32), kScores,
+                                i > 0);
+                tc_commit_warp(&h.scores[q][j % B]);
             }
-            if (lane == 0)
-                tc_commit(&h.empty[stage]);
+            tc_commit_warp(&h.empty[stage]);
             ++taken;
-            __syncwarp();
             return true;
         };
         auto rows = [&](int j) {
             const int stage = taken % S;
             if (!warp_wait(&h.full[stage], (taken / S) & 1))
                 return false;
-            const int t = p.first_tile + j;
-            const int valid = !Tree                 ? p.length - j * kKeyTile
-                              : t < p.tiles_cached ? p.cached - t * kKeyTile
-                                                    : p.length;
-            if (valid < kKeyTile)
+            if (j < n)
             {
-                const int bytes = (kKeyTile - valid) * 128;
-                for (int b = 0; b < kBlocks; ++b)
-                    for (int i = lane * 16; i < bytes; i += 512)
-                        *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128 + i) =
-                            make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
-                __syncwarp();
-            }
-            for (int q = 0; q < NQ; ++q)
-            {
-                if (j >= n[q])
-                    continue;
+                const int t = p.first_tile + j;
+                const int valid = !Tree                 ? p.length - j * kKeyTile
+                                  : t < p.tiles_cached ? p.cached - t * kKeyTile
+                                                        : p.length;
+                if (valid < kKeyTile) // by each MMA warp for its own MMAs
+                {
+                    const int bytes = (kKeyTile - valid) * 128;
+                    for (int b = 0; b < kBlocks; ++b)
+                        for (int i = lane * 16; i < bytes; i += 512)
+                            *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128
+                                                      + i) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
                 if (!warp_wait(&h.weights[q][j % B], (j / B) & 1))
                     return false;
                 tc_fence_after();
-                if (lane == 0)
-                {
-                    const uint32_t d = tmem + Shape::kScoreColumns + q * D, pa = tmem + (q * B + j % B) * kKeyTile;
 #pragma unroll
-                    for (int i = 0; i < kKeyTile / 16; ++i)
-                        tc_mma_ts(d, pa + i * 8, tc_desc_mn(rbase + stage * Shape::kStageBytes + i * 2048, Shape::kBox),
-                                  kRows, j > 0 || i > 0);
-                    tc_commit(&h.done[q][j % B]);
-                }
-                __syncwarp();
+                for (int i = 0; i < kKeyTile / 16; ++i)
+                    tc_mma_ts_warp(obase, sbase + j % B * kKeyTile + i * 8,
+                                   tc_desc_mn(rbase + stage * Shape::kStageBytes + i * 2048, Shape::kBox), kRows,
+                                   j > 0 || i > 0);
+                tc_commit_warp(&h.done[q][j % B]);
             }
-            if (lane == 0)
-                tc_commit(&h.empty[stage]);
+            tc_commit_warp(&h.empty[stage]);
             ++taken;
-            __syncwarp();
             return true;
         };
-        ok = ok && scores(0);
+        bool ok = warp_wait(&h.query, 0) && scores(0);
         for (int j = 0; j < tiles && ok; ++j)
             ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
         // A failed run: the MMAs issued so far end before TMEM is given back.
-        if (!ok && lane == 0)
+        if (!ok)
         {
-            tc_commit(&h.query);
-            mbar_wait(&h.query, 1);
+            tc_commit_warp(&h.drained[q]);
+            mbar_wait(&h.drained[q], 0);
         }
-        __syncwarp();
     }
     else if (warp >= 4)
     {

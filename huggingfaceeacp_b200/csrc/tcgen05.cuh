@@ -130,6 +130,33 @@ __host__ __device__ constexpr uint32_t tc_idesc16(int type, int n, bool b_mn)
            | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (kTcRows >> 4) << 24);
 }
 
+// MMAs and commits by a whole warp, which elects the thread that issues them:
+// without a branch around them the compiler keeps the descriptors in uniform
+// registers. The elected thread is the same each time.
+__device__ __forceinline__ void tc_mma_warp(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n .reg .pred p, e;\n .reg .b32 r;\n setp.ne.b32 p, %4, 0;\n elect.sync r|e, 0xFFFFFFFF;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_ts_warp(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                               uint32_t accumulate)
+{
+    asm volatile("{\n .reg .pred p, e;\n .reg .b32 r;\n setp.ne.b32 p, %4, 0;\n elect.sync r|e, 0xFFFFFFFF;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tc_commit_warp(uint64_t* bar)
+{
+    asm volatile("{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xFFFFFFFF;\n"
+                 " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns, as tc_ld16 and tc_st16.
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r)
 {
