@@ -356,14 +356,17 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             uint64_t* landed = Tree ? h.ready : h.full;
             int taken = 0;
             auto scores = [&](int j) {
-                // S of tile j - 1 is in registers.
-                if (j > 0 && !warp_wait(&h.scores_read, (j - 1) & 1))
-                    return false;
                 for (int b = 0; b < kBlocks; ++b)
                 {
                     const int stage = taken % S;
-                    if (!warp_wait(&landed[stage], (taken / S) & 1))
-                        return false;
+                    if ((b & 1) == 0)
+                    {
+                        // This block and the next, and S of tile j - 1 in registers.
+                        const bool reads = (lane & 2) && b == 0 && j > 0;
+                        if (!warp_wait(reads ? &h.scores_read : &landed[kBlocks == 1 ? stage : stage + (lane & 1)],
+                                       (reads ? j - 1 : taken / S) & 1))
+                            return false;
+                    }
                     tc_fence_after();
                     const uint32_t k = rbase + stage * Shape::kStageBytes;
 #pragma unroll
@@ -380,16 +383,19 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 return true;
             };
             auto rows = [&](int j) {
-                if (!warp_wait(&h.weights[j & 1], (j / 2) & 1))
-                    return false;
                 constexpr int RB = Shape::kRowBuffers, kEach = kBlocks / Shape::kParts; // stages a part
                 const int valid = valid_of(j), buffer = j % RB;
                 for (int part = 0; part < Shape::kParts; ++part)
                 {
                     const int stage = taken % S;
-                    for (int e = 0; e < kEach; ++e)
-                        if (!warp_wait(&landed[stage + e], (taken / S) & 1))
-                            return false;
+                    // The part's stages, the weights, and the part's last O in registers.
+                    const int what = lane & 3;
+                    const bool frees = what == 3 && j >= RB, weighs = what == 2 && part == 0;
+                    if (!warp_wait(frees    ? &h.free[buffer][part]
+                                   : weighs ? &h.weights[j & 1]
+                                            : &landed[stage + (what & (kEach - 1))],
+                                   (frees ? j / RB - 1 : weighs ? j / 2 : taken / S) & 1))
+                        return false;
                     if (!Tree && valid < kKeyTile)
                     {
                         // Rows past the sequence's end: weights of 0, but 0 x NaN is not.
@@ -401,8 +407,6 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    if (j >= RB && !warp_wait(&h.free[buffer][part], (j / RB - 1) & 1))
-                        return false;
                     tc_fence_after();
                     const uint32_t d = tmem + Shape::kRows + buffer * D + part * Shape::kPart;
                     const uint32_t hi = tmem + Shape::kWeights + (j & 1) * 64, lo = hi + 32;

@@ -12,12 +12,14 @@
 // Roles (one warp each, and one warpgroup a query tile):
 //  warp 0   copies: query tiles once, then key and value tiles through a ring,
 //           in the order the MMAs use them (tensor maps; a page is one box);
-//  warp 1   MMAs: S of the next tile is issued before O of this one, so the
-//           tensor core has work while the softmax runs. S has two buffers a
-//           query tile;
-//  warpgroups 1 ..  softmax, a thread a row (its TMEM lane): the tile's scores
-//           to registers, maximum, weights, the weights in T back over the
-//           scores (P, the A operand of O += P V), at the end the row itself.
+//  warps 1, 2  MMAs, a query tile each (one warp for both spent 1930 cycles a
+//           step, most of it in its waits, 60 to 80 cycles for a barrier that is
+//           ready): S of the next tile is issued before O of this one, as soon
+//           as S of this one is in registers;
+//  warpgroups 1, 2  softmax, a thread a row (its TMEM lane): the tile's scores
+//           to registers, maximum, weights, the weights in T back to TMEM in
+//           one of two buffers (P, the A operand of O += P V), at the end the
+//           row itself.
 // The maximum that the weights are taken against follows the true one lazily:
 // only when it would rise by more than 8 (weights up to 2^8) is O scaled in
 // TMEM, which after the first tiles is rare. Weights are rounded to T for the
@@ -57,6 +59,54 @@ struct MmaCall
     float2* part_ml;  // [chunks][rows][heads]
 };
 
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the
+// addition of 1.5 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by the
+// polynomial of least largest relative error (Remez exchange; 7.5e-5 at degree
+// 3, 2.6e-6 at degree 4), n added to the exponent. Below 2^-126 it returns about
+// that, where exp2_approx gives 0.
+template <int Degree>
+__device__ __forceinline__ float2 exp2_poly(float2 x)
+{
+    constexpr float kMagic = 12582912.f;
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 t = __fadd2_rn(x, make_float2(kMagic, kMagic));
+    const float2 n = __fadd2_rn(t, make_float2(-kMagic, -kMagic));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    constexpr float c3[] = {0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f};
+    constexpr float c4[] = {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f,
+                            0.009570102207362652f};
+    const float* c = Degree == 3 ? c3 : c4;
+    float2 p = make_float2(c[Degree], c[Degree]);
+#pragma unroll
+    for (int i = Degree - 1; i >= 0; --i)
+        p = __ffma2_rn(p, f, make_float2(c[i], c[i]));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// The tile's 64 scores of a row to weights 2^(s scale + base), packed in T, and
+// their sum. The special-function unit makes 16 values of 2^x a cycle and SM,
+// which at head width 128 takes as long as the MMAs; of a tile without masked
+// scores (`Mixed`) kPoly of 8 pairs go to the FMA pipe instead.
+template <typename T, bool Mixed>
+__device__ __forceinline__ float weigh(const float* s, float scale, float base, uint32_t* w)
+{
+    constexpr int kPoly = 3, kDegree = std::is_same<T, __nv_bfloat16>::value ? 3 : 4;
+    float2 sum[2] = {};
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+    {
+        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale),
+                                    make_float2(base, base));
+        const float2 e = Mixed && i % 8 * kPoly % 8 < kPoly ? exp2_poly<kDegree>(x)
+                                                           : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+        sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+        w[i] = pack_pair<T>(e.x, e.y);
+    }
+    return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+}
+
 template <int D, int NQ>
 struct MmaShape
 {
@@ -64,8 +114,7 @@ struct MmaShape
     static constexpr int kQueryBytes = NQ * 128 * D * 2;
     static constexpr int kStageBytes = kKeyTile * D * 2;   // one K or V tile
     static constexpr int kBox = kKeyTile * 128;            // one block of it
-    static constexpr int kBuffers = D == 256 ? 4 : 2;      // of scores, a query tile
-    static constexpr int kScoreColumns = NQ * kBuffers * kKeyTile;
+    static constexpr int kScoreColumns = NQ * 2 * kKeyTile; // a query tile's scores and two buffers of weights
     static constexpr int kTmem = kScoreColumns + NQ * D <= 256 ? 256 : 512;
     static constexpr int kCtas = kTmem == 256 ? 2 : 1;     // a SM
     static constexpr int kHead = 1024;                     // barriers and the tile's place
@@ -90,13 +139,14 @@ struct MmaPlace
 
 struct MmaHead
 {
-    uint64_t full[12], empty[12], query, scores[2][4], weights[2][4], done[2][4], drained[2];
+    uint64_t full[12], empty[12], query, scores[2], scores_read[2], weights[2][2], done[2][2], drained[2];
     uint32_t tmem;
     MmaPlace place;
     int parents[kTreeNodes];
 };
 
-// Bounded waits, of a warp together and of one thread.
+// Bounded waits, of a warp together and of one thread. A warp's lanes may name
+// different barriers: it goes on when all have come, for the price of one.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity)
 {
     if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)))
@@ -234,7 +284,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                   const __grid_constant__ CUtensorMap vpages, const __grid_constant__ MmaCall c)
 {
     using Shape = MmaShape<D, NQ>;
-    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks, B = Shape::kBuffers;
+    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks;
     constexpr int kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ __align__(1024) uint8_t smem[];
     MmaHead& h = *reinterpret_cast<MmaHead*>(smem);
@@ -263,11 +313,14 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         }
         mbar_init(&h.query, 1);
         for (int q = 0; q < NQ; ++q)
+        {
             mbar_init(&h.drained[q], 1);
+            mbar_init(&h.scores[q], 1);
+            mbar_init(&h.scores_read[q], 4); // an arrival a warp
+        }
         for (int q = 0; q < NQ; ++q)
-            for (int b = 0; b < B; ++b)
+            for (int b = 0; b < 2; ++b)
             {
-                mbar_init(&h.scores[q][b], 1);
                 mbar_init(&h.weights[q][b], 4); // an arrival a warp
                 mbar_init(&h.done[q][b], 1);
             }
@@ -356,26 +409,24 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         const int q = warp - 1;
         constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false), kRows = tc_idesc16(kType, D, true);
         const uint32_t qbase = smem_addr(queries) + q * Shape::kQueryBytes / NQ, rbase = smem_addr(ring);
-        const uint32_t sbase = tmem + q * B * kKeyTile, obase = tmem + Shape::kScoreColumns + q * D;
+        const uint32_t sbase = tmem + q * 2 * kKeyTile, obase = tmem + Shape::kScoreColumns + q * D;
         const int n = tiles_of(q);
         int taken = 0;
         // S of tile j, from the stage that is next in the ring.
         auto scores = [&](int j) {
             const int stage = taken % S;
-            if (!warp_wait(&h.full[stage], (taken / S) & 1))
+            const bool reads = (lane & 1) && j > 0 && j < n; // S of tile j - 1 is in registers
+            if (!warp_wait(reads ? &h.scores_read[q] : &h.full[stage], (reads ? j - 1 : taken / S) & 1))
                 return false;
             if (j < n)
             {
-                // The buffer's last weights (tile j - B) have been read.
-                if (j >= B && !warp_wait(&h.done[q][j % B], (j / B - 1) & 1))
-                    return false;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
-                    tc_mma_warp(sbase + j % B * kKeyTile, tc_desc(qbase + i / 4 * 128 * 128 + (i & 3) * 32),
+                    tc_mma_warp(sbase, tc_desc(qbase + i / 4 * 128 * 128 + (i & 3) * 32),
                                 tc_desc(rbase + stage * Shape::kStageBytes + i / 4 * Shape::kBox + (i & 3) * 32), kScores,
                                 i > 0);
-                tc_commit_warp(&h.scores[q][j % B]);
+                tc_commit_warp(&h.scores[q]);
             }
             tc_commit_warp(&h.empty[stage]);
             ++taken;
@@ -383,7 +434,8 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         };
         auto rows = [&](int j) {
             const int stage = taken % S;
-            if (!warp_wait(&h.full[stage], (taken / S) & 1))
+            const bool weighs = (lane & 1) && j < n;
+            if (!warp_wait(weighs ? &h.weights[q][j & 1] : &h.full[stage], (weighs ? j / 2 : taken / S) & 1))
                 return false;
             if (j < n)
             {
@@ -401,15 +453,13 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                     fence_proxy_async();
                     __syncwarp();
                 }
-                if (!warp_wait(&h.weights[q][j % B], (j / B) & 1))
-                    return false;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < kKeyTile / 16; ++i)
-                    tc_mma_ts_warp(obase, sbase + j % B * kKeyTile + i * 8,
+                    tc_mma_ts_warp(obase, sbase + kKeyTile + (j & 1) * 32 + i * 8,
                                    tc_desc_mn(rbase + stage * Shape::kStageBytes + i * 2048, Shape::kBox), kRows,
                                    j > 0 || i > 0);
-                tc_commit_warp(&h.done[q][j % B]);
+                tc_commit_warp(&h.done[q][j & 1]);
             }
             tc_commit_warp(&h.empty[stage]);
             ++taken;
@@ -430,7 +480,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         const int q = (warp - 4) >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane; // the TMEM lane
         const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
-        const uint32_t obase = tmem + lanes + Shape::kScoreColumns + q * D;
+        const uint32_t obase = tmem + lanes + Shape::kScoreColumns + q * D, sbase = tmem + lanes + q * 2 * kKeyTile;
         const int n = tiles_of(q);
         const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
         const bool real = row < c.tile_tokens * a.group && token < p.length;
@@ -452,8 +502,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         {
             const int t = p.first_tile + j;
             const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
-            const uint32_t sbase = tmem + lanes + (q * B + j % B) * kKeyTile;
-            if (!warp_wait(&h.scores[q][j % B], (j / B) & 1))
+            if (!warp_wait(&h.scores[q], j & 1))
             {
                 ok = false;
                 break;
@@ -464,8 +513,13 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             tc_ld32(sbase + 32, r + 32);
             tc_wait_ld32(r);
             tc_wait_ld32(r + 32);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&h.scores_read[q]);
             float* s = reinterpret_cast<float*>(r);
             // What the row does not attend to.
+            bool masked = true;
             if (Tree && t >= p.tiles_cached)
             {
 #pragma unroll
@@ -477,7 +531,8 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 const int limit = !Tree                        ? token - j * kKeyTile + 1
                                   : page_there(id, a.pages) ? p.cached - t * kKeyTile
                                                              : 0;
-                if (limit < kKeyTile)
+                masked = __any_sync(0xFFFFFFFFu, limit < kKeyTile);
+                if (masked)
                 {
 #pragma unroll
                     for (int i = 0; i < 64; ++i)
@@ -498,7 +553,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 if (__any_sync(0xFFFFFFFFu, rises))
                 {
                     // O of tile j - 1 is complete before it is scaled.
-                    if (!warp_wait(&h.done[q][(j - 1) % B], ((j - 1) / B) & 1))
+                    if (!warp_wait(&h.done[q][(j - 1) & 1], ((j - 1) / 2) & 1))
                     {
                         ok = false;
                         break;
@@ -521,28 +576,19 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 }
             }
             const float base = m == -INFINITY ? 0.f : -m;
-            float sum[4] = {};
             uint32_t w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-            {
-                const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(scale, scale),
-                                            make_float2(base, base));
-                const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
-                sum[2 * (i & 1)] += e0;
-                sum[2 * (i & 1) + 1] += e1;
-                w[i] = pack_pair<T>(e0, e1);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc_st32(sbase, w);
+            l += masked ? weigh<T, false>(s, scale, base, w) : weigh<T, true>(s, scale, base, w);
+            // The MMAs that read this buffer two tiles back were issued before
+            // S of this tile, whose commit covers them.
+            tc_st32(sbase + kKeyTile + (j & 1) * 32, w);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(&h.weights[q][j % B]);
+                mbar_arrive(&h.weights[q][j & 1]);
         }
         if (ok && n > 0)
-            ok = warp_wait(&h.done[q][(n - 1) % B], ((n - 1) / B) & 1);
+            ok = warp_wait(&h.done[q][(n - 1) & 1], ((n - 1) / 2) & 1);
         if (n > 0)
         {
             tc_fence_after();
