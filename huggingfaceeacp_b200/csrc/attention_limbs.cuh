@@ -204,11 +204,6 @@ __device__ __forceinline__ void set_registers_down()
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-__device__ __forceinline__ void named_barrier(int id, int threads)
-{
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 template <int D, bool Tree>
 __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
     attention_limbs(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -230,7 +225,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
 
     if (warp == 0)
     {
-        const MmaPlace p = find_place<Tree>(c, c.tile_tokens);
+        const MmaPlace p = find_place<Tree>(c, c.tile_tokens, blockIdx.x);
         if (lane == 0)
         {
             h.place = p;
@@ -484,7 +479,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         if (Tree)
             for (int i = tid - 128; i < p.length; i += 256)
                 h.parents[i] = a.parents[p.begin + i];
-        named_barrier(1, 256);
+        named_sync(1, 256);
         float row_factor = exchange[0][0][row] * a.scale_log2;
         if (Tree && real)
             path = tree_path(h.parents, token);
@@ -493,7 +488,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         float kfactor = 1.f, vfactor = 1.f;
         if (Tree)
         {
-            named_barrier(2, 384); // the converters' sample
+            named_sync(2, 384); // the converters' sample
             kfactor = 1.f / split_factor(__uint_as_float(h.sample[0]), 11);
             vfactor = 1.f / split_factor(__uint_as_float(h.sample[1]), 11);
         }
@@ -502,7 +497,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             kfactors = lc.factors + (size_t) p.kv_head * lc.tiles + p.begin / kKeyTile + p.sequence;
             vfactors = kfactors + (size_t) a.kv_heads * lc.tiles;
         }
-        named_barrier(1, 256); // the row factors are read: `exchange` is free
+        named_sync(1, 256); // the row factors are read: `exchange` is free
 
         float acc[kHalf];
 #pragma unroll
@@ -598,7 +593,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 top[i & 3] = fmaxf(top[i & 3], s[i]);
             const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             exchange[j & 1][group][row] = mine;
-            named_barrier(1, 256);
+            named_sync(1, 256);
             const float factor = row_factor * kfactor;
             const float m_new = fmaxf(m, fmaxf(mine, exchange[j & 1][group ^ 1][row]) * factor);
             const float alpha = m == m_new ? 1.f : exp2_approx(m - m_new);
@@ -636,7 +631,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         }
         drain(tiles - 1, alpha_before, vfactor_before);
         exchange[tiles & 1][group][row] = l;
-        named_barrier(1, 256);
+        named_sync(1, 256);
         l += exchange[tiles & 1][group ^ 1][row];
         const bool whole = !Tree || p.whole;
         const int at = p.begin + token;
@@ -661,7 +656,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         if (Tree && !whole && real && group == 0)
             c.part_ml[part] = make_float2(m, l * 0x1p-14f);
         exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
-        named_barrier(1, 256);
+        named_sync(1, 256);
         // Rows that came out not finite: again, half of them by each warpgroup's warp.
         unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && (!finite || exchange[(tiles & 1) ^ 1][group ^ 1][row] != 0.f));
         again &= group ? 0xAAAAAAAAu : 0x55555555u;
@@ -715,7 +710,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 atomicMax(&h.sample[1], __float_as_uint(mv));
             }
         }
-        named_barrier(2, 384); // with the row warps, who wait for the exponents
+        named_sync(2, 384); // with the row warps, who wait for the exponents
         const float factors[2] = {split_factor(__uint_as_float(h.sample[0]), 11),
                                   split_factor(__uint_as_float(h.sample[1]), 11)};
         // A stage: thread t holds 32 channels (one fp32 box's row) of key t / 2.
@@ -745,7 +740,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 // Too large for fp16, or values so small that their halves lose digits.
                 largest *= factor;
                 misfit = misfit || largest > 60000.f || (values && largest > 0.f && largest < 0x1p-6f);
-                named_barrier(3, 128); // all of the stage's fp32 is in registers
+                named_sync(3, 128); // all of the stage's fp32 is in registers
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                 {

@@ -9,17 +9,21 @@
 // a few tokens wide. A CTA takes NQ query tiles of one kv head, over the same
 // keys, in tiles of 64 (a page).
 //
-// Roles (one warp each, and one warpgroup a query tile):
-//  warp 0   copies: query tiles once, then key and value tiles through a ring,
-//           in the order the MMAs use them (tensor maps; a page is one box);
-//  warps 1, 2  MMAs, a query tile each (one warp for both spent 1930 cycles a
-//           step, most of it in its waits, 60 to 80 cycles for a barrier that is
-//           ready): S of the next tile is issued before O of this one, as soon
-//           as S of this one is in registers;
-//  warpgroups 1, 2  softmax, a thread a row (its TMEM lane): the tile's scores
-//           to registers, maximum, weights, the weights in T back to TMEM in
-//           one of two buffers (P, the A operand of O += P V), at the end the
-//           row itself.
+// Roles:
+//  warp 0   places and copies: query tiles, then key and value tiles through a
+//           ring, in the order the MMAs use them (tensor maps; a page is one
+//           box), on into the next unit as far as there is room;
+//  MMAs     a warp for each query tile's S and one for its O, since a warp's
+//           waits and MMAs follow one another: S of the next tile is issued as
+//           soon as S of this one is in registers, O of a tile as soon as its
+//           weights are in TMEM;
+//  softmax  a warpgroup a query tile, a thread a row (its TMEM lane): the tile's
+//           scores to registers, maximum, weights, the weights in T back to TMEM
+//           in one of two buffers (P, the A operand of O += P V), at the end
+//           the row itself.
+// A CTA takes unit after unit: it cancels the launch of a CTA that has not
+// started and does its work (the order stays the grid's, longest rows first), so
+// that the next unit's copies and scores run under this one's last steps.
 // The maximum that the weights are taken against follows the true one lazily:
 // only when it would rise by more than 8 (weights up to 2^8) is O scaled in
 // TMEM, which after the first tiles is rare. Weights are rounded to T for the
@@ -117,32 +121,35 @@ struct MmaShape
     static constexpr int kScoreColumns = NQ * 2 * kKeyTile; // a query tile's scores and two buffers of weights
     static constexpr int kTmem = kScoreColumns + NQ * D <= 256 ? 256 : 512;
     static constexpr int kCtas = kTmem == 256 ? 2 : 1;     // a SM
-    static constexpr int kHead = 1024;                     // barriers and the tile's place
+    static constexpr int kHead = 2048;                     // barriers, places
     static constexpr int kBudget = kCtas == 2 ? 113 * 1024 : 227 * 1024;
     static constexpr int kStagesFit = (kBudget - kHead - kQueryBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
     static constexpr int kSmem = kHead + kQueryBytes + kStages * kStageBytes;
-    static constexpr int kThreads = 128 + 128 * NQ;
+    static constexpr int kThreads = 128 + 128 * NQ + (NQ == 2 ? 32 : 0); // the last warp: MMAs
     static_assert(kScoreColumns + NQ * D <= kTmem && kStages >= 4, "what an SM holds");
 };
 
-// The CTA's place, found once by warp 0.
+// A unit's place.
 struct MmaPlace
 {
-    int sequence; // -1: nothing to do
+    int sequence; // -1: nothing to do; published: no more units
     int begin, length; // its first row, its rows (a tree's nodes)
     int token0, kv_head, chunk;
     int cached, tiles_cached; // a tree's
-    int first_tile, tiles;    // the CTA's key tiles
+    int first_tile, tiles;    // its key tiles
     bool whole;               // the only chunk: finish the rows
 };
 
 struct MmaHead
 {
-    uint64_t full[12], empty[12], query, scores[2], scores_read[2], weights[2][2], done[2][2], drained[2];
+    uint64_t full[12], empty[12], query, query_free, scores[2], scores_read[2], weights[2][2], done[2][2], rows_free[2],
+        place_full[2], place_free[2], next, drained[4];
+    alignas(16) uint4 answer;
     uint32_t tmem;
-    MmaPlace place;
-    int parents[kTreeNodes];
+    int dead; // a wait ran out
+    MmaPlace place[2];
+    int parents[2][kTreeNodes];
 };
 
 // Bounded waits, of a warp together and of one thread. A warp's lanes may name
@@ -164,9 +171,11 @@ __device__ __forceinline__ bool thread_wait(uint64_t* bar, unsigned parity)
 
 // The sequences' tiles of `step` tokens in descending order of their place (the
 // longest rows of keys first), equal places in the sequences' order: unit r of
-// them, by a whole warp.
+// them, by a whole warp. A lane keeps the tile counts of its sequences (lane, lane
+// + 32, ...) in registers; past kKnown of them it reads the offsets again.
 __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequence, int& tile)
 {
+    constexpr int kKnown = 4;
     const int lane = threadIdx.x & 31;
     auto tiles_of = [&](int s) {
         if (s >= a.sequences)
@@ -174,13 +183,22 @@ __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequen
         const int n = bounded_offset(a.offsets, s + 1, a.rows) - bounded_offset(a.offsets, s, a.rows);
         return n > 0 ? (n + step - 1) / step : 0;
     };
+    int known[kKnown], most = 0;
+#pragma unroll
+    for (int i = 0; i < kKnown; ++i)
+        most = max(most, known[i] = tiles_of(lane + 32 * i));
+    for (int s = lane + 32 * kKnown; s < a.sequences; s += 32)
+        most = max(most, tiles_of(s));
     auto from = [&](int t) { // tiles whose place is t or above
         int sum = 0;
-        for (int s = lane; s < a.sequences; s += 32)
+#pragma unroll
+        for (int i = 0; i < kKnown; ++i)
+            sum += max(known[i] - t, 0);
+        for (int s = lane + 32 * kKnown; s < a.sequences; s += 32)
             sum += max(tiles_of(s) - t, 0);
         return __reduce_add_sync(0xFFFFFFFFu, sum);
     };
-    int low = 0, high = (a.rows + step - 1) / step; // from(low) > r >= from(high)
+    int low = 0, high = __reduce_max_sync(0xFFFFFFFFu, most); // from(low) > r >= from(high)
     sequence = -1;
     if (from(0) <= r)
         return;
@@ -194,31 +212,33 @@ __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequen
     }
     tile = low;
     int skip = r - from(low + 1);
-    for (int base = 0; base < a.sequences; base += 32)
+    for (int i = 0; 32 * i < a.sequences; ++i)
     {
-        unsigned has = __ballot_sync(0xFFFFFFFFu, tiles_of(base + lane) > low);
+        const int mine = i == 0 ? known[0] : i == 1 ? known[1] : i == 2 ? known[2] : i == 3 ? known[3] : tiles_of(lane + 32 * i);
+        unsigned has = __ballot_sync(0xFFFFFFFFu, mine > low);
         const int n = __popc(has);
         if (skip < n)
         {
             while (skip--)
                 has &= has - 1;
-            sequence = base + __ffs(has) - 1;
+            sequence = 32 * i + __ffs(has) - 1;
             return;
         }
         skip -= n;
     }
 }
 
-// Where CTA blockIdx.x works, its rows in steps of `step` tokens; by a whole warp.
+// Where unit `unit` (a CTA of the grid) works, its rows in steps of `step` tokens;
+// by a whole warp.
 template <bool Tree>
-__device__ inline MmaPlace find_place(const MmaCall& c, int step)
+__device__ inline MmaPlace find_place(const MmaCall& c, int step, int unit)
 {
     const AttnCall& a = c.a;
     MmaPlace p = {};
     p.sequence = -1;
     if (Tree)
     {
-        int u = blockIdx.x;
+        int u = unit;
         p.chunk = u % c.chunks, u /= c.chunks;
         p.kv_head = u % a.kv_heads, u /= a.kv_heads;
         p.token0 = u % c.row_tiles * step;
@@ -236,8 +256,8 @@ __device__ inline MmaPlace find_place(const MmaCall& c, int step)
     else
     {
         int s, tile = 0;
-        p.kv_head = blockIdx.x % a.kv_heads;
-        find_tile(a, step, blockIdx.x / a.kv_heads, s, tile);
+        p.kv_head = unit % a.kv_heads;
+        find_tile(a, step, unit / a.kv_heads, s, tile);
         if (s >= 0)
         {
             p.sequence = s;
@@ -277,6 +297,59 @@ __device__ __noinline__ void take_again(const MmaCall& c, const MmaPlace& p, int
         c.part_ml[part] = make_float2(m, l);
 }
 
+__device__ __forceinline__ void named_sync(int id, int threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// A failed run: the MMAs that the warp has issued end before TMEM is given back.
+__device__ __forceinline__ void finish_mmas(bool ok, uint64_t* bar)
+{
+    if (!ok)
+    {
+        tc_commit_warp(bar);
+        mbar_wait(bar, 0);
+    }
+}
+
+// Four lanes' 64 bytes each (four rows, 16 registers a lane as chunks of 4) to four
+// chunks of 64 bytes a row: lane i of the four ends with chunk i of rows 0 to 3,
+// so that a store of chunk k writes 64 consecutive bytes of a row.
+__device__ __forceinline__ void turn4(uint32_t (&r)[16])
+{
+    const int lane = threadIdx.x & 3;
+#pragma unroll
+    for (int bit = 1; bit <= 2; bit <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+        {
+            if (c & bit)
+                continue;
+            const bool upper = lane & bit;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                uint32_t& low = r[4 * c + i];
+                uint32_t& high = r[4 * (c | bit) + i];
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, upper ? low : high, bit);
+                (upper ? low : high) = got;
+            }
+        }
+}
+
+// The 16 registers (64 bytes) of each lane's row to `to` + 64 bytes * block, the
+// lanes' rows where `real`, bytes from `end` on left out. `rows`: four lanes' pointers.
+__device__ __forceinline__ void store_rows(uint32_t (&r)[16], char* const (&rows)[4], unsigned real, int at, int end)
+{
+    turn4(r);
+    const int lane = threadIdx.x & 31;
+    at += (lane & 3) * 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (real >> ((lane & ~3) + k) & 1 && at < end)
+            *reinterpret_cast<uint4*>(rows[k] + at) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+}
+
 template <typename T, int D, int NQ, bool Tree>
 __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kCtas)
     attention_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -285,7 +358,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 {
     using Shape = MmaShape<D, NQ>;
     constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks;
-    constexpr int kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ __align__(1024) uint8_t smem[];
     MmaHead& h = *reinterpret_cast<MmaHead*>(smem);
     static_assert(sizeof(MmaHead) <= Shape::kHead, "the head's room");
@@ -294,17 +367,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
     const AttnCall& a = c.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
-    if (warp == 0)
-    {
-        const MmaPlace p = find_place<Tree>(c, c.tile_tokens * NQ);
-        if (lane == 0)
-            h.place = p;
-    }
-    else if (warp == 1)
-    {
-        tc_alloc(&h.tmem, Shape::kTmem);
-    }
-    else if (warp == 2 && lane == 0)
+    if (warp == 0 && lane == 0)
     {
         for (int s = 0; s < S; ++s)
         {
@@ -312,330 +375,449 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             mbar_init(&h.empty[s], NQ); // an arrival an MMA warp
         }
         mbar_init(&h.query, 1);
-        for (int q = 0; q < NQ; ++q)
+        mbar_init(&h.query_free, NQ);
+        mbar_init(&h.next, 1);
+        for (int b = 0; b < 2; ++b)
         {
-            mbar_init(&h.drained[q], 1);
-            mbar_init(&h.scores[q], 1);
-            mbar_init(&h.scores_read[q], 4); // an arrival a warp
+            mbar_init(&h.place_full[b], 1);
+            mbar_init(&h.place_free[b], 6 * NQ); // an arrival a warp but the first
         }
         for (int q = 0; q < NQ; ++q)
+        {
+            mbar_init(&h.scores[q], 1);
+            mbar_init(&h.scores_read[q], 4); // an arrival a warp
+            mbar_init(&h.rows_free[q], 4);
+            mbar_init(&h.drained[q], 1);
+            mbar_init(&h.drained[2 + q], 1);
             for (int b = 0; b < 2; ++b)
             {
-                mbar_init(&h.weights[q][b], 4); // an arrival a warp
+                mbar_init(&h.weights[q][b], 4);
                 mbar_init(&h.done[q][b], 1);
             }
+        }
+        h.dead = 0;
         mbar_fence_init();
+    }
+    else if (warp == 1)
+        tc_alloc(&h.tmem, Shape::kTmem);
+    else if (warp == 2 && lane == 0)
+    {
+        prefetch_map(&qmap);
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
+        if (Tree)
+        {
+            prefetch_map(&kpages);
+            prefetch_map(&vpages);
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (Tree)
         pdl_trigger(); // attention_join may take its place; it waits for this grid's end
-    const MmaPlace p = h.place;
     const uint32_t tmem = h.tmem;
-    if (p.sequence < 0)
-    {
-        if (warp == 1)
-            tc_dealloc(tmem, Shape::kTmem);
-        return;
-    }
     // Key tiles of query tile q: a prompt's tile ends with its last token's.
-    auto tiles_of = [&](int q) {
+    auto tiles_of = [&](const MmaPlace& p, int q) {
         const int t0 = p.token0 + q * c.tile_tokens;
         if (t0 >= p.length)
             return 0;
         return Tree ? p.tiles : (min(t0 + c.tile_tokens, p.length) - 1) / kKeyTile + 1;
     };
-    const int tiles = p.tiles;
-    const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+    // A wait of one of the roles; one that runs out ends the CTA's other waits too.
+    auto wait = [&](uint64_t* bar, unsigned parity) {
+        const bool ok = warp_wait(bar, parity);
+        if (!ok)
+            *(volatile int*) &h.dead = 1;
+        return ok;
+    };
+    // The place of the CTA's i-th unit: false when there is none.
+    auto take = [&](int i, MmaPlace& p) {
+        if (__any_sync(0xFFFFFFFFu, *(volatile int*) &h.dead) || !wait(&h.place_full[i & 1], (i / 2) & 1))
+            return false;
+        p = h.place[i & 1];
+        return p.sequence >= 0;
+    };
+    auto leave = [&](int i) {
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(&h.place_free[i & 1]);
+    };
 
     if (warp == 0)
     {
-        int put = 0, ids = -1;
+        int put = 0, unit = blockIdx.x, i = 0;
         bool ok = true;
+        auto one_wait = [&](uint64_t* bar, unsigned parity) {
+            if (ok && !thread_wait(bar, parity))
+            {
+                *(volatile int*) &h.dead = 1;
+                ok = false;
+            }
+            return ok;
+        };
+        for (int asked = 0; ok; ++asked)
+        {
+            if (lane == 0)
+                ask_next_cta(&h.answer, &h.next);
+            const MmaPlace p = find_place<Tree>(c, c.tile_tokens * NQ, unit);
+            if (p.sequence >= 0)
+            {
+                if (lane == 0 && (i < 2 || one_wait(&h.place_free[i & 1], (i / 2 - 1) & 1)))
+                {
+                    h.place[i & 1] = p;
+                    mbar_arrive(&h.place_full[i & 1]);
+                }
+                const int tiles = p.tiles;
+                const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+                auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id) {
+                    const int stage = put % S;
+                    if (!ok || (put >= S && !one_wait(&h.empty[stage], (put / S - 1) & 1)))
+                        return;
+                    const bool cached = Tree && p.first_tile + j < p.tiles_cached;
+                    // A page that is not there is read past the pool's end: zeros.
+                    const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                           : p.begin + (Tree ? 0 : j * kKeyTile);
+                    mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
+                    for (int b = 0; b < kBlocks; ++b)
+                        tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
+                                    p.kv_head, row, &h.full[stage]);
+                    ++put;
+                };
+                int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
+                for (int j = 0; j <= tiles; ++j)
+                {
+                    int id = -1;
+                    if (Tree)
+                    {
+                        if ((j & 31) == 0)
+                        {
+                            const int t = p.first_tile + j + lane;
+                            ids = t < p.tiles_cached ? table[t] : -1;
+                        }
+                        id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
+                    }
+                    if (lane == 0)
+                    {
+                        if (j < tiles)
+                            load(j, &kmap, &kpages, id);
+                        if (j == 0 && ok && (i == 0 || one_wait(&h.query_free, (i - 1) & 1)))
+                        {
+                            mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
+                            for (int b = 0; b < NQ * kBlocks; ++b)
+                                tensor_load(queries + b * 128 * 128, &qmap, 64 * (b % kBlocks), p.kv_head * a.group,
+                                            p.begin + p.token0 + b / kBlocks * c.tile_tokens, &h.query);
+                        }
+                        if (j > 0)
+                            load(j - 1, &vmap, &vpages, id_before);
+                    }
+                    id_before = id;
+                    __syncwarp();
+                }
+                ++i;
+            }
+            ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+            ok = wait(&h.next, asked & 1) && ok; // an answer is never left behind
+            if (ok && !next_cta(&h.answer, unit))
+                break;
+            __syncwarp(); // the answer has been read
+        }
         if (lane == 0)
         {
-            mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
-            for (int q = 0; q < NQ; ++q)
-                for (int b = 0; b < kBlocks; ++b)
-                    tensor_load(queries + (q * kBlocks + b) * 128 * 128, &qmap, 64 * b, p.kv_head * a.group,
-                                p.begin + p.token0 + q * c.tile_tokens, &h.query);
-        }
-        auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id) {
-            const int stage = put % S;
-            if (put >= S && !thread_wait(&h.empty[stage], (put / S - 1) & 1))
-                return false;
-            const int t = p.first_tile + j;
-            const bool cached = Tree && t < p.tiles_cached;
-            // A page that is not there is read past the pool's end: zeros.
-            const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
-                                   : p.begin + (Tree ? 0 : j * kKeyTile);
-            mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
-            for (int b = 0; b < kBlocks; ++b)
-                tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
-                            p.kv_head, row, &h.full[stage]);
-            ++put;
-            return true;
-        };
-        int id_before = -1; // tile j - 1's page
-        for (int j = 0; j <= tiles; ++j)
-        {
-            int id = -1;
-            if (Tree)
+            if (ok && (i < 2 || one_wait(&h.place_free[i & 1], (i / 2 - 1) & 1)))
             {
-                if ((j & 31) == 0)
-                {
-                    const int t = p.first_tile + j + lane;
-                    ids = t < p.tiles_cached ? table[t] : -1;
-                }
-                id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
+                h.place[i & 1].sequence = -1; // no more units
+                mbar_arrive(&h.place_full[i & 1]);
             }
-            if (lane == 0 && ok)
-                ok = (j == tiles || load(j, &kmap, &kpages, id)) && (j == 0 || load(j - 1, &vmap, &vpages, id_before));
-            id_before = id;
-            __syncwarp();
-        }
-        // Every copy has landed before the CTA may end (only a failed run gets here early).
-        if (lane == 0 && !ok)
-        {
-            mbar_wait(&h.query, 0);
-            for (int i = max(0, put - S); i < put; ++i)
-                mbar_wait(&h.full[i % S], (i / S) & 1);
+            // Every copy has landed before the CTA may end (only a failed run gets here early).
+            if (!ok)
+            {
+                mbar_wait(&h.query, 0);
+                for (int n = max(0, put - S); n < put; ++n)
+                    mbar_wait(&h.full[n % S], (n / S) & 1);
+            }
         }
         __syncwarp();
     }
     else if (warp <= NQ)
     {
+        // S of query tile q: K(j) is item 2 j - 1 of a unit's in the ring, the first item 0.
         const int q = warp - 1;
-        constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false), kRows = tc_idesc16(kType, D, true);
+        constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false);
         const uint32_t qbase = smem_addr(queries) + q * Shape::kQueryBytes / NQ, rbase = smem_addr(ring);
-        const uint32_t sbase = tmem + q * 2 * kKeyTile, obase = tmem + Shape::kScoreColumns + q * D;
-        const int n = tiles_of(q);
-        int taken = 0;
-        // S of tile j, from the stage that is next in the ring.
-        auto scores = [&](int j) {
-            const int stage = taken % S;
-            const bool reads = (lane & 1) && j > 0 && j < n; // S of tile j - 1 is in registers
-            if (!warp_wait(reads ? &h.scores_read[q] : &h.full[stage], (reads ? j - 1 : taken / S) & 1))
-                return false;
-            if (j < n)
-            {
-                tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    tc_mma_warp(sbase, tc_desc(qbase + i / 4 * 128 * 128 + (i & 3) * 32),
-                                tc_desc(rbase + stage * Shape::kStageBytes + i / 4 * Shape::kBox + (i & 3) * 32), kScores,
-                                i > 0);
-                tc_commit_warp(&h.scores[q]);
-            }
-            tc_commit_warp(&h.empty[stage]);
-            ++taken;
-            return true;
-        };
-        auto rows = [&](int j) {
-            const int stage = taken % S;
-            const bool weighs = (lane & 1) && j < n;
-            if (!warp_wait(weighs ? &h.weights[q][j & 1] : &h.full[stage], (weighs ? j / 2 : taken / S) & 1))
-                return false;
-            if (j < n)
-            {
-                const int t = p.first_tile + j;
-                const int valid = !Tree                 ? p.length - j * kKeyTile
-                                  : t < p.tiles_cached ? p.cached - t * kKeyTile
-                                                        : p.length;
-                if (valid < kKeyTile) // by each MMA warp for its own MMAs
-                {
-                    const int bytes = (kKeyTile - valid) * 128;
-                    for (int b = 0; b < kBlocks; ++b)
-                        for (int i = lane * 16; i < bytes; i += 512)
-                            *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128
-                                                      + i) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async();
-                    __syncwarp();
-                }
-                tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < kKeyTile / 16; ++i)
-                    tc_mma_ts_warp(obase, sbase + kKeyTile + (j & 1) * 32 + i * 8,
-                                   tc_desc_mn(rbase + stage * Shape::kStageBytes + i * 2048, Shape::kBox), kRows,
-                                   j > 0 || i > 0);
-                tc_commit_warp(&h.done[q][j & 1]);
-            }
-            tc_commit_warp(&h.empty[stage]);
-            ++taken;
-            return true;
-        };
-        bool ok = warp_wait(&h.query, 0) && scores(0);
-        for (int j = 0; j < tiles && ok; ++j)
-            ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
-        // A failed run: the MMAs issued so far end before TMEM is given back.
-        if (!ok)
+        const uint32_t sbase = tmem + q * 2 * kKeyTile;
+        int first = 0, count = 0; // ring items and tiles of q before this
+        bool ok = true;
+        MmaPlace p;
+        for (int i = 0; ok && take(i, p); ++i)
         {
-            tc_commit_warp(&h.drained[q]);
-            mbar_wait(&h.drained[q], 0);
+            const int tiles = p.tiles, n = tiles_of(p, q);
+            ok = wait(&h.query, i & 1);
+            for (int j = 0; j < tiles && ok; ++j)
+            {
+                const int item = first + max(2 * j - 1, 0), stage = item % S;
+                const bool reads = (lane & 1) && count > 0 && j < n; // S of the last tile is in registers
+                ok = wait(reads ? &h.scores_read[q] : &h.full[stage], (reads ? count - 1 : item / S) & 1);
+                if (!ok)
+                    break;
+                if (j < n)
+                {
+                    tc_fence_after();
+#pragma unroll
+                    for (int b = 0; b < D / 16; ++b)
+                        tc_mma_warp(sbase, tc_desc(qbase + b / 4 * 128 * 128 + (b & 3) * 32),
+                                    tc_desc(rbase + stage * Shape::kStageBytes + b / 4 * Shape::kBox + (b & 3) * 32), kScores,
+                                    b > 0);
+                    tc_commit_warp(&h.scores[q]);
+                    ++count;
+                }
+                tc_commit_warp(&h.empty[stage]);
+            }
+            if (ok)
+                tc_commit_warp(&h.query_free);
+            first += 2 * tiles;
+            leave(i);
         }
+        finish_mmas(!*(volatile int*) &h.dead, &h.drained[q]);
     }
-    else if (warp >= 4)
+    else if (NQ == 2 ? warp == 3 || warp == 12 : warp == 2)
+    {
+        // O of query tile q: V(j) is item 2 j + 2 of a unit's in the ring, the last one its last.
+        const int q = warp == 12 ? 1 : 0;
+        constexpr uint32_t kRows = tc_idesc16(kType, D, true);
+        const uint32_t rbase = smem_addr(ring), wbase = tmem + q * 2 * kKeyTile + kKeyTile;
+        const uint32_t obase = tmem + Shape::kScoreColumns + q * D;
+        int first = 0, count = 0, rows = 0; // ring items, tiles and finished rows of q before this
+        bool ok = true;
+        MmaPlace p;
+        for (int i = 0; ok && take(i, p); ++i)
+        {
+            const int tiles = p.tiles, n = tiles_of(p, q);
+            for (int j = 0; j < tiles && ok; ++j)
+            {
+                const int item = first + min(2 * j + 2, 2 * tiles - 1), stage = item % S;
+                // The weights, and before a unit's first O the last one's in registers.
+                const bool weighs = (lane & 1) && j < n, frees = (lane & 3) == 2 && j == 0 && j < n && rows > 0;
+                ok = wait(frees ? &h.rows_free[q] : weighs ? &h.weights[q][count & 1] : &h.full[stage],
+                          (frees ? rows - 1 : weighs ? count / 2 : item / S) & 1);
+                if (!ok)
+                    break;
+                if (j < n)
+                {
+                    const int t = p.first_tile + j;
+                    const int valid = !Tree                 ? p.length - j * kKeyTile
+                                      : t < p.tiles_cached ? p.cached - t * kKeyTile
+                                                            : p.length;
+                    if (valid < kKeyTile) // by each of the warps for its own MMAs
+                    {
+                        const int bytes = (kKeyTile - valid) * 128;
+                        for (int b = 0; b < kBlocks; ++b)
+                            for (int e = lane * 16; e < bytes; e += 512)
+                                *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128
+                                                          + e) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int b = 0; b < kKeyTile / 16; ++b)
+                        tc_mma_ts_warp(obase, wbase + (count & 1) * 32 + b * 8,
+                                       tc_desc_mn(rbase + stage * Shape::kStageBytes + b * 2048, Shape::kBox), kRows,
+                                       j > 0 || b > 0);
+                    tc_commit_warp(&h.done[q][count & 1]);
+                    ++count;
+                }
+                tc_commit_warp(&h.empty[stage]);
+            }
+            rows += n > 0;
+            first += 2 * tiles;
+            leave(i);
+        }
+        finish_mmas(!*(volatile int*) &h.dead, &h.drained[2 + q]);
+    }
+    else if (warp >= 4 && warp < 4 + 4 * NQ)
     {
         const int q = (warp - 4) >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane; // the TMEM lane
-        const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
-        const uint32_t obase = tmem + lanes + Shape::kScoreColumns + q * D, sbase = tmem + lanes + q * 2 * kKeyTile;
-        const int n = tiles_of(q);
-        const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
-        const bool real = row < c.tile_tokens * a.group && token < p.length;
-        unsigned long long path = 0;
-        if (Tree)
-        {
-            // The warpgroup's copy of the sequence's parents; a row's path from it.
-            for (int i = tid & 127; i < p.length; i += 128)
-                h.parents[i] = a.parents[p.begin + i];
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");
-            if (real)
-                path = tree_path(h.parents, token);
-        }
+        const uint32_t lanes = tmem + ((uint32_t) (quarter * 32) << 16);
+        const uint32_t obase = lanes + Shape::kScoreColumns + q * D, sbase = lanes + q * 2 * kKeyTile;
         const float scale = a.scale_log2;
-        float m = -INFINITY, l = 0.f;
-        int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
+        int count = 0; // tiles before this
         bool ok = true;
-        for (int j = 0; j < n; ++j)
+        MmaPlace p;
+        for (int i = 0; ok && take(i, p); ++i)
         {
-            const int t = p.first_tile + j;
-            const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
-            if (!warp_wait(&h.scores[q], j & 1))
+            const int n = tiles_of(p, q);
+            const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
+            const bool real = row < c.tile_tokens * a.group && token < p.length;
+            const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+            unsigned long long path = 0;
+            if (Tree)
             {
-                ok = false;
-                break;
+                // The sequence's parents, and a row's path from them.
+                int* parents = h.parents[i & 1];
+                for (int e = tid & 127; e < p.length; e += 128)
+                    parents[e] = a.parents[p.begin + e];
+                named_sync(1 + q, 128);
+                if (real)
+                    path = tree_path(parents, token);
             }
-            tc_fence_after();
-            uint32_t r[64];
-            tc_ld32(sbase, r);
-            tc_ld32(sbase + 32, r + 32);
-            tc_wait_ld32(r);
-            tc_wait_ld32(r + 32);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&h.scores_read[q]);
-            float* s = reinterpret_cast<float*>(r);
-            // What the row does not attend to.
-            bool masked = true;
-            if (Tree && t >= p.tiles_cached)
+            float m = -INFINITY, l = 0.f;
+            int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
+            for (int j = 0; j < n; ++j, ++count)
             {
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    s[i] = path >> i & 1 ? s[i] : -INFINITY;
-            }
-            else
-            {
-                const int limit = !Tree                        ? token - j * kKeyTile + 1
-                                  : page_there(id, a.pages) ? p.cached - t * kKeyTile
-                                                             : 0;
-                masked = __any_sync(0xFFFFFFFFu, limit < kKeyTile);
-                if (masked)
+                const int t = p.first_tile + j;
+                const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
+                // S is there, and the weights' buffer has been read (two tiles back).
+                const bool frees = (lane & 1) && count >= 2;
+                ok = wait(frees ? &h.done[q][count & 1] : &h.scores[q], (frees ? count / 2 - 1 : count) & 1);
+                if (!ok)
+                    break;
+                tc_fence_after();
+                uint32_t r[64];
+                tc_ld32(sbase, r);
+                tc_ld32(sbase + 32, r + 32);
+                tc_wait_ld32(r);
+                tc_wait_ld32(r + 32);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&h.scores_read[q]);
+                float* s = reinterpret_cast<float*>(r);
+                // What the row does not attend to.
+                bool masked = true;
+                if (Tree && t >= p.tiles_cached)
                 {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        s[i] = i < limit ? s[i] : -INFINITY;
+                    for (int e = 0; e < 64; ++e)
+                        s[e] = path >> e & 1 ? s[e] : -INFINITY;
                 }
-            }
-            id = id_next;
-            float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int i = 4; i < 64; ++i)
-                top[i & 3] = fmaxf(top[i & 3], s[i]);
-            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-            if (j == 0)
-                m = m_tile;
-            else
-            {
-                const bool rises = m_tile > m + 8.f;
-                if (__any_sync(0xFFFFFFFFu, rises))
+                else
                 {
-                    // O of tile j - 1 is complete before it is scaled.
-                    if (!warp_wait(&h.done[q][(j - 1) & 1], ((j - 1) / 2) & 1))
+                    const int limit = !Tree                        ? token - j * kKeyTile + 1
+                                      : page_there(id, a.pages) ? p.cached - t * kKeyTile
+                                                                 : 0;
+                    masked = __any_sync(0xFFFFFFFFu, limit < kKeyTile);
+                    if (masked)
                     {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const float alpha = rises ? exp2_approx(m - m_tile) : 1.f;
-                    l *= alpha;
-                    m = rises ? m_tile : m;
-#pragma unroll 1
-                    for (int b = 0; b < D; b += 16)
-                    {
-                        uint32_t o[16];
-                        tc_ld16(obase + b, o);
-                        tc_wait_ld(o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tc_st16(obase + b, o);
+                        for (int e = 0; e < 64; ++e)
+                            s[e] = e < limit ? s[e] : -INFINITY;
                     }
                 }
-            }
-            const float base = m == -INFINITY ? 0.f : -m;
-            uint32_t w[32];
-            l += masked ? weigh<T, false>(s, scale, base, w) : weigh<T, true>(s, scale, base, w);
-            // The MMAs that read this buffer two tiles back were issued before
-            // S of this tile, whose commit covers them.
-            tc_st32(sbase + kKeyTile + (j & 1) * 32, w);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&h.weights[q][j & 1]);
-        }
-        if (ok && n > 0)
-            ok = warp_wait(&h.done[q][(n - 1) & 1], ((n - 1) / 2) & 1);
-        if (n > 0)
-        {
-            tc_fence_after();
-            const int at = p.begin + token; // the row of q and out
-            const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
-            const bool whole = !Tree || p.whole;
-            const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
-            bool finite = true;
-#pragma unroll 1
-            for (int b = 0; b < D; b += 16)
-            {
-                uint32_t o[16];
-                tc_ld16(obase + b, o);
-                tc_wait_ld(o);
-                if (b >= a.width || !real)
-                    continue;
+                id = id_next;
+                float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+                for (int e = 4; e < 60; e += 8)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        top[g] = max3(top[g], s[e + 2 * g], s[e + 2 * g + 1]);
+                const float m_tile =
+                    max3(max3(top[0], s[60], s[61]), max3(top[1], s[62], s[63]), fmaxf(top[2], top[3])) * scale;
+                if (j == 0)
+                    m = m_tile;
+                else
                 {
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    const bool rises = m_tile > m + 8.f;
+                    if (__any_sync(0xFFFFFFFFu, rises))
                     {
-                        const float v = __uint_as_float(o[8 * g + i]);
+                        // O of the last tile is complete before it is scaled.
+                        ok = wait(&h.done[q][(count - 1) & 1], ((count - 1) / 2) & 1);
+                        if (!ok)
+                            break;
+                        tc_fence_after();
+                        const float alpha = rises ? exp2_approx(m - m_tile) : 1.f;
+                        l *= alpha;
+                        m = rises ? m_tile : m;
+#pragma unroll 1
+                        for (int b = 0; b < D; b += 16)
+                        {
+                            uint32_t o[16];
+                            tc_ld16(obase + b, o);
+                            tc_wait_ld(o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tc_st16(obase + b, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : -m;
+                uint32_t w[32];
+                l += masked ? weigh<T, false>(s, scale, base, w) : weigh<T, true>(s, scale, base, w);
+                tc_st32(sbase + kKeyTile + (count & 1) * 32, w);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&h.weights[q][count & 1]);
+            }
+            if (n > 0)
+            {
+                ok = ok && wait(&h.done[q][(count - 1) & 1], ((count - 1) / 2) & 1);
+                tc_fence_after();
+                const int at = p.begin + token; // the row of q and out
+                const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
+                const bool whole = !Tree || p.whole;
+                const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
+                bool finite = l < INFINITY;
+                char* mine = whole ? (char*) ((T*) a.out + at * a.out_stride + (size_t) head * a.width)
+                                   : (char*) (c.part_o + part * a.width);
+                const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
+                char* four[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    four[k] = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, (lane & ~3) + k);
+#pragma unroll 1
+                for (int b = 0; b < a.width; b += 32)
+                {
+                    uint32_t o[32];
+                    tc_ld32(obase + b, o);
+                    tc_wait_ld32(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                    {
+                        const float v = __uint_as_float(o[e]);
                         finite = finite && fabsf(v) < INFINITY;
-                        x[i] = scaled == 0.f ? 0.f : v * scaled;
+                        o[e] = __float_as_uint(scaled == 0.f ? 0.f : v * scaled);
                     }
-                    if (b + 8 * g < a.width)
+                    uint32_t x[16];
+                    if (whole)
                     {
-                        if (whole)
-                            store8((T*) a.out + at * a.out_stride + (size_t) head * a.width + b + 8 * g, x);
-                        else
-                            store8(c.part_o + part * a.width + b + 8 * g, x);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            x[e] = pack_pair<T>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+                        store_rows(x, four, rows, 2 * b, 2 * a.width);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+                        {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                x[e] = o[16 * g + e];
+                            store_rows(x, four, rows, 4 * (b + 16 * g), 4 * a.width);
+                        }
                     }
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&h.rows_free[q]);
+                if (Tree && !whole && real)
+                    c.part_ml[part] = make_float2(m, l);
+                // Rows that came out not finite: again, from what they attend to only.
+                unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !finite);
+                while (again)
+                {
+                    const int who = __ffs(again) - 1;
+                    again &= again - 1;
+                    const int at1 = __shfl_sync(0xFFFFFFFFu, at, who), head1 = __shfl_sync(0xFFFFFFFFu, head, who);
+                    take_again<T, Tree>(c, h.place[i & 1], at1, head1);
+                }
             }
-            if (Tree && !whole && real)
-                c.part_ml[part] = make_float2(m, l);
-            // Rows that came out not finite: again, from what they attend to only.
-            unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !(finite && fabsf(l) < INFINITY));
-            while (again)
-            {
-                const int who = __ffs(again) - 1;
-                again &= again - 1;
-                const int at1 = __shfl_sync(0xFFFFFFFFu, at, who), head1 = __shfl_sync(0xFFFFFFFFu, head, who);
-                take_again<T, Tree>(c, h.place, at1, head1);
-            }
+            leave(i);
         }
         tc_fence_before();
     }

@@ -220,6 +220,45 @@ __device__ __forceinline__ void tensor_load(void* dst, const CUtensorMap* map, i
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// Cluster launch control: asks for the grid's next CTA that has not started, to
+// do its work here; the answer (16 bytes) completes on `bar`.
+__device__ __forceinline__ void ask_next_cta(void* answer, uint64_t* bar)
+{
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the last answer has been read
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_addr(answer)),
+                 "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// The x index of the CTA that was taken over; false when all have started (then
+// nothing may be asked again).
+__device__ __forceinline__ bool next_cta(const void* answer, int& x)
+{
+    uint32_t taken, index;
+    asm volatile("{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%2];\n"
+                 " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+                 " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}"
+                 : "=r"(taken), "=r"(index)
+                 : "r"(smem_addr(answer))
+                 : "memory");
+    x = (int) index;
+    return taken;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float r;
