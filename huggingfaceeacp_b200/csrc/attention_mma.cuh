@@ -10,9 +10,12 @@
 // keys, in tiles of 64 (a page).
 //
 // Roles:
-//  warp 0   places and copies: query tiles, then key and value tiles through a
-//           ring, in the order the MMAs use them (tensor maps; a page is one
-//           box), on into the next unit as far as there is room;
+//  warp 0   places and copies: query tiles, then key and value tiles, each
+//           through a ring of its own (tensor maps; a page is one box), on into
+//           the next unit as far as there is room. Of a ring that both passed
+//           through, a warp that takes only the keys would see every other phase of
+//           a stage's barrier, and its parity cannot tell a phase from the one
+//           two before;
 //  MMAs     a warp for each query tile's S and one for its O, since a warp's
 //           waits and MMAs follow one another: S of the next tile is issued as
 //           soon as S of this one is in registers, O of a tile as soon as its
@@ -125,6 +128,7 @@ struct MmaShape
     static constexpr int kBudget = kCtas == 2 ? 113 * 1024 : 227 * 1024;
     static constexpr int kStagesFit = (kBudget - kHead - kQueryBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
+    static constexpr int kKeyStages = kStages / 2, kValueStages = kStages - kKeyStages;
     static constexpr int kSmem = kHead + kQueryBytes + kStages * kStageBytes;
     static constexpr int kThreads = 128 + 128 * NQ + (NQ == 2 ? 32 : 0); // the last warp: MMAs
     static_assert(kScoreColumns + NQ * D <= kTmem && kStages >= 4, "what an SM holds");
@@ -143,7 +147,7 @@ struct MmaPlace
 
 struct MmaHead
 {
-    uint64_t full[12], empty[12], query, query_free, scores[2], scores_read[2], weights[2][2], done[2][2], rows_free[2],
+    uint64_t keys_full[6], keys_free[6], values_full[6], values_free[6], query, query_free, scores[2], scores_read[2], weights[2][2], done[2][2], rows_free[2],
         place_full[2], place_free[2], next, drained[4];
     alignas(16) uint4 answer;
     uint32_t tmem;
@@ -153,7 +157,10 @@ struct MmaHead
 };
 
 // Bounded waits, of a warp together and of one thread. A warp's lanes may name
-// different barriers: it goes on when all have come, for the price of one.
+// different barriers: it goes on when all have come, for the price of one. A poll
+// that finds nothing is held about 4 us by the hardware, so the limit is some 4 s: far
+// above a step, and above the rows that a warp may have to take again meanwhile (32 rows
+// of a million keys).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity)
 {
     if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)))
@@ -357,22 +364,28 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                   const __grid_constant__ CUtensorMap vpages, const __grid_constant__ MmaCall c)
 {
     using Shape = MmaShape<D, NQ>;
-    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks;
+    constexpr int KS = Shape::kKeyStages, VS = Shape::kValueStages, kBlocks = Shape::kBlocks;
     constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     extern __shared__ __align__(1024) uint8_t smem[];
     MmaHead& h = *reinterpret_cast<MmaHead*>(smem);
     static_assert(sizeof(MmaHead) <= Shape::kHead, "the head's room");
     uint8_t* queries = smem + Shape::kHead;
-    uint8_t* ring = queries + Shape::kQueryBytes;
+    uint8_t* keys = queries + Shape::kQueryBytes;
+    uint8_t* values = keys + KS * Shape::kStageBytes;
     const AttnCall& a = c.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
     if (warp == 0 && lane == 0)
     {
-        for (int s = 0; s < S; ++s)
+        for (int s = 0; s < KS; ++s)
         {
-            mbar_init(&h.full[s], 1);
-            mbar_init(&h.empty[s], NQ); // an arrival an MMA warp
+            mbar_init(&h.keys_full[s], 1);
+            mbar_init(&h.keys_free[s], NQ); // an arrival an MMA warp
+        }
+        for (int s = 0; s < VS; ++s)
+        {
+            mbar_init(&h.values_full[s], 1);
+            mbar_init(&h.values_free[s], NQ);
         }
         mbar_init(&h.query, 1);
         mbar_init(&h.query_free, NQ);
@@ -446,7 +459,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 
     if (warp == 0)
     {
-        int put = 0, unit = blockIdx.x, i = 0;
+        int put_keys = 0, put_values = 0, unit = blockIdx.x, i = 0;
         bool ok = true;
         auto one_wait = [&](uint64_t* bar, unsigned parity) {
             if (ok && !thread_wait(bar, parity))
@@ -470,18 +483,19 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 }
                 const int tiles = p.tiles;
                 const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
-                auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id) {
-                    const int stage = put % S;
-                    if (!ok || (put >= S && !one_wait(&h.empty[stage], (put / S - 1) & 1)))
+                auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id, uint8_t* ring, int& put,
+                                int stages, uint64_t* full, uint64_t* free) {
+                    const int stage = put % stages;
+                    if (!ok || (put >= stages && !one_wait(&free[stage], (put / stages - 1) & 1)))
                         return;
                     const bool cached = Tree && p.first_tile + j < p.tiles_cached;
                     // A page that is not there is read past the pool's end: zeros.
                     const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
                                            : p.begin + (Tree ? 0 : j * kKeyTile);
-                    mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
+                    mbar_expect_tx(&full[stage], Shape::kStageBytes);
                     for (int b = 0; b < kBlocks; ++b)
                         tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
-                                    p.kv_head, row, &h.full[stage]);
+                                    p.kv_head, row, &full[stage]);
                     ++put;
                 };
                 int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                     if (lane == 0)
                     {
                         if (j < tiles)
-                            load(j, &kmap, &kpages, id);
+                            load(j, &kmap, &kpages, id, keys, put_keys, KS, h.keys_full, h.keys_free);
                         if (j == 0 && ok && (i == 0 || one_wait(&h.query_free, (i - 1) & 1)))
                         {
                             mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                                             p.begin + p.token0 + b / kBlocks * c.tile_tokens, &h.query);
                         }
                         if (j > 0)
-                            load(j - 1, &vmap, &vpages, id_before);
+                            load(j - 1, &vmap, &vpages, id_before, values, put_values, VS, h.values_full, h.values_free);
                     }
                     id_before = id;
                     __syncwarp();
@@ -533,31 +547,33 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             if (!ok)
             {
                 mbar_wait(&h.query, 0);
-                for (int n = max(0, put - S); n < put; ++n)
-                    mbar_wait(&h.full[n % S], (n / S) & 1);
+                for (int n = max(0, put_keys - KS); n < put_keys; ++n)
+                    mbar_wait(&h.keys_full[n % KS], (n / KS) & 1);
+                for (int n = max(0, put_values - VS); n < put_values; ++n)
+                    mbar_wait(&h.values_full[n % VS], (n / VS) & 1);
             }
         }
         __syncwarp();
     }
     else if (warp <= NQ)
     {
-        // S of query tile q: K(j) is item 2 j - 1 of a unit's in the ring, the first item 0.
+        // S of query tile q.
         const int q = warp - 1;
         constexpr uint32_t kScores = tc_idesc16(kType, kKeyTile, false);
-        const uint32_t qbase = smem_addr(queries) + q * Shape::kQueryBytes / NQ, rbase = smem_addr(ring);
+        const uint32_t qbase = smem_addr(queries) + q * Shape::kQueryBytes / NQ, kbase = smem_addr(keys);
         const uint32_t sbase = tmem + q * 2 * kKeyTile;
-        int first = 0, count = 0; // ring items and tiles of q before this
+        int item = 0, count = 0; // key tiles, and those of q, before this
         bool ok = true;
         MmaPlace p;
         for (int i = 0; ok && take(i, p); ++i)
         {
             const int tiles = p.tiles, n = tiles_of(p, q);
             ok = wait(&h.query, i & 1);
-            for (int j = 0; j < tiles && ok; ++j)
+            for (int j = 0; j < tiles && ok; ++j, ++item)
             {
-                const int item = first + max(2 * j - 1, 0), stage = item % S;
+                const int stage = item % KS;
                 const bool reads = (lane & 1) && count > 0 && j < n; // S of the last tile is in registers
-                ok = wait(reads ? &h.scores_read[q] : &h.full[stage], (reads ? count - 1 : item / S) & 1);
+                ok = wait(reads ? &h.scores_read[q] : &h.keys_full[stage], (reads ? count - 1 : item / KS) & 1);
                 if (!ok)
                     break;
                 if (j < n)
@@ -566,40 +582,39 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 #pragma unroll
                     for (int b = 0; b < D / 16; ++b)
                         tc_mma_warp(sbase, tc_desc(qbase + b / 4 * 128 * 128 + (b & 3) * 32),
-                                    tc_desc(rbase + stage * Shape::kStageBytes + b / 4 * Shape::kBox + (b & 3) * 32), kScores,
+                                    tc_desc(kbase + stage * Shape::kStageBytes + b / 4 * Shape::kBox + (b & 3) * 32), kScores,
                                     b > 0);
                     tc_commit_warp(&h.scores[q]);
                     ++count;
                 }
-                tc_commit_warp(&h.empty[stage]);
+                tc_commit_warp(&h.keys_free[stage]);
             }
             if (ok)
                 tc_commit_warp(&h.query_free);
-            first += 2 * tiles;
             leave(i);
         }
         finish_mmas(!*(volatile int*) &h.dead, &h.drained[q]);
     }
     else if (NQ == 2 ? warp == 3 || warp == 12 : warp == 2)
     {
-        // O of query tile q: V(j) is item 2 j + 2 of a unit's in the ring, the last one its last.
+        // O of query tile q.
         const int q = warp == 12 ? 1 : 0;
         constexpr uint32_t kRows = tc_idesc16(kType, D, true);
-        const uint32_t rbase = smem_addr(ring), wbase = tmem + q * 2 * kKeyTile + kKeyTile;
+        const uint32_t vbase = smem_addr(values), wbase = tmem + q * 2 * kKeyTile + kKeyTile;
         const uint32_t obase = tmem + Shape::kScoreColumns + q * D;
-        int first = 0, count = 0, rows = 0; // ring items, tiles and finished rows of q before this
+        int item = 0, count = 0, rows = 0; // value tiles, those of q, and q's finished units before this
         bool ok = true;
         MmaPlace p;
         for (int i = 0; ok && take(i, p); ++i)
         {
             const int tiles = p.tiles, n = tiles_of(p, q);
-            for (int j = 0; j < tiles && ok; ++j)
+            for (int j = 0; j < tiles && ok; ++j, ++item)
             {
-                const int item = first + min(2 * j + 2, 2 * tiles - 1), stage = item % S;
+                const int stage = item % VS;
                 // The weights, and before a unit's first O the last one's in registers.
                 const bool weighs = (lane & 1) && j < n, frees = (lane & 3) == 2 && j == 0 && j < n && rows > 0;
-                ok = wait(frees ? &h.rows_free[q] : weighs ? &h.weights[q][count & 1] : &h.full[stage],
-                          (frees ? rows - 1 : weighs ? count / 2 : item / S) & 1);
+                ok = wait(frees ? &h.rows_free[q] : weighs ? &h.weights[q][count & 1] : &h.values_full[stage],
+                          (frees ? rows - 1 : weighs ? count / 2 : item / VS) & 1);
                 if (!ok)
                     break;
                 if (j < n)
@@ -613,7 +628,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                         const int bytes = (kKeyTile - valid) * 128;
                         for (int b = 0; b < kBlocks; ++b)
                             for (int e = lane * 16; e < bytes; e += 512)
-                                *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128
+                                *reinterpret_cast<uint4*>(values + stage * Shape::kStageBytes + b * Shape::kBox + valid * 128
                                                           + e) = make_uint4(0, 0, 0, 0);
                         fence_proxy_async();
                         __syncwarp();
@@ -622,15 +637,14 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 #pragma unroll
                     for (int b = 0; b < kKeyTile / 16; ++b)
                         tc_mma_ts_warp(obase, wbase + (count & 1) * 32 + b * 8,
-                                       tc_desc_mn(rbase + stage * Shape::kStageBytes + b * 2048, Shape::kBox), kRows,
+                                       tc_desc_mn(vbase + stage * Shape::kStageBytes + b * 2048, Shape::kBox), kRows,
                                        j > 0 || b > 0);
                     tc_commit_warp(&h.done[q][count & 1]);
                     ++count;
                 }
-                tc_commit_warp(&h.empty[stage]);
+                tc_commit_warp(&h.values_free[stage]);
             }
             rows += n > 0;
-            first += 2 * tiles;
             leave(i);
         }
         finish_mmas(!*(volatile int*) &h.dead, &h.drained[2 + q]);
