@@ -166,16 +166,15 @@ struct LimbShape
     static constexpr int kQueryHalf = kBlocks * 128 * 128;
     static constexpr int kHead = 3072;
     static constexpr int kStagesFit = (227 * 1024 - kHead - 2 * kQueryHalf) / kStageBytes;
-    static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit / 2 * 2; // pairs stay together
+    static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
+    static constexpr int kKeyStages = kStages / 2, kValueStages = kStages - kKeyStages;
     static constexpr int kSmem = kHead + 2 * kQueryHalf + kStages * kStageBytes;
-    static constexpr int kParts = D == 256 ? 2 : 1;      // O in parts of up to 128 channels
-    static constexpr int kPart = D / kParts;
     static constexpr int kRowBuffers = D == 256 ? 1 : 2; // of O
     static constexpr int kThreads = Tree ? 512 : 384;
     // Registers a thread, by warpgroup; at launch 168 or 128 each: the shares
     // add up to that (3 x 168, 4 x 128).
     static constexpr int kLaunchRegisters = Tree ? 128 : 168;
-    static constexpr int kRegistersIssue = 40, kRegistersRows = Tree ? 200 : 232, kRegistersConvert = 72;
+    static constexpr int kRegistersIssue = Tree ? 56 : 72, kRegistersRows = Tree ? 192 : 216, kRegistersConvert = 72;
     static_assert(kRegistersIssue + 2 * kRegistersRows + (Tree ? kRegistersConvert : 0)
                       <= kLaunchRegisters * kThreads / 128,
                   "what the CTA was launched with");
@@ -185,12 +184,16 @@ struct LimbShape
 
 struct LimbHead
 {
-    uint64_t full[12], ready[12], empty[12], query, scores, scores_read, weights[2], done[2][2], free[2][2], drained;
+    uint64_t keys_full[6], keys_ready[6], keys_free[6], values_full[6], values_ready[6], values_free[6];
+    uint64_t query, query_free, scores, scores_read, weights[2], done[2], rows_free[2], place_full[2], place_free[2], next,
+        drained[2];
+    alignas(16) uint4 answer;
     uint32_t tmem;
-    int misfit;              // a tree's value outside the sampled exponent's range
-    unsigned sample[2];      // its largest K and V, as bits
-    MmaPlace place;
-    int parents[kTreeNodes];
+    int dead;           // a wait ran out
+    int misfit[2];      // a unit's value outside its sampled exponent's range
+    unsigned sample[2]; // a unit's largest sampled K and V, as bits
+    MmaPlace place[2];
+    int8_t parents[2][kTreeNodes];
 };
 
 template <int N>
@@ -212,53 +215,57 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
 {
     // Prompts: the maps of K hi, V hi, K lo, V lo. Trees: drafted K, V, paged K, V in fp32.
     using Shape = LimbShape<D, Tree>;
-    constexpr int S = Shape::kStages, kBlocks = Shape::kBlocks, kHalf = D / 2;
+    constexpr int KS = Shape::kKeyStages, VS = Shape::kValueStages, kBlocks = Shape::kBlocks, kHalf = D / 2;
+    constexpr int RB = Shape::kRowBuffers;
     extern __shared__ __align__(1024) uint8_t smem[];
     LimbHead& h = *reinterpret_cast<LimbHead*>(smem);
     float(*exchange)[2][128] = reinterpret_cast<float(*)[2][128]>(smem + Shape::kHead - 2048); // [tile parity][warpgroup][row]
     static_assert(sizeof(LimbHead) <= Shape::kHead - 2048, "the head's room");
     uint8_t* queries = smem + Shape::kHead;
-    uint8_t* ring = queries + 2 * Shape::kQueryHalf;
+    uint8_t* keys = queries + 2 * Shape::kQueryHalf;
+    uint8_t* values = keys + KS * Shape::kStageBytes;
     const MmaCall& c = lc.c;
     const AttnCall& a = c.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
-    if (warp == 0)
+    if (warp == 0 && lane == 0)
     {
-        const MmaPlace p = find_place<Tree>(c, c.tile_tokens, blockIdx.x);
-        if (lane == 0)
+        for (int s = 0; s < 6; ++s)
         {
-            h.place = p;
-            h.misfit = 0;
-            h.sample[0] = h.sample[1] = 0;
-        }
-    }
-    else if (warp == 1)
-    {
-        tc_alloc(&h.tmem, 512);
-    }
-    else if (warp == 2 && lane == 0)
-    {
-        for (int s = 0; s < S; ++s)
-        {
-            mbar_init(&h.full[s], 1);
-            mbar_init(&h.ready[s], 4); // an arrival a converter warp
-            mbar_init(&h.empty[s], 1);
+            mbar_init(&h.keys_full[s], 1);
+            mbar_init(&h.keys_ready[s], 4); // an arrival a converter warp
+            mbar_init(&h.keys_free[s], 1);
+            mbar_init(&h.values_full[s], 1);
+            mbar_init(&h.values_ready[s], 4);
+            mbar_init(&h.values_free[s], 1);
         }
         mbar_init(&h.query, 8); // an arrival a row warp
+        mbar_init(&h.query_free, 1);
         mbar_init(&h.scores, 1);
-        mbar_init(&h.drained, 1);
         mbar_init(&h.scores_read, 8);
+        mbar_init(&h.next, 1);
         for (int b = 0; b < 2; ++b)
         {
             mbar_init(&h.weights[b], 8);
-            for (int i = 0; i < 2; ++i)
-            {
-                mbar_init(&h.done[b][i], 1);
-                mbar_init(&h.free[b][i], Shape::kParts == 2 ? 4 : 8);
-            }
+            mbar_init(&h.done[b], 1);
+            mbar_init(&h.rows_free[b], 8);
+            mbar_init(&h.place_full[b], 1);
+            mbar_init(&h.place_free[b], Tree ? 15 : 11); // an arrival a warp but the one that finds them
+            mbar_init(&h.drained[b], 1);
+            h.misfit[b] = 0;
+            h.sample[b] = 0;
         }
+        h.dead = 0;
         mbar_fence_init();
+    }
+    else if (warp == 1)
+        tc_alloc(&h.tmem, 512);
+    else if (warp == 2 && lane == 0)
+    {
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
+        prefetch_map(&kmap2);
+        prefetch_map(&vmap2);
     }
     tc_fence_before();
     __syncthreads();
@@ -267,18 +274,28 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         pdl_trigger(); // attention_join may take its place; it waits for this grid's end
     else
         pdl_wait(); // split_tiles' halves
-    const MmaPlace p = h.place;
     const uint32_t tmem = h.tmem;
-    if (p.sequence < 0)
-    {
-        if (warp == 1)
-            tc_dealloc(tmem, 512);
-        return;
-    }
-    const int tiles = p.tiles;
-    const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
-    // Keys of tile j that are there.
-    auto valid_of = [&](int j) {
+    // A wait of one of the roles; one that runs out ends the CTA's other waits too.
+    auto wait = [&](uint64_t* bar, unsigned parity) {
+        const bool ok = warp_wait(bar, parity);
+        if (!ok)
+            *(volatile int*) &h.dead = 1;
+        return ok;
+    };
+    // The place of the CTA's i-th unit: false when there is none.
+    auto take = [&](int i, MmaPlace& p) {
+        if (__any_sync(0xFFFFFFFFu, *(volatile int*) &h.dead) || !wait(&h.place_full[i & 1], (i / 2) & 1))
+            return false;
+        p = h.place[i & 1];
+        return p.sequence >= 0;
+    };
+    auto leave = [&](int i) {
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(&h.place_free[i & 1]);
+    };
+    // Keys of the unit's tile j that are there.
+    auto valid_of = [&](const MmaPlace& p, int j) {
         const int t = p.first_tile + j;
         return min(kKeyTile, !Tree                 ? p.length - j * kKeyTile
                              : t < p.tiles_cached ? p.cached - t * kKeyTile
@@ -290,149 +307,211 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         set_registers_down<Shape::kRegistersIssue>();
         if (warp == 0)
         {
-            int put = 0, ids = -1;
+            int put_keys = 0, put_values = 0;
             bool ok = true;
-            // A tile's K or V, block by block.
-            auto load = [&](int j, bool values, int id) {
-                const bool cached = Tree && p.first_tile + j < p.tiles_cached;
-                const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
-                                       : p.begin + (Tree ? 0 : j * kKeyTile);
-                for (int b = 0; b < kBlocks; ++b)
+            auto one_wait = [&](uint64_t* bar, unsigned parity) {
+                if (ok && !thread_wait(bar, parity))
                 {
-                    const int stage = put % S;
-                    if (put >= S && !thread_wait(&h.empty[stage], (put / S - 1) & 1))
-                        return false;
-                    uint8_t* to = ring + stage * Shape::kStageBytes;
-                    mbar_expect_tx(&h.full[stage], Shape::kStageBytes);
+                    *(volatile int*) &h.dead = 1;
+                    ok = false;
+                }
+                return ok;
+            };
+            MmaPlace p;
+            for (int i = 0; ok && take(i, p); ++i)
+            {
+                const int tiles = p.tiles;
+                const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+                // A tile's K or V, block by block.
+                auto load = [&](int j, const CUtensorMap* first, const CUtensorMap* second, int id, uint8_t* ring, int& put,
+                                int stages, uint64_t* full, uint64_t* free) {
+                    const bool cached = Tree && p.first_tile + j < p.tiles_cached;
+                    const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                           : p.begin + (Tree ? 0 : j * kKeyTile);
+                    for (int b = 0; b < kBlocks; ++b)
+                    {
+                        const int stage = put % stages;
+                        if (!ok || (put >= stages && !one_wait(&free[stage], (put / stages - 1) & 1)))
+                            return;
+                        uint8_t* to = ring + stage * Shape::kStageBytes;
+                        mbar_expect_tx(&full[stage], Shape::kStageBytes);
+                        tensor_load(to, Tree && cached ? second : first, 64 * b, p.kv_head, row, &full[stage]);
+                        tensor_load(to + Shape::kBox, Tree ? (cached ? second : first) : second, 64 * b + (Tree ? 32 : 0),
+                                    p.kv_head, row, &full[stage]);
+                        ++put;
+                    }
+                };
+                int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
+                for (int j = 0; j <= tiles; ++j)
+                {
+                    int id = -1;
                     if (Tree)
                     {
-                        const CUtensorMap* map = cached ? (values ? &vmap2 : &kmap2) : (values ? &vmap : &kmap);
-                        tensor_load(to, map, 64 * b, p.kv_head, row, &h.full[stage]);
-                        tensor_load(to + Shape::kBox, map, 64 * b + 32, p.kv_head, row, &h.full[stage]);
+                        if ((j & 31) == 0)
+                        {
+                            const int t = p.first_tile + j + lane;
+                            ids = t < p.tiles_cached ? table[t] : -1;
+                        }
+                        id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
                     }
-                    else
+                    if (lane == 0)
                     {
-                        tensor_load(to, values ? &vmap : &kmap, 64 * b, p.kv_head, row, &h.full[stage]);
-                        tensor_load(to + Shape::kBox, values ? &vmap2 : &kmap2, 64 * b, p.kv_head, row, &h.full[stage]);
+                        if (j < tiles)
+                            load(j, &kmap, &kmap2, id, keys, put_keys, KS, h.keys_full, h.keys_free);
+                        if (j > 0)
+                            load(j - 1, &vmap, &vmap2, id_before, values, put_values, VS, h.values_full, h.values_free);
                     }
-                    ++put;
+                    id_before = id;
+                    __syncwarp();
                 }
-                return true;
-            };
-            int id_before = -1; // tile j - 1's page
-            for (int j = 0; j <= tiles; ++j)
-            {
-                int id = -1;
-                if (Tree)
-                {
-                    if ((j & 31) == 0)
-                    {
-                        const int t = p.first_tile + j + lane;
-                        ids = t < p.tiles_cached ? table[t] : -1;
-                    }
-                    id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
-                }
-                if (lane == 0 && ok)
-                    ok = (j == tiles || load(j, false, id)) && (j == 0 || load(j - 1, true, id_before));
-                id_before = id;
-                __syncwarp();
+                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                leave(i);
             }
             // Every copy has landed before the CTA may end (only a failed run gets here early).
-            if (lane == 0 && !ok)
-                for (int i = max(0, put - S); i < put; ++i)
-                    mbar_wait(&h.full[i % S], (i / S) & 1);
+            if (lane == 0 && *(volatile int*) &h.dead)
+            {
+                for (int n = max(0, put_keys - KS); n < put_keys; ++n)
+                    mbar_wait(&h.keys_full[n % KS], (n / KS) & 1);
+                for (int n = max(0, put_values - VS); n < put_values; ++n)
+                    mbar_wait(&h.values_full[n % VS], (n / VS) & 1);
+            }
             __syncwarp();
         }
         else if (warp == 1)
         {
-            constexpr uint32_t kWide = tc_idesc16(0, 128, false), kNarrow = tc_idesc16(0, 64, false),
-                               kValues = tc_idesc16(0, Shape::kPart, true);
-            const uint32_t qhi = smem_addr(queries), qlo = qhi + Shape::kQueryHalf, rbase = smem_addr(ring);
-            uint64_t* landed = Tree ? h.ready : h.full;
-            int taken = 0;
-            auto scores = [&](int j) {
-                for (int b = 0; b < kBlocks; ++b)
-                {
-                    const int stage = taken % S;
-                    if ((b & 1) == 0)
-                    {
-                        // This block and the next, and S of tile j - 1 in registers.
-                        const bool reads = (lane & 2) && b == 0 && j > 0;
-                        if (!warp_wait(reads ? &h.scores_read : &landed[kBlocks == 1 ? stage : stage + (lane & 1)],
-                                       (reads ? j - 1 : taken / S) & 1))
-                            return false;
-                    }
-                    tc_fence_after();
-                    const uint32_t k = rbase + stage * Shape::kStageBytes;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                    {
-                        const uint32_t at = b * 128 * 128 + i * 32;
-                        tc_mma_warp(tmem + Shape::kScores, tc_desc(qhi + at), tc_desc(k + i * 32), kWide, b > 0 || i > 0);
-                        tc_mma_warp(tmem + Shape::kScores + 64, tc_desc(qlo + at), tc_desc(k + i * 32), kNarrow, 1);
-                    }
-                    tc_commit_warp(&h.empty[stage]);
-                    ++taken;
-                }
-                tc_commit_warp(&h.scores);
-                return true;
-            };
-            auto rows = [&](int j) {
-                constexpr int RB = Shape::kRowBuffers, kEach = kBlocks / Shape::kParts; // stages a part
-                const int valid = valid_of(j), buffer = j % RB;
-                for (int part = 0; part < Shape::kParts; ++part)
-                {
-                    const int stage = taken % S;
-                    // The part's stages, the weights, and the part's last O in registers.
-                    const int what = lane & 3;
-                    const bool frees = what == 3 && j >= RB, weighs = what == 2 && part == 0;
-                    if (!warp_wait(frees    ? &h.free[buffer][part]
-                                   : weighs ? &h.weights[j & 1]
-                                            : &landed[stage + (what & (kEach - 1))],
-                                   (frees ? j / RB - 1 : weighs ? j / 2 : taken / S) & 1))
-                        return false;
-                    if (!Tree && valid < kKeyTile)
-                    {
-                        // Rows past the sequence's end: weights of 0, but 0 x NaN is not.
-                        const int bytes = (kKeyTile - valid) * 128;
-                        for (int box = 0; box < 2 * kEach; ++box)
-                            for (int i = lane * 16; i < bytes; i += 512)
-                                *reinterpret_cast<uint4*>(ring + stage * Shape::kStageBytes + box * Shape::kBox + valid * 128
-                                                          + i) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async();
-                        __syncwarp();
-                    }
-                    tc_fence_after();
-                    const uint32_t d = tmem + Shape::kRows + buffer * D + part * Shape::kPart;
-                    const uint32_t hi = tmem + Shape::kWeights + (j & 1) * 64, lo = hi + 32;
-                    const uint32_t v = rbase + stage * Shape::kStageBytes;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc_mma_ts_warp(d, hi + i * 8, tc_desc_mn(v + Shape::kBox + i * 2048, Shape::kStageBytes), kValues, i > 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc_mma_ts_warp(d, lo + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc_mma_ts_warp(d, hi + i * 8, tc_desc_mn(v + i * 2048, Shape::kStageBytes), kValues, 1);
-                    for (int e = 0; e < kEach; ++e)
-                        tc_commit_warp(&h.empty[stage + e]);
-                    tc_commit_warp(&h.done[buffer][part]);
-                    taken += kEach;
-                }
-                return true;
-            };
-            bool ok = warp_wait(&h.query, 0);
-            tc_fence_after();
-            ok = ok && scores(0);
-            for (int j = 0; j < tiles && ok; ++j)
-                ok = (j + 1 == tiles || scores(j + 1)) && rows(j);
-            // A failed run: the MMAs issued so far end before TMEM is given back.
-            if (!ok)
+            constexpr uint32_t kWide = tc_idesc16(0, 128, false), kNarrow = tc_idesc16(0, 64, false);
+            const uint32_t qhi = smem_addr(queries), qlo = qhi + Shape::kQueryHalf, kbase = smem_addr(keys);
+            uint64_t* landed = Tree ? h.keys_ready : h.keys_full;
+            int item = 0, count = 0; // stages and tiles before this
+            bool ok = true;
+            MmaPlace p;
+            for (int i = 0; ok && take(i, p); ++i)
             {
-                tc_commit_warp(&h.drained);
-                mbar_wait(&h.drained, 0);
+                ok = wait(&h.query, i & 1);
+                for (int j = 0; j < p.tiles && ok; ++j, ++count)
+                {
+                    for (int b = 0; b < kBlocks; ++b, ++item)
+                    {
+                        const int stage = item % KS;
+                        const bool reads = (lane & 1) && b == 0 && count > 0; // S of the last tile is in registers
+                        ok = wait(reads ? &h.scores_read : &landed[stage], (reads ? count - 1 : item / KS) & 1);
+                        if (!ok)
+                            break;
+                        tc_fence_after();
+                        const uint32_t k = kbase + stage * Shape::kStageBytes;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                        {
+                            const uint32_t at = b * 128 * 128 + e * 32;
+                            tc_mma_warp(tmem + Shape::kScores, tc_desc(qhi + at), tc_desc(k + e * 32), kWide, b > 0 || e > 0);
+                            tc_mma_warp(tmem + Shape::kScores + 64, tc_desc(qlo + at), tc_desc(k + e * 32), kNarrow, 1);
+                        }
+                        tc_commit_warp(&h.keys_free[stage]);
+                    }
+                    if (ok)
+                        tc_commit_warp(&h.scores);
+                }
+                if (ok)
+                    tc_commit_warp(&h.query_free);
+                leave(i);
             }
+            finish_mmas(!*(volatile int*) &h.dead, &h.drained[0]);
+        }
+        else if (warp == 2)
+        {
+            constexpr uint32_t kValues = tc_idesc16(0, 64, true);
+            const uint32_t vbase = smem_addr(values);
+            uint64_t* landed = Tree ? h.values_ready : h.values_full;
+            int item = 0, count = 0;
+            bool ok = true;
+            MmaPlace p;
+            for (int i = 0; ok && take(i, p); ++i)
+            {
+                for (int j = 0; j < p.tiles && ok; ++j, ++count)
+                {
+                    const int valid = valid_of(p, j), buffer = count % RB;
+                    for (int b = 0; b < kBlocks; ++b, ++item)
+                    {
+                        // The stage, the weights, and the buffer's last O in registers.
+                        const int stage = item % VS, what = lane & 3;
+                        const bool frees = what == 1 && b == 0 && count >= RB, weighs = what == 2 && b == 0;
+                        ok = wait(frees ? &h.rows_free[buffer] : weighs ? &h.weights[count & 1] : &landed[stage],
+                                  (frees ? count / RB - 1 : weighs ? count / 2 : item / VS) & 1);
+                        if (!ok)
+                            break;
+                        if (!Tree && valid < kKeyTile)
+                        {
+                            // Rows past the sequence's end: weights of 0, but 0 x NaN is not.
+                            const int bytes = (kKeyTile - valid) * 128;
+                            for (int box = 0; box < 2; ++box)
+                                for (int e = lane * 16; e < bytes; e += 512)
+                                    *reinterpret_cast<uint4*>(values + stage * Shape::kStageBytes + box * Shape::kBox
+                                                              + valid * 128 + e) = make_uint4(0, 0, 0, 0);
+                            fence_proxy_async();
+                            __syncwarp();
+                        }
+                        tc_fence_after();
+                        const uint32_t d = tmem + Shape::kRows + buffer * D + b * 64;
+                        const uint32_t hi = tmem + Shape::kWeights + (count & 1) * 64, lo = hi + 32;
+                        const uint32_t v = vbase + stage * Shape::kStageBytes;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tc_mma_ts_warp(d, hi + e * 8, tc_desc_mn(v + Shape::kBox + e * 2048, Shape::kBox), kValues, e > 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tc_mma_ts_warp(d, lo + e * 8, tc_desc_mn(v + e * 2048, Shape::kBox), kValues, 1);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tc_mma_ts_warp(d, hi + e * 8, tc_desc_mn(v + e * 2048, Shape::kBox), kValues, 1);
+                        tc_commit_warp(&h.values_free[stage]);
+                    }
+                    if (ok)
+                        tc_commit_warp(&h.done[buffer]);
+                }
+                leave(i);
+            }
+            finish_mmas(!*(volatile int*) &h.dead, &h.drained[1]);
+        }
+        else
+        {
+            // The units' places, found while the unit before is worked on.
+            int unit = blockIdx.x, i = 0;
+            bool ok = true;
+            auto publish = [&](const MmaPlace& p) {
+                ok = ok && (i < 2 || wait(&h.place_free[i & 1], (i / 2 - 1) & 1));
+                if (ok && lane == 0)
+                {
+                    h.place[i & 1] = p;
+                    mbar_arrive(&h.place_full[i & 1]);
+                }
+                ++i;
+            };
+            if (Tree)
+            {
+                const long long total = tiles_between(c, 0, a.sequences), per = tiles_per_cta(c, total);
+                const long long end = min(total, (blockIdx.x + 1) * per);
+                for (long long at = blockIdx.x * per; at < end && ok;)
+                {
+                    const MmaPlace p = tree_place(c, at, end, blockIdx.x);
+                    at += p.tiles;
+                    publish(p);
+                }
+            }
+            for (int asked = 0; !Tree && ok; ++asked)
+            {
+                if (lane == 0)
+                    ask_next_cta(&h.answer, &h.next);
+                const MmaPlace p = prompt_place(c, c.tile_tokens, unit);
+                if (p.sequence >= 0)
+                    publish(p);
+                ok = wait(&h.next, asked & 1) && ok; // an answer is never left behind
+                if (ok && !next_cta(&h.answer, unit))
+                    break;
+                __syncwarp(); // the answer has been read
+            }
+            MmaPlace end = {};
+            end.sequence = -1; // no more units
+            publish(end);
         }
     }
     else if (warp < 12)
@@ -441,230 +520,245 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         const int group = (warp - 4) >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane; // the TMEM lane
         const uint32_t lanes = tmem + ((uint32_t) (quarter * 32) << 16);
-        const int token = p.token0 + row / a.group, head = p.kv_head * a.group + row % a.group;
-        const bool real = row < c.tile_tokens * a.group && token < p.length;
-
-        // The queries' halves, a row a warp: lane c the channels [8 c, 8 c + 8).
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i)
-        {
-            const int r = (warp - 4) * 16 + i, t = p.token0 + r / a.group;
-            float x[8] = {};
-            if (r < c.tile_tokens * a.group && t < p.length && lane * 8 < a.width)
-                load8((const float*) a.q + (p.begin + t) * a.q_stride + (size_t) (p.kv_head * a.group + r % a.group) * a.width
-                          + lane * 8, x);
-            float m = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                m = fmaxf(m, finite_abs(x[e]));
-            const float factor = split_factor(warp_max(m), 15);
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                split_pair(x[2 * e], x[2 * e + 1], factor, hi[e], lo[e]);
-            if (lane < D / 8)
-            {
-                uint8_t* to = queries + (lane >> 3) * 128 * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-            if (lane == 0)
-                exchange[0][0][r] = 1.f / factor;
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-            mbar_arrive(&h.query);
-        unsigned long long path = 0;
-        if (Tree)
-            for (int i = tid - 128; i < p.length; i += 256)
-                h.parents[i] = a.parents[p.begin + i];
-        named_sync(1, 256);
-        float row_factor = exchange[0][0][row] * a.scale_log2;
-        if (Tree && real)
-            path = tree_path(h.parents, token);
-        const float* kfactors = nullptr;
-        const float* vfactors = nullptr;
-        float kfactor = 1.f, vfactor = 1.f;
-        if (Tree)
-        {
-            named_sync(2, 384); // the converters' sample
-            kfactor = 1.f / split_factor(__uint_as_float(h.sample[0]), 11);
-            vfactor = 1.f / split_factor(__uint_as_float(h.sample[1]), 11);
-        }
-        else
-        {
-            kfactors = lc.factors + (size_t) p.kv_head * lc.tiles + p.begin / kKeyTile + p.sequence;
-            vfactors = kfactors + (size_t) a.kv_heads * lc.tiles;
-        }
-        named_sync(1, 256); // the row factors are read: `exchange` is free
-
-        float acc[kHalf];
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-            acc[i] = 0.f;
-        float m = -INFINITY, l = 0.f, alpha_before = 1.f, vfactor_before = 1.f;
-        int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
-        bool ok = true;
-        // After a wait that ran out the loop goes on without waits, so that the
+        int count = 0; // tiles before this
+        // After a wait that ran out a unit goes on without waits, so that the
         // warps' barriers still match.
-        // acc = acc * alpha + (O of tile j) * factor
-        auto drain = [&](int j, float alpha, float factor) {
-            constexpr int RB = Shape::kRowBuffers;
-            const int buffer = j % RB, part = Shape::kParts == 2 ? group : 0;
-            ok = ok && warp_wait(&h.done[buffer][part], (j / RB) & 1);
-            tc_fence_after();
-            const uint32_t at = lanes + Shape::kRows + buffer * D + group * kHalf;
-            const bool scales = __any_sync(0xFFFFFFFFu, alpha != 1.f);
-#pragma unroll
-            for (int b = 0; b < kHalf; b += 16)
-            {
-                uint32_t o[16];
-                tc_ld16(at + b, o);
-                tc_wait_ld(o);
-                if (scales)
-                {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        acc[b + i] *= alpha;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    acc[b + i] = fmaf(__uint_as_float(o[i]), factor, acc[b + i]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (ok && lane == 0)
-                mbar_arrive(&h.free[buffer][part]);
-        };
-        for (int j = 0; j < tiles; ++j)
+        bool ok = true;
+        MmaPlace p;
+        for (int i = 0;; ++i)
         {
-            const int t = p.first_tile + j;
-            const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
-            if (!Tree)
+            if (any_stops(5, Tree ? 384 : 256, !ok || !take(i, p)))
+                break;
+            const int tiles = p.tiles;
+            const int token = p.token0 + row / a.group, head = p.kv_head * a.group + row % a.group;
+            const bool real = row < c.tile_tokens * a.group && token < p.length;
+            const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+
+            // The queries' halves, a row a warp: lane c the channels [8 c, 8 c + 8).
+            ok = ok && (i == 0 || wait(&h.query_free, (i - 1) & 1));
+            named_sync(1, 256); // `exchange` is free
+#pragma unroll 4
+            for (int e = 0; e < 16; ++e)
             {
-                kfactor = kfactors[j];
-                vfactor = vfactors[j];
-            }
-            ok = ok && warp_wait(&h.scores, j & 1);
-            tc_fence_after();
-            float s[32];
+                const int r = (warp - 4) * 16 + e, t = p.token0 + r / a.group;
+                float x[8] = {};
+                if (r < c.tile_tokens * a.group && t < p.length && lane * 8 < a.width)
+                    load8((const float*) a.q + (p.begin + t) * a.q_stride
+                              + (size_t) (p.kv_head * a.group + r % a.group) * a.width + lane * 8, x);
+                float largest = 0.f;
 #pragma unroll
-            for (int b = 0; b < 32; b += 16)
-            {
-                uint32_t large[16], small[16];
-                tc_ld16(lanes + Shape::kScores + group * 32 + b, large);
-                tc_ld16(lanes + Shape::kScores + 64 + group * 32 + b, small);
-                tc_wait_ld(large);
-                tc_wait_ld(small);
+                for (int k = 0; k < 8; ++k)
+                    largest = fmaxf(largest, finite_abs(x[k]));
+                const float factor = split_factor(warp_max(largest), 15);
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[b + i] = __uint_as_float(large[i]) + __uint_as_float(small[i]);
+                for (int k = 0; k < 4; ++k)
+                    split_pair(x[2 * k], x[2 * k + 1], factor, hi[k], lo[k]);
+                if (lane < D / 8)
+                {
+                    uint8_t* to = queries + (lane >> 3) * 128 * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                if (lane == 0)
+                    exchange[0][0][r] = 1.f / factor;
             }
-            tc_fence_before();
+            fence_proxy_async();
             __syncwarp();
             if (ok && lane == 0)
-                mbar_arrive(&h.scores_read);
-            // What the row does not attend to.
-            if (Tree && t >= p.tiles_cached)
+                mbar_arrive(&h.query);
+            if (Tree)
+                for (int e = tid - 128; e < p.length; e += 256)
+                    h.parents[i & 1][e] = (int8_t) min(max(a.parents[p.begin + e], -1), kTreeNodes);
+            named_sync(1, 256);
+            const float row_factor = exchange[0][0][row] * a.scale_log2;
+            unsigned path = 0; // of the half's keys
+            if (Tree && real)
+                path = (unsigned) (tree_path(h.parents[i & 1], token) >> (32 * group));
+            const float* kfactors = nullptr;
+            const float* vfactors = nullptr;
+            float kfactor = 1.f, vfactor = 1.f;
+            if (Tree)
             {
-                const uint32_t bits = (uint32_t) (path >> (32 * group));
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    s[i] = bits >> i & 1 ? s[i] : -INFINITY;
+                named_sync(2, 384); // the converters' sample
+                kfactor = 1.f / split_factor(__uint_as_float(h.sample[0]), 11);
+                vfactor = 1.f / split_factor(__uint_as_float(h.sample[1]), 11);
+                named_sync(4, 384); // it has been read
             }
             else
             {
-                const int limit = (!Tree                        ? token - j * kKeyTile + 1
-                                   : page_there(id, a.pages) ? p.cached - t * kKeyTile
-                                                              : 0)
-                                  - 32 * group;
-                if (limit < 32)
+                kfactors = lc.factors + (size_t) p.kv_head * lc.tiles + p.begin / kKeyTile + p.sequence;
+                vfactors = kfactors + (size_t) a.kv_heads * lc.tiles;
+                named_sync(1, 256); // the row factors have been read
+            }
+
+            float acc[kHalf];
+#pragma unroll
+            for (int e = 0; e < kHalf; ++e)
+                acc[e] = 0.f;
+            float m = -INFINITY, l = 0.f, alpha_before = 1.f, vfactor_before = 1.f;
+            int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
+            // acc = acc * alpha + (O of the n-th tile) * factor
+            auto drain = [&](int n, float alpha, float factor) {
+                ok = ok && wait(&h.done[n % RB], (n / RB) & 1);
+                tc_fence_after();
+                const uint32_t at = lanes + Shape::kRows + n % RB * D + group * kHalf;
+                const bool scales = __any_sync(0xFFFFFFFFu, alpha != 1.f);
+#pragma unroll
+                for (int b = 0; b < kHalf; b += 32)
+                {
+                    uint32_t o[32];
+                    tc_ld32(at + b, o);
+                    tc_wait_ld32(o);
+                    if (scales)
+                    {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            acc[b + e] *= alpha;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        acc[b + e] = fmaf(__uint_as_float(o[e]), factor, acc[b + e]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (ok && lane == 0)
+                    mbar_arrive(&h.rows_free[n % RB]);
+            };
+            for (int j = 0; j < tiles; ++j, ++count)
+            {
+                const int t = p.first_tile + j;
+                const int id_next = Tree && t + 1 < p.tiles_cached ? table[t + 1] : -1;
+                if (!Tree)
+                {
+                    kfactor = kfactors[j];
+                    vfactor = vfactors[j];
+                }
+                // S is there. The weights' buffer is free: the MMAs that read it two
+                // tiles back ended before O of that tile was drained.
+                ok = ok && wait(&h.scores, count & 1);
+                tc_fence_after();
+                float s[32];
+                {
+                    uint32_t large[32], small[32];
+                    tc_ld32(lanes + Shape::kScores + group * 32, large);
+                    tc_ld32(lanes + Shape::kScores + 64 + group * 32, small);
+                    tc_wait_ld32(large);
+                    tc_wait_ld32(small);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        s[e] = __uint_as_float(large[e]) + __uint_as_float(small[e]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (ok && lane == 0)
+                    mbar_arrive(&h.scores_read);
+                // What the row does not attend to.
+                if (Tree && t >= p.tiles_cached)
                 {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        s[i] = i < limit ? s[i] : -INFINITY;
+                    for (int e = 0; e < 32; ++e)
+                        s[e] = path >> e & 1 ? s[e] : -INFINITY;
                 }
-            }
-            id = id_next;
-            float top[4] = {s[0], s[1], s[2], s[3]};
+                else
+                {
+                    const int limit = (!Tree                        ? token - j * kKeyTile + 1
+                                       : page_there(id, a.pages) ? p.cached - t * kKeyTile
+                                                                  : 0)
+                                      - 32 * group;
+                    if (limit < 32)
+                    {
 #pragma unroll
-            for (int i = 4; i < 32; ++i)
-                top[i & 3] = fmaxf(top[i & 3], s[i]);
-            const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            exchange[j & 1][group][row] = mine;
+                        for (int e = 0; e < 32; ++e)
+                            s[e] = e < limit ? s[e] : -INFINITY;
+                    }
+                }
+                id = id_next;
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int e = 4; e < 28; e += 8)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        top[g] = max3(top[g], s[e + 2 * g], s[e + 2 * g + 1]);
+                const float mine = max3(max3(top[0], s[28], s[29]), max3(top[1], s[30], s[31]), fmaxf(top[2], top[3]));
+                exchange[j & 1][group][row] = mine;
+                named_sync(1, 256);
+                const float factor = row_factor * kfactor;
+                const float m_new = fmaxf(m, fmaxf(mine, exchange[j & 1][group ^ 1][row]) * factor);
+                const float alpha = m == m_new ? 1.f : exp2_approx(m - m_new);
+                const float base = 14.f - (m_new == -INFINITY ? 0.f : m_new);
+                m = m_new;
+                float2 sum[2] = {};
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                {
+                    const float2 x = __ffma2_rn(make_float2(s[2 * e], s[2 * e + 1]), make_float2(factor, factor),
+                                                make_float2(base, base));
+                    const float2 w = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                    sum[e & 1] = __fadd2_rn(sum[e & 1], w);
+                    const __half2 hh = __floats2half2_rn(w.x, w.y);
+                    const float2 back = __half22float2(hh);
+                    hi[e] = *reinterpret_cast<const uint32_t*>(&hh);
+                    lo[e] = pack_pair<__half>(w.x - back.x, w.y - back.y);
+                }
+                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                const uint32_t wbase = lanes + Shape::kWeights + (count & 1) * 64 + group * 16;
+                tc_st16(wbase, hi);
+                tc_st16(wbase + 32, lo);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (ok && lane == 0)
+                    mbar_arrive(&h.weights[count & 1]);
+                if (j > 0)
+                    drain(count - 1, alpha_before, vfactor_before);
+                alpha_before = alpha;
+                vfactor_before = vfactor;
+            }
+            drain(count - 1, alpha_before, vfactor_before);
+            exchange[tiles & 1][group][row] = l;
             named_sync(1, 256);
-            const float factor = row_factor * kfactor;
-            const float m_new = fmaxf(m, fmaxf(mine, exchange[j & 1][group ^ 1][row]) * factor);
-            const float alpha = m == m_new ? 1.f : exp2_approx(m - m_new);
-            const float base = 14.f - (m_new == -INFINITY ? 0.f : m_new);
-            m = m_new;
-            float sum[4] = {};
-            uint32_t hi[16], lo[16];
+            l += exchange[tiles & 1][group ^ 1][row];
+            const bool whole = !Tree || p.whole;
+            const int at = p.begin + token;
+            const size_t part = (size_t) p.part * c.part_rows + row;
+            // The weights' 2^14: cancels in a finished row, is taken off a part's.
+            const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 0x1p-14f;
+            bool finite = l < INFINITY && (!Tree || !*(volatile int*) &h.misfit[i & 1]);
+            char* mine = (char*) (whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width
+                                        : c.part_o + part * a.width);
+            const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
+            char* four[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int k = 0; k < 4; ++k)
+                four[k] = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, (lane & ~3) + k);
+#pragma unroll
+            for (int b = 0; b < kHalf; b += 16)
             {
-                const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(factor, factor),
-                                            make_float2(base, base));
-                const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
-                sum[2 * (i & 1)] += e0;
-                sum[2 * (i & 1) + 1] += e1;
-                const __half2 hh = __floats2half2_rn(e0, e1);
-                const float2 back = __half22float2(hh);
-                hi[i] = *reinterpret_cast<const uint32_t*>(&hh);
-                lo[i] = pack_pair<__half>(e0 - back.x, e1 - back.y);
+                uint32_t x[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                {
+                    finite = finite && fabsf(acc[b + e]) < INFINITY;
+                    x[e] = __float_as_uint(scaled == 0.f ? 0.f : acc[b + e] * scaled);
+                }
+                store_rows(x, four, rows, 4 * (group * kHalf + b), 4 * a.width);
             }
-            l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            // The MMAs that read this buffer two tiles back ended before S of this tile.
-            const uint32_t wbase = lanes + Shape::kWeights + (j & 1) * 64 + group * 16;
-            tc_st16(wbase, hi);
-            tc_st16(wbase + 32, lo);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (ok && lane == 0)
-                mbar_arrive(&h.weights[j & 1]);
-            if (j > 0)
-                drain(j - 1, alpha_before, vfactor_before);
-            alpha_before = alpha;
-            vfactor_before = vfactor;
-        }
-        drain(tiles - 1, alpha_before, vfactor_before);
-        exchange[tiles & 1][group][row] = l;
-        named_sync(1, 256);
-        l += exchange[tiles & 1][group ^ 1][row];
-        const bool whole = !Tree || p.whole;
-        const int at = p.begin + token;
-        const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
-        // The weights' 2^14: cancels in a finished row, is taken off a chunk's.
-        const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 0x1p-14f;
-        bool finite = l < INFINITY && (!Tree || !h.misfit);
-        float* to = whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width : c.part_o + part * a.width;
-#pragma unroll
-        for (int b = 0; b < kHalf; b += 4)
-        {
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
+            if (Tree && !whole && real && group == 0)
+                c.part_ml[part] = make_float2(m, l * 0x1p-14f);
+            exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
+            named_sync(1, 256);
+            // Rows that came out not finite: again, half of them by each warpgroup's warp.
+            unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && (!finite || exchange[(tiles & 1) ^ 1][group ^ 1][row] != 0.f));
+            again &= group ? 0xAAAAAAAAu : 0x55555555u;
+            while (again)
             {
-                finite = finite && fabsf(acc[b + i]) < INFINITY;
-                x[i] = scaled == 0.f ? 0.f : acc[b + i] * scaled;
+                const int who = __ffs(again) - 1;
+                again &= again - 1;
+                take_again<float, Tree>(c, h.place[i & 1], __shfl_sync(0xFFFFFFFFu, at, who), __shfl_sync(0xFFFFFFFFu, head, who));
             }
-            if (real && group * kHalf + b < a.width)
-                *reinterpret_cast<float4*>(to + group * kHalf + b) = make_float4(x[0], x[1], x[2], x[3]);
-        }
-        if (Tree && !whole && real && group == 0)
-            c.part_ml[part] = make_float2(m, l * 0x1p-14f);
-        exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
-        named_sync(1, 256);
-        // Rows that came out not finite: again, half of them by each warpgroup's warp.
-        unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && (!finite || exchange[(tiles & 1) ^ 1][group ^ 1][row] != 0.f));
-        again &= group ? 0xAAAAAAAAu : 0x55555555u;
-        while (again)
-        {
-            const int who = __ffs(again) - 1;
-            again &= again - 1;
-            take_again<float, Tree>(c, h.place, __shfl_sync(0xFFFFFFFFu, at, who), __shfl_sync(0xFFFFFFFFu, head, who));
+            leave(i);
         }
         tc_fence_before();
     }
@@ -672,98 +766,116 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
     {
         set_registers_down<Shape::kRegistersConvert>();
         const int t = tid - 384;
-        // The exponents: the largest of 16 keys spread over the CTA's, an eighth
-        // of their channels a thread.
-        {
-            const int end = min((p.first_tile + tiles) * kKeyTile, p.cached), from = p.first_tile * kKeyTile;
-            const int key = t >> 3;
-            const float* k = nullptr;
-            const float* v = nullptr;
-            if (end > from)
-            {
-                const int j = from + (int) ((long long) (end - from) * key / 16);
-                const int page = table[j >> kPageLog];
-                if (page_there(page, a.pages))
-                {
-                    const size_t at = (((size_t) page << kPageLog) + (j & (kPagePositions - 1))) * a.kv_heads + p.kv_head;
-                    k = (const float*) a.key_pages + at * a.width;
-                    v = (const float*) a.value_pages + at * a.width;
-                }
-            }
-            else
-            {
-                const int r = p.begin + p.length * key / 16;
-                k = (const float*) a.k + r * a.k_stride + (size_t) p.kv_head * a.width;
-                v = (const float*) a.v + r * a.v_stride + (size_t) p.kv_head * a.width;
-            }
-            float mk = 0.f, mv = 0.f;
-            for (int i = (t & 7) * 4; k && i < a.width; i += 32)
-            {
-                const float4 x = *reinterpret_cast<const float4*>(k + i), y = *reinterpret_cast<const float4*>(v + i);
-                mk = fmaxf(fmaxf(mk, fmaxf(finite_abs(x.x), finite_abs(x.y))), fmaxf(finite_abs(x.z), finite_abs(x.w)));
-                mv = fmaxf(fmaxf(mv, fmaxf(finite_abs(y.x), finite_abs(y.y))), fmaxf(finite_abs(y.z), finite_abs(y.w)));
-            }
-            mk = warp_max(mk), mv = warp_max(mv);
-            if (lane == 0)
-            {
-                atomicMax(&h.sample[0], __float_as_uint(mk));
-                atomicMax(&h.sample[1], __float_as_uint(mv));
-            }
-        }
-        named_sync(2, 384); // with the row warps, who wait for the exponents
-        const float factors[2] = {split_factor(__uint_as_float(h.sample[0]), 11),
-                                  split_factor(__uint_as_float(h.sample[1]), 11)};
         // A stage: thread t holds 32 channels (one fp32 box's row) of key t / 2.
         const int key = t >> 1, box = t & 1;
-        int taken = 0;
-        bool misfit = false, ok = true;
-        auto convert = [&](int j, int values) {
-            const bool there = key < valid_of(j);
-            const float factor = factors[values];
-            for (int b = 0; b < kBlocks; ++b)
-            {
-                const int stage = taken % S;
-                ok = ok && warp_wait(&h.full[stage], (taken / S) & 1);
-                uint8_t* at = ring + stage * Shape::kStageBytes + key * 128;
-                uint32_t hi[16], lo[16];
-                float largest = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                {
-                    float4 x = *reinterpret_cast<const float4*>(at + box * Shape::kBox + ((i ^ (key & 7)) << 4));
-                    if (!there)
-                        x = make_float4(0.f, 0.f, 0.f, 0.f); // behind the sequence: whatever the page holds
-                    largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-                    split_pair(x.x, x.y, factor, hi[2 * i], lo[2 * i]);
-                    split_pair(x.z, x.w, factor, hi[2 * i + 1], lo[2 * i + 1]);
-                }
-                // Too large for fp16, or values so small that their halves lose digits.
-                largest *= factor;
-                misfit = misfit || largest > 60000.f || (values && largest > 0.f && largest < 0x1p-6f);
-                named_sync(3, 128); // all of the stage's fp32 is in registers
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    const int chunk = ((box * 4 + i) ^ (key & 7)) << 4;
-                    *reinterpret_cast<uint4*>(at + chunk) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-                    *reinterpret_cast<uint4*>(at + Shape::kBox + chunk) =
-                        make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-                }
-                if (misfit)
-                    h.misfit = 1;
-                fence_proxy_async();
-                __syncwarp();
-                if (ok && lane == 0)
-                    mbar_arrive(&h.ready[stage]);
-                ++taken;
-            }
-        };
-        for (int j = 0; j <= tiles; ++j)
+        int taken_keys = 0, taken_values = 0;
+        bool ok = true; // as with the row warps
+        MmaPlace p;
+        for (int i = 0;; ++i)
         {
-            if (j < tiles)
-                convert(j, 0);
-            if (j > 0)
-                convert(j - 1, 1);
+            if (any_stops(5, 384, !ok || !take(i, p)))
+                break;
+            const int tiles = p.tiles;
+            const int* table = a.table + (size_t) p.sequence * a.table_stride;
+            // The exponents: the largest of 16 keys spread over the unit's, an
+            // eighth of their channels a thread.
+            {
+                const int end = min((p.first_tile + tiles) * kKeyTile, p.cached), from = p.first_tile * kKeyTile;
+                const int which = t >> 3;
+                const float* k = nullptr;
+                const float* v = nullptr;
+                if (end > from)
+                {
+                    const int j = from + (int) ((long long) (end - from) * which / 16);
+                    const int page = table[j >> kPageLog];
+                    if (page_there(page, a.pages))
+                    {
+                        const size_t at = (((size_t) page << kPageLog) + (j & (kPagePositions - 1))) * a.kv_heads + p.kv_head;
+                        k = (const float*) a.key_pages + at * a.width;
+                        v = (const float*) a.value_pages + at * a.width;
+                    }
+                }
+                else
+                {
+                    const int r = p.begin + p.length * which / 16;
+                    k = (const float*) a.k + r * a.k_stride + (size_t) p.kv_head * a.width;
+                    v = (const float*) a.v + r * a.v_stride + (size_t) p.kv_head * a.width;
+                }
+                float mk = 0.f, mv = 0.f;
+                for (int e = (t & 7) * 4; k && e < a.width; e += 32)
+                {
+                    const float4 x = *reinterpret_cast<const float4*>(k + e), y = *reinterpret_cast<const float4*>(v + e);
+                    mk = fmaxf(fmaxf(mk, fmaxf(finite_abs(x.x), finite_abs(x.y))), fmaxf(finite_abs(x.z), finite_abs(x.w)));
+                    mv = fmaxf(fmaxf(mv, fmaxf(finite_abs(y.x), finite_abs(y.y))), fmaxf(finite_abs(y.z), finite_abs(y.w)));
+                }
+                mk = warp_max(mk), mv = warp_max(mv);
+                if (lane == 0)
+                {
+                    atomicMax(&h.sample[0], __float_as_uint(mk));
+                    atomicMax(&h.sample[1], __float_as_uint(mv));
+                }
+            }
+            named_sync(2, 384); // with the row warps, who wait for the exponents
+            const float factors[2] = {split_factor(__uint_as_float(h.sample[0]), 11),
+                                      split_factor(__uint_as_float(h.sample[1]), 11)};
+            named_sync(4, 384);
+            if (t == 0)
+            {
+                h.sample[0] = h.sample[1] = 0;
+                h.misfit[(i & 1) ^ 1] = 0; // the last unit's has been read: its rows are stored
+            }
+            named_sync(3, 128);
+            bool misfit = false;
+            auto convert = [&](int j, float factor, bool is_value, uint8_t* ring, int& taken, int stages, uint64_t* full,
+                               uint64_t* ready) {
+                const bool there = key < valid_of(p, j);
+                for (int b = 0; b < kBlocks; ++b)
+                {
+                    const int stage = taken % stages;
+                    ok = ok && wait(&full[stage], (taken / stages) & 1);
+                    uint8_t* at = ring + stage * Shape::kStageBytes + key * 128;
+                    uint32_t hi[16], lo[16];
+                    float largest = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                    {
+                        float4 x = *reinterpret_cast<const float4*>(at + box * Shape::kBox + ((e ^ (key & 7)) << 4));
+                        if (!there)
+                            x = make_float4(0.f, 0.f, 0.f, 0.f); // behind the sequence: whatever the page holds
+                        largest = fmaxf(fmaxf(largest, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+                        split_pair(x.x, x.y, factor, hi[2 * e], lo[2 * e]);
+                        split_pair(x.z, x.w, factor, hi[2 * e + 1], lo[2 * e + 1]);
+                    }
+                    // Too large for fp16, or values so small that their halves lose digits.
+                    largest *= factor;
+                    misfit = misfit || largest > 60000.f || (is_value && largest > 0.f && largest < 0x1p-6f);
+                    named_sync(3, 128); // all of the stage's fp32 is in registers
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        const int chunk = ((box * 4 + e) ^ (key & 7)) << 4;
+                        *reinterpret_cast<uint4*>(at + chunk) =
+                            make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+                        *reinterpret_cast<uint4*>(at + Shape::kBox + chunk) =
+                            make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
+                    }
+                    if (misfit)
+                        *(volatile int*) &h.misfit[i & 1] = 1;
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (ok && lane == 0)
+                        mbar_arrive(&ready[stage]);
+                    ++taken;
+                }
+            };
+            for (int j = 0; j <= tiles; ++j)
+            {
+                if (j < tiles)
+                    convert(j, factors[0], false, keys, taken_keys, KS, h.keys_full, h.keys_ready);
+                if (j > 0)
+                    convert(j - 1, factors[1], true, values, taken_values, VS, h.values_full, h.values_ready);
+            }
+            leave(i);
         }
     }
     __syncthreads();

@@ -10,9 +10,10 @@
 // keys, in tiles of 64 (a page).
 //
 // Roles:
-//  warp 0   places and copies: query tiles, then key and value tiles, each
-//           through a ring of its own (tensor maps; a page is one box), on into
-//           the next unit as far as there is room. Of a ring that both passed
+//  places   a warp finds the next unit while this one is worked on;
+//  copies   query tiles, then key and value tiles, each through a ring of its
+//           own (tensor maps; a page is one box), on into the next unit as far
+//           as there is room. Of a ring that both passed
 //           through, a warp that takes only the keys would see every other phase of
 //           a stage's barrier, and its parity cannot tell a phase from the one
 //           two before;
@@ -24,7 +25,7 @@
 //           scores to registers, maximum, weights, the weights in T back to TMEM
 //           in one of two buffers (P, the A operand of O += P V), at the end
 //           the row itself.
-// A CTA takes unit after unit: it cancels the launch of a CTA that has not
+// A CTA takes unit after unit. Of prompts, it cancels the launch of a CTA that has not
 // started and does its work (the order stays the grid's, longest rows first), so
 // that the next unit's copies and scores run under this one's last steps.
 // The maximum that the weights are taken against follows the true one lazily:
@@ -39,9 +40,9 @@
 // attend to it: every row that comes out not finite is taken again by
 // attention_row, which reads only what the row attends to.
 //
-// A tree's keys may be cut into chunks over several CTAs (`chunk_tiles` tiles
-// each): each leaves its rows' maximum, sum and unnormalised O in the
-// workspace, and attention_join puts them together.
+// A batch of trees is shared out evenly in key tiles, so a query tile's keys may
+// lie with several CTAs: each leaves its rows' maximum, sum and unnormalised O in
+// the workspace, and attention_join puts them together.
 #pragma once
 
 #include "attention_rows.cuh"
@@ -58,12 +59,11 @@ __device__ unsigned g_operator_error;
 struct MmaCall
 {
     AttnCall a;
-    int tile_tokens;  // tokens of a query tile: 128 / group
-    int row_tiles;    // a tree's CTAs along its nodes
-    int chunk_tiles;  // key tiles of a chunk (a tree's)
-    int chunks;       // most chunks of a sequence; 1: the rows are finished here
-    float* part_o;    // [chunks][rows][heads][width]
-    float2* part_ml;  // [chunks][rows][heads]
+    int tile_tokens; // tokens of a query tile: 128 / group
+    int ctas;        // a tree's: its key tiles are shared out to that many
+    int part_rows;   // rows of a part: a query tile's at most
+    float* part_o;   // [2 ctas][part_rows][width]
+    float2* part_ml; // [2 ctas][part_rows]
 };
 
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the
@@ -130,7 +130,7 @@ struct MmaShape
     static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
     static constexpr int kKeyStages = kStages / 2, kValueStages = kStages - kKeyStages;
     static constexpr int kSmem = kHead + kQueryBytes + kStages * kStageBytes;
-    static constexpr int kThreads = 128 + 128 * NQ + (NQ == 2 ? 32 : 0); // the last warp: MMAs
+    static constexpr int kThreads = 128 + 128 * NQ + (NQ == 2 ? 64 : 0); // the last warps: MMAs, places
     static_assert(kScoreColumns + NQ * D <= kTmem && kStages >= 4, "what an SM holds");
 };
 
@@ -139,10 +139,10 @@ struct MmaPlace
 {
     int sequence; // -1: nothing to do; published: no more units
     int begin, length; // its first row, its rows (a tree's nodes)
-    int token0, kv_head, chunk;
+    int token0, kv_head, part;
     int cached, tiles_cached; // a tree's
     int first_tile, tiles;    // its key tiles
-    bool whole;               // the only chunk: finish the rows
+    bool whole;               // all of its keys: finish the rows
 };
 
 struct MmaHead
@@ -235,45 +235,114 @@ __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequen
     }
 }
 
-// Where unit `unit` (a CTA of the grid) works, its rows in steps of `step` tokens;
-// by a whole warp.
-template <bool Tree>
-__device__ inline MmaPlace find_place(const MmaCall& c, int step, int unit)
+// Where unit `unit` (a CTA of the grid) of packed prompts works, its rows in steps
+// of `step` tokens; by a whole warp.
+__device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
 {
     const AttnCall& a = c.a;
     MmaPlace p = {};
-    p.sequence = -1;
-    if (Tree)
+    int s, tile = 0;
+    p.kv_head = unit % a.kv_heads;
+    find_tile(a, step, unit / a.kv_heads, s, tile);
+    p.sequence = s;
+    if (s >= 0)
     {
-        int u = unit;
-        p.chunk = u % c.chunks, u /= c.chunks;
-        p.kv_head = u % a.kv_heads, u /= a.kv_heads;
-        p.token0 = u % c.row_tiles * step;
-        const int s = u / c.row_tiles;
         p.begin = bounded_offset(a.offsets, s, a.rows);
-        p.length = min(bounded_offset(a.offsets, s + 1, a.rows) - p.begin, a.max_nodes);
-        p.cached = min(max(a.lengths[s], 0), a.max_length);
-        p.tiles_cached = (p.cached + kKeyTile - 1) / kKeyTile;
-        p.first_tile = p.chunk * c.chunk_tiles;
-        p.tiles = min(c.chunk_tiles, p.tiles_cached + 1 - p.first_tile); // + 1: the drafted tile
-        p.whole = p.tiles_cached < c.chunk_tiles;
-        if (p.token0 < p.length && p.tiles > 0)
-            p.sequence = s;
+        p.length = bounded_offset(a.offsets, s + 1, a.rows) - p.begin;
+        p.token0 = tile * step;
+        p.tiles = (min(p.token0 + step, p.length) - 1) / kKeyTile + 1;
+        p.whole = true;
     }
-    else
+    return p;
+}
+
+// A batch of trees is one row of key tiles: sequence after sequence, in it query tile
+// after query tile of each kv head, of each its cached tiles and the drafted one.
+// Every CTA takes `per` of them in a piece, whatever sequences it falls on, so
+// that sequences of any lengths keep all CTAs busy to the end. A query tile that a
+// CTA holds whole is finished there; of one that several share, each leaves a
+// part: part 2 cta of the query tile that its piece begins in, part 2 cta + 1 of the
+// one that begins in its piece.
+struct TreeRow
+{
+    int nodes, cached, tiles, query_tiles; // of a sequence; tiles a query tile
+    __device__ long long total() const { return (long long) tiles * query_tiles; }
+};
+
+__device__ __forceinline__ TreeRow tree_row(const MmaCall& c, int s)
+{
+    const AttnCall& a = c.a;
+    TreeRow r = {};
+    if (s >= a.sequences)
+        return r;
+    const int begin = bounded_offset(a.offsets, s, a.rows);
+    r.nodes = max(min(bounded_offset(a.offsets, s + 1, a.rows) - begin, a.max_nodes), 0);
+    r.cached = min(max(a.lengths[s], 0), a.max_length);
+    r.tiles = (r.cached + kKeyTile - 1) / kKeyTile + 1;
+    r.query_tiles = (r.nodes + c.tile_tokens - 1) / c.tile_tokens * a.kv_heads;
+    return r;
+}
+
+// The tiles of sequences [begin, end); by a whole warp.
+__device__ inline long long tiles_between(const MmaCall& c, int begin, int end)
+{
+    long long sum = 0;
+#pragma unroll 4
+    for (int s = begin + (threadIdx.x & 31); s < end; s += 32)
+        sum += tree_row(c, s).total();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    return sum;
+}
+
+// A CTA's piece: at least four tiles, so that few rows are not cut into more parts than
+// they are worth.
+__device__ __forceinline__ long long tiles_per_cta(const MmaCall& c, long long total)
+{
+    return max((total + c.ctas - 1) / c.ctas, 4ll);
+}
+
+// The place of the tiles from `at` on, up to `end`; by a whole warp. `cta` takes them.
+__device__ inline MmaPlace tree_place(const MmaCall& c, long long at, long long end, int cta)
+{
+    const AttnCall& a = c.a;
+    const int lane = threadIdx.x & 31;
+    MmaPlace p = {};
+    p.sequence = -1;
+    long long before = 0;
+    for (int base = 0; base < a.sequences; base += 32)
     {
-        int s, tile = 0;
-        p.kv_head = unit % a.kv_heads;
-        find_tile(a, step, unit / a.kv_heads, s, tile);
-        if (s >= 0)
+        const TreeRow mine = tree_row(c, base + lane);
+        long long sum = mine.total();
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
         {
-            p.sequence = s;
-            p.begin = bounded_offset(a.offsets, s, a.rows);
-            p.length = bounded_offset(a.offsets, s + 1, a.rows) - p.begin;
-            p.token0 = tile * step;
-            p.tiles = (min(p.token0 + step, p.length) - 1) / kKeyTile + 1;
-            p.whole = true;
+            const long long up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+            if (lane >= o)
+                sum += up;
         }
+        const unsigned beyond = __ballot_sync(0xFFFFFFFFu, before + sum > at);
+        if (beyond)
+        {
+            const int who = __ffs(beyond) - 1;
+            const long long start = before + __shfl_sync(0xFFFFFFFFu, sum - mine.total(), who);
+            const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), query_tile = (int) ((at - start) / tiles);
+            const int within = (int) ((at - start) % tiles);
+            p.sequence = base + who;
+            p.begin = bounded_offset(a.offsets, p.sequence, a.rows);
+            p.length = __shfl_sync(0xFFFFFFFFu, mine.nodes, who);
+            p.cached = __shfl_sync(0xFFFFFFFFu, mine.cached, who);
+            p.tiles_cached = tiles - 1;
+            p.kv_head = query_tile % a.kv_heads;
+            p.token0 = query_tile / a.kv_heads * c.tile_tokens;
+            p.first_tile = within;
+            p.tiles = (int) min((long long) (tiles - p.first_tile), end - at);
+            p.whole = p.tiles == tiles;
+            p.part = 2 * cta + (p.first_tile == 0);
+            return p;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, sum, 31);
     }
     return p;
 }
@@ -297,7 +366,7 @@ __device__ __noinline__ void take_again(const MmaCall& c, const MmaPlace& p, int
     if (at < a.width)
         load8((const T*) a.q + row * a.q_stride + (size_t) head * a.width + at, q);
     attend_row<T, Tree>(a, keys, p.kv_head, q, from, to, m, l, acc);
-    const size_t part = ((size_t) p.chunk * a.rows + row) * a.heads + head;
+    const size_t part = (size_t) p.part * c.part_rows + (row - p.begin - p.token0) * a.group + head % a.group;
     if (at < a.width)
         store8(c.part_o + part * a.width + at, acc);
     if (at == 0)
@@ -307,6 +376,19 @@ __device__ __noinline__ void take_again(const MmaCall& c, const MmaPlace& p, int
 __device__ __forceinline__ void named_sync(int id, int threads)
 {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Whether any of the barrier's threads wants to stop: warps that share barriers leave
+// their loops together.
+__device__ __forceinline__ bool any_stops(int id, int threads, bool stop)
+{
+    uint32_t any;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.or.aligned.pred q, %1, %2, p;\n"
+                 " selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(any)
+                 : "r"(id), "r"(threads), "r"((uint32_t) stop)
+                 : "memory");
+    return any;
 }
 
 // A failed run: the MMAs that the warp has issued end before TMEM is given back.
@@ -393,7 +475,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         for (int b = 0; b < 2; ++b)
         {
             mbar_init(&h.place_full[b], 1);
-            mbar_init(&h.place_free[b], 6 * NQ); // an arrival a warp but the first
+            mbar_init(&h.place_free[b], 6 * NQ + 1); // an arrival a warp but the one that finds them
         }
         for (int q = 0; q < NQ; ++q)
         {
@@ -459,7 +541,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 
     if (warp == 0)
     {
-        int put_keys = 0, put_values = 0, unit = blockIdx.x, i = 0;
+        int put_keys = 0, put_values = 0;
         bool ok = true;
         auto one_wait = [&](uint64_t* bar, unsigned parity) {
             if (ok && !thread_wait(bar, parity))
@@ -469,91 +551,110 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             }
             return ok;
         };
-        for (int asked = 0; ok; ++asked)
+        MmaPlace p;
+        for (int i = 0; ok && take(i, p); ++i)
+        {
+            const int tiles = p.tiles;
+            const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+            auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id, uint8_t* ring, int& put,
+                            int stages, uint64_t* full, uint64_t* free) {
+                const int stage = put % stages;
+                if (!ok || (put >= stages && !one_wait(&free[stage], (put / stages - 1) & 1)))
+                    return;
+                const bool cached = Tree && p.first_tile + j < p.tiles_cached;
+                // A page that is not there is read past the pool's end: zeros.
+                const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                       : p.begin + (Tree ? 0 : j * kKeyTile);
+                mbar_expect_tx(&full[stage], Shape::kStageBytes);
+                for (int b = 0; b < kBlocks; ++b)
+                    tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
+                                p.kv_head, row, &full[stage]);
+                ++put;
+            };
+            int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
+            for (int j = 0; j <= tiles; ++j)
+            {
+                int id = -1;
+                if (Tree)
+                {
+                    if ((j & 31) == 0)
+                    {
+                        const int t = p.first_tile + j + lane;
+                        ids = t < p.tiles_cached ? table[t] : -1;
+                    }
+                    id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
+                }
+                if (lane == 0)
+                {
+                    if (j < tiles)
+                        load(j, &kmap, &kpages, id, keys, put_keys, KS, h.keys_full, h.keys_free);
+                    if (j == 0 && ok && (i == 0 || one_wait(&h.query_free, (i - 1) & 1)))
+                    {
+                        mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
+                        for (int b = 0; b < NQ * kBlocks; ++b)
+                            tensor_load(queries + b * 128 * 128, &qmap, 64 * (b % kBlocks), p.kv_head * a.group,
+                                        p.begin + p.token0 + b / kBlocks * c.tile_tokens, &h.query);
+                    }
+                    if (j > 0)
+                        load(j - 1, &vmap, &vpages, id_before, values, put_values, VS, h.values_full, h.values_free);
+                }
+                id_before = id;
+                __syncwarp();
+            }
+            ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+            leave(i);
+        }
+        // Every copy has landed before the CTA may end (only a failed run gets here early).
+        if (lane == 0 && *(volatile int*) &h.dead)
+        {
+            mbar_wait(&h.query, 0);
+            for (int n = max(0, put_keys - KS); n < put_keys; ++n)
+                mbar_wait(&h.keys_full[n % KS], (n / KS) & 1);
+            for (int n = max(0, put_values - VS); n < put_values; ++n)
+                mbar_wait(&h.values_full[n % VS], (n / VS) & 1);
+        }
+        __syncwarp();
+    }
+    else if (warp == (NQ == 2 ? 13 : 3))
+    {
+        // The units' places, found while the unit before is worked on.
+        int unit = blockIdx.x, i = 0;
+        bool ok = true;
+        auto publish = [&](const MmaPlace& p) {
+            ok = ok && (i < 2 || wait(&h.place_free[i & 1], (i / 2 - 1) & 1));
+            if (ok && lane == 0)
+            {
+                h.place[i & 1] = p;
+                mbar_arrive(&h.place_full[i & 1]);
+            }
+            ++i;
+        };
+        if (Tree)
+        {
+            const long long total = tiles_between(c, 0, a.sequences), per = tiles_per_cta(c, total);
+            const long long end = min(total, (blockIdx.x + 1) * per);
+            for (long long at = blockIdx.x * per; at < end && ok;)
+            {
+                const MmaPlace p = tree_place(c, at, end, blockIdx.x);
+                at += p.tiles;
+                publish(p);
+            }
+        }
+        for (int asked = 0; !Tree && ok; ++asked)
         {
             if (lane == 0)
                 ask_next_cta(&h.answer, &h.next);
-            const MmaPlace p = find_place<Tree>(c, c.tile_tokens * NQ, unit);
+            const MmaPlace p = prompt_place(c, c.tile_tokens * NQ, unit);
             if (p.sequence >= 0)
-            {
-                if (lane == 0 && (i < 2 || one_wait(&h.place_free[i & 1], (i / 2 - 1) & 1)))
-                {
-                    h.place[i & 1] = p;
-                    mbar_arrive(&h.place_full[i & 1]);
-                }
-                const int tiles = p.tiles;
-                const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
-                auto load = [&](int j, const CUtensorMap* drafted, const CUtensorMap* paged, int id, uint8_t* ring, int& put,
-                                int stages, uint64_t* full, uint64_t* free) {
-                    const int stage = put % stages;
-                    if (!ok || (put >= stages && !one_wait(&free[stage], (put / stages - 1) & 1)))
-                        return;
-                    const bool cached = Tree && p.first_tile + j < p.tiles_cached;
-                    // A page that is not there is read past the pool's end: zeros.
-                    const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
-                                           : p.begin + (Tree ? 0 : j * kKeyTile);
-                    mbar_expect_tx(&full[stage], Shape::kStageBytes);
-                    for (int b = 0; b < kBlocks; ++b)
-                        tensor_load(ring + stage * Shape::kStageBytes + b * Shape::kBox, cached ? paged : drafted, 64 * b,
-                                    p.kv_head, row, &full[stage]);
-                    ++put;
-                };
-                int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
-                for (int j = 0; j <= tiles; ++j)
-                {
-                    int id = -1;
-                    if (Tree)
-                    {
-                        if ((j & 31) == 0)
-                        {
-                            const int t = p.first_tile + j + lane;
-                            ids = t < p.tiles_cached ? table[t] : -1;
-                        }
-                        id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
-                    }
-                    if (lane == 0)
-                    {
-                        if (j < tiles)
-                            load(j, &kmap, &kpages, id, keys, put_keys, KS, h.keys_full, h.keys_free);
-                        if (j == 0 && ok && (i == 0 || one_wait(&h.query_free, (i - 1) & 1)))
-                        {
-                            mbar_expect_tx(&h.query, NQ * kBlocks * 128 * a.group * c.tile_tokens);
-                            for (int b = 0; b < NQ * kBlocks; ++b)
-                                tensor_load(queries + b * 128 * 128, &qmap, 64 * (b % kBlocks), p.kv_head * a.group,
-                                            p.begin + p.token0 + b / kBlocks * c.tile_tokens, &h.query);
-                        }
-                        if (j > 0)
-                            load(j - 1, &vmap, &vpages, id_before, values, put_values, VS, h.values_full, h.values_free);
-                    }
-                    id_before = id;
-                    __syncwarp();
-                }
-                ++i;
-            }
-            ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                publish(p);
             ok = wait(&h.next, asked & 1) && ok; // an answer is never left behind
             if (ok && !next_cta(&h.answer, unit))
                 break;
             __syncwarp(); // the answer has been read
         }
-        if (lane == 0)
-        {
-            if (ok && (i < 2 || one_wait(&h.place_free[i & 1], (i / 2 - 1) & 1)))
-            {
-                h.place[i & 1].sequence = -1; // no more units
-                mbar_arrive(&h.place_full[i & 1]);
-            }
-            // Every copy has landed before the CTA may end (only a failed run gets here early).
-            if (!ok)
-            {
-                mbar_wait(&h.query, 0);
-                for (int n = max(0, put_keys - KS); n < put_keys; ++n)
-                    mbar_wait(&h.keys_full[n % KS], (n / KS) & 1);
-                for (int n = max(0, put_values - VS); n < put_values; ++n)
-                    mbar_wait(&h.values_full[n % VS], (n / VS) & 1);
-            }
-        }
-        __syncwarp();
+        MmaPlace end = {};
+        end.sequence = -1; // no more units
+        publish(end);
     }
     else if (warp <= NQ)
     {
@@ -659,8 +760,11 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         int count = 0; // tiles before this
         bool ok = true;
         MmaPlace p;
-        for (int i = 0; ok && take(i, p); ++i)
+        for (int i = 0;; ++i)
         {
+            const bool stop = !ok || !take(i, p);
+            if (Tree ? any_stops(1 + q, 128, stop) : stop)
+                break;
             const int n = tiles_of(p, q);
             const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
             const bool real = row < c.tile_tokens * a.group && token < p.length;
@@ -771,7 +875,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 ok = ok && wait(&h.done[q][(count - 1) & 1], ((count - 1) / 2) & 1);
                 tc_fence_after();
                 const int at = p.begin + token; // the row of q and out
-                const size_t part = ((size_t) p.chunk * a.rows + at) * a.heads + head;
+                const size_t part = (size_t) p.part * c.part_rows + row;
                 const bool whole = !Tree || p.whole;
                 const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
                 bool finite = l < INFINITY;
@@ -840,40 +944,47 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         tc_dealloc(tmem, Shape::kTmem);
 }
 
-// Joins a tree's chunks: a warp a (row, head), lane c the channels [8 c, 8 c + 8).
-// Rows of one chunk are finished already.
+// Joins a query tile's parts: a warp a (row, head), lane c the channels [8 c, 8 c +
+// 8). What one CTA held whole is finished already.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ MmaCall c)
 {
-    pdl_wait();
     const AttnCall& a = c.a;
     const long long unit = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
     const int row = (int) (unit / a.heads), head = (int) (unit % a.heads), at = (threadIdx.x & 31) * 8;
-    if (row >= a.rows)
-        return;
-    const int s = sequence_of(a.offsets, a.sequences, a.rows, row);
-    if (s < 0 || row - bounded_offset(a.offsets, s, a.rows) >= a.max_nodes)
-        return;
-    const int tiles = (min(max(a.lengths[s], 0), a.max_length) + kKeyTile - 1) / kKeyTile + 1;
-    const int chunks = (tiles + c.chunk_tiles - 1) / c.chunk_tiles;
-    if (chunks == 1)
-        return;
-    float m = -INFINITY;
-    for (int i = 0; i < chunks; ++i)
-        m = fmaxf(m, c.part_ml[((size_t) i * a.rows + row) * a.heads + head].x);
-    float l = 0.f, acc[8] = {};
-    for (int i = 0; i < chunks; ++i)
+    const int s = row < a.rows ? sequence_of(a.offsets, a.sequences, a.rows, row) : -1;
+    const int node = s < 0 ? 0 : row - bounded_offset(a.offsets, s, a.rows);
+    if (s < 0 || node >= a.max_nodes)
     {
-        const size_t part = ((size_t) i * a.rows + row) * a.heads + head;
-        const float2 ml = c.part_ml[part];
-        if (ml.y == 0.f) // nothing attended in this chunk
+        pdl_wait();
+        return;
+    }
+    const TreeRow mine = tree_row(c, s);
+    const long long before = tiles_between(c, 0, s), total = before + tiles_between(c, s, a.sequences);
+    const long long per = tiles_per_cta(c, total);
+    const long long first =
+        before + (long long) (node / c.tile_tokens * a.kv_heads + head / a.group) * mine.tiles;
+    const int from = (int) (first / per), to = (int) ((first + mine.tiles - 1) / per);
+    pdl_wait();
+    if (from == to)
+        return;
+    const int within = node % c.tile_tokens * a.group + head % a.group;
+    auto part_of = [&](int cta) { return (size_t) (2 * cta + (cta == from)) * c.part_rows + within; };
+    float m = -INFINITY;
+    for (int i = from; i <= to; ++i)
+        m = fmaxf(m, c.part_ml[part_of(i)].x);
+    float l = 0.f, acc[8] = {};
+    for (int i = from; i <= to; ++i)
+    {
+        const float2 ml = c.part_ml[part_of(i)];
+        if (ml.y == 0.f) // nothing attended there
             continue;
         const float w = ml.x == m ? 1.f : exp2f(ml.x - m);
         l += w * ml.y;
         if (at < a.width)
         {
             float x[8];
-            load8(c.part_o + part * a.width + at, x);
+            load8(c.part_o + part_of(i) * a.width + at, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 acc[e] = fmaf(w, x[e], acc[e]);

@@ -117,7 +117,8 @@ struct RowKeys
 
 // Bit i set for the nodes on the path from node n up (n < 64 nodes of a tree,
 // parents within the tree; a parent that is not before its child ends the path).
-__device__ __forceinline__ unsigned long long tree_path(const int* parents, int n)
+template <typename Int>
+__device__ __forceinline__ unsigned long long tree_path(const Int* parents, int n)
 {
     unsigned long long path = 0;
     for (int i = n; i >= 0;)

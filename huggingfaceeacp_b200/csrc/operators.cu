@@ -245,29 +245,16 @@ bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int h
 // ---- attention_mma ---------------------------------------------------------------
 constexpr int kSms = 148; // a B200's; the work is cut for it wherever the call is checked
 
-// How a tree's keys are cut: `chunks` chunks of `chunk_tiles` key tiles at most.
-// A CTA a (sequence, kv head, row tile, chunk): chunks enough for about three
-// CTAs a place on the GPU at the longest length, so that shorter sequences and
-// the last CTAs leave little of it idle, but at least four tiles each.
-struct TreePlan
+// A tree's CTAs, one a place on the GPU, and the rows of a part that it leaves.
+int tree_ctas(int dtype, int width)
 {
-    int row_tiles, chunk_tiles, chunks;
-};
-
-TreePlan tree_plan(int dtype, int sequences, int heads, int kv_heads, int width, int max_nodes, int max_length)
-{
-    const int tokens = 128 / (heads / kv_heads);
-    const int row_tiles = (max_nodes + tokens - 1) / tokens;
-    const int tiles = (max_length + kKeyTile - 1) / kKeyTile + 1;
-    const int64_t units = (int64_t) sequences * kv_heads * row_tiles, places = kSms * (dtype != HF_DTYPE_F32 && width <= 128 ? 2 : 1);
-    const int64_t wanted = std::min<int64_t>((3 * places + units - 1) / units, (tiles + 3) / 4);
-    const int chunk_tiles = (int) ((tiles + wanted - 1) / std::max<int64_t>(wanted, 1));
-    return {row_tiles, chunk_tiles, (tiles + chunk_tiles - 1) / chunk_tiles};
+    return kSms * (dtype != HF_DTYPE_F32 && width <= 128 ? 2 : 1);
 }
 
-uint64_t part_bytes(const TreePlan& plan, int rows, int heads, int width)
+int part_rows(int heads, int kv_heads, int max_nodes)
 {
-    return plan.chunks == 1 ? 0 : (uint64_t) plan.chunks * rows * heads * (4 * (uint64_t) width + 8);
+    const int group = heads / kv_heads;
+    return std::min(128 / group, max_nodes) * group;
 }
 
 template <typename T, int D, int NQ, bool Tree>
@@ -293,7 +280,6 @@ int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
     MmaCall c = {};
     c.a = a;
     c.tile_tokens = 128 / a.group;
-    c.chunks = 1;
     // Two query tiles a CTA read the keys half as often; with fewer of them
     // than SMs the rows are spread over twice the CTAs instead.
     const int64_t pairs = (int64_t) a.rows * a.heads / 256;
@@ -315,17 +301,14 @@ int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
                    : launch_mma<T, 64, 1, false>(maps, c, ctas, device, stream);
 }
 
-// A tree's call and its CTAs.
-int64_t tree_call(MmaCall* c, const AttnCall& a, const TreePlan& plan, void* workspace)
+void tree_call(MmaCall* c, int dtype, const AttnCall& a, void* workspace)
 {
     c->a = a;
     c->tile_tokens = 128 / a.group;
-    c->row_tiles = plan.row_tiles;
-    c->chunk_tiles = plan.chunk_tiles;
-    c->chunks = plan.chunks;
+    c->ctas = tree_ctas(dtype, a.width);
+    c->part_rows = part_rows(a.heads, a.kv_heads, a.max_nodes);
     c->part_o = (float*) workspace;
-    c->part_ml = (float2*) (c->part_o + (size_t) plan.chunks * a.rows * a.heads * a.width);
-    return (int64_t) a.sequences * a.kv_heads * plan.row_tiles * plan.chunks;
+    c->part_ml = (float2*) (c->part_o + (size_t) 2 * c->ctas * c->part_rows * a.width);
 }
 
 template <typename T>
@@ -336,14 +319,13 @@ int join(const MmaCall& c, cudaStream_t stream)
 }
 
 template <typename T>
-int tree_mma(int dtype, const AttnCall& a, const TreePlan& plan, void* workspace, int device, cudaStream_t stream)
+int tree_mma(int dtype, const AttnCall& a, void* workspace, int device, cudaStream_t stream)
 {
     MmaCall c = {};
-    const int64_t ctas = tree_call(&c, a, plan, workspace);
+    tree_call(&c, dtype, a, workspace);
+    const int ctas = c.ctas;
     CUtensorMap maps[5] = {};
     const int64_t positions = (int64_t) a.pages * kPagePositions;
-    if (ctas > INT32_MAX)
-        return HF_E_SHAPE;
     if (!encode_rows(&maps[0], dtype, a.q, a.width, a.heads, a.rows, a.q_stride, a.group, c.tile_tokens)
         || !encode_rows(&maps[1], dtype, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kKeyTile)
         || !encode_rows(&maps[2], dtype, a.v, a.width, a.kv_heads, a.rows, a.v_stride, 1, kKeyTile)
@@ -353,7 +335,7 @@ int tree_mma(int dtype, const AttnCall& a, const TreePlan& plan, void* workspace
     const int rc = a.width > 128  ? launch_mma<T, 256, 1, true>(maps, c, ctas, device, stream)
                    : a.width > 64 ? launch_mma<T, 128, 1, true>(maps, c, ctas, device, stream)
                                   : launch_mma<T, 64, 1, true>(maps, c, ctas, device, stream);
-    return rc || plan.chunks == 1 ? rc : join<T>(c, stream);
+    return rc ? rc : join<T>(c, stream);
 }
 
 // ---- attention_limbs (fp32) --------------------------------------------------------
@@ -393,7 +375,6 @@ int packed_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t st
     LimbCall l = {};
     l.c.a = a;
     l.c.tile_tokens = 128 / a.group;
-    l.c.chunks = 1;
     l.limbs = (__half*) workspace;
     l.tiles = limb_tiles(a.rows, a.sequences);
     const size_t limb = (size_t) a.rows * a.kv_heads * a.width;
@@ -414,13 +395,12 @@ int packed_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t st
                           : launch_limbs<64, false>(maps, l, ctas, device, stream);
 }
 
-int tree_limbs(const AttnCall& a, const TreePlan& plan, void* workspace, int device, cudaStream_t stream)
+int tree_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t stream)
 {
     LimbCall l = {};
     MmaCall& c = l.c;
-    const int64_t ctas = tree_call(&c, a, plan, workspace);
-    if (ctas > INT32_MAX)
-        return HF_E_SHAPE;
+    tree_call(&c, HF_DTYPE_F32, a, workspace);
+    const int ctas = c.ctas;
     CUtensorMap maps[4] = {};
     const int64_t positions = (int64_t) a.pages * kPagePositions, kvw = (int64_t) a.kv_heads * a.width;
     if (!encode_rows(&maps[0], HF_DTYPE_F32, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kKeyTile)
@@ -431,7 +411,7 @@ int tree_limbs(const AttnCall& a, const TreePlan& plan, void* workspace, int dev
     const int rc = a.width > 128  ? launch_limbs<256, true>(maps, l, ctas, device, stream)
                    : a.width > 64 ? launch_limbs<128, true>(maps, l, ctas, device, stream)
                                   : launch_limbs<64, true>(maps, l, ctas, device, stream);
-    return rc || plan.chunks == 1 ? rc : join<float>(c, stream);
+    return rc ? rc : join<float>(c, stream);
 }
 
 int check_packed_sizes(const hf_attention_packed* call)
@@ -461,8 +441,8 @@ uint64_t packed_workspace(const hf_attention_packed& call)
 
 uint64_t tree_workspace(const hf_page_cache& c, const hf_attention_tree& call)
 {
-    const TreePlan plan = tree_plan(c.dtype, c.sequences, call.heads, call.kv_heads, call.head_width, call.max_nodes, call.max_length);
-    return part_bytes(plan, call.rows, call.heads, call.head_width);
+    return (uint64_t) 2 * tree_ctas(c.dtype, call.head_width) * part_rows(call.heads, call.kv_heads, call.max_nodes)
+           * (4 * call.head_width + 8);
 }
 } // namespace
 
@@ -654,21 +634,20 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
     a.table_stride = c.table_stride;
     a.max_nodes = call->max_nodes;
     a.max_length = std::min(call->max_length, c.table_stride * kPagePositions);
-    const TreePlan plan = tree_plan(c.dtype, c.sequences, a.heads, a.kv_heads, a.width, a.max_nodes, call->max_length);
     const uint64_t bytes = tree_workspace(c, *call);
-    if (bytes && !aligned(call->workspace))
+    if (!aligned(call->workspace))
         return HF_E_INVALID;
     if (call->workspace_bytes < bytes)
         return HF_E_CAPACITY;
     const DeviceOf on(a.q);
     if (on.status)
         return on.status;
-    if (!on.holds(bytes ? call->workspace : nullptr, a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
+    if (!on.holds(call->workspace, a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
     if (c.dtype == HF_DTYPE_F32)
-        return tree_limbs(a, plan, call->workspace, on.current, st);
-    return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, plan, call->workspace, on.current, st)
-                                    : tree_mma<__half>(c.dtype, a, plan, call->workspace, on.current, st);
+        return tree_limbs(a, call->workspace, on.current, st);
+    return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, call->workspace, on.current, st)
+                                    : tree_mma<__half>(c.dtype, a, call->workspace, on.current, st);
 }
 }
