@@ -267,6 +267,19 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         prefetch_map(&kmap2);
         prefetch_map(&vmap2);
     }
+    // The first place is found while the barriers and TMEM are made.
+    MmaPlace first = {};
+    TreePlaces places;
+    if (warp == 3)
+    {
+        if (Tree)
+        {
+            places.begin(c, blockIdx.x);
+            first = places.next(c);
+        }
+        else
+            first = prompt_place(c, c.tile_tokens, blockIdx.x);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -488,20 +501,14 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             };
             if (Tree)
             {
-                const long long total = tiles_between(c, 0, a.sequences), per = tiles_per_cta(c, total);
-                const long long end = min(total, (blockIdx.x + 1) * per);
-                for (long long at = blockIdx.x * per; at < end && ok;)
-                {
-                    const MmaPlace p = tree_place(c, at, end, blockIdx.x);
-                    at += p.tiles;
+                for (MmaPlace p = first; p.sequence >= 0 && ok; p = places.next(c))
                     publish(p);
-                }
             }
             for (int asked = 0; !Tree && ok; ++asked)
             {
                 if (lane == 0)
                     ask_next_cta(&h.answer, &h.next);
-                const MmaPlace p = prompt_place(c, c.tile_tokens, unit);
+                const MmaPlace p = asked == 0 ? first : prompt_place(c, c.tile_tokens, unit);
                 if (p.sequence >= 0)
                     publish(p);
                 ok = wait(&h.next, asked & 1) && ok; // an answer is never left behind
@@ -537,31 +544,47 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             // The queries' halves, a row a warp: lane c the channels [8 c, 8 c + 8).
             ok = ok && (i == 0 || wait(&h.query_free, (i - 1) & 1));
             named_sync(1, 256); // `exchange` is free
-#pragma unroll 4
-            for (int e = 0; e < 16; ++e)
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half)
             {
-                const int r = (warp - 4) * 16 + e, t = p.token0 + r / a.group;
-                float x[8] = {};
-                if (r < c.tile_tokens * a.group && t < p.length && lane * 8 < a.width)
-                    load8((const float*) a.q + (p.begin + t) * a.q_stride
-                              + (size_t) (p.kv_head * a.group + r % a.group) * a.width + lane * 8, x);
-                float largest = 0.f;
+                float x[8][8];
+                int t = ((warp - 4) * 16 + half * 8) / a.group, g = ((warp - 4) * 16 + half * 8) % a.group;
+                const float* from = (const float*) a.q + (long long) (p.begin + p.token0) * a.q_stride
+                                    + (size_t) p.kv_head * a.group * a.width + lane * 8;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    largest = fmaxf(largest, finite_abs(x[k]));
-                const float factor = split_factor(warp_max(largest), 15);
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    split_pair(x[2 * k], x[2 * k + 1], factor, hi[k], lo[k]);
-                if (lane < D / 8)
+                for (int e = 0; e < 8; ++e)
                 {
-                    uint8_t* to = queries + (lane >> 3) * 128 * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        x[e][k] = 0.f;
+                    if (t < c.tile_tokens && p.token0 + t < p.length && lane * 8 < a.width)
+                        load8(from + t * a.q_stride + (size_t) g * a.width, x[e]);
+                    if (++g == a.group)
+                        g = 0, ++t;
                 }
-                if (lane == 0)
-                    exchange[0][0][r] = 1.f / factor;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    const int r = (warp - 4) * 16 + half * 8 + e;
+                    float largest = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        largest = fmaxf(largest, finite_abs(x[e][k]));
+                    const float factor =
+                        split_factor(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(largest))), 15);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        split_pair(x[e][2 * k], x[e][2 * k + 1], factor, hi[k], lo[k]);
+                    if (lane < D / 8)
+                    {
+                        uint8_t* to = queries + (lane >> 3) * 128 * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+                        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    if (lane == 0)
+                        exchange[0][0][r] = 1.f / factor;
+                }
             }
             fence_proxy_async();
             __syncwarp();
@@ -725,7 +748,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             const size_t part = (size_t) p.part * c.part_rows + row;
             // The weights' 2^14: cancels in a finished row, is taken off a part's.
             const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 0x1p-14f;
-            bool finite = l < INFINITY && (!Tree || !*(volatile int*) &h.misfit[i & 1]);
+            float2 check = make_float2(l * 0.f, Tree && *(volatile int*) &h.misfit[i & 1] ? NAN : 0.f); // 0 for finite values
             char* mine = (char*) (whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width
                                         : c.part_o + part * a.width);
             const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
@@ -738,15 +761,19 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             {
                 uint32_t x[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
+                for (int e = 0; e < 16; e += 2)
                 {
-                    finite = finite && fabsf(acc[b + e]) < INFINITY;
-                    x[e] = __float_as_uint(scaled == 0.f ? 0.f : acc[b + e] * scaled);
+                    const float2 v = make_float2(acc[b + e], acc[b + e + 1]);
+                    check = __ffma2_rn(v, make_float2(0.f, 0.f), check);
+                    const float2 y = __fmul2_rn(v, make_float2(scaled, scaled));
+                    x[e] = __float_as_uint(y.x);
+                    x[e + 1] = __float_as_uint(y.y);
                 }
                 store_rows(x, four, rows, 4 * (group * kHalf + b), 4 * a.width);
             }
             if (Tree && !whole && real && group == 0)
                 c.part_ml[part] = make_float2(m, l * 0x1p-14f);
+            const bool finite = check.x + check.y == 0.f;
             exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
             named_sync(1, 256);
             // Rows that came out not finite: again, half of them by each warpgroup's warp.

@@ -263,10 +263,11 @@ __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
 // CTA holds whole is finished there; of one that several share, each leaves a
 // part: part 2 cta of the query tile that its piece begins in, part 2 cta + 1 of the
 // one that begins in its piece.
+// The host refuses calls of 2^30 tiles and more.
 struct TreeRow
 {
     int nodes, cached, tiles, query_tiles; // of a sequence; tiles a query tile
-    __device__ long long total() const { return (long long) tiles * query_tiles; }
+    __device__ int total() const { return tiles * query_tiles; }
 };
 
 __device__ __forceinline__ TreeRow tree_row(const MmaCall& c, int s)
@@ -284,68 +285,79 @@ __device__ __forceinline__ TreeRow tree_row(const MmaCall& c, int s)
 }
 
 // The tiles of sequences [begin, end); by a whole warp.
-__device__ inline long long tiles_between(const MmaCall& c, int begin, int end)
+__device__ inline int tiles_between(const MmaCall& c, int begin, int end)
 {
-    long long sum = 0;
+    int sum = 0;
 #pragma unroll 4
     for (int s = begin + (threadIdx.x & 31); s < end; s += 32)
         sum += tree_row(c, s).total();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    return sum;
+    return __reduce_add_sync(0xFFFFFFFFu, sum);
 }
 
-// A CTA's piece: at least four tiles, so that few rows are not cut into more parts than
+// A CTA's piece: at least two tiles, so that few rows are not cut into more parts than
 // they are worth.
-__device__ __forceinline__ long long tiles_per_cta(const MmaCall& c, long long total)
+__device__ __forceinline__ int tiles_per_cta(const MmaCall& c, int total)
 {
-    return max((total + c.ctas - 1) / c.ctas, 4ll);
+    return max((total + c.ctas - 1) / c.ctas, 2);
 }
 
-// The place of the tiles from `at` on, up to `end`; by a whole warp. `cta` takes them.
-__device__ inline MmaPlace tree_place(const MmaCall& c, long long at, long long end, int cta)
+// The places of CTA `cta`'s piece one after another; by a whole warp.
+struct TreePlaces
 {
-    const AttnCall& a = c.a;
-    const int lane = threadIdx.x & 31;
-    MmaPlace p = {};
-    p.sequence = -1;
-    long long before = 0;
-    for (int base = 0; base < a.sequences; base += 32)
+    TreeRow known; // the lane's of the first 32 sequences
+    int at, end, cta;
+
+    __device__ void begin(const MmaCall& c, int which)
     {
-        const TreeRow mine = tree_row(c, base + lane);
-        long long sum = mine.total();
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-        {
-            const long long up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-            if (lane >= o)
-                sum += up;
-        }
-        const unsigned beyond = __ballot_sync(0xFFFFFFFFu, before + sum > at);
-        if (beyond)
-        {
-            const int who = __ffs(beyond) - 1;
-            const long long start = before + __shfl_sync(0xFFFFFFFFu, sum - mine.total(), who);
-            const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), query_tile = (int) ((at - start) / tiles);
-            const int within = (int) ((at - start) % tiles);
-            p.sequence = base + who;
-            p.begin = bounded_offset(a.offsets, p.sequence, a.rows);
-            p.length = __shfl_sync(0xFFFFFFFFu, mine.nodes, who);
-            p.cached = __shfl_sync(0xFFFFFFFFu, mine.cached, who);
-            p.tiles_cached = tiles - 1;
-            p.kv_head = query_tile % a.kv_heads;
-            p.token0 = query_tile / a.kv_heads * c.tile_tokens;
-            p.first_tile = within;
-            p.tiles = (int) min((long long) (tiles - p.first_tile), end - at);
-            p.whole = p.tiles == tiles;
-            p.part = 2 * cta + (p.first_tile == 0);
-            return p;
-        }
-        before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+        cta = which;
+        known = tree_row(c, threadIdx.x & 31);
+        const int total = __reduce_add_sync(0xFFFFFFFFu, known.total()) + tiles_between(c, 32, c.a.sequences);
+        const int per = tiles_per_cta(c, total);
+        at = min(total, cta * per);
+        end = min(total, at + per);
     }
-    return p;
-}
+    __device__ MmaPlace next(const MmaCall& c)
+    {
+        const AttnCall& a = c.a;
+        const int lane = threadIdx.x & 31;
+        MmaPlace p = {};
+        p.sequence = -1;
+        for (int base = 0, before = 0; base < a.sequences && at < end; base += 32)
+        {
+            const TreeRow mine = base ? tree_row(c, base + lane) : known;
+            int sum = mine.total();
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+            {
+                const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                if (lane >= o)
+                    sum += up;
+            }
+            const unsigned beyond = __ballot_sync(0xFFFFFFFFu, before + sum > at);
+            if (beyond)
+            {
+                const int who = __ffs(beyond) - 1;
+                const int start = before + __shfl_sync(0xFFFFFFFFu, sum - mine.total(), who);
+                const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), query_tile = (at - start) / tiles;
+                p.sequence = base + who;
+                p.begin = bounded_offset(a.offsets, p.sequence, a.rows);
+                p.length = __shfl_sync(0xFFFFFFFFu, mine.nodes, who);
+                p.cached = __shfl_sync(0xFFFFFFFFu, mine.cached, who);
+                p.tiles_cached = tiles - 1;
+                p.kv_head = query_tile % a.kv_heads;
+                p.token0 = query_tile / a.kv_heads * c.tile_tokens;
+                p.first_tile = at - start - query_tile * tiles;
+                p.tiles = min(tiles - p.first_tile, end - at);
+                p.whole = p.tiles == tiles;
+                p.part = 2 * cta + (p.first_tile == 0);
+                at += p.tiles;
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+        }
+        return p;
+    }
+};
 
 // A row that came out not finite, by a whole warp: the same keys again, read
 // only where the row attends to them.
@@ -360,8 +372,8 @@ __device__ __noinline__ void take_again(const MmaCall& c, const MmaPlace& p, int
     }
     const int at = (threadIdx.x & 31) * 8;
     const RowKeys keys = row_keys<Tree>(a, p.sequence, p.begin, row);
-    const int from = p.first_tile * kKeyTile, end = p.first_tile + p.tiles;
-    const int to = end > p.tiles_cached ? keys.cached + keys.drafted : end * kKeyTile;
+    const int from = min(p.first_tile * kKeyTile, keys.cached), end = p.first_tile + p.tiles;
+    const int to = end > p.tiles_cached ? keys.cached + keys.drafted : min(end * kKeyTile, keys.cached);
     float q[8] = {}, acc[8], m, l;
     if (at < a.width)
         load8((const T*) a.q + row * a.q_stride + (size_t) head * a.width + at, q);
@@ -506,6 +518,19 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             prefetch_map(&vpages);
         }
     }
+    // The first place is found while the barriers and TMEM are made.
+    MmaPlace first = {};
+    TreePlaces places;
+    if (warp == (NQ == 2 ? 13 : 3))
+    {
+        if (Tree)
+        {
+            places.begin(c, blockIdx.x);
+            first = places.next(c);
+        }
+        else
+            first = prompt_place(c, c.tile_tokens * NQ, blockIdx.x);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -631,20 +656,14 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         };
         if (Tree)
         {
-            const long long total = tiles_between(c, 0, a.sequences), per = tiles_per_cta(c, total);
-            const long long end = min(total, (blockIdx.x + 1) * per);
-            for (long long at = blockIdx.x * per; at < end && ok;)
-            {
-                const MmaPlace p = tree_place(c, at, end, blockIdx.x);
-                at += p.tiles;
+            for (MmaPlace p = first; p.sequence >= 0 && ok; p = places.next(c))
                 publish(p);
-            }
         }
         for (int asked = 0; !Tree && ok; ++asked)
         {
             if (lane == 0)
                 ask_next_cta(&h.answer, &h.next);
-            const MmaPlace p = prompt_place(c, c.tile_tokens * NQ, unit);
+            const MmaPlace p = asked == 0 ? first : prompt_place(c, c.tile_tokens * NQ, unit);
             if (p.sequence >= 0)
                 publish(p);
             ok = wait(&h.next, asked & 1) && ok; // an answer is never left behind
@@ -877,8 +896,9 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 const int at = p.begin + token; // the row of q and out
                 const size_t part = (size_t) p.part * c.part_rows + row;
                 const bool whole = !Tree || p.whole;
+                // Nothing attended: 0 (O is 0, or NaN and the row taken again).
                 const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
-                bool finite = l < INFINITY;
+                float2 check = make_float2(l * 0.f, 0.f); // stays 0 for finite values
                 char* mine = whole ? (char*) ((T*) a.out + at * a.out_stride + (size_t) head * a.width)
                                    : (char*) (c.part_o + part * a.width);
                 const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
@@ -893,11 +913,13 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                     tc_ld32(obase + b, o);
                     tc_wait_ld32(o);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
+                    for (int e = 0; e < 32; e += 2)
                     {
-                        const float v = __uint_as_float(o[e]);
-                        finite = finite && fabsf(v) < INFINITY;
-                        o[e] = __float_as_uint(scaled == 0.f ? 0.f : v * scaled);
+                        const float2 v = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                        check = __ffma2_rn(v, make_float2(0.f, 0.f), check);
+                        const float2 y = __fmul2_rn(v, make_float2(scaled, scaled));
+                        o[e] = __float_as_uint(y.x);
+                        o[e + 1] = __float_as_uint(y.y);
                     }
                     uint32_t x[16];
                     if (whole)
@@ -926,7 +948,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 if (Tree && !whole && real)
                     c.part_ml[part] = make_float2(m, l);
                 // Rows that came out not finite: again, from what they attend to only.
-                unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !finite);
+                unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !(check.x + check.y == 0.f));
                 while (again)
                 {
                     const int who = __ffs(again) - 1;
@@ -960,34 +982,45 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
         return;
     }
     const TreeRow mine = tree_row(c, s);
-    const long long before = tiles_between(c, 0, s), total = before + tiles_between(c, s, a.sequences);
-    const long long per = tiles_per_cta(c, total);
-    const long long first =
-        before + (long long) (node / c.tile_tokens * a.kv_heads + head / a.group) * mine.tiles;
-    const int from = (int) (first / per), to = (int) ((first + mine.tiles - 1) / per);
+    const int before = tiles_between(c, 0, s), per = tiles_per_cta(c, before + tiles_between(c, s, a.sequences));
+    const int first = before + (node / c.tile_tokens * a.kv_heads + head / a.group) * mine.tiles;
+    const int from = first / per, to = (first + mine.tiles - 1) / per;
     pdl_wait();
     if (from == to)
         return;
     const int within = node % c.tile_tokens * a.group + head % a.group;
     auto part_of = [&](int cta) { return (size_t) (2 * cta + (cta == from)) * c.part_rows + within; };
-    float m = -INFINITY;
-    for (int i = from; i <= to; ++i)
-        m = fmaxf(m, c.part_ml[part_of(i)].x);
-    float l = 0.f, acc[8] = {};
-    for (int i = from; i <= to; ++i)
+    // 32 parts at a time, a lane's maximum and sum each; four parts' rows in flight.
+    float m = -INFINITY, l = 0.f, acc[8] = {};
+    for (int base = from; base <= to; base += 32)
     {
-        const float2 ml = c.part_ml[part_of(i)];
-        if (ml.y == 0.f) // nothing attended there
-            continue;
-        const float w = ml.x == m ? 1.f : exp2f(ml.x - m);
-        l += w * ml.y;
-        if (at < a.width)
-        {
-            float x[8];
-            load8(c.part_o + part_of(i) * a.width + at, x);
+        const int lane = threadIdx.x & 31, count = min(32, to + 1 - base);
+        const float2 ml = lane < count ? c.part_ml[part_of(base + lane)] : make_float2(-INFINITY, 0.f);
+        const float m_new = fmaxf(m, warp_max(ml.y == 0.f ? -INFINITY : ml.x));
+        const float alpha = m == m_new ? 1.f : exp2f(m - m_new);
+        // A part in which nothing was attended weighs nothing.
+        const float weight = ml.y == 0.f ? 0.f : ml.x == m_new ? 1.f : exp2f(ml.x - m_new);
+        l = l * alpha + warp_sum(weight * ml.y);
+        m = m_new;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                acc[e] = fmaf(w, x[e], acc[e]);
+        for (int e = 0; e < 8; ++e)
+            acc[e] *= alpha;
+        for (int i = 0; i < count; i += 4)
+        {
+            float x[4][8] = {};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < count && at < a.width)
+                    load8(c.part_o + part_of(base + i + k) * a.width + at, x[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                const float w = __shfl_sync(0xFFFFFFFFu, weight, (i + k) & 31);
+                if (i + k < count && w != 0.f)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        acc[e] = fmaf(w, x[k][e], acc[e]);
+            }
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

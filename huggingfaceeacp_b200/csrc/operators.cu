@@ -431,6 +431,10 @@ int check_tree_sizes(const hf_page_cache* cache, hf_page_cache* c, const hf_atte
         return rc;
     if (call->max_nodes > HF_TREE_NODES || c->kv_width != call->kv_heads * call->head_width)
         return HF_E_SHAPE;
+    // The kernels count key tiles in 32 bits.
+    const int64_t tokens = 128 / (call->heads / call->kv_heads), row_tiles = (call->max_nodes + tokens - 1) / tokens;
+    if ((call->max_length / kKeyTile + 2) * row_tiles > (1 << 30) / ((int64_t) c->sequences * call->kv_heads))
+        return HF_E_SHAPE;
     return HF_OK;
 }
 

@@ -307,6 +307,37 @@ def test_tree_siblings_do_not_reach_each_other(kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("length", [0, 1, 63, 64, 65, 128, 200, 257, 1000])
+def test_tree_infinities_wherever_the_keys_are_cut(kind, length):
+    """Infinite values in the cache's first and last position and in one node: rows are exact in every other channel, for
+    caches whose tiles fall differently on the CTAs."""
+    code, dtype = ref.TYPES[kind]
+    parents, h, kv, d = [-1, 0, 0, 1], 4, 2, 64
+    cache = Cache(kind, 1, 18, kv, d, [length, 70], 17, 24)
+    at = cache.table.tolist()[0]
+    for j, channel in ((0, 5), (length - 1, 9)):
+        if 0 <= j < length:
+            cache.values[0, at[j // PAGE], j % PAGE, channel] = math.inf
+    g = torch.Generator("cuda").manual_seed(25)
+    q, k, v = (_normal(g, 8, n, d, dtype=dtype) for n in (h, kv, kv))
+    v[2, 0, 11] = -math.inf
+    out = torch.empty_like(q)
+    plan = native.TreeAttention(code, h, kv, d)
+    offsets, up = _ints([0, 4, 8]), _ints(parents * 2)
+    room = _room(plan.workspace_bytes(2, 8, 4, 1000))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(), 8, 4,
+             1000, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q, k, v, [4, 4], [parents] * 2, cache.keys[0].view(cache.shape), cache.values[0].view(cache.shape),
+                              cache.table.tolist(), [length, 70], d ** -0.5)
+    fine = torch.isfinite(expected)
+    assert torch.equal(torch.isfinite(out), fine)
+    tol = ref.tolerance(expected.nan_to_num(0, 0, 0), size.nan_to_num(0, 0, 0), q, cache.keys[0].view(-1, kv, d), d ** -0.5,
+                        length + 8, dtype)
+    assert bool(((out.double() - expected).abs() <= tol)[fine].all())
+    assert bool((out.double()[~fine] == expected[~fine]).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_tree_pages_that_are_not_there_and_bounds(kind):
     """Page ids outside the pool are not attended; lengths and node counts are bounded by the call's."""
     lengths = [200, 130]
