@@ -320,63 +320,62 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         set_registers_down<Shape::kRegistersIssue>();
         if (warp == 0)
         {
+            // K and V each in its own order, whichever ring has room: one that waits
+            // for its MMAs must not hold up the other (K tile by tile ahead of V,
+            // a V that had room came late and a step took 5000 cycles).
             int put_keys = 0, put_values = 0;
             bool ok = true;
-            auto one_wait = [&](uint64_t* bar, unsigned parity) {
-                if (ok && !thread_wait(bar, parity))
-                {
-                    *(volatile int*) &h.dead = 1;
-                    ok = false;
-                }
-                return ok;
-            };
             MmaPlace p;
             for (int i = 0; ok && take(i, p); ++i)
             {
-                const int tiles = p.tiles;
-                const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
-                // A tile's K or V, block by block.
-                auto load = [&](int j, const CUtensorMap* first, const CUtensorMap* second, int id, uint8_t* ring, int& put,
-                                int stages, uint64_t* full, uint64_t* free) {
-                    const bool cached = Tree && p.first_tile + j < p.tiles_cached;
-                    const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
-                                           : p.begin + (Tree ? 0 : j * kKeyTile);
-                    for (int b = 0; b < kBlocks; ++b)
+                if (lane == 0)
+                {
+                    const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
+                    struct
                     {
+                        int tile, block, id, id_next;
+                    } next[2];
+                    auto page_of = [&](int j) {
+                        const int t = p.first_tile + j;
+                        return Tree && t < p.tiles_cached ? table[t] : -1;
+                    };
+                    for (int r = 0; r < 2; ++r)
+                        next[r] = {0, 0, page_of(0), page_of(1)};
+                    auto load = [&](int r, const CUtensorMap* drafted, const CUtensorMap* paged, uint8_t* ring, int& put,
+                                    int stages, uint64_t* full, uint64_t* free) {
                         const int stage = put % stages;
-                        if (!ok || (put >= stages && !one_wait(&free[stage], (put / stages - 1) & 1)))
-                            return;
+                        if (next[r].tile == p.tiles || (put >= stages && !mbar_test(&free[stage], (put / stages - 1) & 1)))
+                            return false;
+                        const bool cached = Tree && p.first_tile + next[r].tile < p.tiles_cached;
+                        const int id = next[r].id, b = next[r].block;
+                        // A page that is not there is read past the pool's end: zeros.
+                        const int row = cached ? (page_there(id, a.pages) ? id : a.pages) * kPagePositions
+                                               : p.begin + (Tree ? 0 : next[r].tile * kKeyTile);
                         uint8_t* to = ring + stage * Shape::kStageBytes;
                         mbar_expect_tx(&full[stage], Shape::kStageBytes);
-                        tensor_load(to, Tree && cached ? second : first, 64 * b, p.kv_head, row, &full[stage]);
-                        tensor_load(to + Shape::kBox, Tree ? (cached ? second : first) : second, 64 * b + (Tree ? 32 : 0),
+                        tensor_load(to, Tree && cached ? paged : drafted, 64 * b, p.kv_head, row, &full[stage]);
+                        tensor_load(to + Shape::kBox, Tree ? (cached ? paged : drafted) : paged, 64 * b + (Tree ? 32 : 0),
                                     p.kv_head, row, &full[stage]);
                         ++put;
-                    }
-                };
-                int id_before = -1, ids = -1; // tile j - 1's page; 32 tiles' pages
-                for (int j = 0; j <= tiles; ++j)
-                {
-                    int id = -1;
-                    if (Tree)
+                        if (++next[r].block == kBlocks)
+                            next[r] = {next[r].tile + 1, 0, next[r].id_next, page_of(next[r].tile + 2)};
+                        return true;
+                    };
+                    unsigned idle = 0;
+                    while ((next[0].tile < p.tiles || next[1].tile < p.tiles) && ok)
                     {
-                        if ((j & 31) == 0)
+                        const bool k = load(0, &kmap, &kmap2, keys, put_keys, KS, h.keys_full, h.keys_free);
+                        const bool v = load(1, &vmap, &vmap2, values, put_values, VS, h.values_full, h.values_free);
+                        idle = k || v ? 0 : idle + 1;
+                        if (idle == 1u << 26) // some seconds
                         {
-                            const int t = p.first_tile + j + lane;
-                            ids = t < p.tiles_cached ? table[t] : -1;
+                            flag_error(&g_operator_error, kErrWaitTimeout);
+                            *(volatile int*) &h.dead = 1;
+                            ok = false;
                         }
-                        id = __shfl_sync(0xFFFFFFFFu, ids, j & 31);
                     }
-                    if (lane == 0)
-                    {
-                        if (j < tiles)
-                            load(j, &kmap, &kmap2, id, keys, put_keys, KS, h.keys_full, h.keys_free);
-                        if (j > 0)
-                            load(j - 1, &vmap, &vmap2, id_before, values, put_values, VS, h.values_full, h.values_free);
-                    }
-                    id_before = id;
-                    __syncwarp();
                 }
+                __syncwarp();
                 ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
                 leave(i);
             }

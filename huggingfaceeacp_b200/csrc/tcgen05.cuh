@@ -220,6 +220,17 @@ __device__ __forceinline__ void tensor_load(void* dst, const CUtensorMap* map, i
                  : "memory");
 }
 
+// Whether the phase with the given parity is over, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, unsigned parity)
+{
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return done;
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
 {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
