@@ -169,7 +169,10 @@ struct LimbShape
     static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
     static constexpr int kKeyStages = kStages / 2, kValueStages = kStages - kKeyStages;
     static constexpr int kSmem = kHead + 2 * kQueryHalf + kStages * kStageBytes;
-    static constexpr int kRowBuffers = D == 256 ? 1 : 2; // of O
+    // O: two buffers, or at width 256 (all that TMEM has left) one in two halves, so
+    // that a half is drained while the MMAs fill the other.
+    static constexpr int kRowBuffers = D == 256 ? 1 : 2;
+    static constexpr bool kHalves = D == 256;
     static constexpr int kThreads = Tree ? 512 : 384;
     // Registers a thread, by warpgroup; at launch 168 or 128 each: the shares
     // add up to that (3 x 168, 4 x 128).
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         {
             mbar_init(&h.weights[b], 8);
             mbar_init(&h.done[b], 1);
-            mbar_init(&h.rows_free[b], 8);
+            mbar_init(&h.rows_free[b], Shape::kHalves ? 4 : 8);
             mbar_init(&h.place_full[b], 1);
             mbar_init(&h.place_free[b], Tree ? 15 : 11); // an arrival a warp but the one that finds them
             mbar_init(&h.drained[b], 1);
@@ -445,9 +448,10 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     for (int b = 0; b < kBlocks; ++b, ++item)
                     {
                         // The stage, the weights, and the buffer's last O in registers.
-                        const int stage = item % VS, what = lane & 3;
-                        const bool frees = what == 1 && b == 0 && count >= RB, weighs = what == 2 && b == 0;
-                        ok = wait(frees ? &h.rows_free[buffer] : weighs ? &h.weights[count & 1] : &landed[stage],
+                        const int stage = item % VS, what = lane & 3, part = Shape::kHalves ? b / 2 : buffer;
+                        const bool frees = what == 1 && (b == 0 || (Shape::kHalves && b == 2)) && count >= RB;
+                        const bool weighs = what == 2 && b == 0;
+                        ok = wait(frees ? &h.rows_free[part] : weighs ? &h.weights[count & 1] : &landed[stage],
                                   (frees ? count / RB - 1 : weighs ? count / 2 : item / VS) & 1);
                         if (!ok)
                             break;
@@ -476,9 +480,9 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                         for (int e = 0; e < 4; ++e)
                             tc_mma_ts_warp(d, hi + e * 8, tc_desc_mn(v + e * 2048, Shape::kBox), kValues, 1);
                         tc_commit_warp(&h.values_free[stage]);
+                        if (b == kBlocks - 1 || (Shape::kHalves && b == 1))
+                            tc_commit_warp(&h.done[part]);
                     }
-                    if (ok)
-                        tc_commit_warp(&h.done[buffer]);
                 }
                 leave(i);
             }
@@ -622,7 +626,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             int id = Tree && p.first_tile < p.tiles_cached ? table[p.first_tile] : -1;
             // acc = acc * alpha + (O of the n-th tile) * factor
             auto drain = [&](int n, float alpha, float factor) {
-                ok = ok && wait(&h.done[n % RB], (n / RB) & 1);
+                const int part = Shape::kHalves ? group : n % RB;
+                ok = ok && wait(&h.done[part], (n / RB) & 1);
                 tc_fence_after();
                 const uint32_t at = lanes + Shape::kRows + n % RB * D + group * kHalf;
                 const bool scales = __any_sync(0xFFFFFFFFu, alpha != 1.f);
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (ok && lane == 0)
-                    mbar_arrive(&h.rows_free[n % RB]);
+                    mbar_arrive(&h.rows_free[part]);
             };
             for (int j = 0; j < tiles; ++j, ++count)
             {
@@ -657,7 +662,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     vfactor = vfactors[j];
                 }
                 // S is there. The weights' buffer is free: the MMAs that read it two
-                // tiles back ended before O of that tile was drained.
+                // tiles back ended before O of that tile was drained, by both
+                // warpgroups before the last tile's exchange.
                 ok = ok && wait(&h.scores, count & 1);
                 tc_fence_after();
                 float s[32];
