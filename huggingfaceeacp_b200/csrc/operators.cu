@@ -55,16 +55,30 @@ public:
     int current = 0;
 
 private:
+    // By the driver's call: about a third of the runtime's time, and a call asks for ten
+    // pointers.
     static bool on_device(const void* p, int* device)
     {
-        cudaPointerAttributes a;
-        if (cudaPointerGetAttributes(&a, p) != cudaSuccess)
+        using Query = CUresult (*)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+        static std::atomic<Query> known {nullptr};
+        Query query = known.load(std::memory_order_relaxed);
+        if (!query)
         {
-            cudaGetLastError();
-            return false;
+            void* f = nullptr;
+            cudaDriverEntryPointQueryResult found;
+            if (cudaGetDriverEntryPointByVersion("cuPointerGetAttributes", &f, 12000, cudaEnableDefault, &found) != cudaSuccess
+                || found != cudaDriverEntryPointSuccess)
+                return false;
+            known.store(query = (Query) f, std::memory_order_relaxed);
         }
-        *device = a.device;
-        return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged;
+        unsigned type = 0;
+        int ordinal = -1;
+        CUpointer_attribute which[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+        void* values[2] = {&type, &ordinal};
+        if (query(2, which, values, (CUdeviceptr) p) != CUDA_SUCCESS || type != CU_MEMORYTYPE_DEVICE || ordinal < 0)
+            return false;
+        *device = ordinal;
+        return true;
     }
     bool here(const void* p) const
     {
@@ -155,9 +169,28 @@ PageBook book_of(const hf_page_cache& c, void* workspace)
     return b;
 }
 
+// The bookkeeping kernel, `Book<true>` where the book fits shared memory.
+template <typename Kernel, typename... Args>
+cudaError_t launch_book(Kernel small, Kernel large, std::atomic<uint64_t>& ready, int device, cudaStream_t stream,
+                        const PageBook& b, Args... args)
+{
+    const int64_t words = (int64_t) b.pages + b.sequences;
+    if (words > kSmallBook)
+        return launch(false, large, dim3(1), dim3(kBookThreads), 0, stream, b, args...);
+    const uint64_t bit = 1ull << (device & 63); // devices whose kernel has its shared memory
+    if (!(ready.load(std::memory_order_relaxed) & bit))
+    {
+        const cudaError_t e = cudaFuncSetAttribute(small, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kSmallBook);
+        if (e != cudaSuccess)
+            return e;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return launch(false, small, dim3(1), dim3(kBookThreads), (size_t) words * 4, stream, b, args...);
+}
+
 int copy_rows(const PageBook& b, int most, int device, cudaStream_t stream)
 {
-    const long long units = (long long) most * b.layers * 2;
+    const long long units = (long long) most * b.layers * 2 * ((kPagePositions * b.row_bytes + 32767) / 32768);
     const int grid = (int) std::min<long long>(std::max<long long>(units, 1), (long long) sm_count(device) * 8);
     return status_of(launch(true, pages_copy_rows, dim3(grid), dim3(256), 0, stream, b));
 }
@@ -501,8 +534,9 @@ int hf_cuda_pages_update(const hf_page_cache* cache, const int32_t* release, int
         return HF_E_INVALID;
     const PageBook b = book_of(c, workspace);
     cudaStream_t s = (cudaStream_t) stream;
-    const cudaError_t e = launch(false, pages_update_book, dim3(1), dim3(kBookThreads), 0, s, b, release, (int) releases,
-                                 forks, (int) fork_count, grow, result);
+    static std::atomic<uint64_t> ready {0};
+    const cudaError_t e = launch_book(pages_update_book<true>, pages_update_book<false>, ready, on.current, s, b, release,
+                                      (int) releases, forks, (int) fork_count, grow, result);
     if (e != cudaSuccess || !grow)
         return status_of(e);
     return copy_rows(b, c.sequences, on.current, s);
@@ -525,7 +559,9 @@ int hf_cuda_pages_compact(const hf_page_cache* cache, int32_t* live, void* works
         return HF_E_INVALID;
     const PageBook b = book_of(c, workspace);
     cudaStream_t s = (cudaStream_t) stream;
-    const cudaError_t e = launch(false, pages_compact_book, dim3(1), dim3(kBookThreads), 0, s, b, live);
+    static std::atomic<uint64_t> ready {0};
+    const cudaError_t e =
+        launch_book(pages_compact_book<true>, pages_compact_book<false>, ready, on.current, s, b, live);
     if (e != cudaSuccess)
         return HF_E_CUDA;
     return copy_rows(b, c.pages / 2 + 1, on.current, s);
