@@ -500,6 +500,14 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     h.place[i & 1] = p;
                     mbar_arrive(&h.place_full[i & 1]);
                 }
+                // The unit's queries on their way to L2 while the one before is worked on.
+                if (p.sequence >= 0)
+                    for (int t = lane; t < c.tile_tokens && p.token0 + t < p.length; t += 32)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                                         (const float*) a.q + (long long) (p.begin + p.token0 + t) * a.q_stride
+                                         + (size_t) p.kv_head * a.group * a.width),
+                                     "r"(a.group * a.width * 4)
+                                     : "memory");
                 ++i;
             };
             if (Tree)
@@ -565,16 +573,38 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     if (++g == a.group)
                         g = 0, ++t;
                 }
+                // The rows' largest values, eight at once: each step halves the rows that
+                // a lane holds, until lanes 4 e .. 4 e + 3 hold row e's (NaN left out; an
+                // infinity makes its row NaN, which is what it is).
+                float top[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                {
+                    const float(&v)[8] = x[e];
+                    top[e] = max3(max3(max3(0.f, fabsf(v[0]), fabsf(v[1])), fabsf(v[2]), fabsf(v[3])),
+                                  max3(0.f, fabsf(v[4]), fabsf(v[5])), max3(0.f, fabsf(v[6]), fabsf(v[7])));
+                }
+#pragma unroll
+                for (int rows = 4; rows >= 1; rows >>= 1)
+                {
+                    const bool upper = lane & (4 * rows);
+#pragma unroll
+                    for (int e = 0; e < rows; ++e)
+                    {
+                        const float other = __shfl_xor_sync(0xFFFFFFFFu, upper ? top[e] : top[e + rows], 4 * rows);
+                        top[e] = fmaxf(upper ? top[e + rows] : top[e], other);
+                    }
+                }
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], 2));
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], 1));
+                const float mine = split_factor(top[0], 15);
+                if ((lane & 3) == 0)
+                    exchange[0][0][(warp - 4) * 16 + half * 8 + lane / 4] = 1.f / mine;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                 {
                     const int r = (warp - 4) * 16 + half * 8 + e;
-                    float largest = 0.f;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        largest = fmaxf(largest, finite_abs(x[e][k]));
-                    const float factor =
-                        split_factor(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(largest))), 15);
+                    const float factor = __shfl_sync(0xFFFFFFFFu, mine, 4 * e);
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -585,8 +615,6 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                         *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *reinterpret_cast<uint4*>(to + Shape::kQueryHalf) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    if (lane == 0)
-                        exchange[0][0][r] = 1.f / factor;
                 }
             }
             fence_proxy_async();
@@ -756,25 +784,34 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             float2 check = make_float2(l * 0.f, Tree && *(volatile int*) &h.misfit[i & 1] ? NAN : 0.f); // 0 for finite values
             char* mine = (char*) (whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width
                                         : c.part_o + part * a.width);
-            const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
-            char* four[4];
+            // Through the queries' room (their last MMA is over): a row a thread in,
+            // a row a warp out, 16-byte chunk c of row r at chunk c ^ r.
+            constexpr int kChunks = kHalf / 4;
+            float4* room = reinterpret_cast<float4*>(queries) + (warp - 4) * 32 * kChunks;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                four[k] = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, (lane & ~3) + k);
-#pragma unroll
-            for (int b = 0; b < kHalf; b += 16)
+            for (int b = 0; b < kChunks; ++b)
             {
-                uint32_t x[16];
+                float2 v[2];
 #pragma unroll
-                for (int e = 0; e < 16; e += 2)
+                for (int e = 0; e < 2; ++e)
                 {
-                    const float2 v = make_float2(acc[b + e], acc[b + e + 1]);
-                    check = __ffma2_rn(v, make_float2(0.f, 0.f), check);
-                    const float2 y = __fmul2_rn(v, make_float2(scaled, scaled));
-                    x[e] = __float_as_uint(y.x);
-                    x[e + 1] = __float_as_uint(y.y);
+                    v[e] = make_float2(acc[4 * b + 2 * e], acc[4 * b + 2 * e + 1]);
+                    check = __ffma2_rn(v[e], make_float2(0.f, 0.f), check);
+                    v[e] = __fmul2_rn(v[e], make_float2(scaled, scaled));
                 }
-                store_rows(x, four, rows, 4 * (group * kHalf + b), 4 * a.width);
+                room[lane * kChunks + (b ^ lane & (kChunks - 1))] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            }
+            __syncwarp();
+            const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
+            constexpr int kAtOnce = 32 / kChunks; // rows
+            const int chunk = lane & (kChunks - 1), channel = group * kHalf + 4 * chunk;
+#pragma unroll 4
+            for (int r0 = 0; r0 < 32; r0 += kAtOnce)
+            {
+                const int r = r0 + lane / kChunks;
+                char* to = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, r);
+                if (rows >> r & 1 && channel < a.width)
+                    *reinterpret_cast<float4*>(to + 4 * channel) = room[r * kChunks + (chunk ^ r & (kChunks - 1))];
             }
             if (Tree && !whole && real && group == 0)
                 c.part_ml[part] = make_float2(m, l * 0x1p-14f);

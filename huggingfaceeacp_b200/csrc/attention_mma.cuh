@@ -258,11 +258,15 @@ __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
 
 // A batch of trees is one row of key tiles: sequence after sequence, in it query tile
 // after query tile of each kv head, of each its cached tiles and the drafted one.
-// Every CTA takes `per` of them in a piece, whatever sequences it falls on, so
-// that sequences of any lengths keep all CTAs busy to the end. A query tile that a
-// CTA holds whole is finished there; of one that several share, each leaves a
-// part: part 2 cta of the query tile that its piece begins in, part 2 cta + 1 of the
-// one that begins in its piece.
+// It is cut for the CTAs in one of two ways:
+//  few query tiles (a CTA's share is less than half of one): each is cut into pieces
+//  of at most `per` tiles, no more pieces than CTAs. A CTA takes one piece: a
+//  second would cost it another start (about 10 us of a 60 us call of 16 trees in
+//  fp32);
+//  many: every CTA takes `per` tiles in a row, whatever query tiles they fall on, so
+//  that sequences of any lengths keep all CTAs busy to the end.
+// A query tile that a CTA holds whole is finished there; of one that several share, each
+// leaves a part: part 2 cta + 1 where the query tile begins in a row of many, else 2 cta.
 // The host refuses calls of 2^30 tiles and more.
 struct TreeRow
 {
@@ -284,38 +288,52 @@ __device__ __forceinline__ TreeRow tree_row(const MmaCall& c, int s)
     return r;
 }
 
-// The tiles of sequences [begin, end); by a whole warp.
-__device__ inline int tiles_between(const MmaCall& c, int begin, int end)
+struct TreeCut
 {
-    int sum = 0;
-#pragma unroll 4
-    for (int s = begin + (threadIdx.x & 31); s < end; s += 32)
-        sum += tree_row(c, s).total();
-    return __reduce_add_sync(0xFFFFFFFFu, sum);
+    bool few;
+    int per;
+    __device__ int pieces(int tiles) const { return (tiles + per - 1) / per; } // few: of a query tile
+};
+
+// How a call's row is cut, and its tiles; by a whole warp, `known` the lane's of the
+// first 32 sequences. At least two tiles a CTA: a part costs about one.
+__device__ inline TreeCut cut_trees(const MmaCall& c, const TreeRow& known, int& total)
+{
+    const int lane = threadIdx.x & 31, sequences = c.a.sequences;
+    total = known.total();
+    int query_tiles = known.query_tiles;
+    for (int s = lane + 32; s < sequences; s += 32)
+    {
+        const TreeRow r = tree_row(c, s);
+        total += r.total();
+        query_tiles += r.query_tiles;
+    }
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    query_tiles = __reduce_add_sync(0xFFFFFFFFu, query_tiles);
+    // The sum of n / per, each rounded up, is at most total / per + query_tiles.
+    const bool few = 2 * query_tiles <= c.ctas;
+    const int share = few ? c.ctas - query_tiles : c.ctas;
+    return {few, max((total + share - 1) / share, 2)};
 }
 
-// A CTA's piece: at least two tiles, so that few rows are not cut into more parts than
-// they are worth.
-__device__ __forceinline__ int tiles_per_cta(const MmaCall& c, int total)
-{
-    return max((total + c.ctas - 1) / c.ctas, 2);
-}
-
-// The places of CTA `cta`'s piece one after another; by a whole warp.
+// The places of CTA `cta` one after another; by a whole warp.
 struct TreePlaces
 {
     TreeRow known; // the lane's of the first 32 sequences
-    int at, end, cta;
+    TreeCut cut;
+    int at, end, cta; // tiles; few: pieces
 
     __device__ void begin(const MmaCall& c, int which)
     {
+        int total;
         cta = which;
         known = tree_row(c, threadIdx.x & 31);
-        const int total = __reduce_add_sync(0xFFFFFFFFu, known.total()) + tiles_between(c, 32, c.a.sequences);
-        const int per = tiles_per_cta(c, total);
-        at = min(total, cta * per);
-        end = min(total, at + per);
+        cut = cut_trees(c, known, total);
+        at = cut.few ? cta : min(total, cta * cut.per);
+        end = cut.few ? cta + 1 : min(total, at + cut.per);
     }
+    // A sequence's tiles, or pieces, in the row.
+    __device__ int share(const TreeRow& r) const { return cut.few ? r.query_tiles * cut.pieces(r.tiles) : r.total(); }
     __device__ MmaPlace next(const MmaCall& c)
     {
         const AttnCall& a = c.a;
@@ -325,7 +343,7 @@ struct TreePlaces
         for (int base = 0, before = 0; base < a.sequences && at < end; base += 32)
         {
             const TreeRow mine = base ? tree_row(c, base + lane) : known;
-            int sum = mine.total();
+            int sum = share(mine);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1)
             {
@@ -337,8 +355,9 @@ struct TreePlaces
             if (beyond)
             {
                 const int who = __ffs(beyond) - 1;
-                const int start = before + __shfl_sync(0xFFFFFFFFu, sum - mine.total(), who);
-                const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), query_tile = (at - start) / tiles;
+                const int within = at - before - __shfl_sync(0xFFFFFFFFu, sum - share(mine), who);
+                const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), each = cut.few ? cut.pieces(tiles) : tiles;
+                const int query_tile = within / each, rest = within - query_tile * each;
                 p.sequence = base + who;
                 p.begin = bounded_offset(a.offsets, p.sequence, a.rows);
                 p.length = __shfl_sync(0xFFFFFFFFu, mine.nodes, who);
@@ -346,11 +365,21 @@ struct TreePlaces
                 p.tiles_cached = tiles - 1;
                 p.kv_head = query_tile % a.kv_heads;
                 p.token0 = query_tile / a.kv_heads * c.tile_tokens;
-                p.first_tile = at - start - query_tile * tiles;
-                p.tiles = min(tiles - p.first_tile, end - at);
+                if (cut.few) // pieces as even as they go
+                {
+                    p.first_tile = (int) ((long long) tiles * rest / each);
+                    p.tiles = (int) ((long long) tiles * (rest + 1) / each) - p.first_tile;
+                    p.part = 2 * cta;
+                    at = end;
+                }
+                else
+                {
+                    p.first_tile = rest;
+                    p.tiles = min(tiles - rest, end - at);
+                    p.part = 2 * cta + (rest == 0);
+                    at += p.tiles;
+                }
                 p.whole = p.tiles == tiles;
-                p.part = 2 * cta + (p.first_tile == 0);
-                at += p.tiles;
                 break;
             }
             before += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -982,14 +1011,25 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
         return;
     }
     const TreeRow mine = tree_row(c, s);
-    const int before = tiles_between(c, 0, s), per = tiles_per_cta(c, before + tiles_between(c, s, a.sequences));
-    const int first = before + (node / c.tile_tokens * a.kv_heads + head / a.group) * mine.tiles;
-    const int from = first / per, to = (first + mine.tiles - 1) / per;
+    const TreeRow known = tree_row(c, threadIdx.x & 31);
+    int total;
+    const TreeCut cut = cut_trees(c, known, total);
+    int before = 0;
+    for (int base = 0; base < s; base += 32)
+    {
+        const int lane = threadIdx.x & 31;
+        const TreeRow r = base ? tree_row(c, base + lane) : known;
+        before += base + lane < s ? (cut.few ? r.query_tiles * cut.pieces(r.tiles) : r.total()) : 0;
+    }
+    before = __reduce_add_sync(0xFFFFFFFFu, before);
+    const int query_tile = node / c.tile_tokens * a.kv_heads + head / a.group;
+    const int each = cut.few ? cut.pieces(mine.tiles) : mine.tiles, first = before + query_tile * each;
+    const int from = cut.few ? first : first / cut.per, to = cut.few ? first + each - 1 : (first + each - 1) / cut.per;
     pdl_wait();
     if (from == to)
         return;
     const int within = node % c.tile_tokens * a.group + head % a.group;
-    auto part_of = [&](int cta) { return (size_t) (2 * cta + (cta == from)) * c.part_rows + within; };
+    auto part_of = [&](int cta) { return (size_t) (2 * cta + (!cut.few && cta == from)) * c.part_rows + within; };
     // 32 parts at a time, a lane's maximum and sum each; four parts' rows in flight.
     float m = -INFINITY, l = 0.f, acc[8] = {};
     for (int base = from; base <= to; base += 32)
