@@ -77,6 +77,7 @@ struct LimbCall
 __global__ void __launch_bounds__(256) split_tiles(const __grid_constant__ LimbCall l)
 {
     __shared__ float row_max[kKeyTile];
+    pdl_wait();
     pdl_trigger();
     const AttnCall& a = l.c.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, at = lane * 8;
@@ -270,7 +271,9 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         prefetch_map(&kmap2);
         prefetch_map(&vmap2);
     }
-    // The first place is found while the barriers and TMEM are made.
+    // Of prompts: split_tiles' halves, of trees whatever is ahead in the stream.
+    pdl_wait();
+    // The first place is found while TMEM is made.
     MmaPlace first = {};
     TreePlaces places;
     if (warp == 3)
@@ -288,8 +291,6 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
     tc_fence_after();
     if (Tree)
         pdl_trigger(); // attention_join may take its place; it waits for this grid's end
-    else
-        pdl_wait(); // split_tiles' halves
     const uint32_t tmem = h.tmem;
     // A wait of one of the roles; one that runs out ends the CTA's other waits too.
     auto wait = [&](uint64_t* bar, unsigned parity) {

@@ -547,7 +547,8 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             prefetch_map(&vpages);
         }
     }
-    // The first place is found while the barriers and TMEM are made.
+    pdl_wait(); // the set-up above ran beside the end of the kernel ahead in the stream
+    // The first place is found while TMEM is made.
     MmaPlace first = {};
     TreePlaces places;
     if (warp == (NQ == 2 ? 13 : 3))

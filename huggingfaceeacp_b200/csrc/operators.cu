@@ -176,7 +176,7 @@ cudaError_t launch_book(Kernel small, Kernel large, std::atomic<uint64_t>& ready
 {
     const int64_t words = (int64_t) b.pages + b.sequences;
     if (words > kSmallBook)
-        return launch(false, large, dim3(1), dim3(kBookThreads), 0, stream, b, args...);
+        return launch(true, large, dim3(1), dim3(kBookThreads), 0, stream, b, args...);
     const uint64_t bit = 1ull << (device & 63); // devices whose kernel has its shared memory
     if (!(ready.load(std::memory_order_relaxed) & bit))
     {
@@ -185,7 +185,7 @@ cudaError_t launch_book(Kernel small, Kernel large, std::atomic<uint64_t>& ready
             return e;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    return launch(false, small, dim3(1), dim3(kBookThreads), (size_t) words * 4, stream, b, args...);
+    return launch(true, small, dim3(1), dim3(kBookThreads), (size_t) words * 4, stream, b, args...);
 }
 
 int copy_rows(const PageBook& b, int most, int device, cudaStream_t stream)
@@ -303,7 +303,7 @@ int launch_mma(const CUtensorMap (&maps)[5], const MmaCall& c, int64_t ctas, int
             return HF_E_CUDA;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    return status_of(launch(false, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
+    return status_of(launch(true, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
                             maps[1], maps[2], maps[3], maps[4], c));
 }
 
@@ -399,7 +399,7 @@ int launch_limbs(const CUtensorMap (&maps)[4], const LimbCall& l, int64_t ctas, 
             return HF_E_CUDA;
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    return status_of(launch(!Tree, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
+    return status_of(launch(true, kernel, dim3((unsigned) ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
                             maps[1], maps[2], maps[3], l));
 }
 
@@ -421,7 +421,7 @@ int packed_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t st
         if (!encode_rows(&maps[i], HF_DTYPE_F16, l.limbs + limb_of[i] * limb, a.width, a.kv_heads, a.rows,
                          (int64_t) a.kv_heads * a.width, 1, kKeyTile))
             return HF_E_CUDA;
-    if (launch(false, split_tiles, dim3(l.tiles, a.kv_heads, 2), dim3(256), 0, stream, l) != cudaSuccess)
+    if (launch(true, split_tiles, dim3(l.tiles, a.kv_heads, 2), dim3(256), 0, stream, l) != cudaSuccess)
         return HF_E_CUDA;
     return a.width > 128  ? launch_limbs<256, false>(maps, l, ctas, device, stream)
            : a.width > 64 ? launch_limbs<128, false>(maps, l, ctas, device, stream)
@@ -602,7 +602,7 @@ int hf_cuda_pages_write(const hf_page_cache* cache, int32_t layer, const void* k
     w.index = index;
     w.rows = rows;
     w.source_rows = source_rows;
-    return status_of(launch(false, pages_write_rows, dim3((unsigned) (rows + 7) / 8), dim3(256), 0, (cudaStream_t) stream, w));
+    return status_of(launch(true, pages_write_rows, dim3((unsigned) (rows + 7) / 8), dim3(256), 0, (cudaStream_t) stream, w));
 }
 
 int hf_cuda_attention_packed_workspace(const hf_attention_packed* call, uint64_t* bytes)

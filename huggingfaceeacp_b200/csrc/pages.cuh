@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
     extern __shared__ int shared[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kBookThreads / 32;
+    pdl_wait();
     pdl_trigger();
     const BookView<Small> v = open_book<Small>(b, shared);
 
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_book(const PageBoo
 {
     extern __shared__ int shared[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
     pdl_trigger();
     const BookView<Small> v = open_book<Small>(b, shared);
     int live = 0;
