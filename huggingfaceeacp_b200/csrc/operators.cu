@@ -174,7 +174,7 @@ template <typename Kernel, typename... Args>
 cudaError_t launch_book(Kernel small, Kernel large, std::atomic<uint64_t>& ready, int device, cudaStream_t stream,
                         const PageBook& b, Args... args)
 {
-    const int64_t words = (int64_t) b.pages + b.sequences;
+    const int64_t words = book_words(b.pages, b.sequences);
     if (words > kSmallBook)
         return launch(true, large, dim3(1), dim3(kBookThreads), 0, stream, b, args...);
     const uint64_t bit = 1ull << (device & 63); // devices whose kernel has its shared memory

@@ -83,29 +83,56 @@ __device__ __forceinline__ int block_scan(int v, int* total)
     return before + sum - v;
 }
 
-// The book's counts and lengths in shared memory, where a few thousand fit
-// (kSmallBook): one round trip to L2 brings them all, and the phases then run at
-// shared memory's latency instead of L2's (a step of 16 sequences over 256 pages:
-// 12.4 us a pass in L2). Larger books stay where they are and are read past L1.
-constexpr int kSmallBook = 24 * 1024; // pages + sequences
+// The book's counts and lengths, the scratch and the call's lists in shared memory
+// where they fit (kSmallBook words): one round trip to L2 brings them all, and the
+// phases then run at shared memory's latency instead of L2's. Larger books stay where
+// they are and are read past L1.
+constexpr int kSmallBook = 48 * 1024;
+
+__host__ __device__ constexpr long long book_words(long long pages, long long sequences)
+{
+    return 2 * pages + 7 * sequences; // refs, free ids; lengths, last, first, grow, forks, release
+}
 
 template <bool Small>
 struct BookView
 {
     int* lengths;
     int* refs;
-    __device__ int length(int s) const { return Small ? lengths[s] : __ldcg(&lengths[s]); }
-    __device__ int ref(int id) const { return Small ? refs[id] : __ldcg(&refs[id]); }
+    int* last;  // [sequences] scratch: a fork's length, then the page that a sequence would write into
+    int* first; // [sequences] scratch: where its new pages begin among the free ones
+    int* free_ids;
+    const int* release;
+    const int* forks;
+    const int* grow;
+    __device__ int at(const int* p, int i) const { return Small ? p[i] : __ldcg(&p[i]); }
+    __device__ int length(int s) const { return at(lengths, s); }
+    __device__ int ref(int id) const { return at(refs, id); }
 };
 
 template <bool Small>
-__device__ __forceinline__ BookView<Small> open_book(const PageBook& b, int* shared)
+__device__ __forceinline__ BookView<Small> open_book(const PageBook& b, int* shared, const int* release, int releases,
+                                                     const int* forks, int fork_count, const int* grow)
 {
     if (!Small)
-        return {b.lengths, b.refs};
-    const BookView<Small> v = {shared, shared + b.sequences};
-    for (int i = threadIdx.x; i < b.sequences; i += kBookThreads)
+        return {b.lengths, b.refs, b.per_sequence, b.per_sequence + b.sequences, b.free_ids, release, forks, grow};
+    const int n = b.sequences;
+    int* lists = shared + 2 * b.pages + 3 * n;
+    const BookView<Small> v = {shared + 2 * b.pages, shared, shared + 2 * b.pages + n, shared + 2 * b.pages + 2 * n,
+                               shared + b.pages, lists, lists + n, grow ? lists + 3 * n : nullptr};
+    for (int i = threadIdx.x; i < n; i += kBookThreads)
+    {
         v.lengths[i] = b.lengths[i];
+        if (grow)
+            lists[3 * n + i] = grow[i];
+        if (i < releases)
+            lists[i] = release[i];
+        if (i < fork_count)
+        {
+            lists[n + 2 * i] = forks[2 * i];
+            lists[n + 2 * i + 1] = forks[2 * i + 1];
+        }
+    }
     for (int i = threadIdx.x; i < b.pages; i += kBookThreads)
         v.refs[i] = b.refs[i];
     __syncthreads();
@@ -136,11 +163,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
     constexpr int kWarps = kBookThreads / 32;
     pdl_wait();
     pdl_trigger();
-    const BookView<Small> v = open_book<Small>(b, shared);
+    const BookView<Small> v = open_book<Small>(b, shared, release, releases, forks, fork_count, grow);
 
     for (int i = warp; i < releases; i += kWarps)
     {
-        const int s = release[i];
+        const int s = v.release[i];
         if ((unsigned) s >= (unsigned) b.sequences)
             continue;
         int length = 0;
@@ -160,16 +187,16 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
     __syncthreads();
 
     // Forks: every pair's length is taken before any target is filled.
-    int* fork_length = b.per_sequence;
+    int* fork_length = v.last;
     if (fork_count > 0)
     {
         for (int i = warp; i < fork_count; i += kWarps)
         {
-            const int source = forks[2 * i], target = forks[2 * i + 1];
+            const int source = v.forks[2 * i], target = v.forks[2 * i + 1];
             bool ok = (unsigned) source < (unsigned) b.sequences && (unsigned) target < (unsigned) b.sequences
                       && v.length(target) <= 0;
             for (int e = lane; e < i && ok; e += 32)
-                ok = forks[2 * e + 1] != target;
+                ok = v.forks[2 * e + 1] != target;
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (lane == 0)
                 fork_length[i] = ok ? v.length(source) : 0;
@@ -177,12 +204,12 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
         __syncthreads();
         for (int i = warp; i < fork_count; i += kWarps)
         {
-            const int length = __ldcg(&fork_length[i]);
+            const int length = v.at(fork_length, i);
             if (length <= 0)
                 continue;
             const int held = pages_of(length, b.table_stride);
-            const int* from = b.table + (size_t) forks[2 * i] * b.table_stride;
-            int* to = b.table + (size_t) forks[2 * i + 1] * b.table_stride;
+            const int* from = b.table + (size_t) v.forks[2 * i] * b.table_stride;
+            int* to = b.table + (size_t) v.forks[2 * i + 1] * b.table_stride;
             for (int j = lane; j < held; j += 32)
             {
                 const int id = __ldcg(&from[j]);
@@ -191,7 +218,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
                     atomicAdd(&v.refs[id], 1);
             }
             if (lane == 0)
-                v.lengths[forks[2 * i + 1]] = length;
+                v.lengths[v.forks[2 * i + 1]] = length;
         }
         __syncthreads();
     }
@@ -199,8 +226,8 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
     // Growth: last[s] is the partly filled page that sequence s would write
     // into, -1 when there is none; it is copied while more than one sequence
     // holds it, those before s that have moved off it no longer counted.
-    int* last = b.per_sequence;
-    int* first = b.per_sequence + b.sequences;
+    int* last = v.last;
+    int* first = v.first;
     int wanted = 0, past = 0;
     if (grow)
     {
@@ -208,7 +235,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
         {
             const int length = max(v.length(s), 0);
             int id = -1;
-            if (grow[s] > 0 && (length & (kPagePositions - 1)) && length >> kPageLog < b.table_stride)
+            if (v.grow[s] > 0 && (length & (kPagePositions - 1)) && length >> kPageLog < b.table_stride)
                 id = __ldcg(&b.table[(size_t) s * b.table_stride + (length >> kPageLog)]);
             last[s] = page_there(id, b.pages) && v.ref(id) > 1 ? id : -1;
         }
@@ -217,26 +244,26 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
         {
             const int s = base + tid;
             int need = 0, over = 0;
-            if (s < b.sequences && grow[s] > 0)
+            if (s < b.sequences && v.grow[s] > 0)
             {
                 const int length = max(v.length(s), 0);
-                const long long grown = (long long) length + grow[s];
+                const long long grown = (long long) length + v.grow[s];
                 over = grown > (long long) b.table_stride * kPagePositions;
                 need = over ? 0 : pages_of(grown, b.table_stride) - pages_of(length, b.table_stride);
-                const int id = __ldcg(&last[s]);
+                const int id = v.at(last, s);
                 if (id >= 0)
                 {
                     int holders = v.ref(id);
                     for (int e = 0; e < s; ++e)
-                        holders -= __ldcg(&last[e]) == id;
+                        holders -= v.at(last, e) == id;
                     need += holders > 1 ? 1 : 0;
                     if (holders > 1)
                         need |= 1 << 30; // the copy, kept beside the count
                 }
             }
-            int total, overs;
+            int total;
             const int before = block_scan(need & 0x3FFFFFFF, &total);
-            block_scan(over, &overs);
+            const int overs = __syncthreads_count(over);
             if (s < b.sequences)
                 first[s] = (wanted + before) | (need & (1 << 30));
             wanted = min(wanted + total, 1 << 29); // need <= 2^20: no sum overflows; this many are never there
@@ -262,7 +289,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
             if (free_here[k])
             {
                 if (at < wanted)
-                    b.free_ids[at] = base + 4 * tid + k;
+                    v.free_ids[at] = base + 4 * tid + k;
                 ++at;
             }
         room += total;
@@ -274,8 +301,8 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
         for (int base = 0; base < b.sequences; base += kBookThreads)
         {
             const int s = base + tid;
-            const bool grows = s < b.sequences && grow[s] > 0;
-            const int entry = grows ? __ldcg(&first[s]) : 0;
+            const bool grows = s < b.sequences && v.grow[s] > 0;
+            const int entry = grows ? v.at(first, s) : 0;
             const bool copies = entry & (1 << 30);
             int total;
             const int slot = copied + block_scan(copies, &total);
@@ -285,11 +312,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
             int* row = b.table + (size_t) s * b.table_stride;
             const int length = max(v.length(s), 0);
             const int held = pages_of(length, b.table_stride);
-            const int need = pages_of((long long) length + grow[s], b.table_stride) - held;
+            const int need = pages_of((long long) length + v.grow[s], b.table_stride) - held;
             int at = entry & 0x3FFFFFFF;
             if (copies)
             {
-                const int id = __ldcg(&last[s]), fresh = __ldcg(&b.free_ids[at++]);
+                const int id = v.at(last, s), fresh = v.at(v.free_ids, at++);
                 b.copies[slot] = {id, fresh, length & (kPagePositions - 1)};
                 row[held - 1] = fresh;
                 v.refs[fresh] = 1;
@@ -297,11 +324,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_update_book(const PageBook
             }
             for (int j = 0; j < need; ++j)
             {
-                const int fresh = __ldcg(&b.free_ids[at + j]);
+                const int fresh = v.at(v.free_ids, at + j);
                 row[held + j] = fresh;
                 v.refs[fresh] = 1;
             }
-            v.lengths[s] = length + grow[s];
+            v.lengths[s] = length + v.grow[s];
         }
     if (tid == 0)
     {
@@ -322,14 +349,10 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_book(const PageBoo
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_trigger();
-    const BookView<Small> v = open_book<Small>(b, shared);
+    const BookView<Small> v = open_book<Small>(b, shared, nullptr, 0, nullptr, 0, nullptr);
     int live = 0;
-    {
-        int mine = 0;
-        for (int id = tid; id < b.pages; id += kBookThreads)
-            mine += v.ref(id) > 0;
-        block_scan(mine, &live);
-    }
+    for (int base = 0; base < b.pages; base += kBookThreads)
+        live += __syncthreads_count(base + tid < b.pages && v.ref(base + tid) > 0);
     int leaves = 0, holes = 0;
     for (int base = 0; base < b.pages; base += kBookThreads)
     {
@@ -337,19 +360,19 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_book(const PageBoo
         const bool held = id < b.pages && v.ref(id) > 0;
         const bool leaves_here = held && id >= live, hole = id < live && !held;
         int total;
-        const int at = leaves + block_scan(leaves_here, &total);
-        leaves += total;
-        const int hole_at = holes + block_scan(hole, &total);
-        holes += total;
+        const int both = block_scan(leaves_here | hole << 16, &total); // 1024 of each at most
+        const int at = leaves + (both & 0xFFFF), hole_at = holes + (both >> 16);
+        leaves += total & 0xFFFF;
+        holes += total >> 16;
         if (leaves_here)
             b.copies[at].source = id;
         if (hole)
-            b.free_ids[hole_at] = id;
+            v.free_ids[hole_at] = id;
     }
     __syncthreads();
     for (int i = tid; i < leaves; i += kBookThreads)
     {
-        const int source = __ldcg(&b.copies[i].source), target = __ldcg(&b.free_ids[i]);
+        const int source = __ldcg(&b.copies[i].source), target = v.at(v.free_ids, i);
         b.copies[i] = {source, target, kPagePositions};
         b.renamed[source] = target;
         v.refs[target] = v.ref(source);
