@@ -13,6 +13,14 @@ pytestmark = pytest.mark.gpu
 
 PAGE = native.PAGE_ROWS
 TYPES = ["f32", "bf16", "f16"]
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    native.operators_sync(0, _stream())
+
+
 HEADS = [(8, 1, 256), (8, 2, 128), (4, 4, 64), (6, 2, 96), (7, 1, 80), (3, 3, 8), (10, 2, 40), (2, 2, 200)]
 
 
@@ -584,6 +592,95 @@ def test_two_calls_side_by_side():
     for q, k, v, _, out, _ in runs:
         expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
         ref.close(out, expected, size, q, k, d ** -0.5, 333)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(128, 1, 64), (70, 1, 128), (130, 2, 40)], ids=str)
+def test_many_heads_over_one(kind, heads):
+    """65 to 128 query heads over a kv head: a query tile is a single token."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    lengths = [67, 2]
+    g = torch.Generator("cuda").manual_seed(70)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, 67)
+    cache = Cache(kind, 1, 8, kv, d, [130, 0], 4, 71)
+    _tree(cache, 0, h, kv, d, [3, 2], [[-1, 0, 0], [-1, -1]], 72, 130)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_caches_past_32_bits(kind):
+    """Pages whose first element lies past 2^32 bytes and 2^31 elements of the pool, in every operator that takes pages."""
+    code, dtype = ref.TYPES[kind]
+    kv, d = 4, 128
+    pages = 2 ** 31 // (PAGE * kv * d) + 40  # past 2^31 elements
+    pools = [torch.empty(pages, PAGE, kv * d, dtype=dtype, device="cuda") for _ in range(2)]
+    low, high = [0, 3], list(range(pages - 8, pages))
+    g = torch.Generator("cuda").manual_seed(73)
+    for pool in pools:
+        for p in low + high:
+            pool[p] = _normal(g, PAGE, kv * d, dtype=dtype)
+    table, lengths = [[high[1], low[0], high[5], -1], [high[0], -1, -1, -1]], [150, 64]
+    refs = [0] * pages
+    for p in (high[1], low[0], high[5], high[0]):
+        refs[p] = 1
+    cache = Cache.__new__(Cache)
+    cache.keys, cache.values = (pool[None] for pool in pools)
+    cache.shape, cache.kind, cache.code, cache.dtype = (pages, PAGE, kv, d), kind, code, dtype
+    cache.table, cache.lengths, cache.refs = _ints(table), _ints(lengths), _ints(refs)
+    cache.native = native.PageCache(code, 1, pages, kv * d, 2, 4, pools[0].data_ptr(), pools[1].data_ptr(),
+                                    cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr())
+    cache.room, cache.result = _room(cache.native.workspace_bytes), _ints([0, 0, 0])
+    _tree(cache, 0, 8, kv, d, [4, 1], [[-1, 0, 0, 1], [-1]], 74, 150)
+    rows, offsets, index = _normal(g, 70, 2 * kv * d, dtype=dtype), _ints([0, 30, 33]), _ints([i * 2 for i in range(33)])
+    k, v = rows.split(kv * d, 1)
+    cache.native.write(0, k.data_ptr(), v.data_ptr(), offsets.data_ptr(), 33, source_rows=70, index=index.data_ptr(),
+                       k_stride=rows.stride(0), v_stride=rows.stride(0), stream=_stream())
+    for pool, source in ((pools[0], k), (pools[1], v)):
+        for s, begin, count in ((0, 0, 30), (1, 30, 3)):
+            for i in range(count):
+                j = lengths[s] - count + i
+                assert torch.equal(pool[table[s][j // PAGE], j % PAGE], source[(begin + i) * 2])
+    kept = [[pool[p].clone() for p in (high[0], high[1], high[5])] for pool in pools]
+    cache.native.compact(cache.result.data_ptr(), **cache.kw())
+    assert cache.result.tolist()[0] == 4
+    assert cache.table.tolist() == [[2, 0, 3, -1], [1, -1, -1, -1]] and cache.refs[:5].tolist() == [1, 1, 1, 1, 0]
+    for pool, was in zip(pools, kept):
+        for target, rows_of in zip((1, 2, 3), was):
+            assert torch.equal(pool[target], rows_of)
+
+
+def test_the_default_stream_and_no_stream_argument():
+    g = torch.Generator("cuda").manual_seed(75)
+    (q, k, v), stride = _fused(g, 90, 8, 1, 256, torch.float32)
+    out = torch.empty(q.shape, device="cuda")
+    torch.cuda.synchronize()
+    kept = _run_packed(native.F32, q, k, v, out, [90], stride, stream=0)
+    torch.cuda.synchronize()
+    assert kept
+    expected, size = ref.packed(q, k, v, [90], 1 / 16)
+    ref.close(out, expected, size, q, k, 1 / 16, 90)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_long_prompts_and_caches(kind):
+    """More tiles than any buffer holds, more units than CTAs: a few rows each against the formula."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, n = 4, 2, 64, 6000
+    g = torch.Generator("cuda").manual_seed(76)
+    (q, k, v), stride = _fused(g, n + 7, h, kv, d, dtype)
+    out = torch.empty(q.shape, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, [n, 7], stride)
+    at = torch.tensor([0, 1, 63, 64, 2999, 4096, n - 1], device="cuda")
+    seen = torch.arange(n, device="cuda") <= at[:, None]
+    expected, size = ref.attend(q[at], k[:n], v[:n], seen, d ** -0.5)
+    ref.close(out[at], expected, size, q[at], k, d ** -0.5, n)
+    lengths = [9000, 17, 4500]
+    cache = Cache(kind, 1, 220, kv, d, lengths, 145, 77)
+    _tree(cache, 0, h, kv, d, [2, 5, 64], [_branching(i, i) for i in (2, 5, 64)], 78, 9000)
 
 
 def test_host_memory_is_refused():
