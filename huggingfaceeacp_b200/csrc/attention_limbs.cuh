@@ -190,12 +190,12 @@ struct LimbHead
 {
     uint64_t keys_full[6], keys_ready[6], keys_free[6], values_full[6], values_ready[6], values_free[6];
     uint64_t query, query_free, scores, scores_read, weights[2], done[2], rows_free[2], place_full[2], place_free[2], next,
-        drained[2];
+        sampled[2], drained[2];
     alignas(16) uint4 answer;
     uint32_t tmem;
     int dead;           // a wait ran out
-    int misfit[2];      // a unit's value outside its sampled exponent's range
-    unsigned sample[2]; // a unit's largest sampled K and V, as bits
+    int misfit[2];         // a unit's value outside its sampled exponent's range
+    unsigned sample[2][2]; // a unit's largest sampled K and V, as bits
     MmaPlace place[2];
     int8_t parents[2][kTreeNodes];
 };
@@ -256,8 +256,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             mbar_init(&h.place_full[b], 1);
             mbar_init(&h.place_free[b], Tree ? 15 : 11); // an arrival a warp but the one that finds them
             mbar_init(&h.drained[b], 1);
-            h.misfit[b] = 0;
-            h.sample[b] = 0;
+            mbar_init(&h.sampled[b], 4); // an arrival a converter warp
         }
         h.dead = 0;
         mbar_fence_init();
@@ -546,11 +545,12 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         MmaPlace p;
         for (int i = 0;; ++i)
         {
-            if (any_stops(5, Tree ? 384 : 256, !ok || !take(i, p)))
+            if (any_stops(5, 256, !ok || !take(i, p)))
                 break;
             const int tiles = p.tiles;
             const int token = p.token0 + row / a.group, head = p.kv_head * a.group + row % a.group;
             const bool real = row < c.tile_tokens * a.group && token < p.length;
+            const bool idle = !__any_sync(0xFFFFFFFFu, real); // no row of the warp's: it keeps the others' step only
             const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
 
             // The queries' halves, a row a warp: lane c the channels [8 c, 8 c + 8).
@@ -561,6 +561,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             {
                 float x[8][8];
                 int t = ((warp - 4) * 16 + half * 8) / a.group, g = ((warp - 4) * 16 + half * 8) % a.group;
+                if (t >= min(c.tile_tokens, p.length - p.token0))
+                    break; // rows that are not there may hold anything: it stays with them
                 const float* from = (const float*) a.q + (long long) (p.begin + p.token0) * a.q_stride
                                     + (size_t) p.kv_head * a.group * a.width + lane * 8;
 #pragma unroll
@@ -635,17 +637,16 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             float kfactor = 1.f, vfactor = 1.f;
             if (Tree)
             {
-                named_sync(2, 384); // the converters' sample
-                kfactor = 1.f / split_factor(__uint_as_float(h.sample[0]), 11);
-                vfactor = 1.f / split_factor(__uint_as_float(h.sample[1]), 11);
-                named_sync(4, 384); // it has been read
+                ok = ok && wait(&h.sampled[i & 1], (i / 2) & 1);
+                kfactor = 1.f / split_factor(__uint_as_float(h.sample[i & 1][0]), 11);
+                vfactor = 1.f / split_factor(__uint_as_float(h.sample[i & 1][1]), 11);
             }
             else
             {
                 kfactors = lc.factors + (size_t) p.kv_head * lc.tiles + p.begin / kKeyTile + p.sequence;
                 vfactors = kfactors + (size_t) a.kv_heads * lc.tiles;
-                named_sync(1, 256); // the row factors have been read
             }
+            named_sync(1, 256); // the row factors have been read
 
             float acc[kHalf];
 #pragma unroll
@@ -663,6 +664,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
 #pragma unroll
                 for (int b = 0; b < kHalf; b += 32)
                 {
+                    if (idle)
+                        break;
                     uint32_t o[32];
                     tc_ld32(at + b, o);
                     tc_wait_ld32(o);
@@ -695,6 +698,18 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 // warpgroups before the last tile's exchange.
                 ok = ok && wait(&h.scores, count & 1);
                 tc_fence_after();
+                if (idle)
+                {
+                    if (ok && lane == 0)
+                    {
+                        mbar_arrive(&h.scores_read);
+                        mbar_arrive(&h.weights[count & 1]);
+                    }
+                    named_sync(1, 256);
+                    if (j > 0)
+                        drain(count - 1, 1.f, 0.f);
+                    continue;
+                }
                 float s[32];
                 {
                     uint32_t large[32], small[32];
@@ -792,6 +807,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
 #pragma unroll
             for (int b = 0; b < kChunks; ++b)
             {
+                if (idle)
+                    break;
                 float2 v[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
@@ -807,7 +824,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             constexpr int kAtOnce = 32 / kChunks; // rows
             const int chunk = lane & (kChunks - 1), channel = group * kHalf + 4 * chunk;
 #pragma unroll 4
-            for (int r0 = 0; r0 < 32; r0 += kAtOnce)
+            for (int r0 = 0; r0 < 32 && !idle; r0 += kAtOnce)
             {
                 const int r = r0 + lane / kChunks;
                 char* to = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, r);
@@ -843,12 +860,18 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         MmaPlace p;
         for (int i = 0;; ++i)
         {
-            if (any_stops(5, 384, !ok || !take(i, p)))
+            if (any_stops(2, 128, !ok || !take(i, p)))
                 break;
             const int tiles = p.tiles;
             const int* table = a.table + (size_t) p.sequence * a.table_stride;
             // The exponents: the largest of 16 keys spread over the unit's, an
-            // eighth of their channels a thread.
+            // eighth of their channels a thread. The row warps have left the unit
+            // before the last, whose slot this is.
+            if (t < 2)
+                h.sample[i & 1][t] = 0;
+            if (t == 2)
+                h.misfit[i & 1] = 0;
+            named_sync(3, 128);
             {
                 const int end = min((p.first_tile + tiles) * kKeyTile, p.cached), from = p.first_tile * kKeyTile;
                 const int which = t >> 3;
@@ -881,20 +904,15 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                 mk = warp_max(mk), mv = warp_max(mv);
                 if (lane == 0)
                 {
-                    atomicMax(&h.sample[0], __float_as_uint(mk));
-                    atomicMax(&h.sample[1], __float_as_uint(mv));
+                    atomicMax(&h.sample[i & 1][0], __float_as_uint(mk));
+                    atomicMax(&h.sample[i & 1][1], __float_as_uint(mv));
                 }
             }
-            named_sync(2, 384); // with the row warps, who wait for the exponents
-            const float factors[2] = {split_factor(__uint_as_float(h.sample[0]), 11),
-                                      split_factor(__uint_as_float(h.sample[1]), 11)};
-            named_sync(4, 384);
-            if (t == 0)
-            {
-                h.sample[0] = h.sample[1] = 0;
-                h.misfit[(i & 1) ^ 1] = 0; // the last unit's has been read: its rows are stored
-            }
             named_sync(3, 128);
+            const float factors[2] = {split_factor(__uint_as_float(h.sample[i & 1][0]), 11),
+                                      split_factor(__uint_as_float(h.sample[i & 1][1]), 11)};
+            if (lane == 0)
+                mbar_arrive(&h.sampled[i & 1]);
             bool misfit = false;
             auto convert = [&](int j, float factor, bool is_value, uint8_t* ring, int& taken, int stages, uint64_t* full,
                                uint64_t* ready) {

@@ -817,6 +817,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             const int n = tiles_of(p, q);
             const int token = p.token0 + q * c.tile_tokens + row / a.group, head = p.kv_head * a.group + row % a.group;
             const bool real = row < c.tile_tokens * a.group && token < p.length;
+            const bool idle = !__any_sync(0xFFFFFFFFu, real); // no row of the warp's: it keeps the others' step only
             const int* table = Tree ? a.table + (size_t) p.sequence * a.table_stride : nullptr;
             unsigned long long path = 0;
             if (Tree)
@@ -841,6 +842,15 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 if (!ok)
                     break;
                 tc_fence_after();
+                if (idle)
+                {
+                    if (lane == 0)
+                    {
+                        mbar_arrive(&h.scores_read[q]);
+                        mbar_arrive(&h.weights[q][count & 1]);
+                    }
+                    continue;
+                }
                 uint32_t r[64];
                 tc_ld32(sbase, r);
                 tc_ld32(sbase + 32, r + 32);
@@ -937,7 +947,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 for (int k = 0; k < 4; ++k)
                     four[k] = (char*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) mine, (lane & ~3) + k);
 #pragma unroll 1
-                for (int b = 0; b < a.width; b += 32)
+                for (int b = 0; b < a.width && !idle; b += 32)
                 {
                     uint32_t o[32];
                     tc_ld32(obase + b, o);
