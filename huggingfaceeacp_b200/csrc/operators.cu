@@ -3,6 +3,7 @@
 // state: every check is made on the host before the first launch.
 #include <hf_cuda.h>
 
+#include "attention_few.cuh"
 #include "attention_limbs.cuh"
 #include "attention_mma.cuh"
 #include "attention_rows.cuh"
@@ -254,10 +255,10 @@ EncodeTiled encoder()
 }
 
 // [rows][heads][width] elements, rows `stride` elements apart, in boxes of 128
-// bytes of channels x box_heads x box_rows with the 128-byte swizzle; zeros
-// outside.
+// bytes of channels x box_heads x box_rows with the 128-byte swizzle, or of `plain`
+// channels without one; zeros outside.
 bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int heads, int64_t rows, int64_t stride,
-                 int box_heads, int box_rows)
+                 int box_heads, int box_rows, int plain = 0)
 {
     const EncodeTiled encode = encoder();
     const int size = size_of(dtype);
@@ -266,11 +267,11 @@ bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int h
                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const cuuint64_t dims[3] = {(cuuint64_t) width, (cuuint64_t) heads, (cuuint64_t) rows};
     const cuuint64_t strides[2] = {(cuuint64_t) width * size, (cuuint64_t) stride * size};
-    const cuuint32_t box[3] = {(cuuint32_t) (128 / size), (cuuint32_t) box_heads, (cuuint32_t) box_rows};
+    const cuuint32_t box[3] = {(cuuint32_t) (plain ? plain : 128 / size), (cuuint32_t) box_heads, (cuuint32_t) box_rows};
     const cuuint32_t ones[3] = {1, 1, 1};
     return encode
            && encode(map, type, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
                   == CUDA_SUCCESS;
 }
@@ -428,11 +429,43 @@ int packed_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t st
                           : launch_limbs<64, false>(maps, l, ctas, device, stream);
 }
 
+template <int D>
+int launch_few(const AttnCall& a, const MmaCall& c, int device, cudaStream_t stream)
+{
+    using Shape = FewShape<D>;
+    CUtensorMap maps[4] = {};
+    const int64_t positions = (int64_t) a.pages * kPagePositions, kvw = (int64_t) a.kv_heads * a.width;
+    if (!encode_rows(&maps[0], HF_DTYPE_F32, a.k, a.width, a.kv_heads, a.rows, a.k_stride, 1, kFewKeys, D)
+        || !encode_rows(&maps[1], HF_DTYPE_F32, a.v, a.width, a.kv_heads, a.rows, a.v_stride, 1, kFewKeys, D)
+        || !encode_rows(&maps[2], HF_DTYPE_F32, a.key_pages, a.width, a.kv_heads, positions, kvw, 1, kFewKeys, D)
+        || !encode_rows(&maps[3], HF_DTYPE_F32, a.value_pages, a.width, a.kv_heads, positions, kvw, 1, kFewKeys, D))
+        return HF_E_CUDA;
+    static std::atomic<uint64_t> ready {0}; // devices whose kernel has its shared memory
+    const uint64_t bit = 1ull << (device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit))
+    {
+        if (cudaFuncSetAttribute(attention_few<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess)
+            return HF_E_CUDA;
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return status_of(launch(true, attention_few<D>, dim3(c.ctas), dim3(Shape::kThreads), Shape::kSmem, stream, maps[0],
+                            maps[1], maps[2], maps[3], c));
+}
+
 int tree_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t stream)
 {
     LimbCall l = {};
     MmaCall& c = l.c;
     tree_call(&c, HF_DTYPE_F32, a, workspace);
+    // Up to eight rows a kv head the FMAs keep up with HBM, and nothing has to be
+    // turned into halves.
+    if (c.part_rows <= kFewRows)
+    {
+        const int rc = a.width > 128  ? launch_few<256>(a, c, device, stream)
+                       : a.width > 64 ? launch_few<128>(a, c, device, stream)
+                                      : launch_few<64>(a, c, device, stream);
+        return rc ? rc : join<float>(c, stream);
+    }
     const int ctas = c.ctas;
     CUtensorMap maps[4] = {};
     const int64_t positions = (int64_t) a.pages * kPagePositions, kvw = (int64_t) a.kv_heads * a.width;
