@@ -10,8 +10,8 @@
 // Work. The key tiles are shared out to the CTAs as for the other trees. Tiles pass
 // through a ring in halves of 32 keys, K then V, each one tensor-map copy; warp w
 // takes keys 4 w to 4 w + 3 of each. A lane holds 4 channels of every 128 (the
-// queries and the sums of all eight rows, in registers), so a key's row is read by
-// conflict-free 16-byte loads; the 4 x 8 scores are summed over the lanes by halving
+// sums of all eight rows, in registers; the queries lie in shared memory, since nine
+// warps get 168 registers each), so rows are read by conflict-free 16-byte loads; the 4 x 8 scores are summed over the lanes by halving
 // (31 shuffles: lane r + 8 k ends with row r, key k). Each warp has its own running
 // maximum and sum over its own keys, and its own rows of O; the warps meet at the
 // end of a unit. No fp32 chain is longer than a warp's keys.
@@ -33,7 +33,8 @@ struct FewShape
     static constexpr int kHead = 1024;
     static constexpr int kMeet = kFewWarps * kFewRows * (D + 2) * 4; // the warps' rows at the end of a unit
     static constexpr int kStages = D == 256 ? 4 : 8;
-    static constexpr int kSmem = kHead + kMeet + kStages * kStageBytes;
+    static constexpr int kQueries = kFewRows * D * 4;
+    static constexpr int kSmem = kHead + kMeet + kQueries + kStages * kStageBytes;
     static constexpr int kThreads = 32 * (kFewWarps + 1);
     static_assert(kSmem <= 227 * 1024 && kStages % 4 == 0, "what an SM holds; a unit's items begin at any stage");
 };
@@ -57,7 +58,8 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
     FewHead& h = *reinterpret_cast<FewHead*>(smem);
     static_assert(sizeof(FewHead) <= Shape::kHead, "the head's room");
     uint8_t* ring = smem + Shape::kHead;
-    float* meet = reinterpret_cast<float*>(ring + S * Shape::kStageBytes);
+    float4* queries = reinterpret_cast<float4*>(ring + S * Shape::kStageBytes); // [row][channel]
+    float* meet = reinterpret_cast<float*>(ring + S * Shape::kStageBytes + Shape::kQueries);
     const AttnCall& a = c.a;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
 
@@ -161,19 +163,25 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
         const MmaPlace p = h.place[i & 1];
         const int* table = a.table + (size_t) p.sequence * a.table_stride;
         const int rows = min(p.length - p.token0, c.tile_tokens) * a.group; // at most eight
-        float4 q[kFewRows][V], acc[kFewRows][V];
+        float4 acc[kFewRows][V];
 #pragma unroll
         for (int r = 0; r < kFewRows; ++r)
 #pragma unroll
             for (int v = 0; v < V; ++v)
-            {
-                const int channel = 128 * v + 4 * lane, token = p.begin + p.token0 + r / a.group;
-                q[r][v] = acc[r][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < rows && channel < a.width)
-                    q[r][v] = *reinterpret_cast<const float4*>((const float*) a.q + token * a.q_stride
-                                                               + (size_t) (p.kv_head * a.group + r % a.group) * a.width
-                                                               + channel);
-            }
+                acc[r][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        // A row a warp; the warps' meeting at the end of the last unit freed the room.
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+        {
+            const int channel = 128 * v + 4 * lane, token = p.begin + p.token0 + warp / a.group;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (warp < rows && channel < a.width)
+                x = *reinterpret_cast<const float4*>((const float*) a.q + token * a.q_stride
+                                                     + (size_t) (p.kv_head * a.group + warp % a.group) * a.width + channel);
+            if (channel < D)
+                queries[warp * (D / 4) + 32 * v + lane] = x;
+        }
+        named_sync(2, 32 * kFewWarps);
         unsigned long long path = 0;
         if (row < rows)
             path = tree_path(a.parents + p.begin, p.token0 + row / a.group);
@@ -190,28 +198,37 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
                 const int ks = item % S, vs = (item + 1) % S;
                 ok = ok && warp_wait(&h.full[ks], (item / S) & 1);
                 float s[4 * kFewRows];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
                 {
-                    const float4* from =
-                        reinterpret_cast<const float4*>(ring + ks * Shape::kStageBytes + (4 * warp + k) * D * 4);
-                    float4 x[V];
+                    float4 x[4][V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v)
-                        x[v] = 128 * v + 4 * lane < D ? from[32 * v + lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int v = 0; v < V; ++v)
+                            x[k][v] = 128 * v + 4 * lane < D
+                                          ? reinterpret_cast<const float4*>(ring + ks * Shape::kStageBytes
+                                                                            + (4 * warp + k) * D * 4)[32 * v + lane]
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int r = 0; r < kFewRows; ++r)
                     {
-                        float dot = 0.f;
+                        float dot[4] = {};
 #pragma unroll
                         for (int v = 0; v < V; ++v)
                         {
-                            dot = fmaf(q[r][v].x, x[v].x, dot);
-                            dot = fmaf(q[r][v].y, x[v].y, dot);
-                            dot = fmaf(q[r][v].z, x[v].z, dot);
-                            dot = fmaf(q[r][v].w, x[v].w, dot);
+                            const float4 q = 128 * v + 4 * lane < D ? queries[r * (D / 4) + 32 * v + lane]
+                                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                            {
+                                dot[k] = fmaf(q.x, x[k][v].x, dot[k]);
+                                dot[k] = fmaf(q.y, x[k][v].y, dot[k]);
+                                dot[k] = fmaf(q.z, x[k][v].z, dot[k]);
+                                dot[k] = fmaf(q.w, x[k][v].w, dot[k]);
+                            }
                         }
-                        s[8 * k + r] = dot;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            s[8 * k + r] = dot[k];
                     }
                 }
                 __syncwarp();

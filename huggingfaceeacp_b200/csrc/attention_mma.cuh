@@ -259,7 +259,7 @@ __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
 // A batch of trees is one row of key tiles: sequence after sequence, in it query tile
 // after query tile of each kv head, of each its cached tiles and the drafted one.
 // It is cut for the CTAs in one of two ways:
-//  few query tiles (a CTA's share is less than half of one): each is cut into pieces
+//  few query tiles (a CTA's share is less than a quarter of one): each is cut into pieces
 //  of at most `per` tiles, no more pieces than CTAs. A CTA takes one piece: a
 //  second would cost it another start (about 10 us of a 60 us call of 16 trees in
 //  fp32);
@@ -311,7 +311,7 @@ __device__ inline TreeCut cut_trees(const MmaCall& c, const TreeRow& known, int&
     total = __reduce_add_sync(0xFFFFFFFFu, total);
     query_tiles = __reduce_add_sync(0xFFFFFFFFu, query_tiles);
     // The sum of n / per, each rounded up, is at most total / per + query_tiles.
-    const bool few = 2 * query_tiles <= c.ctas;
+    const bool few = 4 * query_tiles <= c.ctas;
     const int share = few ? c.ctas - query_tiles : c.ctas;
     return {few, max((total + share - 1) / share, 2)};
 }
