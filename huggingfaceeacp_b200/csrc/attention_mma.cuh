@@ -13,10 +13,9 @@
 //  places   a warp finds the next unit while this one is worked on;
 //  copies   query tiles, then key and value tiles, each through a ring of its
 //           own (tensor maps; a page is one box), on into the next unit as far
-//           as there is room. Of a ring that both passed
-//           through, a warp that takes only the keys would see every other phase of
-//           a stage's barrier, and its parity cannot tell a phase from the one
-//           two before;
+//           as there is room. (Of one ring for both, a warp that takes only the
+//           keys would see every other phase of a stage's barrier, and its parity
+//           cannot tell a phase from the one two before.)
 //  MMAs     a warp for each query tile's S and one for its O, since a warp's
 //           waits and MMAs follow one another: S of the next tile is issued as
 //           soon as S of this one is in registers, O of a tile as soon as its
@@ -43,6 +42,17 @@
 // A batch of trees is shared out evenly in key tiles, so a query tile's keys may
 // lie with several CTAs: each leaves its rows' maximum, sum and unnormalised O in
 // the workspace, and attention_join puts them together.
+//
+// Measured (B200, CUDA events). Prompts, 4 x 4096 tokens, 32 heads of 128 over 8:
+// 510 us, 1,075 TFLOP/s, 0.65 of the measured cuBLAS rate, the tensor pipe active
+// 52 % of the time; 8 heads of 256 over one: 1,198 TFLOP/s, 59 %. Bound by the
+// softmax warps: a step of both query tiles (256 rows x 64 keys) takes some 1,700
+// cycles, 1,000 of them the weights, whose special-function (640), FMA (540) and
+// ALU (580) time two warps a scheduler overlap only partly; its MMAs take 1,280
+// (N = 64 scores are bound by the 6 KB that each reads from shared memory, 48
+// cycles instead of 32). Tried and no faster: two warpgroups a query tile, the
+// tiles' warps taking turns, 2 or 4 of 8 pairs on the FMA pipe. Trees, one token for
+// each of 64 caches of 4,000: 167 us for 1.07 GB, 0.97 of the measured copy rate.
 #pragma once
 
 #include "attention_rows.cuh"

@@ -414,7 +414,7 @@ int hf_cuda_operators_sync(int device, void* stream);
  * outside every sequence are neither read nor written. head_width is a multiple
  * of 8 up to 256, heads / kv_heads at most 128. `scale` (> 0) multiplies the scores.
  * A value or key row that holds infinities or NaN reaches only the rows that
- * attend to it. */
+ * attend to it. `out` may not overlap q, k or v. */
 typedef struct hf_attention_packed
 {
     int32_t dtype;
