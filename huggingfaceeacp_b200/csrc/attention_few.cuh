@@ -362,6 +362,8 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
             }
             if (!p.whole && lane == 0)
                 c.part_ml[part] = make_float2(top, sum);
+            if (p.first_tile == 0 && warp % a.group == 0 && lane == 0)
+                c.spans[(size_t) at * a.kv_heads + p.kv_head] = span_of(p, blockIdx.x);
             __syncwarp();
             if (__any_sync(0xFFFFFFFFu, ok && !(check == 0.f)))
                 take_again<float, true>(c, h.place[i & 1], at, head);

@@ -172,7 +172,7 @@ struct LimbShape
     static constexpr int kBox = kKeyTile * 128;          // 64 keys x 64 channels of one half
     static constexpr int kStageBytes = 2 * kBox;
     static constexpr int kQueryHalf = kBlocks * 128 * 128;
-    static constexpr int kHead = 3072;
+    static constexpr int kHead = 3 * 1024;
     static constexpr int kStagesFit = (227 * 1024 - kHead - 2 * kQueryHalf) / kStageBytes;
     static constexpr int kStages = kStagesFit > 12 ? 12 : kStagesFit;
     static constexpr int kKeyStages = kStages / 2, kValueStages = kStages - kKeyStages;
@@ -268,8 +268,6 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         h.dead = 0;
         mbar_fence_init();
     }
-    else if (warp == 1)
-        tc_alloc(&h.tmem, 512);
     else if (warp == 2 && lane == 0)
     {
         prefetch_map(&kmap);
@@ -278,7 +276,10 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
         prefetch_map(&vmap2);
     }
     // Of prompts: split_tiles' halves, of trees whatever is ahead in the stream.
+    // TMEM is asked for behind it: that kernel may still want it.
     pdl_wait();
+    if (warp == 1)
+        tc_alloc(&h.tmem, 512);
     // The first place is found while TMEM is made.
     MmaPlace first = {};
     TreePlaces places;
@@ -840,6 +841,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             }
             if (Tree && !whole && real && group == 0)
                 c.part_ml[part] = make_float2(m, l * 0x1p-14f);
+            if (Tree && real && group == 0 && p.first_tile == 0 && row % a.group == 0)
+                c.spans[(size_t) at * a.kv_heads + p.kv_head] = span_of(p, blockIdx.x);
             const bool finite = check.x + check.y == 0.f;
             exchange[(tiles & 1) ^ 1][group][row] = finite ? 0.f : 1.f;
             named_sync(1, 256);

@@ -74,7 +74,9 @@ struct MmaCall
     int part_rows;   // rows of a part: a query tile's at most
     float* part_o;   // [2 ctas][part_rows][width]
     float2* part_ml; // [2 ctas][part_rows]
+    int2* spans;     // [rows][kv_heads]: the first and the last CTA that hold a row's keys (few: first | kFew)
 };
+constexpr int kFew = 1 << 30;
 
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the
 // addition of 1.5 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by the
@@ -152,6 +154,8 @@ struct MmaPlace
     int token0, kv_head, part;
     int cached, tiles_cached; // a tree's
     int first_tile, tiles;    // its key tiles
+    int last_cta;             // a tree's that begins here: who holds its last tile
+    bool few;
     bool whole;               // all of its keys: finish the rows
 };
 
@@ -245,6 +249,32 @@ __device__ inline void find_tile(const AttnCall& a, int step, int r, int& sequen
     }
 }
 
+// The same of more sequences than a lane keeps, in the sequences' order, each one's
+// last tile first: tile j of sequence s has number begin_s / step + s + j, so a search
+// 32 ways at a time finds it (in descending order of place each unit would cost a
+// pass over all sequences).
+__device__ inline void find_tile_of_many(const AttnCall& a, int step, int r, int& sequence, int& tile)
+{
+    const int lane = threadIdx.x & 31;
+    int low = -1, high = a.sequences; // the number of low's first tile <= r < that of high's
+    while (high - low > 1)
+    {
+        const int stride = (high - low + 31) / 32, s = low + (lane + 1) * stride;
+        const bool below = s < high && bounded_offset(a.offsets, s, a.rows) / step + s <= r;
+        const int n = __popc(__ballot_sync(0xFFFFFFFFu, below));
+        low += n * stride;
+        high = min(high, low + stride);
+    }
+    sequence = -1;
+    if (low < 0)
+        return;
+    const int begin = bounded_offset(a.offsets, low, a.rows);
+    const int length = bounded_offset(a.offsets, low + 1, a.rows) - begin, tiles = (length + step - 1) / step;
+    tile = tiles - 1 - (r - begin / step - low);
+    if (length > 0 && tile >= 0)
+        sequence = low;
+}
+
 // Where unit `unit` (a CTA of the grid) of packed prompts works, its rows in steps
 // of `step` tokens; by a whole warp.
 __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
@@ -253,7 +283,10 @@ __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
     MmaPlace p = {};
     int s, tile = 0;
     p.kv_head = unit % a.kv_heads;
-    find_tile(a, step, unit / a.kv_heads, s, tile);
+    if (a.sequences <= 128)
+        find_tile(a, step, unit / a.kv_heads, s, tile);
+    else
+        find_tile_of_many(a, step, unit / a.kv_heads, s, tile);
     p.sequence = s;
     if (s >= 0)
     {
@@ -331,7 +364,8 @@ struct TreePlaces
 {
     TreeRow known; // the lane's of the first 32 sequences
     TreeCut cut;
-    int at, end, cta; // tiles; few: pieces
+    int at, end, cta;       // tiles; few: pieces
+    int base = 0, before = 0; // the 32 sequences to go on from, and what lies before them
 
     __device__ void begin(const MmaCall& c, int which)
     {
@@ -350,7 +384,7 @@ struct TreePlaces
         const int lane = threadIdx.x & 31;
         MmaPlace p = {};
         p.sequence = -1;
-        for (int base = 0, before = 0; base < a.sequences && at < end; base += 32)
+        for (; base < a.sequences && at < end; base += 32)
         {
             const TreeRow mine = base ? tree_row(c, base + lane) : known;
             int sum = share(mine);
@@ -380,6 +414,8 @@ struct TreePlaces
                     p.first_tile = (int) ((long long) tiles * rest / each);
                     p.tiles = (int) ((long long) tiles * (rest + 1) / each) - p.first_tile;
                     p.part = 2 * cta;
+                    p.last_cta = cta + each - 1;
+                    p.few = true;
                     at = end;
                 }
                 else
@@ -387,6 +423,7 @@ struct TreePlaces
                     p.first_tile = rest;
                     p.tiles = min(tiles - rest, end - at);
                     p.part = 2 * cta + (rest == 0);
+                    p.last_cta = (at + tiles - 1) / cut.per; // where rest is 0
                     at += p.tiles;
                 }
                 p.whole = p.tiles == tiles;
@@ -397,6 +434,12 @@ struct TreePlaces
         return p;
     }
 };
+
+// What a unit that begins its query tile leaves for attention_join.
+__device__ __forceinline__ int2 span_of(const MmaPlace& p, int cta)
+{
+    return make_int2(p.few ? cta | kFew : cta, p.last_cta);
+}
 
 // A row that came out not finite, by a whole warp: the same keys again, read
 // only where the row attends to them.
@@ -544,8 +587,6 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         h.dead = 0;
         mbar_fence_init();
     }
-    else if (warp == 1)
-        tc_alloc(&h.tmem, Shape::kTmem);
     else if (warp == 2 && lane == 0)
     {
         prefetch_map(&qmap);
@@ -557,7 +598,11 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
             prefetch_map(&vpages);
         }
     }
-    pdl_wait(); // the set-up above ran beside the end of the kernel ahead in the stream
+    // The set-up above ran beside the end of the kernel ahead in the stream. TMEM is
+    // asked for behind it: that kernel may still want it.
+    pdl_wait();
+    if (warp == 1)
+        tc_alloc(&h.tmem, Shape::kTmem);
     // The first place is found while TMEM is made.
     MmaPlace first = {};
     TreePlaces places;
@@ -997,6 +1042,8 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                     mbar_arrive(&h.rows_free[q]);
                 if (Tree && !whole && real)
                     c.part_ml[part] = make_float2(m, l);
+                if (Tree && real && p.first_tile == 0 && row % a.group == 0)
+                    c.spans[(size_t) at * a.kv_heads + p.kv_head] = span_of(p, blockIdx.x);
                 // Rows that came out not finite: again, from what they attend to only.
                 unsigned again = __ballot_sync(0xFFFFFFFFu, ok && real && !(check.x + check.y == 0.f));
                 while (again)
@@ -1031,26 +1078,14 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
         pdl_wait();
         return;
     }
-    const TreeRow mine = tree_row(c, s);
-    const TreeRow known = tree_row(c, threadIdx.x & 31);
-    int total;
-    const TreeCut cut = cut_trees(c, known, total);
-    int before = 0;
-    for (int base = 0; base < s; base += 32)
-    {
-        const int lane = threadIdx.x & 31;
-        const TreeRow r = base ? tree_row(c, base + lane) : known;
-        before += base + lane < s ? (cut.few ? r.query_tiles * cut.pieces(r.tiles) : r.total()) : 0;
-    }
-    before = __reduce_add_sync(0xFFFFFFFFu, before);
-    const int query_tile = node / c.tile_tokens * a.kv_heads + head / a.group;
-    const int each = cut.few ? cut.pieces(mine.tiles) : mine.tiles, first = before + query_tile * each;
-    const int from = cut.few ? first : first / cut.per, to = cut.few ? first + each - 1 : (first + each - 1) / cut.per;
     pdl_wait();
+    const int2 span = c.spans[(size_t) row * a.kv_heads + head / a.group];
+    const bool few = span.x & kFew;
+    const int from = span.x & ~kFew, to = span.y;
     if (from == to)
         return;
     const int within = node % c.tile_tokens * a.group + head % a.group;
-    auto part_of = [&](int cta) { return (size_t) (2 * cta + (!cut.few && cta == from)) * c.part_rows + within; };
+    auto part_of = [&](int cta) { return (size_t) (2 * cta + (!few && cta == from)) * c.part_rows + within; };
     // 32 parts at a time, a lane's maximum and sum each; four parts' rows in flight.
     float m = -INFINITY, l = 0.f, acc[8] = {};
     for (int base = from; base <= to; base += 32)

@@ -343,6 +343,7 @@ void tree_call(MmaCall* c, int dtype, const AttnCall& a, void* workspace)
     c->part_rows = part_rows(a.heads, a.kv_heads, a.max_nodes);
     c->part_o = (float*) workspace;
     c->part_ml = (float2*) (c->part_o + (size_t) 2 * c->ctas * c->part_rows * a.width);
+    c->spans = (int2*) (c->part_ml + (size_t) 2 * c->ctas * c->part_rows);
 }
 
 template <typename T>
@@ -512,7 +513,8 @@ uint64_t packed_workspace(const hf_attention_packed& call)
 uint64_t tree_workspace(const hf_page_cache& c, const hf_attention_tree& call)
 {
     return (uint64_t) 2 * tree_ctas(c.dtype, call.head_width) * part_rows(call.heads, call.kv_heads, call.max_nodes)
-           * (4 * call.head_width + 8);
+           * (4 * call.head_width + 8)
+           + (uint64_t) 8 * call.rows * call.kv_heads;
 }
 } // namespace
 

@@ -595,6 +595,44 @@ def test_two_calls_side_by_side():
 
 
 @pytest.mark.parametrize("kind", TYPES)
+def test_thousands_of_sequences(kind):
+    """More sequences than a warp keeps in registers, many of them empty: prompts and decode steps."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, n = 4, 2, 64, 3000
+    lengths = [0 if i % 3 == 1 else (i * 7) % 20 if i % 50 else 90 + i % 60 for i in range(n)]
+    g = torch.Generator("cuda").manual_seed(80)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    begin = 0
+    for i, length in enumerate(lengths):
+        if length and i % 97 in (0, 50):
+            rows = slice(begin, begin + length)
+            expected, size = ref.packed(q[rows], k[rows], v[rows], [length], d ** -0.5)
+            ref.close(out[rows], expected, size, q[rows], k[rows], d ** -0.5, length)
+        begin += length
+    assert not bool(torch.isnan(out).any())
+    cached = [(i * 11) % 150 for i in range(n)]
+    cache = Cache(kind, 1, sum(-(-x // PAGE) for x in cached) + 2, kv, d, cached, 3, 81)
+    nodes = [1 if i % 4 else 0 for i in range(n)]
+    (q, k, v), stride = _fused(g, sum(nodes), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    plan, offsets, up = native.TreeAttention(code, h, kv, d), _ints(_offsets(nodes)), _ints([-1] * sum(nodes))
+    room = _room(plan.workspace_bytes(n, len(q), 1, 150))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(),
+             len(q), 1, 150, q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(),
+             workspace_bytes=room.numel(), stream=_stream())
+    assert not bool(torch.isnan(out).any())
+    at, table = _offsets(nodes), cache.table.tolist()
+    for s in range(0, n, 61):
+        rows = slice(at[s], at[s + 1])
+        if nodes[s]:
+            expected, size = ref.tree(q[rows], k[rows], v[rows], [1], [[-1]], cache.keys[0].view(cache.shape),
+                                      cache.values[0].view(cache.shape), [table[s]], [cached[s]], d ** -0.5)
+            ref.close(out[rows], expected, size, q[rows], cache.keys[0].view(-1, kv, d), d ** -0.5, 151)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("heads", [(128, 1, 64), (70, 1, 128), (130, 2, 40)], ids=str)
 def test_many_heads_over_one(kind, heads):
     """65 to 128 query heads over a kv head: a query tile is a single token."""
