@@ -314,10 +314,16 @@ int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
     MmaCall c = {};
     c.a = a;
     c.tile_tokens = 128 / a.group;
-    // Two query tiles a CTA read the keys half as often; with fewer of them
-    // than SMs the rows are spread over twice the CTAs instead.
+    // Two query tiles a CTA read the keys half as often (300 prompts of 100 to 400 tokens,
+    // 32 heads on 8 of 128: 367 us, with one tile 422); with fewer of them than SMs
+    // the rows are spread over twice the CTAs instead. Of prompts of less than three
+    // tiles a second one is mostly empty, and what a unit costs to begin and to end
+    // counts: two CTAs a SM of one tile each overlap it (4096 prompts of up to 16 tokens:
+    // 453 us, with two tiles 852; 2048 of up to 64: 322 and 440; 1000 of 50 to 150: 463
+    // and 463).
     const int64_t pairs = (int64_t) a.rows * a.heads / 256;
-    const int nq = a.width <= 128 && pairs >= kSms ? 2 : 1;
+    const bool shorts = a.rows < 3LL * c.tile_tokens * a.sequences;
+    const int nq = a.width <= 128 && pairs >= kSms && !shorts ? 2 : 1;
     const int64_t ctas = ((int64_t) a.rows / (c.tile_tokens * nq) + a.sequences) * a.kv_heads;
     CUtensorMap maps[5] = {};
     if (!encode_rows(&maps[0], dtype, a.q, a.width, a.heads, a.rows, a.q_stride, a.group, c.tile_tokens)

@@ -109,6 +109,22 @@ def test_packed_prompts_of_many_sequences(kind):
     ref.close(out, expected, size, q, k, 64 ** -0.5, max(lengths))
 
 
+@pytest.mark.parametrize("heads", [(16, 4, 128), (12, 12, 64)], ids=str)
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths", [[i * 37 % 41 for i in range(300)], [95, 97] * 20, [700, 400, 1, 0, 1300, 650]],
+                         ids=["short", "between", "long"])
+def test_packed_prompts_that_fill_every_sm(kind, heads, lengths):
+    """Enough rows for two query tiles a CTA, taken where the prompts are long, or one where they are short."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    g = torch.Generator("cuda").manual_seed(31)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    out = torch.full(q.shape, math.nan, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, max(lengths))
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("heads", [(8, 1, 256), (4, 2, 128), (5, 5, 72)], ids=str)
 def test_packed_rows_outside_every_sequence_are_left_alone(kind, heads):
