@@ -71,6 +71,7 @@ struct MmaCall
     AttnCall a;
     int tile_tokens; // tokens of a query tile: 128 / group
     int ctas;        // a tree's: its key tiles are shared out to that many
+    int start;       // a tree's: what a unit's start and end cost, in key tiles
     int part_rows;   // rows of a part: a query tile's at most
     float* part_o;   // [2 ctas][part_rows][width]
     float2* part_ml; // [2 ctas][part_rows]
@@ -307,7 +308,8 @@ __device__ inline MmaPlace prompt_place(const MmaCall& c, int step, int unit)
 //  second would cost it another start (about 10 us of a 60 us call of 16 trees in
 //  fp32);
 //  many: every CTA takes `per` tiles in a row, whatever query tiles they fall on, so
-//  that sequences of any lengths keep all CTAs busy to the end.
+//  that sequences of any lengths keep all CTAs busy to the end. Each query tile is
+//  preceded by `start` tiles that nobody reads: what it costs to begin and to end.
 // A query tile that a CTA holds whole is finished there; of one that several share, each
 // leaves a part: part 2 cta + 1 where the query tile begins in a row of many, else 2 cta.
 // The host refuses calls of 2^30 tiles and more.
@@ -356,6 +358,8 @@ __device__ inline TreeCut cut_trees(const MmaCall& c, const TreeRow& known, int&
     // The sum of n / per, each rounded up, is at most total / per + query_tiles.
     const bool few = 4 * query_tiles <= c.ctas;
     const int share = few ? c.ctas - query_tiles : c.ctas;
+    if (!few)
+        total += c.start * query_tiles;
     return {few, max((total + share - 1) / share, 2)};
 }
 
@@ -377,7 +381,10 @@ struct TreePlaces
         end = cut.few ? cta + 1 : min(total, at + cut.per);
     }
     // A sequence's tiles, or pieces, in the row.
-    __device__ int share(const TreeRow& r) const { return cut.few ? r.query_tiles * cut.pieces(r.tiles) : r.total(); }
+    __device__ int share(const MmaCall& c, const TreeRow& r) const
+    {
+        return r.query_tiles * (cut.few ? cut.pieces(r.tiles) : r.tiles + c.start);
+    }
     __device__ MmaPlace next(const MmaCall& c)
     {
         const AttnCall& a = c.a;
@@ -387,7 +394,7 @@ struct TreePlaces
         for (; base < a.sequences && at < end; base += 32)
         {
             const TreeRow mine = base ? tree_row(c, base + lane) : known;
-            int sum = share(mine);
+            int sum = share(c, mine);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1)
             {
@@ -399,8 +406,8 @@ struct TreePlaces
             if (beyond)
             {
                 const int who = __ffs(beyond) - 1;
-                const int within = at - before - __shfl_sync(0xFFFFFFFFu, sum - share(mine), who);
-                const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), each = cut.few ? cut.pieces(tiles) : tiles;
+                const int within = at - before - __shfl_sync(0xFFFFFFFFu, sum - share(c, mine), who);
+                const int tiles = __shfl_sync(0xFFFFFFFFu, mine.tiles, who), each = cut.few ? cut.pieces(tiles) : tiles + c.start;
                 const int query_tile = within / each, rest = within - query_tile * each;
                 p.sequence = base + who;
                 p.begin = bounded_offset(a.offsets, p.sequence, a.rows);
@@ -420,11 +427,14 @@ struct TreePlaces
                 }
                 else
                 {
-                    p.first_tile = rest;
-                    p.tiles = min(tiles - rest, end - at);
-                    p.part = 2 * cta + (rest == 0);
-                    p.last_cta = (at + tiles - 1) / cut.per; // where rest is 0
-                    at += p.tiles;
+                    const int begin = at - rest; // the query tile's place in the row
+                    p.first_tile = max(rest - c.start, 0);
+                    p.tiles = min(each, end - begin) - c.start - p.first_tile;
+                    p.part = 2 * cta + (p.first_tile == 0);
+                    p.last_cta = (begin + each - 1) / cut.per; // where first_tile is 0
+                    at = min(begin + each, end);
+                    if (p.tiles <= 0) // the CTA ends before its first key tile
+                        p.sequence = -1;
                 }
                 p.whole = p.tiles == tiles;
                 break;

@@ -279,6 +279,13 @@ bool encode_rows(CUtensorMap* map, int dtype, const void* base, int width, int h
 // ---- attention_mma ---------------------------------------------------------------
 constexpr int kSms = 148; // a B200's; the work is cut for it wherever the call is checked
 
+// What it costs a unit of a tree's to begin and to end, in key tiles (it is counted in
+// where the tiles are shared out): 48 decode steps of 50 to 2500 tokens, 32 heads on 8
+// of 128, bf16: 74 us with 0, 61 with 2, 59 with 4, 59 with 6; 48 trees of 15 nodes over
+// 50 to 1500, fp32: 215, 186, 172, 164, of 50 to 3000, 8 heads on one of 256: 105, 89,
+// 79, 85; on plain FMAs, 64 steps of 200 to 2048: 49, 47, 49, 52.
+constexpr int kStart = 4, kFewStart = 2;
+
 // A tree's CTAs, one a place on the GPU, and the rows of a part that it leaves.
 int tree_ctas(int dtype, int width)
 {
@@ -346,6 +353,7 @@ void tree_call(MmaCall* c, int dtype, const AttnCall& a, void* workspace)
     c->a = a;
     c->tile_tokens = 128 / a.group;
     c->ctas = tree_ctas(dtype, a.width);
+    c->start = kStart;
     c->part_rows = part_rows(a.heads, a.kv_heads, a.max_nodes);
     c->part_o = (float*) workspace;
     c->part_ml = (float2*) (c->part_o + (size_t) 2 * c->ctas * c->part_rows * a.width);
@@ -468,6 +476,7 @@ int tree_limbs(const AttnCall& a, void* workspace, int device, cudaStream_t stre
     // turned into halves.
     if (c.part_rows <= kFewRows)
     {
+        c.start = kFewStart;
         const int rc = a.width > 128  ? launch_few<256>(a, c, device, stream)
                        : a.width > 64 ? launch_few<128>(a, c, device, stream)
                                       : launch_few<64>(a, c, device, stream);
@@ -506,7 +515,7 @@ int check_tree_sizes(const hf_page_cache* cache, hf_page_cache* c, const hf_atte
         return HF_E_SHAPE;
     // The kernels count key tiles in 32 bits.
     const int64_t tokens = 128 / (call->heads / call->kv_heads), row_tiles = (call->max_nodes + tokens - 1) / tokens;
-    if ((call->max_length / kKeyTile + 2) * row_tiles > (1 << 30) / ((int64_t) c->sequences * call->kv_heads))
+    if ((call->max_length / kKeyTile + 2 + kStart) * row_tiles > (1 << 30) / ((int64_t) c->sequences * call->kv_heads))
         return HF_E_SHAPE;
     return HF_OK;
 }

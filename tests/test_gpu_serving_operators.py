@@ -295,6 +295,17 @@ def test_decode_steps_of_many_sequences(kind):
     _tree(cache, 0, 8, 2, 128, [1] * 40, [[-1]] * 40, 16, 300)
 
 
+@pytest.mark.parametrize("nodes", [1, 5])
+@pytest.mark.parametrize("sequences", [38, 39, 41, 56, 67, 75, 113])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_trees_cut_at_every_place(kind, sequences, nodes):
+    """One long cache among short and empty ones: CTAs begin and end on every tile of a sequence and before its first."""
+    lengths = [(i * 61) % 131 for i in range(sequences)]
+    lengths[sequences // 3] = 4000
+    cache = Cache(kind, 1, sum((n + PAGE - 1) // PAGE for n in lengths) + 3, 4, 64, lengths, 63, 32)
+    _tree(cache, 0, 8, 4, 64, [nodes] * sequences, [_branching(nodes, 2)] * sequences, 33, 4000)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_tree_garbage_in_the_cache_is_not_read(kind):
     """Page rows past a length, free pages, and drafted rows behind the last sequence hold NaN."""
