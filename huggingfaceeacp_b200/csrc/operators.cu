@@ -4,6 +4,7 @@
 #include <hf_cuda.h>
 
 #include "attention_few.cuh"
+#include "attention_short.cuh"
 #include "attention_limbs.cuh"
 #include "attention_mma.cuh"
 #include "attention_rows.cuh"
@@ -296,6 +297,31 @@ int part_rows(int heads, int kv_heads, int max_nodes)
 {
     const int group = heads / kv_heads;
     return std::min(128 / group, max_nodes) * group;
+}
+
+// Whether a call of at most `keys` keys a row goes to attention_short, which takes
+// 3.5 us and 0.07 us a key on the GPU, and some 0.3 us for 1000 keys of all rows
+// where they fill it. Bounds where the other kernels become as fast (us on the GPU,
+// short and other; a launch less saves 1 to 3 us of the caller's on top):
+//  trees, one row of 21, 101, 251 keys: fp32 4.6 and 11.5, 10.4 and 13.3, 20 and 14;
+//  bf16 4.7 and 9, 10.8 and 10.4, 21 and 10.8. 16 rows of 31: bf16 7.0 and 10.2; a tree of
+//  8 nodes on 60: fp32 9.9 and 16.6, bf16 9.5 and 9.2; of 40: fp32 36 and 18, bf16 30 and 9;
+//  a prompt of 8, 32, 64 tokens, 8 heads of 256: fp32 4.0 and 20, 6.1 and 21, 13.4 and 21;
+//  bf16 3.8 and 7.5, 5.2 and 7.5, 9.1 and 7.4; 32 heads of 128, 32 tokens: fp32 13 and 19,
+//  bf16 10.4 and 6.3.
+bool is_short(const AttnCall& a, int dtype, bool tree, int64_t keys)
+{
+    const int64_t most = dtype == HF_DTYPE_F32 ? 32768 : tree ? 24576 : 8192; // keys of all rows
+    return keys <= 112 && (int64_t) a.rows * a.heads * keys <= most;
+}
+
+template <bool Tree>
+int attend_short(int dtype, const AttnCall& a, cudaStream_t stream)
+{
+    const dim3 grid((unsigned) (a.rows * a.heads)), block(32 * kShortWarps);
+    return status_of(dtype == HF_DTYPE_F32    ? launch(true, attention_short<float, Tree>, grid, block, 0, stream, a)
+                     : dtype == HF_DTYPE_BF16 ? launch(true, attention_short<__nv_bfloat16, Tree>, grid, block, 0, stream, a)
+                                              : launch(true, attention_short<__half, Tree>, grid, block, 0, stream, a));
 }
 
 template <typename T, int D, int NQ, bool Tree>
@@ -685,6 +711,8 @@ int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
     if (!on.holds(bytes ? call->workspace : nullptr, a.k, a.v, a.out, a.offsets))
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
+    if (is_short(a, call->dtype, false, a.rows))
+        return attend_short<false>(call->dtype, a, st);
     if (call->dtype == HF_DTYPE_F32)
         return packed_limbs(a, call->workspace, on.current, st);
     return call->dtype == HF_DTYPE_BF16 ? packed_mma<__nv_bfloat16>(call->dtype, a, on.current, st)
@@ -735,6 +763,8 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
     if (!on.holds(call->workspace, a.k, a.v, a.out, a.offsets, a.parents, a.key_pages, a.value_pages, a.table, a.lengths))
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
+    if (is_short(a, c.dtype, true, (int64_t) a.max_length + a.max_nodes))
+        return attend_short<true>(c.dtype, a, st);
     if (c.dtype == HF_DTYPE_F32)
         return tree_limbs(a, call->workspace, on.current, st);
     return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, call->workspace, on.current, st)

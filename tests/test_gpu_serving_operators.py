@@ -295,6 +295,46 @@ def test_decode_steps_of_many_sequences(kind):
     _tree(cache, 0, 8, 2, 128, [1] * 40, [[-1]] * 40, 16, 300)
 
 
+@pytest.mark.parametrize("heads", [(4, 1, 256), (6, 2, 40), (3, 3, 128)], ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths", [[1], [5, 0, 1, 9], [0, 0], [2] * 12], ids=str)
+def test_packed_calls_of_a_few_rows(kind, heads, lengths):
+    """The smallest calls; rows before and behind the prompts hold NaN and are left alone."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    before, used = 2, sum(lengths)
+    g = torch.Generator("cuda").manual_seed(34)
+    (q, k, v), stride = _fused(g, before + used + 3, h, kv, d, dtype)
+    for x in (q, k, v):
+        x[:before] = math.nan
+        x[before + used:] = math.nan
+    out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride, begin=before)
+    rows = slice(before, before + used)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5, begin=before)
+    if used:
+        ref.close(out[rows], expected[rows], size[rows], q[rows], k[rows], d ** -0.5, max(lengths))
+    assert bool((out[:before] == 7.0).all()) and bool((out[before + used:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads", [(4, 1, 256), (6, 2, 40), (3, 3, 128)], ids=str)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths,nodes", [([0], [1]), ([47], [1]), ([70, 0, 1, 64], [3, 1, 0, 7]), ([90, 65, 3] * 5, [1] * 15)],
+                         ids=str)
+def test_tree_calls_of_a_few_rows(kind, heads, lengths, nodes):
+    """The smallest calls; page rows past a length, free pages and rows behind the last sequence hold NaN."""
+    h, kv, d = heads
+    pages = sum((n + PAGE - 1) // PAGE for n in lengths) + 2
+    cache = Cache(kind, 1, pages, kv, d, lengths, 2, 35)
+    for pool in (cache.keys, cache.values):
+        held = torch.zeros(pages, PAGE, dtype=torch.bool)
+        for row, n in zip(cache.table.tolist(), lengths):
+            for j in range(n):
+                held[row[j // PAGE], j % PAGE] = True
+        pool[0][~held.cuda()] = math.nan
+    _tree(cache, 0, h, kv, d, nodes, [_branching(n, n) for n in nodes], 36, max(lengths), poison=True)
+
+
 @pytest.mark.parametrize("nodes", [1, 5])
 @pytest.mark.parametrize("sequences", [38, 39, 41, 56, 67, 75, 113])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
