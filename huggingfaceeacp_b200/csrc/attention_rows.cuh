@@ -149,9 +149,9 @@ __device__ __forceinline__ RowKeys row_keys(const AttnCall& a, int s, int begin,
 }
 
 // m, l and the lane's 8 channels of the unnormalised row over keys [from, to)
-// of the row's list, Batch keys' loads in flight. All 32 lanes call it.
-template <typename T, bool Tree, int Batch = 1>
-__device__ __forceinline__ void attend_row(const AttnCall& a, const RowKeys& keys, int kv_head, const float (&q)[8], int from, int to,
+// of the row's list. All 32 lanes call it.
+template <typename T, bool Tree>
+__device__ void attend_row(const AttnCall& a, const RowKeys& keys, int kv_head, const float (&q)[8], int from, int to,
                            float& m, float& l, float (&acc)[8])
 {
     const int lane = threadIdx.x & 31, c = lane * 8;
@@ -191,31 +191,22 @@ __device__ __forceinline__ void attend_row(const AttnCall& a, const RowKeys& key
         if (!seen)
             continue;
         float score = -INFINITY;
-        for (unsigned left = seen; left;)
+        for (unsigned left = seen; left; left &= left - 1)
         {
-            int who[Batch]; // -1: no key left
-            float x[Batch][8];
-#pragma unroll
-            for (int n = 0; n < Batch; ++n)
+            const int i = __ffs(left) - 1;
+            const T* p = (const T*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) kp, i);
+            float dot = 0.f;
+            if (channels)
             {
-                who[n] = __ffs(left) - 1;
-                left &= left - 1;
-                const T* p = (const T*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) kp, max(who[n], 0));
-                if (channels && who[n] >= 0)
-                    load8(p + c, x[n]);
-            }
+                float x[8];
+                load8(p + c, x);
 #pragma unroll
-            for (int n = 0; n < Batch; ++n)
-            {
-                float dot = 0.f;
-                if (channels && who[n] >= 0)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        dot = fmaf(q[e], x[n][e], dot);
-                dot = warp_sum(dot);
-                if (lane == who[n])
-                    score = dot * a.scale_log2;
+                for (int e = 0; e < 8; ++e)
+                    dot = fmaf(q[e], x[e], dot);
             }
+            dot = warp_sum(dot);
+            if (lane == i)
+                score = dot * a.scale_log2;
         }
         // A NaN score must reach the row: fmaxf drops it, the sums keep it.
         const float m_new = fmaxf(m, warp_max(score));
@@ -223,27 +214,18 @@ __device__ __forceinline__ void attend_row(const AttnCall& a, const RowKeys& key
         const float weight = kp ? (score == -INFINITY ? 0.f : exp2f(score - m_new)) : 0.f;
         l = l * alpha + warp_sum(weight);
         float part[8] = {};
-        for (unsigned left = seen; left;)
+        for (unsigned left = seen; left; left &= left - 1)
         {
-            int who[Batch];
-            float x[Batch][8];
-#pragma unroll
-            for (int n = 0; n < Batch; ++n)
+            const int i = __ffs(left) - 1;
+            const T* p = (const T*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) vp, i);
+            const float w = __shfl_sync(0xFFFFFFFFu, weight, i);
+            if (channels)
             {
-                who[n] = __ffs(left) - 1;
-                left &= left - 1;
-                const T* p = (const T*) __shfl_sync(0xFFFFFFFFu, (unsigned long long) vp, max(who[n], 0));
-                if (channels && who[n] >= 0)
-                    load8(p + c, x[n]);
-            }
+                float x[8];
+                load8(p + c, x);
 #pragma unroll
-            for (int n = 0; n < Batch; ++n)
-            {
-                const float w = __shfl_sync(0xFFFFFFFFu, weight, max(who[n], 0));
-                if (channels && who[n] >= 0)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        part[e] = fmaf(w, x[n][e], part[e]);
+                for (int e = 0; e < 8; ++e)
+                    part[e] = fmaf(w, x[e], part[e]);
             }
         }
 #pragma unroll

@@ -316,7 +316,7 @@ bool is_short(const AttnCall& a, int dtype, bool tree, int64_t keys)
 }
 
 template <bool Tree>
-int attend_short(int dtype, const AttnCall& a, cudaStream_t stream)
+int short_call(int dtype, const AttnCall& a, cudaStream_t stream)
 {
     const dim3 grid((unsigned) (a.rows * a.heads)), block(32 * kShortWarps);
     return status_of(dtype == HF_DTYPE_F32    ? launch(true, attention_short<float, Tree>, grid, block, 0, stream, a)
@@ -712,7 +712,7 @@ int hf_cuda_attention_packed(const hf_attention_packed* call, void* stream)
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
     if (is_short(a, call->dtype, false, a.rows))
-        return attend_short<false>(call->dtype, a, st);
+        return short_call<false>(call->dtype, a, st);
     if (call->dtype == HF_DTYPE_F32)
         return packed_limbs(a, call->workspace, on.current, st);
     return call->dtype == HF_DTYPE_BF16 ? packed_mma<__nv_bfloat16>(call->dtype, a, on.current, st)
@@ -764,7 +764,7 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
         return HF_E_INVALID;
     cudaStream_t st = (cudaStream_t) stream;
     if (is_short(a, c.dtype, true, (int64_t) a.max_length + a.max_nodes))
-        return attend_short<true>(c.dtype, a, st);
+        return short_call<true>(c.dtype, a, st);
     if (c.dtype == HF_DTYPE_F32)
         return tree_limbs(a, call->workspace, on.current, st);
     return c.dtype == HF_DTYPE_BF16 ? tree_mma<__nv_bfloat16>(c.dtype, a, call->workspace, on.current, st)
