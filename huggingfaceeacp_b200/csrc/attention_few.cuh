@@ -5,7 +5,7 @@
 // A cached position is read once and meets 8 rows, 4 operations for each 4 bytes and
 // row: about 3,200 issue slots a scheduler and 64-key tile at width 256 against the
 // 5,400 cycles that the tile takes to arrive at 44 GB/s an SM. Measured (B200), 64
-// sequences of 200 to 2,048 tokens, the engine's heads: 50 us a call for 122 MB, a tile
+// sequences of 200 to 2,048 tokens, the engine's heads: 47 us a call for 122 MB, a tile
 // in 6,300 cycles, the rest its start, the warps' meeting and the join.
 // (attention_limbs, whose converters take 8,000 cycles a tile: 91 us.)
 //
