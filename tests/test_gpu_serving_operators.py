@@ -433,6 +433,49 @@ def test_tree_pages_that_are_not_there_and_bounds(kind):
     assert bool((out[5:] == 7.0).all())
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("bound", [60, 109, 110, 150])
+def test_tree_bounds_in_short_and_long_calls(kind, bound):
+    """The call's bounds and missing pages on both sides of 112 keys, where the kernels change."""
+    cache = Cache(kind, 1, 6, 1, 64, [200, 180], 4, 37, table=[[2, -1, 5, 77777], [-5, 0, 1, -1]])
+    g = torch.Generator("cuda").manual_seed(38)
+    (q, k, v), stride = _fused(g, 7, 4, 1, 64, cache.dtype)
+    out = torch.full(q.shape, 7.0, dtype=cache.dtype, device="cuda")
+    plan, offsets, up = native.TreeAttention(cache.code, 4, 1, 64), _ints([0, 2, 7]), _ints([-1, 0, -1, 0, 1, 2, 3])
+    room = _room(plan.workspace_bytes(2, 7, 3, bound))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(), 7, 3,
+             bound, q_stride=stride, k_stride=stride, v_stride=stride, workspace=room.data_ptr(),
+             workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q[:5], k[:5], v[:5], [2, 3], [[-1, 0], [-1, 0, 1]], cache.keys[0].view(cache.shape),
+                              cache.values[0].view(cache.shape), cache.table.tolist(), [bound, bound], 64 ** -0.5)
+    everything = torch.cat([k[:5], cache.keys[0].view(-1, 1, 64)])
+    ref.close(out[:5], expected, size, q[:5], everything, 64 ** -0.5, bound + 3)
+    assert bool((out[5:] == 7.0).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("length", [10, 128, 300])
+def test_tree_siblings_in_short_and_long_calls(kind, length):
+    """A sibling's value of NaN or infinity stays with its own descendants, over caches of either kernel."""
+    code, dtype = ref.TYPES[kind]
+    parents, h, kv, d = [-1, 0, 0, 1, 2, 2], 4, 1, 128
+    cache = Cache(kind, 1, 6, kv, d, [length], 5, 39)
+    g = torch.Generator("cuda").manual_seed(40)
+    q, k, v = (_normal(g, 6, n, d, dtype=dtype) for n in (h, kv, kv))
+    v[1], v[2] = math.inf, math.nan
+    out = torch.empty_like(q)
+    plan = native.TreeAttention(code, h, kv, d)
+    offsets, up = _ints([0, 6]), _ints(parents)
+    room = _room(plan.workspace_bytes(1, 6, 6, length))
+    plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(), 6, 6,
+             length, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q, k, v, [6], [parents], cache.keys[0].view(cache.shape), cache.values[0].view(cache.shape),
+                              cache.table.tolist(), [length], d ** -0.5)
+    everything = torch.cat([k, cache.keys[0].view(-1, kv, d)])
+    ref.close(out[:1], expected[:1], size[:1], q, everything, d ** -0.5, length + 6)
+    assert bool((out[[1, 3]] == math.inf).all()) and bool(torch.isnan(out[[2, 4, 5]]).all())
+
+
 # ---- the cache's steps ---------------------------------------------------------------------------------------------
 
 
