@@ -36,8 +36,8 @@
 // Value rows past a sequence's last key are set to zero in shared memory before
 // the MMA (their weights are 0, but 0 x NaN is not). Inside a sequence a
 // masked value that is not finite makes the tile's sums NaN for rows that do not
-// attend to it: every row that comes out not finite is taken again by
-// attention_row, which reads only what the row attends to.
+// attend to it: every row that comes out not finite, or has a score of NaN or
+// infinity, is taken again by attention_row, which reads only what the row attends to.
 //
 // A batch of trees is shared out evenly in key tiles, so a query tile's keys may
 // lie with several CTAs: each leaves its rows' maximum, sum and unnormalised O in
@@ -83,7 +83,8 @@ constexpr int kFew = 1 << 30;
 // addition of 1.5 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by the
 // polynomial of least largest relative error (Remez exchange; 7.5e-5 at degree
 // 3, 2.6e-6 at degree 4), n added to the exponent. Below 2^-126 it returns about
-// that, where exp2_approx gives 0.
+// that, where exp2_approx gives 0, and for NaN too: its callers look for NaN in the
+// scores' maximum.
 template <int Degree>
 __device__ __forceinline__ float2 exp2_poly(float2 x)
 {
@@ -953,9 +954,13 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 for (int e = 4; e < 60; e += 8)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
-                        top[g] = max3(top[g], s[e + 2 * g], s[e + 2 * g + 1]);
-                const float m_tile =
-                    max3(max3(top[0], s[60], s[61]), max3(top[1], s[62], s[63]), fmaxf(top[2], top[3])) * scale;
+                        top[g] = max3_nan(top[g], s[e + 2 * g], s[e + 2 * g + 1]);
+                const float m_tile = max3_nan(max3_nan(top[0], s[60], s[61]), max3_nan(top[1], s[62], s[63]),
+                                              max_nan(top[2], top[3]))
+                                     * scale;
+                // A score of NaN or infinity, of which exp2_poly would make a number: the row is taken again.
+                if (!(m_tile < INFINITY))
+                    l = NAN;
                 if (j == 0)
                     m = m_tile;
                 else

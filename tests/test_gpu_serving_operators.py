@@ -839,3 +839,65 @@ def test_host_memory_is_refused():
         with pytest.raises(native.HFError) as e:
             plan.run(*(x.data_ptr() for x in args), offsets.data_ptr(), 1, 64, stream=_stream())
         assert e.value.code == native.HF_E_INVALID
+
+
+# ---- keys that are not finite --------------------------------------------------------------------------------------
+
+
+def _run_tree(cache, q, k, v, nodes, parents, max_length, layer=0):
+    """The operator's rows and the formula's (with the rows' sizes)."""
+    h, d = q.shape[1:]
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    plan = native.TreeAttention(cache.code, h, k.shape[1], d)
+    offsets, up = _ints(_offsets(nodes)), _ints([p for row in parents for p in row])
+    room = _room(plan.workspace_bytes(len(nodes), len(q), max(nodes), max_length))
+    plan.run(cache.native, layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(),
+             len(q), max(nodes), max_length, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q, k, v, nodes, parents, cache.keys[layer].view(cache.shape), cache.values[layer].view(cache.shape),
+                              cache.table.tolist(), cache.lengths.tolist(), d ** -0.5)
+    return out, expected, size
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 1, 256), (4, 2, 64)], ids=str)
+def test_a_key_alone_that_is_not_finite_in_a_prompt(kind, value, heads):
+    """At every place of 16 in a tile, its value finite: what the rows in its own tile and in later ones come to is the
+    formula's (a score of infinity or NaN makes the row NaN, one of minus infinity weighs nothing)."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    lengths = [200, 30]
+    for place in range(16):
+        g = torch.Generator("cuda").manual_seed(90 + place)
+        (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+        k[64 + place + 16 * (place % 4), 0, 5] = value
+        out = torch.full(q.shape, math.inf, dtype=dtype, device="cuda")
+        _run_packed(code, q, k, v, out, lengths, stride)
+        expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+        assert bool(torch.isnan(expected).any()) and bool(torch.isfinite(expected[:64]).all())
+        ref.close(out, expected, size, q, k, d ** -0.5, max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads,nodes", [((8, 2, 128), 1), ((8, 1, 256), 5), ((4, 2, 64), 20)], ids=str)
+def test_a_key_alone_that_is_not_finite_in_the_cache(kind, value, heads, nodes):
+    """The same in a full cached page, for decode steps and trees whose keys lie with one CTA and with several."""
+    h, kv, d = heads
+    lengths = [300, 70, 4000]
+    parents = [_branching(nodes, s) for s in range(3)]
+    cache = Cache(kind, 1, 75, kv, d, lengths, 63, 91)
+    g = torch.Generator("cuda").manual_seed(92)
+    for place in range(16):
+        q, k, v = (_normal(g, 3 * nodes, n, d, dtype=cache.dtype) for n in (h, kv, kv))
+        at = []
+        for s, j in ((0, 64 + place), (1, place + 48), (2, 640 + place)):
+            page = cache.table.tolist()[s][j // PAGE]
+            at.append((page, j % PAGE, cache.keys[0, page, j % PAGE, 3].item()))
+            cache.keys[0, page, j % PAGE, 3] = value
+        out, expected, size = _run_tree(cache, q, k, v, [nodes] * 3, parents, 4000)
+        assert bool(torch.isnan(expected).any()) and (kv == 1 or bool(torch.isfinite(expected[:, h // kv:]).all()))
+        everything = torch.cat([k, cache.keys[0].view(-1, kv, d)])
+        ref.close(out, expected, size, q, everything, d ** -0.5, 4064)
+        for page, j, was in at:
+            cache.keys[0, page, j, 3] = was
