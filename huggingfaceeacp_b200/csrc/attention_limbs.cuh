@@ -805,7 +805,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
             const size_t part = (size_t) p.part * c.part_rows + row;
             // The weights' 2^14: cancels in a finished row, is taken off a part's.
             const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 0x1p-14f;
-            float2 check = make_float2(l * 0.f, Tree && *(volatile int*) &h.misfit[i & 1] ? NAN : 0.f); // 0 for finite values
+            // 0 for finite values. A maximum of minus infinity may be of masked keys or of such scores.
+            float2 check = make_float2(l * 0.f, m == -INFINITY || (Tree && *(volatile int*) &h.misfit[i & 1]) ? NAN : 0.f);
             char* mine = (char*) (whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width
                                         : c.part_o + part * a.width);
             // Through the queries' room (their last MMA is over): a row a thread in,

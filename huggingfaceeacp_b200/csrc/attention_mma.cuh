@@ -1008,7 +1008,9 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                 const bool whole = !Tree || p.whole;
                 // Nothing attended: 0 (O is 0, or NaN and the row taken again).
                 const float scaled = !ok ? NAN : l == 0.f ? 0.f : whole ? 1.f / l : 1.f;
-                float2 check = make_float2(l * 0.f, 0.f); // stays 0 for finite values
+                // Stays 0 for finite values. A maximum of minus infinity may be of masked keys or
+                // of such scores.
+                float2 check = make_float2(l * 0.f, m == -INFINITY ? NAN : 0.f);
                 char* mine = whole ? (char*) ((T*) a.out + at * a.out_stride + (size_t) head * a.width)
                                    : (char*) (c.part_o + part * a.width);
                 const unsigned rows = __ballot_sync(0xFFFFFFFFu, real);
@@ -1134,7 +1136,7 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
             }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = finish_factor(m, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         acc[e] = l == 0.f ? 0.f : acc[e] * inv;

@@ -10,7 +10,7 @@
 // m_new)), and each block's weighted values are summed apart and then added to
 // the row, so that no fp32 chain is longer than 32 + keys / 32. A key that the
 // row does not attend to is not read, whatever it holds. A row that attends to
-// nothing is 0.
+// nothing is 0; one whose every score is minus infinity is NaN, as by the formula.
 #pragma once
 
 #include "common.cuh"
@@ -148,6 +148,21 @@ __device__ __forceinline__ RowKeys row_keys(const AttnCall& a, int s, int begin,
     return k;
 }
 
+// The weight of a score against the largest so far. Where that is minus infinity every
+// score is (or NaN): each weighs 1, so that the sum tells such keys from none at all,
+// and drops out as soon as a larger one comes (the sums are scaled by 2^-inf).
+__device__ __forceinline__ float weight_of(float score, float m)
+{
+    return score == -INFINITY && m == -INFINITY ? 1.f : exp2f(score - m);
+}
+
+// What a finished row's sums are multiplied with: 0 of a row that attends to nothing,
+// NaN where every score is minus infinity and the formula has no weights.
+__device__ __forceinline__ float finish_factor(float m, float l)
+{
+    return l == 0.f ? 0.f : m == -INFINITY ? NAN : 1.f / l;
+}
+
 // m, l and the lane's 8 channels of the unnormalised row over keys [from, to)
 // of the row's list. All 32 lanes call it.
 template <typename T, bool Tree>
@@ -211,7 +226,7 @@ __device__ void attend_row(const AttnCall& a, const RowKeys& keys, int kv_head, 
         // A NaN score must reach the row: fmaxf drops it, the sums keep it.
         const float m_new = fmaxf(m, warp_max(score));
         const float alpha = m == m_new ? 1.f : exp2f(m - m_new);
-        const float weight = kp ? (score == -INFINITY ? 0.f : exp2f(score - m_new)) : 0.f;
+        const float weight = kp ? weight_of(score, m_new) : 0.f;
         l = l * alpha + warp_sum(weight);
         float part[8] = {};
         for (unsigned left = seen; left; left &= left - 1)
@@ -245,7 +260,7 @@ __device__ void attention_row(const AttnCall& a, int s, int begin, int row, int 
         load8((const T*) a.q + row * a.q_stride + (size_t) h * a.width + c, q);
     const RowKeys keys = row_keys<Tree>(a, s, begin, row);
     attend_row<T, Tree>(a, keys, h / a.group, q, 0, keys.cached + keys.drafted, m, l, acc);
-    const float inv = l == 0.f ? 0.f : 1.f / l; // nothing attended: the row is 0
+    const float inv = finish_factor(m, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         acc[e] = l == 0.f ? 0.f : acc[e] * inv;

@@ -86,7 +86,7 @@ __device__ __forceinline__ void attend_short(const AttnCall& a, const RowKeys& k
         // A NaN score must reach the row: fmaxf drops it, the sums keep it.
         const float m_new = fmaxf(m, warp_max(score));
         const float alpha = m == m_new ? 1.f : exp2f(m - m_new);
-        const float weight = kp ? (score == -INFINITY ? 0.f : exp2f(score - m_new)) : 0.f;
+        const float weight = kp ? weight_of(score, m_new) : 0.f;
         l = l * alpha + warp_sum(weight);
         float part[8] = {};
         for (unsigned left = seen; left;)
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 4) attention_short(const __g
         for (int e = 0; e < 8; ++e)
             acc[e] = fmaf(weight, x[e], acc[e]);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = finish_factor(m, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         acc[e] = l == 0.f ? 0.f : acc[e] * inv;

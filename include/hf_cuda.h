@@ -413,8 +413,10 @@ int hf_cuda_operators_sync(int device, void* stream);
  * elements apart (0 = packed; views of one fused q|k|v row are fine). Rows
  * outside every sequence are neither read nor written. head_width is a multiple
  * of 8 up to 256, heads / kv_heads at most 128. `scale` (> 0) multiplies the scores.
- * A value or key row that holds infinities or NaN reaches only the rows that
- * attend to it. `out` may not overlap q, k or v. */
+ * A value or key row that holds infinities or NaN reaches the rows that attend
+ * to it, by the formula (a score of infinity or NaN makes the row NaN, one of
+ * minus infinity weighs nothing, and of no other scores the row is NaN), and no
+ * others. `out` may not overlap q, k or v. */
 typedef struct hf_attention_packed
 {
     int32_t dtype;

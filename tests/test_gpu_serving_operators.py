@@ -901,3 +901,45 @@ def test_a_key_alone_that_is_not_finite_in_the_cache(kind, value, heads, nodes):
         ref.close(out, expected, size, q, everything, d ** -0.5, 4064)
         for page, j, was in at:
             cache.keys[0, page, j, 3] = was
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths", [[200, 1], [40, 1, 2], [700]], ids=str)
+def test_prompt_rows_whose_every_score_is_minus_infinity(kind, lengths):
+    """The formula has no weights for them: NaN, not the 0 of a row that attends to nothing. Later rows are finite."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = 4, 2, 64
+    g = torch.Generator("cuda").manual_seed(93)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    q[:, :, 5] = q[:, :, 5].abs() + 0.25
+    for begin in _offsets(lengths)[:-1]:
+        k[begin:begin + 3, 0, 5] = -math.inf
+    out = torch.zeros(q.shape, dtype=dtype, device="cuda")
+    _run_packed(code, q, k, v, out, lengths, stride)
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    assert bool(torch.isnan(expected[0, :2]).all()) and bool(torch.isfinite(expected[3:lengths[0]]).all())
+    ref.close(out, expected, size, q, k, d ** -0.5, max(lengths))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("length", [20, 60, 300, 4000])
+@pytest.mark.parametrize("nodes", [1, 7])
+@pytest.mark.parametrize("lowest", [0.5, 1.0])
+def test_tree_rows_whose_scores_are_minus_infinity(kind, length, nodes, lowest):
+    """Half of the cache, or all of it and the nodes: the parts of a row in which every score is minus infinity weigh
+    nothing beside others, and of nothing else the row is NaN."""
+    h, kv, d = 4, 2, 64
+    cache = Cache(kind, 1, 70, kv, d, [length, 33], 63, 94)
+    g = torch.Generator("cuda").manual_seed(95)
+    parents = [_branching(nodes, 3), _branching(nodes, 4)]
+    q, k, v = (_normal(g, 2 * nodes, n, d, dtype=cache.dtype) for n in (h, kv, kv))
+    q[:, :, 5] = q[:, :, 5].abs() + 0.25
+    row = cache.table.tolist()[0]
+    for j in range(int(length * lowest)):
+        cache.keys[0, row[j // PAGE], j % PAGE, 5] = -math.inf
+    if lowest == 1:
+        k[:nodes, 0, 5] = -math.inf
+    out, expected, size = _run_tree(cache, q, k, v, [nodes] * 2, parents, max(length, 33))
+    assert bool(torch.isnan(expected[:nodes, :2]).all()) == (lowest == 1) and bool(torch.isfinite(expected[:, 2:]).all())
+    everything = torch.cat([k, cache.keys[0].view(-1, kv, d)])
+    ref.close(out, expected, size, q, everything, d ** -0.5, length + 64)
