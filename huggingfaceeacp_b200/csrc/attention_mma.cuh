@@ -56,6 +56,7 @@
 #pragma once
 
 #include "attention_rows.cuh"
+#include "key_span.cuh"
 #include "tcgen05.cuh"
 
 namespace hfk
@@ -77,7 +78,6 @@ struct MmaCall
     float2* part_ml; // [2 ctas][part_rows]
     int2* spans;     // [rows][kv_heads]: the first and the last CTA that hold a row's keys (few: first | kFew)
 };
-constexpr int kFew = 1 << 30;
 
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (the
 // addition of 1.5 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by the
@@ -1096,9 +1096,19 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
         return;
     }
     pdl_wait();
-    const int2 span = c.spans[(size_t) row * a.kv_heads + head / a.group];
-    const bool few = span.x & kFew;
-    const int from = span.x & ~kFew, to = span.y;
+    const int2 words = c.spans[(size_t) row * a.kv_heads + head / a.group];
+    const KeySpan span = key_span(words.x, words.y, c.ctas);
+    // A wait has run out (here or, until hf_cuda_operators_sync has told it, in an earlier
+    // call): rows, parts and spans may be missing, so every row is NaN.
+    if (__ldcg(&g_operator_error) || !span.there)
+    {
+        const float none[8] = {NAN, NAN, NAN, NAN, NAN, NAN, NAN, NAN};
+        if (at < a.width)
+            store8((T*) a.out + row * a.out_stride + (size_t) head * a.width + at, none);
+        return;
+    }
+    const bool few = span.few;
+    const int from = span.first, to = span.last;
     if (from == to)
         return;
     const int within = node % c.tile_tokens * a.group + head % a.group;

@@ -399,8 +399,9 @@ int hf_cuda_quantize_q8(const float* values, int64_t first, int64_t count, int64
  * bounded by the kernels: offsets are taken as ascending within [0, rows],
  * lengths within the bounds given, and a page id outside the pool is a page
  * that is not there (its positions are not attended, read or written). Waits
- * inside the kernels are bounded: one that ran out leaves NaN rows and is
- * reported by hf_cuda_operators_sync. */
+ * inside the kernels are bounded: a call in which one ran out leaves rows that
+ * are NaN or, of packed prompts, not written, hf_cuda_operators_sync reports it,
+ * and until then the rows of tree calls on that device are NaN. */
 enum { HF_DTYPE_F32 = 0, HF_DTYPE_BF16 = 1, HF_DTYPE_F16 = 2 };
 /* Waits for `stream`; HF_E_DEVICE when a wait of an operator's kernel has run out on
  * `device` since the last call (and clears it). */
