@@ -57,6 +57,7 @@
 
 #include "attention_rows.cuh"
 #include "key_span.cuh"
+#include "phases.cuh"
 #include "tcgen05.cuh"
 
 namespace hfk
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
 
     if (warp == 0)
     {
-        int put_keys = 0, put_values = 0;
+        int put_keys = 0, put_values = 0, put_queries = 0;
         bool ok = true;
         auto one_wait = [&](uint64_t* bar, unsigned parity) {
             if (ok && !thread_wait(bar, parity))
@@ -715,6 +716,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
                         for (int b = 0; b < NQ * kBlocks; ++b)
                             tensor_load(queries + b * 128 * 128, &qmap, 64 * (b % kBlocks), p.kv_head * a.group,
                                         p.begin + p.token0 + b / kBlocks * c.tile_tokens, &h.query);
+                        ++put_queries;
                     }
                     if (j > 0)
                         load(j - 1, &vmap, &vpages, id_before, values, put_values, VS, h.values_full, h.values_free);
@@ -728,7 +730,8 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         // Every copy has landed before the CTA may end (only a failed run gets here early).
         if (lane == 0 && *(volatile int*) &h.dead)
         {
-            mbar_wait(&h.query, 0);
+            if (put_queries)
+                mbar_wait(&h.query, last_parity(put_queries));
             for (int n = max(0, put_keys - KS); n < put_keys; ++n)
                 mbar_wait(&h.keys_full[n % KS], (n / KS) & 1);
             for (int n = max(0, put_values - VS); n < put_values; ++n)

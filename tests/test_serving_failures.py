@@ -1,5 +1,5 @@
-"""What the serving operators' second kernel does with what a call leaves whose wait ran out: the spans that it reads are
-bounded (here, without a GPU) and its rows are NaN (with one)."""
+"""What the serving operators do once a wait has run out: copies in flight are waited for, the spans that the second kernel
+reads are bounded (without a GPU), and its rows are NaN (with one)."""
 import os
 import subprocess
 
@@ -37,12 +37,43 @@ int main()
 
 
 def test_spans_that_no_cta_left_are_not_followed(tmp_path):
-    source, program = str(tmp_path / "spans.cpp"), str(tmp_path / "spans")
-    with open(source, "w") as f:
-        f.write(SPANS)
-    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{CSRC}", source, "-o", program], check=True)
-    result = subprocess.run([program], capture_output=True, text=True)
+    result = _host_program(tmp_path, SPANS)
     assert result.returncode == 0, result.stdout
+
+
+PHASES = """
+#include "phases.cuh"
+#include <cstdio>
+using namespace hfk;
+int main()
+{
+    int wrong = 0;
+    for (int begun = 1; begun < 9; ++begun)
+        for (int over = begun - 1; over <= begun; ++over) // the last use in flight, then over
+        {
+            const bool returns = (unsigned) (over & 1) != last_parity(begun); // the current phase has the other parity
+            wrong += returns != (over == begun);
+        }
+    std::printf("%d\\n", wrong);
+    return wrong != 0;
+}
+"""
+
+
+def _host_program(tmp_path, text):
+    source, program = str(tmp_path / "program.cpp"), str(tmp_path / "program")
+    with open(source, "w") as f:
+        f.write(text)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{CSRC}", source, "-o", program], check=True)
+    return subprocess.run([program], capture_output=True, text=True)
+
+
+def test_a_failed_call_waits_for_the_last_copy_of_queries(tmp_path):
+    """A CTA may not end while a copy into its shared memory is in flight: the wait names that copy's phase."""
+    result = _host_program(tmp_path, PHASES)
+    assert result.returncode == 0, result.stdout
+    with open(os.path.join(CSRC, "attention_mma.cuh")) as f:
+        assert "mbar_wait(&h.query, last_parity(put_queries))" in f.read()
 
 
 @pytest.mark.gpu
