@@ -1091,28 +1091,21 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
     const AttnCall& a = c.a;
     const long long unit = (long long) blockIdx.x * 8 + (threadIdx.x >> 5);
     const int row = (int) (unit / a.heads), head = (int) (unit % a.heads), at = (threadIdx.x & 31) * 8;
-    const int s = row < a.rows ? sequence_of(a.offsets, a.sequences, a.rows, row) : -1;
-    const int node = s < 0 ? 0 : row - bounded_offset(a.offsets, s, a.rows);
-    if (s < 0 || node >= a.max_nodes)
-    {
-        pdl_wait();
-        return;
-    }
+    // The offsets too are behind the wait: the kernel ahead has waited for who wrote them, but nothing says
+    // that its trigger hands that on. (The search ahead of the wait: 0.3 us of 14 less.)
     pdl_wait();
-    const int2 words = c.spans[(size_t) row * a.kv_heads + head / a.group];
-    const KeySpan span = key_span(words.x, words.y, c.ctas);
-    // A wait has run out (here or, until hf_cuda_operators_sync has told it, in an earlier
-    // call): rows, parts and spans may be missing, so every row is NaN.
-    if (__ldcg(&g_operator_error) || !span.there)
-    {
-        const float none[8] = {NAN, NAN, NAN, NAN, NAN, NAN, NAN, NAN};
-        if (at < a.width)
-            store8((T*) a.out + row * a.out_stride + (size_t) head * a.width + at, none);
+    if (row >= a.rows)
         return;
-    }
+    const int2 words = c.spans[(size_t) row * a.kv_heads + head / a.group]; // on its way beside the search
+    const unsigned failed = __ldcg(&g_operator_error);
+    int begin;
+    const int s = sequence_of_row(a, row, begin), node = row - begin;
+    if (s < 0 || node >= a.max_nodes)
+        return;
+    const KeySpan span = key_span(words.x, words.y, c.ctas);
     const bool few = span.few;
     const int from = span.first, to = span.last;
-    if (from == to)
+    if (from == to && !failed)
         return;
     const int within = node % c.tile_tokens * a.group + head % a.group;
     auto part_of = [&](int cta) { return (size_t) (2 * cta + (!few && cta == from)) * c.part_rows + within; };
@@ -1149,10 +1142,12 @@ __global__ void __launch_bounds__(256) attention_join(const __grid_constant__ Mm
             }
         }
     }
-    const float inv = finish_factor(m, l);
+    // A wait has run out (here or, until hf_cuda_operators_sync has told it, in an earlier
+    // call): rows, parts and spans may be missing, so every row is NaN.
+    const float inv = failed || !span.there ? NAN : finish_factor(m, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        acc[e] = l == 0.f ? 0.f : acc[e] * inv;
+        acc[e] *= inv; // 0 where nothing was attended
     if (at < a.width)
         store8((T*) a.out + row * a.out_stride + (size_t) head * a.width + at, acc);
 }

@@ -130,6 +130,25 @@ __device__ __forceinline__ unsigned long long tree_path(const Int* parents, int 
     return path;
 }
 
+// The sequence whose rows hold `row` and its first row, -1 for none: the last one that
+// begins there or before, by a whole warp, 32 ways at a time.
+__device__ __forceinline__ int sequence_of_row(const AttnCall& a, int row, int& begin)
+{
+    const int lane = threadIdx.x & 31;
+    int s = -1, high = a.sequences;
+    while (high - s > 1)
+    {
+        const int stride = (high - s + 31) / 32, probe = s + (lane + 1) * stride;
+        const int below = __popc(__ballot_sync(0xFFFFFFFFu, probe < high && bounded_offset(a.offsets, probe, a.rows) <= row));
+        s += below * stride;
+        high = min(high, s + stride);
+    }
+    if (s < 0)
+        return -1;
+    begin = bounded_offset(a.offsets, s, a.rows);
+    return row < bounded_offset(a.offsets, s + 1, a.rows) ? s : -1;
+}
+
 template <bool Tree>
 __device__ __forceinline__ RowKeys row_keys(const AttnCall& a, int s, int begin, int row)
 {

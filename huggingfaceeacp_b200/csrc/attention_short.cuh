@@ -131,20 +131,10 @@ __global__ void __launch_bounds__(32 * kShortWarps, 4) attention_short(const __g
     pdl_trigger();
     if (at < a.width)
         load8((const T*) a.q + row * a.q_stride + (size_t) head * a.width + at, q);
-    // The row's sequence: the last one that begins at the row or before it, 32 ways at a time.
-    int s = -1, high = a.sequences;
-    while (high - s > 1)
-    {
-        const int stride = (high - s + 31) / 32, probe = s + (lane + 1) * stride;
-        const int below = __popc(__ballot_sync(0xFFFFFFFFu, probe < high && bounded_offset(a.offsets, probe, a.rows) <= row));
-        s += below * stride;
-        high = min(high, s + stride);
-    }
-    if (s < 0 || row >= bounded_offset(a.offsets, s + 1, a.rows))
+    int begin;
+    const int s = sequence_of_row(a, row, begin);
+    if (s < 0 || (Tree && row - begin >= a.max_nodes))
         return; // the CTA together
-    const int begin = bounded_offset(a.offsets, s, a.rows);
-    if (Tree && row - begin >= a.max_nodes)
-        return;
     const RowKeys keys = row_keys<Tree>(a, s, begin, row);
     const int count = keys.cached + keys.drafted, share = (count + kShortWarps - 1) / kShortWarps;
     attend_short<T, Tree>(a, keys, head / a.group, q, min(warp * share, count), min((warp + 1) * share, count), m, l, acc);

@@ -20,10 +20,12 @@ struct KeySpan
 };
 
 // A call in which a wait ran out leaves spans unwritten: what the workspace holds
-// there may be anything, and is not followed.
+// there may be anything, and becomes a span of no CTA.
 HFK_BOTH inline KeySpan key_span(int x, int y, int ctas)
 {
     const int first = x & ~kFew;
-    return {first, y, (x & kFew) != 0, first >= 0 && first <= y && y < ctas};
+    if (first < 0 || first > y || y >= ctas)
+        return {0, -1, false, false};
+    return {first, y, (x & kFew) != 0, true};
 }
 } // namespace hfk

@@ -29,6 +29,7 @@ int main()
                     fits = fits || ((x == first || x == (kFew | first)) && y >= first && y < ctas);
                 wrong += s.there != fits;
                 wrong += s.there && (s.first < 0 || s.last >= ctas || s.first > s.last || s.few != (x >= kFew));
+                wrong += !s.there && s.first <= s.last;
             }
     std::printf("%d\\n", wrong);
     return wrong != 0;
