@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
                 m_new = fmaxf(m_new, __shfl_xor_sync(0xFFFFFFFFu, m_new, 8));
                 m_new = fmaxf(m_new, __shfl_xor_sync(0xFFFFFFFFu, m_new, 16));
                 const float alpha = m == m_new ? 1.f : exp2_approx(m - m_new);
-                const float weight = !seen ? 0.f : score == -INFINITY && m_new == -INFINITY ? 1.f : exp2_approx(score - m_new);
+                const float weight = seen && score != -INFINITY ? exp2_approx(score - m_new) : 0.f;
                 l = l * alpha + weight;
                 m = m_new;
                 if (__any_sync(0xFFFFFFFFu, alpha != 1.f))
@@ -344,9 +344,10 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
             }
             const int at = p.begin + p.token0 + warp / a.group, head = p.kv_head * a.group + warp % a.group;
             const size_t part = (size_t) p.part * c.part_rows + warp;
-            const float scaled = !ok ? NAN : p.whole ? finish_factor(top, sum) : sum == 0.f ? 0.f : 1.f;
+            const float scaled = !ok ? NAN : sum == 0.f ? 0.f : p.whole ? 1.f / sum : 1.f;
             float* to = p.whole ? (float*) a.out + at * a.out_stride + (size_t) head * a.width : c.part_o + part * a.width;
-            float check = sum * 0.f; // stays 0 for finite values
+            // Stays 0 for finite values. A maximum of minus infinity may be of masked keys or of such scores.
+            float check = top == -INFINITY ? NAN : sum * 0.f;
             for (int channel = 2 * lane; channel < a.width; channel += 64)
             {
                 float2 x = make_float2(0.f, 0.f);
