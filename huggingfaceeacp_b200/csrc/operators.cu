@@ -21,6 +21,32 @@ static_assert(kPagePositions == HF_PAGE_ROWS && kTreeNodes == HF_TREE_NODES, "th
 
 namespace
 {
+// A function of the driver's, looked up once; null when it is not there.
+template <typename F>
+F driver_call(std::atomic<F>& known, const char* name)
+{
+    if (F f = known.load(std::memory_order_relaxed))
+        return f;
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion(name, &f, 12000, cudaEnableDefault, &found) != cudaSuccess
+        || found != cudaDriverEntryPointSuccess)
+        return nullptr;
+    known.store((F) f, std::memory_order_relaxed);
+    return (F) f;
+}
+
+// Whether the calling thread has a current context: one that has not used the device
+// yet has none, and tensor maps cannot be encoded there.
+bool has_context()
+{
+    using Current = CUresult (*)(CUcontext*);
+    static std::atomic<Current> known {nullptr};
+    const Current current = driver_call(known, "cuCtxGetCurrent");
+    CUcontext context = nullptr;
+    return current && current(&context) == CUDA_SUCCESS && context;
+}
+
 // Makes the device that holds `p` current, and the caller's again at the end.
 class DeviceOf
 {
@@ -30,7 +56,8 @@ public:
         int device = 0;
         if (!on_device(p, &device))
             return;
-        if (cudaGetDevice(&before) != cudaSuccess || (device != before && cudaSetDevice(device) != cudaSuccess))
+        if (cudaGetDevice(&before) != cudaSuccess
+            || ((device != before || !has_context()) && cudaSetDevice(device) != cudaSuccess))
         {
             status = HF_E_CUDA;
             return;
@@ -63,21 +90,12 @@ private:
     {
         using Query = CUresult (*)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
         static std::atomic<Query> known {nullptr};
-        Query query = known.load(std::memory_order_relaxed);
-        if (!query)
-        {
-            void* f = nullptr;
-            cudaDriverEntryPointQueryResult found;
-            if (cudaGetDriverEntryPointByVersion("cuPointerGetAttributes", &f, 12000, cudaEnableDefault, &found) != cudaSuccess
-                || found != cudaDriverEntryPointSuccess)
-                return false;
-            known.store(query = (Query) f, std::memory_order_relaxed);
-        }
+        const Query query = driver_call(known, "cuPointerGetAttributes");
         unsigned type = 0;
         int ordinal = -1;
         CUpointer_attribute which[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
         void* values[2] = {&type, &ordinal};
-        if (query(2, which, values, (CUdeviceptr) p) != CUDA_SUCCESS || type != CU_MEMORYTYPE_DEVICE || ordinal < 0)
+        if (!query || query(2, which, values, (CUdeviceptr) p) != CUDA_SUCCESS || type != CU_MEMORYTYPE_DEVICE || ordinal < 0)
             return false;
         *device = ordinal;
         return true;
@@ -244,15 +262,7 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
 EncodeTiled encoder()
 {
     static std::atomic<EncodeTiled> known {nullptr};
-    if (EncodeTiled e = known.load(std::memory_order_relaxed))
-        return e;
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess
-        || found != cudaDriverEntryPointSuccess)
-        return nullptr;
-    known.store((EncodeTiled) f, std::memory_order_relaxed);
-    return (EncodeTiled) f;
+    return driver_call(known, "cuTensorMapEncodeTiled");
 }
 
 // [rows][heads][width] elements, rows `stride` elements apart, in boxes of 128

@@ -2,6 +2,7 @@
 64-bit implementations (serving_reference.py): types, head layouts, lengths around the page and tile borders, strided
 views, empty sequences, garbage outside the rows in use, captured graphs, and a serving run of all of them together."""
 import math
+import threading
 
 import pytest
 
@@ -943,3 +944,32 @@ def test_tree_rows_whose_scores_are_minus_infinity(kind, length, nodes, lowest):
     assert bool(torch.isnan(expected[:nodes, :2]).all()) == (lowest == 1) and bool(torch.isfinite(expected[:, 2:]).all())
     everything = torch.cat([k, cache.keys[0].view(-1, kv, d)])
     ref.close(out, expected, size, q, everything, d ** -0.5, length + 64)
+
+
+# ---- who calls -----------------------------------------------------------------------------------------------------
+
+
+def test_a_thread_that_has_not_used_the_device():
+    """A fresh thread has no current context of its own yet."""
+    g = torch.Generator("cuda").manual_seed(96)
+    (q, k, v), stride = _fused(g, 300, 8, 1, 256, torch.float32)
+    out = torch.empty(q.shape, device="cuda")
+    stream, failed = _stream(), []
+    plan, offsets = native.PackedAttention(native.F32, 8, 1, 256), _ints([0, 300])
+    room = _room(plan.workspace_bytes(1, 300))
+    torch.cuda.synchronize()
+
+    def call():
+        try:
+            plan.run(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), 1, 300, q_stride=stride,
+                     k_stride=stride, v_stride=stride, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=stream)
+        except native.HFError as e:
+            failed.append(e)
+
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not failed
+    expected, size = ref.packed(q, k, v, [300], 1 / 16)
+    ref.close(out, expected, size, q, k, 1 / 16, 300)
