@@ -747,54 +747,79 @@ class PageCache:
         _refused(rc, "page write")
 
 
+class _Calls:
+    """A plan's call structs that are not in use. Each call takes one for itself and gives it back (list operations are
+    atomic), since another thread may call while this one is in the library; making one anew costs 0.7 us more."""
+
+    def __init__(self, kind, *fixed):
+        self.kind, self.fixed, self.spare = kind, fixed, []
+
+    def take(self):
+        try:
+            return self.spare.pop()
+        except IndexError:
+            call = self.kind(*self.fixed)
+            return call, ctypes.byref(call)
+
+
 class PackedAttention:
     """Causal attention of packed prompts (hf_cuda_attention_packed) for one choice of heads; run() takes device addresses.
-    `scale` defaults to head_width ** -0.5. Nothing is kept of a call: threads may share one."""
+    `scale` defaults to head_width ** -0.5. Threads may share one."""
 
     def __init__(self, dtype: int, heads: int, kv_heads: int, head_width: int, scale: float | None = None):
         self.lib = cuda()
-        self.heads = (dtype, heads, kv_heads, head_width)
-        self.scale = head_width ** -0.5 if scale is None else scale
+        self.calls = _Calls(PackedStruct, dtype, heads, kv_heads, head_width, 0, 0,
+                            head_width ** -0.5 if scale is None else scale)
 
     def workspace_bytes(self, sequences: int, rows: int) -> int:
-        size, call = ctypes.c_uint64(0), PackedStruct(*self.heads, sequences, rows, self.scale)
-        _refused(self.lib.hf_cuda_attention_packed_workspace(ctypes.byref(call), ctypes.byref(size)), "packed attention")
+        size, (c, ref) = ctypes.c_uint64(0), self.calls.take()
+        c.sequences, c.rows = sequences, rows
+        _refused(self.lib.hf_cuda_attention_packed_workspace(ref, ctypes.byref(size)), "packed attention")
+        self.calls.spare.append((c, ref))
         return size.value
 
     def run(self, q: int, k: int, v: int, out: int, offsets: int, sequences: int, rows: int, q_stride: int = 0,
             k_stride: int = 0, v_stride: int = 0, out_stride: int = 0, workspace: int = 0, workspace_bytes: int = 0,
             stream: int | None = None):
-        call = PackedStruct(*self.heads, sequences, rows, self.scale, q, k, v, out, q_stride, k_stride, v_stride, out_stride,
-                            offsets, workspace, workspace_bytes)
-        _refused(self.lib.hf_cuda_attention_packed(ctypes.byref(call), stream), "packed attention")
+        c, ref = self.calls.take()
+        c.q, c.k, c.v, c.out, c.offsets, c.sequences, c.rows = q, k, v, out, offsets, sequences, rows
+        c.q_stride, c.k_stride, c.v_stride, c.out_stride = q_stride, k_stride, v_stride, out_stride
+        c.workspace, c.workspace_bytes = workspace, workspace_bytes
+        _refused(self.lib.hf_cuda_attention_packed(ref, stream), "packed attention")
+        self.calls.spare.append((c, ref))
 
 
 class TreeAttention:
     """Attention of drafted trees, or of single tokens, over a layer of a PageCache (hf_cuda_attention_tree) for one choice
-    of heads; run() takes device addresses. `scale` defaults to head_width ** -0.5. Nothing is kept of a call: threads may
-    share one."""
+    of heads; run() takes device addresses. `scale` defaults to head_width ** -0.5. Threads may share one."""
 
     def __init__(self, dtype: int, heads: int, kv_heads: int, head_width: int, scale: float | None = None):
         self.lib = cuda()
         self.dtype = dtype
-        self.heads = (heads, kv_heads, head_width)
-        self.scale = head_width ** -0.5 if scale is None else scale
+        self.kv_width = kv_heads * head_width
+        self.calls = _Calls(TreeStruct, heads, kv_heads, head_width, 0, 0, 0, 0,
+                            head_width ** -0.5 if scale is None else scale)
 
     def workspace_bytes(self, sequences: int, rows: int, max_nodes: int, max_length: int) -> int:
-        size, call = ctypes.c_uint64(0), TreeStruct(*self.heads, rows, max_nodes, max_length, 0, self.scale)
-        cache = PageCacheStruct(self.dtype, 1, 1, call.kv_heads * call.head_width, sequences, 1)
-        _refused(self.lib.hf_cuda_attention_tree_workspace(ctypes.byref(cache), ctypes.byref(call), ctypes.byref(size)),
-                 "tree attention")
+        size, (c, ref) = ctypes.c_uint64(0), self.calls.take()
+        cache = PageCacheStruct(self.dtype, 1, 1, self.kv_width, sequences, 1)
+        c.rows, c.max_nodes, c.max_length, c.layer = rows, max_nodes, max_length, 0
+        _refused(self.lib.hf_cuda_attention_tree_workspace(ctypes.byref(cache), ref, ctypes.byref(size)), "tree attention")
+        self.calls.spare.append((c, ref))
         return size.value
 
     def run(self, cache: PageCache, layer: int, q: int, k: int, v: int, out: int, offsets: int, parents: int, rows: int,
             max_nodes: int, max_length: int, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, out_stride: int = 0,
             workspace: int = 0, workspace_bytes: int = 0, stream: int | None = None):
-        call = TreeStruct(*self.heads, rows, max_nodes, max_length, layer, self.scale, q, k, v, out, q_stride, k_stride,
-                          v_stride, out_stride, offsets, parents, workspace, workspace_bytes)
         if cache.struct.dtype != self.dtype:
             raise HFError(HF_E_INVALID, "the cache holds another element type")
-        _refused(self.lib.hf_cuda_attention_tree(cache.ref, ctypes.byref(call), stream), "tree attention")
+        c, ref = self.calls.take()
+        c.q, c.k, c.v, c.out, c.offsets, c.parents, c.rows = q, k, v, out, offsets, parents, rows
+        c.q_stride, c.k_stride, c.v_stride, c.out_stride = q_stride, k_stride, v_stride, out_stride
+        c.max_nodes, c.max_length, c.layer, c.workspace, c.workspace_bytes = (max_nodes, max_length, layer, workspace,
+                                                                              workspace_bytes)
+        _refused(self.lib.hf_cuda_attention_tree(cache.ref, ref, stream), "tree attention")
+        self.calls.spare.append((c, ref))
 
 
 NCCL_ID_BYTES = 128  # hf_cuda.h HF_NCCL_ID_BYTES
