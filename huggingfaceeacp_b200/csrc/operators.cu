@@ -119,6 +119,12 @@ bool aligned(const void* p)
     return p && (uintptr_t) p % 16 == 0;
 }
 
+// An int32 array; `optional` ones may be null.
+bool words(const void* p, bool optional = false)
+{
+    return p ? (uintptr_t) p % 4 == 0 : optional;
+}
+
 // A row stride in elements: the width when 0; false when rows would overlap or
 // are not 16-byte aligned.
 bool row_stride(int64_t* stride, int64_t width, int size)
@@ -157,7 +163,7 @@ int check_cache(const hf_page_cache* cache, hf_page_cache* c)
 {
     if (const int rc = check_cache_sizes(cache, c))
         return rc;
-    return aligned(c->keys) && aligned(c->values) && c->table && c->lengths && c->refs ? HF_OK : HF_E_INVALID;
+    return aligned(c->keys) && aligned(c->values) && words(c->table) && words(c->lengths) && words(c->refs) ? HF_OK : HF_E_INVALID;
 }
 
 uint64_t book_bytes(const hf_page_cache& c)
@@ -232,7 +238,7 @@ template <typename Call>
 int check_rows(const Call& call, int size, int heads, int kv_heads, int width, AttnCall* a)
 {
     int64_t q = call.q_stride, k = call.k_stride, v = call.v_stride, o = call.out_stride;
-    if (!aligned(call.q) || !aligned(call.k) || !aligned(call.v) || !aligned(call.out) || !call.offsets
+    if (!aligned(call.q) || !aligned(call.k) || !aligned(call.v) || !aligned(call.out) || !words(call.offsets)
         || !row_stride(&q, (int64_t) heads * width, size) || !row_stride(&k, (int64_t) kv_heads * width, size)
         || !row_stride(&v, (int64_t) kv_heads * width, size) || !row_stride(&o, (int64_t) heads * width, size))
         return HF_E_INVALID;
@@ -607,8 +613,8 @@ int hf_cuda_pages_update(const hf_page_cache* cache, const int32_t* release, int
     hf_page_cache c;
     if (const int rc = check_cache(cache, &c))
         return rc;
-    if (releases < 0 || releases > c.sequences || fork_count < 0 || fork_count > c.sequences || !result
-        || (releases && !release) || (fork_count && !forks) || !aligned(workspace))
+    if (releases < 0 || releases > c.sequences || fork_count < 0 || fork_count > c.sequences || !words(result)
+        || !words(release, !releases) || !words(forks, !fork_count) || !words(grow, true) || !aligned(workspace))
         return HF_E_INVALID;
     if (workspace_bytes < book_bytes(c))
         return HF_E_CAPACITY;
@@ -634,7 +640,7 @@ int hf_cuda_pages_compact(const hf_page_cache* cache, int32_t* live, void* works
     hf_page_cache c;
     if (const int rc = check_cache(cache, &c))
         return rc;
-    if (!live || !aligned(workspace))
+    if (!words(live) || !aligned(workspace))
         return HF_E_INVALID;
     if (workspace_bytes < book_bytes(c))
         return HF_E_CAPACITY;
@@ -661,7 +667,7 @@ int hf_cuda_pages_write(const hf_page_cache* cache, int32_t layer, const void* k
     if (const int rc = check_cache(cache, &c))
         return rc;
     const int size = size_of(c.dtype);
-    if (layer < 0 || layer >= c.layers || rows < 0 || source_rows < 0 || !offsets || !aligned(k) || !aligned(v)
+    if (layer < 0 || layer >= c.layers || rows < 0 || source_rows < 0 || !words(offsets) || !words(index, true) || !aligned(k) || !aligned(v)
         || !row_stride(&k_stride, c.kv_width, size) || !row_stride(&v_stride, c.kv_width, size))
         return HF_E_INVALID;
     if (rows == 0 || source_rows == 0)
@@ -750,7 +756,7 @@ int hf_cuda_attention_tree(const hf_page_cache* cache, const hf_attention_tree* 
     const int size = size_of(c.dtype);
     if (const int rc = check_rows(*call, size, call->heads, call->kv_heads, call->head_width, &a))
         return rc;
-    if (!aligned(c.keys) || !aligned(c.values) || !c.table || !c.lengths || !call->parents)
+    if (!aligned(c.keys) || !aligned(c.values) || !words(c.table) || !words(c.lengths) || !words(call->parents))
         return HF_E_INVALID;
     a.sequences = c.sequences;
     a.parents = call->parents;

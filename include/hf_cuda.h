@@ -392,10 +392,10 @@ int hf_cuda_quantize_q8(const float* values, int64_t first, int64_t count, int64
  * replayed side by side) need one each. Element type of queries, keys, values,
  * outputs and pages: HF_DTYPE_*; scores, softmax statistics and sums are fp32
  * in all of them. Refused before anything is launched: a null pointer, a count
- * out of range, memory that is not 16-byte aligned or not device memory, a
- * stride that is no multiple of 16 bytes (HF_E_INVALID); a shape they do not
- * serve (HF_E_SHAPE); a workspace that is too small (HF_E_CAPACITY). What the
- * host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
+ * out of range, memory that is not 16-byte aligned (int32 arrays: 4) or not
+ * device memory, a stride that is no multiple of 16 bytes (HF_E_INVALID); a
+ * shape they do not serve (HF_E_SHAPE); a workspace that is too small
+ * (HF_E_CAPACITY). What the host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
  * bounded by the kernels: offsets are taken as ascending within [0, rows],
  * lengths within the bounds given, and a page id outside the pool is a page
  * that is not there (its positions are not attended, read or written). Waits

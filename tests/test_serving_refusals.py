@@ -106,3 +106,30 @@ def test_tree_cache_must_match():
             "max_nodes": 5, "max_length": 200, "workspace": GOOD, "workspace_bytes": 1 << 40}
     assert _code(native.TreeAttention(native.BF16, 8, 2, 64).run, cache=_cache(kv_width=64), **args) == native.HF_E_SHAPE
     assert _code(native.TreeAttention(native.F32, 8, 2, 64).run, cache=_cache(), **args) == native.HF_E_INVALID
+
+
+def test_int32_arrays_off_their_border():
+    """Refused ahead of the workspace's size: a kernel would fault on them."""
+    for name in ("table", "lengths", "refs"):
+        cache = _cache(**{name: GOOD + 2})
+        assert _code(cache.update, GOOD, GOOD, 0) == native.HF_E_INVALID
+        assert _code(cache.compact, GOOD, GOOD, 0) == native.HF_E_INVALID
+        assert _code(cache.write, 0, GOOD, GOOD, GOOD, 5) == native.HF_E_INVALID
+    lists = {"result": GOOD, "release": GOOD, "releases": 1, "forks": GOOD, "fork_count": 1, "grow": GOOD}
+    assert _code(_cache().update, **lists, workspace=GOOD, workspace_bytes=0) == native.HF_E_CAPACITY
+    for name in ("result", "release", "forks", "grow"):
+        bad = {**lists, name: GOOD + 1}
+        assert _code(_cache().update, **bad, workspace=GOOD, workspace_bytes=0) == native.HF_E_INVALID
+    assert _code(_cache().compact, GOOD + 3, GOOD, 0) == native.HF_E_INVALID
+    for name in ("offsets", "index"):
+        args = {"layer": 0, "k": GOOD, "v": GOOD, "offsets": GOOD, "rows": 0, "index": GOOD, name: GOOD + 2}
+        assert _code(_cache().write, **args) == native.HF_E_INVALID
+    rows = {"q": GOOD, "k": GOOD, "v": GOOD, "out": GOOD, "offsets": GOOD, "rows": 9, "workspace": GOOD, "workspace_bytes": 0}
+    prompt, step = native.PackedAttention(native.F32, 8, 2, 64), native.TreeAttention(native.BF16, 8, 2, 64)
+    assert _code(prompt.run, **rows, sequences=2) == native.HF_E_CAPACITY
+    assert _code(prompt.run, **{**rows, "offsets": GOOD + 2}, sequences=2) == native.HF_E_INVALID
+    tree = {**rows, "cache": _cache(), "layer": 0, "parents": GOOD, "max_nodes": 5, "max_length": 200}
+    assert _code(step.run, **tree) == native.HF_E_CAPACITY
+    for bad in ({"offsets": GOOD + 1}, {"parents": GOOD + 2}, {"cache": _cache(table=GOOD + 1)},
+                {"cache": _cache(lengths=GOOD + 2)}):
+        assert _code(step.run, **{**tree, **bad}) == native.HF_E_INVALID
