@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
         int put = 0;
         bool ok = true;
         auto one_wait = [&](uint64_t* bar, unsigned parity) {
-            if (ok && !thread_wait(bar, parity))
+            if (ok && !lone_wait(bar, parity))
             {
                 *(volatile int*) &h.dead = 1;
                 ok = false;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
     for (int i = 0;; ++i)
     {
         const bool come = ok && !__any_sync(0xFFFFFFFFu, *(volatile int*) &h.dead)
-                          && warp_wait(&h.place_full[i & 1], (i / 2) & 1);
+                          && same_wait(&h.place_full[i & 1], (i / 2) & 1);
         if (any_stops(1, 32 * kFewWarps, !come || h.place[i & 1].sequence < 0))
             break;
         const MmaPlace p = h.place[i & 1];
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
             {
                 const int first = half * kFewKeys + 4 * warp; // the warp's keys of the tile
                 const int ks = item % S, vs = (item + 1) % S;
-                ok = ok && warp_wait(&h.full[ks], (item / S) & 1);
+                ok = ok && same_wait(&h.full[ks], (item / S) & 1);
                 float s[4 * kFewRows];
                 {
                     float4 x[4][V];
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(FewShape<D>::kThreads, 1)
                                                     acc[r][v].w * scale);
                     }
                 }
-                ok = ok && warp_wait(&h.full[vs], ((item + 1) / S) & 1);
+                ok = ok && same_wait(&h.full[vs], ((item + 1) / S) & 1);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                 {

@@ -301,7 +301,14 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
     const uint32_t tmem = h.tmem;
     // A wait of one of the roles; one that runs out ends the CTA's other waits too.
     auto wait = [&](uint64_t* bar, unsigned parity) {
-        const bool ok = warp_wait(bar, parity);
+        const bool ok = same_wait(bar, parity);
+        if (!ok)
+            *(volatile int*) &h.dead = 1;
+        return ok;
+    };
+    // The same where lanes wait for different barriers.
+    auto wait_for_all = [&](uint64_t* bar, unsigned parity) {
+        const bool ok = warp_wait<2>(bar, parity);
         if (!ok)
             *(volatile int*) &h.dead = 1;
         return ok;
@@ -372,13 +379,17 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                             next[r] = {next[r].tile + 1, 0, next[r].id_next, page_of(next[r].tile + 2)};
                         return true;
                     };
-                    unsigned idle = 0;
+                    bool idle = false;
+                    unsigned begun = 0;
                     while ((next[0].tile < p.tiles || next[1].tile < p.tiles) && ok)
                     {
                         const bool k = load(0, &kmap, &kmap2, keys, put_keys, KS, h.keys_full, h.keys_free);
                         const bool v = load(1, &vmap, &vmap2, values, put_values, VS, h.values_full, h.values_free);
-                        idle = k || v ? 0 : idle + 1;
-                        if (idle == 1u << 26) // some seconds
+                        const unsigned now = wait_ticks();
+                        if (k || v || !idle)
+                            begun = now;
+                        idle = !k && !v;
+                        if (now - begun > kWaitTicks)
                         {
                             flag_error(&g_operator_error, kErrWaitTimeout);
                             *(volatile int*) &h.dead = 1;
@@ -417,7 +428,7 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                     {
                         const int stage = item % KS;
                         const bool reads = (lane & 1) && b == 0 && count > 0; // S of the last tile is in registers
-                        ok = wait(reads ? &h.scores_read : &landed[stage], (reads ? count - 1 : item / KS) & 1);
+                        ok = wait_for_all(reads ? &h.scores_read : &landed[stage], (reads ? count - 1 : item / KS) & 1);
                         if (!ok)
                             break;
                         tc_fence_after();
@@ -459,8 +470,8 @@ __global__ void __launch_bounds__(LimbShape<D, Tree>::kThreads, 1)
                         const int stage = item % VS, what = lane & 3, part = Shape::kHalves ? b / 2 : buffer;
                         const bool frees = what == 1 && (b == 0 || (Shape::kHalves && b == 2)) && count >= RB;
                         const bool weighs = what == 2 && b == 0;
-                        ok = wait(frees ? &h.rows_free[part] : weighs ? &h.weights[count & 1] : &landed[stage],
-                                  (frees ? count / RB - 1 : weighs ? count / 2 : item / VS) & 1);
+                        ok = wait_for_all(frees ? &h.rows_free[part] : weighs ? &h.weights[count & 1] : &landed[stage],
+                                          (frees ? count / RB - 1 : weighs ? count / 2 : item / VS) & 1);
                         if (!ok)
                             break;
                         if (!Tree && valid < kKeyTile)

@@ -174,20 +174,76 @@ struct MmaHead
 };
 
 // Bounded waits, of a warp together and of one thread. A warp's lanes may name
-// different barriers: it goes on when all have come, for the price of one. A poll
-// that finds nothing is held about 4 us by the hardware, so the limit is some 4 s: far
-// above a step, and above the rows that a warp may have to take again meanwhile (32 rows
-// of a million keys).
+// different barriers: it goes on when all have come, for the price of one.
+//
+// The limit is in time: the hardware holds a poll that finds nothing for 4 us while all
+// of a warp's lanes wait, and for 0.09 us once some have gone on, so that a number of
+// polls says little. After 8 to 9 ticks of 2^32 ns, some 36 s, a wait gives up: far
+// above a step, and above the rows that a warp may have to take again meanwhile, at
+// 0.43 us a key and row (32 rows of two million keys; in attention_limbs 16 at 0.52).
+// Where it is known how the lanes wait, polls are counted: same_wait, of a warp whose
+// lanes all wait for one barrier (34 s), and lone_wait, of one thread (24 s).
+//
+// The loop has one way on and one out: with a second way on (a slower loop behind it, a
+// call, a look at whether rows are taken again) the compiler no longer sees that the
+// lanes go together, and calls take 5 to 60 % longer. The clock is read after every
+// `Polls`, which decides between a wait's length and the code's. Measured with 1, 2, 4
+// and 8: prompts of 32 heads of 128, 4 x 4096 tokens 515, 509, 509, 513 us, 2048 of up to
+// 64 tokens 307, 295, 262, 274; of width 256 479, 464, 464, 452; 2048 decode steps of 10 to
+// 600 tokens 878, 886, 926, 1014, one tree of 63 14.7, 14.9, 15.9, 15.5. (48 fp32 decode
+// steps on FMAs: 94.6, 95.2, 95.6, 95.6, with counted polls 93.3.)
+constexpr unsigned kWaitTicks = 8;
+
+__device__ __forceinline__ unsigned wait_ticks()
+{
+    unsigned t;
+    asm volatile("mov.u32 %0, %%globaltimer_hi;" : "=r"(t));
+    return t;
+}
+
+template <int Polls>
+__device__ __forceinline__ bool timed_wait(uint64_t* bar, unsigned parity)
+{
+    unsigned begun = 0;
+    for (bool first = true;; first = false)
+    {
+#pragma unroll
+        for (int i = 0; i < Polls; ++i)
+            if (mbar_wait(bar, parity, 1))
+                return true;
+        const unsigned now = wait_ticks();
+        if (first)
+            begun = now;
+        if (now - begun > kWaitTicks)
+            return false;
+    }
+}
+template <int Polls>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity)
 {
-    if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)))
+    if (__all_sync(0xFFFFFFFFu, timed_wait<Polls>(bar, parity)))
         return true;
     flag_error(&g_operator_error, kErrWaitTimeout);
     return false;
 }
+template <int Polls>
 __device__ __forceinline__ bool thread_wait(uint64_t* bar, unsigned parity)
 {
-    if (mbar_wait(bar, parity))
+    if (timed_wait<Polls>(bar, parity))
+        return true;
+    flag_error(&g_operator_error, kErrWaitTimeout);
+    return false;
+}
+__device__ __forceinline__ bool same_wait(uint64_t* bar, unsigned parity)
+{
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, 1u << 23)))
+        return true;
+    flag_error(&g_operator_error, kErrWaitTimeout);
+    return false;
+}
+__device__ __forceinline__ bool lone_wait(uint64_t* bar, unsigned parity)
+{
+    if (mbar_wait(bar, parity, 1u << 28))
         return true;
     flag_error(&g_operator_error, kErrWaitTimeout);
     return false;
@@ -554,6 +610,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
     using Shape = MmaShape<D, NQ>;
     constexpr int KS = Shape::kKeyStages, VS = Shape::kValueStages, kBlocks = Shape::kBlocks;
     constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    constexpr int kPolls = Tree ? 1 : D == 256 ? 8 : 4; // see timed_wait
     extern __shared__ __align__(1024) uint8_t smem[];
     MmaHead& h = *reinterpret_cast<MmaHead*>(smem);
     static_assert(sizeof(MmaHead) <= Shape::kHead, "the head's room");
@@ -643,7 +700,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
     };
     // A wait of one of the roles; one that runs out ends the CTA's other waits too.
     auto wait = [&](uint64_t* bar, unsigned parity) {
-        const bool ok = warp_wait(bar, parity);
+        const bool ok = warp_wait<kPolls>(bar, parity);
         if (!ok)
             *(volatile int*) &h.dead = 1;
         return ok;
@@ -666,7 +723,7 @@ __global__ void __launch_bounds__(MmaShape<D, NQ>::kThreads, MmaShape<D, NQ>::kC
         int put_keys = 0, put_values = 0, put_queries = 0;
         bool ok = true;
         auto one_wait = [&](uint64_t* bar, unsigned parity) {
-            if (ok && !thread_wait(bar, parity))
+            if (ok && !thread_wait<kPolls>(bar, parity))
             {
                 *(volatile int*) &h.dead = 1;
                 ok = false;

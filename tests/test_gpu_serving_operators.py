@@ -973,3 +973,26 @@ def test_a_thread_that_has_not_used_the_device():
     assert not failed
     expected, size = ref.packed(q, k, v, [300], 1 / 16)
     ref.close(out, expected, size, q, k, 1 / 16, 300)
+
+
+@pytest.mark.parametrize("kind,n", [("bf16", 120064), ("f16", 20096), ("f32", 40064)])
+def test_rows_taken_again_over_many_keys(kind, n):
+    """An infinite value near a long prompt's end: the rows of its tile are taken again over all of their keys, a warp's 32
+    (fp32: 16) in 0.3 to 1.7 s, and what waits for them waits on. (bf16: by the second of a CTA's two query tiles.)"""
+    code, dtype = ref.TYPES[kind]
+    g = torch.Generator("cuda").manual_seed(99)
+    q, k, v = (_normal(g, n, 1, 8, dtype=dtype) for _ in range(3))
+    bad = n - 30
+    v[bad, 0, 3] = math.inf
+    out = torch.empty_like(q)
+    kept = _run_packed(code, q, k, v, out, [n], 8)
+    torch.cuda.synchronize()
+    assert kept
+    at = torch.tensor([0, n // 2, n - 128, n - 65, bad - 1, bad, n - 1], device="cuda")
+    seen = torch.arange(n, device="cuda") <= at[:, None]
+    expected, size = ref.attend(q[at], k, v, seen, 8 ** -0.5)
+    fine = torch.isfinite(expected)
+    assert int((~fine).sum()) == 2 and torch.equal(torch.isfinite(out[at]), fine)
+    tol = ref.tolerance(expected.nan_to_num(0, 0, 0), size.nan_to_num(0, 0, 0), q, k, 8 ** -0.5, n, dtype)
+    assert bool(((out[at].double() - expected).abs() <= tol)[fine].all())
+    assert not bool(torch.isnan(out).any())
