@@ -996,3 +996,114 @@ def test_rows_taken_again_over_many_keys(kind, n):
     tol = ref.tolerance(expected.nan_to_num(0, 0, 0), size.nan_to_num(0, 0, 0), q, k, 8 ** -0.5, n, dtype)
     assert bool(((out[at].double() - expected).abs() <= tol)[fine].all())
     assert not bool(torch.isnan(out).any())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_a_call_repeated_gives_the_same_bits(kind):
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, lengths = 8, 2, 128, [900, 3, 0, 400, 131]
+    g = torch.Generator("cuda").manual_seed(97)
+    (q, k, v), stride = _fused(g, sum(lengths), h, kv, d, dtype)
+    prompts = [torch.empty(q.shape, dtype=dtype, device="cuda") for _ in range(4)]
+    for out in prompts:
+        _run_packed(code, q, k, v, out, lengths, stride)
+    cached = [3000, 700, 0, 64, 1900]
+    cache = Cache(kind, 1, 100, kv, d, cached, 47, 98)
+    trees = []
+    for nodes in (1, 12):
+        q, k, v = (_normal(g, 5 * nodes, n, d, dtype=dtype) for n in (h, kv, kv))
+        trees.append([_run_tree(cache, q, k, v, [nodes] * 5, [_branching(nodes, s) for s in range(5)], 3000)[0]
+                      for _ in range(4)])
+    for first, *others in (prompts, *trees):
+        for other in others:
+            assert torch.equal(first.view(torch.uint8), other.view(torch.uint8))
+
+# ---- what the documentation allows ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("sequences", [1, 5, 200])
+def test_a_batch_without_a_row(kind, sequences):
+    """Every sequence is empty: nothing is read or written, in calls of many rows and of few."""
+    code, dtype = ref.TYPES[kind]
+    for rows in (4, 900):
+        q, k, v = (torch.full((rows, n, 64), math.nan, dtype=dtype, device="cuda") for n in (8, 2, 2))
+        out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+        _run_packed(code, q, k, v, out, [0] * sequences, 0, begin=rows // 2)
+        assert bool((out == 7.0).all())
+        cache = Cache(kind, 1, 3, 2, 64, [0] * sequences, 2, 101)
+        plan, offsets, up = native.TreeAttention(code, 8, 2, 64), _ints([rows // 2] * (sequences + 1)), _ints([-1] * rows)
+        room = _room(plan.workspace_bytes(sequences, rows, 5, 128))
+        plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(), up.data_ptr(),
+                 rows, 5, 128, workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+        assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(8, 1, 256), (4, 2, 40), (16, 4, 128)], ids=str)
+@pytest.mark.parametrize("lengths", [[20, 5], [300, 1, 77], [700] * 6], ids=str)
+def test_rows_of_every_operand_further_apart(kind, heads, lengths):
+    """A row stride of its own for q, k, v and out; what lies between out's rows stays."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d = heads
+    rows = sum(lengths)
+    g = torch.Generator("cuda").manual_seed(102)
+    wide = [_normal(g, rows, n * d + 8 * (i + 1), dtype=dtype) for i, n in enumerate((h, kv, kv, h))]
+    wide[3].fill_(7.0)
+    q, k, v, out = (x[:, 8 * (i + 1):].unflatten(1, (-1, d)) for i, x in enumerate(wide))
+    offsets = _ints(_offsets(lengths))
+    strides = dict(zip(("q_stride", "k_stride", "v_stride", "out_stride"), (x.stride(0) for x in wide)))
+    plan = native.PackedAttention(code, h, kv, d)
+    room = _room(plan.workspace_bytes(len(lengths), rows))
+    plan.run(*(x.data_ptr() for x in (q, k, v, out)), offsets.data_ptr(), len(lengths), rows, **strides,
+             workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.packed(q, k, v, lengths, d ** -0.5)
+    ref.close(out, expected, size, q, k, d ** -0.5, max(lengths))
+    assert bool((wide[3][:, :32] == 7.0).all())
+    nodes = [min(n, 9) for n in lengths]
+    cache = Cache(kind, 1, 40, kv, d, [200, 70, 0, 333, 64, 1][:len(lengths)], 6, 103)
+    parents = [_branching(n, i) for i, n in enumerate(nodes)]
+    wide[3].fill_(7.0)
+    used, step = sum(nodes), native.TreeAttention(code, h, kv, d)
+    offsets, up = _ints(_offsets(nodes)), _ints([p for row in parents for p in row])
+    room = _room(step.workspace_bytes(len(nodes), used, 9, 333))
+    step.run(cache.native, 0, *(x.data_ptr() for x in (q, k, v, out)), offsets.data_ptr(), up.data_ptr(), used, 9, 333, **strides,
+             workspace=room.data_ptr(), workspace_bytes=room.numel(), stream=_stream())
+    expected, size = ref.tree(q[:used], k[:used], v[:used], nodes, parents, cache.keys[0].view(cache.shape),
+                              cache.values[0].view(cache.shape), cache.table.tolist(), cache.lengths.tolist(), d ** -0.5)
+    everything = torch.cat([k[:used], cache.keys[0].view(-1, kv, d)])
+    ref.close(out[:used], expected, size, q[:used], everything, d ** -0.5, 342)
+    assert bool((wide[3][:, :32] == 7.0).all()) and bool((wide[3][used:] == 7.0).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_graphs_side_by_side(kind):
+    """Two captured steps replayed at once on two streams, a workspace each, over one cache."""
+    code, dtype = ref.TYPES[kind]
+    h, kv, d, lengths = 8, 2, 128, [1500, 300, 64]
+    cache = Cache(kind, 1, 40, kv, d, lengths, 24, 104)
+    g = torch.Generator("cuda").manual_seed(105)
+    runs = []
+    for nodes in (1, 6):
+        q, k, v = (_normal(g, 3 * nodes, n, d, dtype=dtype) for n in (h, kv, kv))
+        out, parents = torch.empty_like(q), [_branching(nodes, s) for s in range(3)]
+        plan = native.TreeAttention(code, h, kv, d)
+        offsets, up = _ints(_offsets([nodes] * 3)), _ints([p for row in parents for p in row])
+        room = _room(plan.workspace_bytes(3, len(q), nodes, 1500))
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(20):
+                plan.run(cache.native, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), offsets.data_ptr(),
+                         up.data_ptr(), len(q), nodes, 1500, workspace=room.data_ptr(), workspace_bytes=room.numel(),
+                         stream=_stream())
+        runs.append((graph, stream, q, k, v, out, nodes, parents, plan, offsets, up, room))
+    for _ in range(5):
+        for graph, stream, *_rest in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, q, k, v, out, nodes, parents, *_rest in runs:
+        expected, size = ref.tree(q, k, v, [nodes] * 3, parents, cache.keys[0].view(cache.shape),
+                                  cache.values[0].view(cache.shape), cache.table.tolist(), lengths, d ** -0.5)
+        ref.close(out, expected, size, q, torch.cat([k, cache.keys[0].view(-1, kv, d)]), d ** -0.5, 1506)
