@@ -12,9 +12,12 @@
 // Exponents: of a query, its row's; of keys and values a tile's (prompts:
 // split_tiles takes the tile's largest value) or the CTA's (trees: from 16 of its keys);
 // the weights 2^(s - m) are taken times 2^14, which cancels in the end. Where an
-// exponent does not fit its tile (values 2^16 apart, or more than 16 times the
-// trees' sample) the tile's factor is NaN, and like every row that comes out
-// not finite, its rows are taken again by attention_row.
+// exponent does not fit its tile (rows 2^16 apart; in trees keys or values above some
+// 29 to 59 times the sample's largest, or 32 channels of a value below 2^-17 of it) the
+// tile's factor is NaN, and like every row that comes out not finite, its rows are
+// taken again by attention_row. Rows are looked at, not channels: one whose values are
+// all small next to its tile's keeps an error of 2^-39 of the tile's largest value (trees:
+// 2^-35 of the sample's), which is more than fp32's below some 2^-20 of it.
 //
 // Work. As in attention_mma: 128 rows (tokens x a kv head's heads) a unit, 64-key
 // tiles, longest rows first, unit after unit. K and V pass through rings of 16 KB

@@ -45,14 +45,15 @@
 //
 // Measured (B200, CUDA events). Prompts, 4 x 4096 tokens, 32 heads of 128 over 8:
 // 510 us, 1,075 TFLOP/s, 0.65 of the measured cuBLAS rate, the tensor pipe active
-// 52 % of the time; 8 heads of 256 over one: 1,198 TFLOP/s, 59 %. Bound by the
+// 52 % of the time; 8 heads of 256 over one: 1,212 TFLOP/s, 59 %. Bound by the
 // softmax warps: a step of both query tiles (256 rows x 64 keys) takes some 1,700
 // cycles, 1,000 of them the weights, whose special-function (640), FMA (540) and
 // ALU (580) time two warps a scheduler overlap only partly; its MMAs take 1,280
 // (N = 64 scores are bound by the 6 KB that each reads from shared memory, 48
 // cycles instead of 32). Tried and no faster: two warpgroups a query tile, the
 // tiles' warps taking turns, 2 or 4 of 8 pairs on the FMA pipe. Trees, one token for
-// each of 64 caches of 4,000: 167 us for 1.07 GB, 0.97 of the measured copy rate.
+// each of 64 caches of 4,000: 163 us in this kernel (profiled alone) for 1.07 GB, 1.0 of
+// the measured copy rate; the call, with attention_join and its start, 189.
 #pragma once
 
 #include "attention_rows.cuh"

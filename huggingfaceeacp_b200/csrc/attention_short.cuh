@@ -15,7 +15,7 @@ constexpr int kShortWarps = 4, kShortKeys = 8;
 
 // attend_row with the loads of kShortKeys keys in flight. (The tiled kernels, which call
 // attend_row for the rows that they take again, have no registers for this one: with it
-// the trees of 64 caches of 4000 took 204 us instead of 188.)
+// a call for 64 caches of 4000 took 204 us instead of 188.)
 template <typename T, bool Tree>
 __device__ __forceinline__ void attend_short(const AttnCall& a, const RowKeys& keys, int kv_head, const float (&q)[8],
                                              int from, int to, float& m, float& l, float (&acc)[8])

@@ -68,7 +68,6 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// `count` arrivals at once.
 // Polls the phase with the given parity; returns false when the poll budget
 // runs out (the caller records kErrWaitTimeout and skips the stage).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, unsigned parity, unsigned limit = kSpinLimit)

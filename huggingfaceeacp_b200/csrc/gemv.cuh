@@ -206,6 +206,7 @@ constexpr int kStageQuants = 32768;
 constexpr int kStageScales = kStageQuants / 16;
 constexpr int kMaxSlabRows = 64; // rows a CTA may own when WPR > 1 (partials live in shared memory)
 
+// `count` arrivals at once.
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar, unsigned count)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");

@@ -298,9 +298,9 @@ constexpr int kSms = 148; // a B200's; the work is cut for it wherever the call 
 
 // What it costs a unit of a tree's to begin and to end, in key tiles (it is counted in
 // where the tiles are shared out): 48 decode steps of 50 to 2500 tokens, 32 heads on 8
-// of 128, bf16: 74 us with 0, 61 with 2, 59 with 4, 59 with 6; 48 trees of 15 nodes over
-// 50 to 1500, fp32: 215, 186, 172, 164, of 50 to 3000, 8 heads on one of 256: 105, 89,
-// 79, 85; on plain FMAs, 64 steps of 200 to 2048: 49, 47, 49, 52.
+// of 128, bf16: 75 us with 0, 60 with 2, 60 with 4, 61 with 6; 48 trees of 15 nodes over
+// 50 to 1500, fp32: 218, 187, 171, 164, of 50 to 3000, 8 heads on one of 256: 107, 91,
+// 82, 86; on plain FMAs, 64 steps of 200 to 2048: 52, 47, 50, 54.
 constexpr int kStart = 4, kFewStart = 2;
 
 // A tree's CTAs, one a place on the GPU, and the rows of a part that it leaves.
@@ -319,12 +319,12 @@ int part_rows(int heads, int kv_heads, int max_nodes)
 // 3.5 us and 0.07 us a key on the GPU, and some 0.3 us for 1000 keys of all rows
 // where they fill it. Bounds where the other kernels become as fast (us on the GPU,
 // short and other; a launch less saves 1 to 3 us of the caller's on top):
-//  trees, one row of 21, 101, 251 keys: fp32 4.6 and 11.5, 10.4 and 13.3, 20 and 14;
-//  bf16 4.7 and 9, 10.8 and 10.4, 21 and 10.8. 16 rows of 31: bf16 7.0 and 10.2; a tree of
-//  8 nodes on 60: fp32 9.9 and 16.6, bf16 9.5 and 9.2; of 40: fp32 36 and 18, bf16 30 and 9;
-//  a prompt of 8, 32, 64 tokens, 8 heads of 256: fp32 4.0 and 20, 6.1 and 21, 13.4 and 21;
-//  bf16 3.8 and 7.5, 5.2 and 7.5, 9.1 and 7.4; 32 heads of 128, 32 tokens: fp32 13 and 19,
-//  bf16 10.4 and 6.3.
+//  trees, one row of 21, 101, 251 keys: fp32 5.2 and 12.0, 10.7 and 14.2, 21 and 15;
+//  bf16 4.9 and 9.9, 10.9 and 11.8, 21 and 11.7. 16 rows of 31: bf16 7.3 and 10.8; a tree
+//  of 8 nodes on 60: fp32 10.1 and 17, bf16 9.6 and 9.9; of 40: fp32 37 and 19, bf16 31 and
+//  10; a prompt of 8, 32, 64 tokens, 8 heads of 256: fp32 4.0 and 21, 5.9 and 22, 13.1 and
+//  21; bf16 3.8 and 7.9, 5.2 and 8.1, 9.1 and 7.9; 32 heads of 128, 32 tokens: fp32 12.6
+//  and 18.5, bf16 10.3 and 6.7.
 bool is_short(const AttnCall& a, int dtype, bool tree, int64_t keys)
 {
     const int64_t most = dtype == HF_DTYPE_F32 ? 32768 : tree ? 24576 : 8192; // keys of all rows
@@ -364,12 +364,12 @@ int packed_mma(int dtype, const AttnCall& a, int device, cudaStream_t stream)
     c.a = a;
     c.tile_tokens = 128 / a.group;
     // Two query tiles a CTA read the keys half as often (300 prompts of 100 to 400 tokens,
-    // 32 heads on 8 of 128: 367 us, with one tile 422); with fewer of them than SMs
+    // 32 heads on 8 of 128: 345 us, with one tile 390); with fewer of them than SMs
     // the rows are spread over twice the CTAs instead. Of prompts of less than three
     // tiles a second one is mostly empty, and what a unit costs to begin and to end
     // counts: two CTAs a SM of one tile each overlap it (4096 prompts of up to 16 tokens:
-    // 453 us, with two tiles 852; 2048 of up to 64: 322 and 440; 1000 of 50 to 150: 463
-    // and 463).
+    // 357 us, with two tiles 644; 2048 of up to 64: 267 and 366; 1000 of 50 to 150: 441
+    // and 439).
     const int64_t pairs = (int64_t) a.rows * a.heads / 256;
     const bool shorts = a.rows < 3LL * c.tile_tokens * a.sequences;
     const int nq = a.width <= 128 && pairs >= kSms && !shorts ? 2 : 1;

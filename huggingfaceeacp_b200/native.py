@@ -705,7 +705,8 @@ def _refused(rc: int, what: str):
 
 
 def operators_sync(device: int = 0, stream: int | None = None):
-    """Waits for `stream`; raises when an operator's kernel gave up a wait on `device` (hf_cuda_operators_sync)."""
+    """Waits for `stream`; raises when an operator's kernel has given up a wait on `device` since the last call
+    (hf_cuda_operators_sync). Until that is told, the rows of tree calls on that device are NaN."""
     rc = cuda().hf_cuda_operators_sync(device, stream)
     if rc:
         raise HFError(rc, "an operator's kernel gave up a wait" if rc == HF_E_DEVICE else "CUDA error")

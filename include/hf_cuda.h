@@ -391,17 +391,26 @@ int hf_cuda_quantize_q8(const float* values, int64_t first, int64_t count, int64
  * between calls; calls that may overlap on the GPU (other streams, graphs
  * replayed side by side) need one each. Element type of queries, keys, values,
  * outputs and pages: HF_DTYPE_*; scores, softmax statistics and sums are fp32
- * in all of them. Refused before anything is launched: a null pointer, a count
- * out of range, memory that is not 16-byte aligned (int32 arrays: 4) or not
- * device memory, a stride that is no multiple of 16 bytes (HF_E_INVALID); a
- * shape they do not serve (HF_E_SHAPE); a workspace that is too small
- * (HF_E_CAPACITY). What the host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
+ * in all of them.
+ *   Rounding besides the result's own, once: in bf16 and fp16 a weight is rounded
+ * to the type for its product with the value (their sum is not), and its
+ * exponential is off by up to 8e-5 (bf16) or 3e-6 of itself. In fp32, products of
+ * prompts and of more than eight query rows a kv head are made of operands of 22
+ * bits: a query is off by up to 2^-22 of itself or 2^-39 of its row's largest
+ * value, a key or value by 2^-22 of itself or 2^-39 (trees: 2^-35) of the largest
+ * one near it (of 64 rows; trees: of the cached rows of its sequence).
+ *   Refused before anything is launched: a null pointer, a count out of range,
+ * memory that is not 16-byte aligned (int32 arrays: 4) or not device memory, a
+ * stride that is no multiple of 16 bytes (HF_E_INVALID); a shape they do not
+ * serve (HF_E_SHAPE); a workspace that is too small (HF_E_CAPACITY). What the
+ * host cannot see (offsets, lengths, page ids, parents: int32 device arrays) is
  * bounded by the kernels: offsets are taken as ascending within [0, rows],
  * lengths within the bounds given, and a page id outside the pool is a page
- * that is not there (its positions are not attended, read or written). Waits
- * inside the kernels are bounded: a call in which one ran out leaves rows that
- * are NaN or, of packed prompts, not written, hf_cuda_operators_sync reports it,
- * and until then the rows of tree calls on that device are NaN. */
+ * that is not there (its positions are not attended, read or written).
+ *   Waits inside the kernels are bounded (about half a minute): a call in which
+ * one ran out leaves rows that are NaN or, of packed prompts, not written,
+ * hf_cuda_operators_sync reports it, and until then the rows of tree calls on
+ * that device are NaN. */
 enum { HF_DTYPE_F32 = 0, HF_DTYPE_BF16 = 1, HF_DTYPE_F16 = 2 };
 /* Waits for `stream`; HF_E_DEVICE when a wait of an operator's kernel has run out on
  * `device` since the last call (and clears it). */
@@ -412,8 +421,9 @@ int hf_cuda_operators_sync(int device, void* stream);
  * rows up to i; query head h reads kv head h / (heads / kv_heads). Rows of q and
  * out are [heads][head_width], of k and v [kv_heads][head_width], `*_stride`
  * elements apart (0 = packed; views of one fused q|k|v row are fine). Rows
- * outside every sequence are neither read nor written. head_width is a multiple
- * of 8 up to 256, heads / kv_heads at most 128. `scale` (> 0) multiplies the scores.
+ * outside every sequence are neither read nor written, and sequences may all be
+ * empty, but `rows` and `sequences` are at least 1. head_width is a multiple of 8
+ * up to 256, heads / kv_heads at most 128. `scale` (> 0) multiplies the scores.
  * A value or key row that holds infinities or NaN reaches the rows that attend
  * to it, by the formula (a score of infinity or NaN makes the row NaN, one of
  * minus infinity weighs nothing, and of no other scores the row is NaN), and no
@@ -473,7 +483,7 @@ int hf_cuda_pages_workspace(const hf_page_cache* cache, uint64_t* bytes);
  *  release  the `releases` sequences listed (at most `sequences`; one listed
  *           twice is released once, ids out of range are ignored) give their
  *           pages back and have length 0;
- *  fork     of `fork_count` pairs (source, target), each target that is empty and
+ *  fork     of `fork_count` pairs (source, target; at most `sequences`), each target that is empty and
  *           that no earlier pair names becomes a copy of its source as the
  *           releases left it, sharing all of its pages; other pairs are ignored;
  *  grow     every sequence s grows by grow[s] positions (grow null = none, counts
