@@ -193,7 +193,10 @@ struct MmaHead
 // 64 tokens 307, 295, 262, 274; of width 256 479, 464, 464, 452; 2048 decode steps of 10 to
 // 600 tokens 878, 886, 926, 1014, one tree of 63 14.7, 14.9, 15.9, 15.5. (48 fp32 decode
 // steps on FMAs: 94.6, 95.2, 95.6, 95.6, with counted polls 93.3.)
-constexpr unsigned kWaitTicks = 8;
+#ifndef HFK_WAIT_TICKS // a test shortens it
+#define HFK_WAIT_TICKS 8
+#endif
+constexpr unsigned kWaitTicks = HFK_WAIT_TICKS;
 
 __device__ __forceinline__ unsigned wait_ticks()
 {

@@ -77,10 +77,21 @@ def test_a_failed_call_waits_for_the_last_copy_of_queries(tmp_path):
         assert "mbar_wait(&h.query, last_parity(put_queries))" in f.read()
 
 
+def _device_program(tmp_path, source, *flags):
+    program = str(tmp_path / "program")
+    subprocess.run([build.NVCC, *build.ARCH, "-std=c++17", "-O1", *flags, f"-I{build.INCLUDE}", f"-I{CSRC}",
+                    os.path.join(os.path.dirname(os.path.abspath(__file__)), source), "-o", program], check=True)
+    return subprocess.run([program], capture_output=True, text=True, timeout=120)
+
+
 @pytest.mark.gpu
 def test_the_join_of_a_failed_call_is_nan(tmp_path):
-    program = str(tmp_path / "join")
-    subprocess.run([build.NVCC, *build.ARCH, "-std=c++17", "-O1", f"-I{build.INCLUDE}", f"-I{CSRC}",
-                    os.path.join(os.path.dirname(os.path.abspath(__file__)), "join_harness.cu"), "-o", program], check=True)
-    result = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    result = _device_program(tmp_path, "join_harness.cu")
+    assert result.returncode == 0, result.stdout + result.stderr
+
+
+@pytest.mark.gpu
+def test_a_wait_without_an_arrival_ends(tmp_path):
+    """However its lanes wait, it returns and sets the error word; what has come is not kept waiting."""
+    result = _device_program(tmp_path, "wait_harness.cu", "-DHFK_WAIT_TICKS=0")
     assert result.returncode == 0, result.stdout + result.stderr
