@@ -1107,3 +1107,28 @@ def test_graphs_side_by_side(kind):
         expected, size = ref.tree(q, k, v, [nodes] * 3, parents, cache.keys[0].view(cache.shape),
                                   cache.values[0].view(cache.shape), cache.table.tolist(), lengths, d ** -0.5)
         ref.close(out, expected, size, q, torch.cat([k, cache.keys[0].view(-1, kv, d)]), d ** -0.5, 1506)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1e-6, 1e-9])
+def test_fp32_channels_far_below_the_others(scale):
+    """Every 17th channel of the values is `scale` times as large as the others. Two fp16 halves under their tile's exponent are
+    off by half of 2^-24 where the largest value is at least 2^14 (trees: 2^10 of their sample's), so the error is the
+    tolerance of the channel itself and 2^-39 (2^-35) of the largest value: weights sum to one."""
+    h, d = 8, 256
+    g = torch.Generator("cuda").manual_seed(106)
+    (q, k, v), stride = _fused(g, 340, h, 1, d, torch.float32)
+    v[:, :, 3::17] *= scale
+    out = torch.empty(q.shape, device="cuda")
+    _run_packed(native.F32, q, k, v, out, [300, 40], stride)
+    expected, size = ref.packed(q, k, v, [300, 40], 1 / 16)
+    tol = ref.tolerance(expected, size, q, k, 1 / 16, 300, torch.float32) + 2.0 ** -39 * float(v.abs().max())
+    assert bool(((out.double() - expected).abs() <= tol).all())
+    cache = Cache("f32", 1, 24, 1, d, [1000, 300], 20, 107)
+    cache.values[:, :, :, 3::17] *= scale
+    q, k, v = (_normal(g, 20, n, d, dtype=torch.float32) for n in (h, 1, 1))
+    v[:, :, 3::17] *= scale
+    out, expected, size = _run_tree(cache, q, k, v, [10, 10], [_branching(10, 1), _branching(10, 2)], 1000)
+    everything = torch.cat([k, cache.keys[0].view(-1, 1, d)])
+    tol = ref.tolerance(expected, size, q, everything, 1 / 16, 1010, torch.float32)
+    tol += 2.0 ** -35 * float(cache.values.abs().max())
+    assert bool(((out.double() - expected).abs() <= tol).all())
